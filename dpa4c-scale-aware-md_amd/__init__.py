@@ -17,7 +17,7 @@ import os
 
 import numpy as np
 
-from . import dpa4c, model, systems  # noqa: F401
+from . import dpa4c, model, ops, systems  # noqa: F401
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdpamd.so")
@@ -37,7 +37,7 @@ EXPORTED = ("dp_create", "dp_destroy", "dp_get_info", "dp_last_error", "dp_compu
             "dp_graph_stats", "dp_compute_canonical_graph_device", "dp_compute_edges_device",
             "dp_compute_edges_device_f32",
             "dp_debug_copy", "dp_debug_keep", "dp_debug_fused_rows", "dp_debug_few_rows",
-            "dp_debug_fitting_form", "dp_stage_times", "dp_device_bytes")
+            "dp_debug_fitting_form", "dp_stage_times", "dp_device_bytes") + ops.EXPORTED
 
 
 class DeepmdException(RuntimeError):
@@ -87,6 +87,7 @@ def lib():
         L.dp_device_bytes.argtypes = [P]
         L.dp_device_bytes.restype = C.c_size_t
         _ = D
+        ops.bind(L)
         _LIB = L
     return _LIB
 

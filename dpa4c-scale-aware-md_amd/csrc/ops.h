@@ -1,0 +1,82 @@
+// Operators of trainable heads (embedding lookup, gated block): arguments and launches
+// of their kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace dpamd {
+
+// activations, with the codes of the model files
+enum { kActTanh = 0, kActSilu = 1, kActGelu = 2 };
+
+// ---- tile products (product.h) ----
+enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2 };
+
+// A 16-bit operand: row length in elements; elements between its pieces (fp32 only).
+// 16-byte aligned, ld a multiple of 8, and the contiguous side ends at a multiple of 8
+// or is followed by zeros up to one.
+struct Operand {
+  const unsigned short* p;
+  long ld;
+  long plane;
+};
+
+// h, dg and du in operand form: [M][ldh], pieces plane_h apart; saved: [M][N] pairs (g, u).
+struct EpiArgs {
+  unsigned short* h;
+  unsigned short *dg, *du;
+  long ldh, plane_h;
+  float* saved;
+};
+
+struct ProductArgs {
+  Operand a[2], b[2];
+  int M, N, K;  // N: columns of one B matrix
+  int cols;     // columns written: N, or N and the zeros up to ldh
+  int segs;     // 2: K runs over a[0], b[0] and then over a[1], b[1]
+  int mats;     // 2: the columns of b[0] and then those of b[1], each to its own out
+  int split;    // slices of K, each to its own part of `partial`
+  int tiles_m, tiles_n, tiles_n1;  // tiles_n1: those of one matrix
+  int act;
+  float* partial;
+  long ldp;  // cols up to a multiple of 4
+  void* out[2];
+  long ldo[2];
+  bool vec[2];
+  EpiArgs epi;
+};
+
+// What a product is: which layouts and epilogue.
+enum ProductKind {
+  kProdGate,      // x Wg, x Wu -> h                    rows k-contiguous by columns
+  kProdDown,      // h Wd -> y
+  kProdGateGrad,  // dy Wd^T -> dg, du, h               both k-contiguous
+  kProdInput,     // dg Wg^T + du Wu^T -> dx
+  kProdWeight     // x^T dg, x^T du;  h^T dy            both k-strided
+};
+
+// How a product is cut: tile shape and slices of K, and the workspace its slices need.
+struct ProductPlan {
+  int shape, split;
+  size_t bytes;
+};
+ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu);
+void run_product(hipStream_t st, ProductKind what, int elem, const ProductPlan& plan, ProductArgs& args);
+
+// [rows][cols] of the caller's type into operand form, zeros up to ld.
+void pack_operand(hipStream_t st, int elem, const void* src, long ld_src, long rows, long cols, unsigned short* dst,
+                  long ld, long plane);
+// rows x row_bytes of zeros, rows `stride` bytes apart (a kernel: may be captured)
+void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride);
+
+// ---- lookup (lookup.hip) ----
+void lookup_rows(hipStream_t st, int elem, long n, int vocab, int width, const int* ids,
+                 const void* table, long ld_table, float scale, void* out, long ld_out);
+size_t lookup_grad_bytes(long n, int vocab, int width);
+void lookup_grad(hipStream_t st, int elem, long n, int vocab, int width, const int* ids, const void* dout,
+                 long ld, float scale, void* dtable, long ld_table, char* ws);
+
+}  // namespace dpamd

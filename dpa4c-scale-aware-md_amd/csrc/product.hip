@@ -1,0 +1,63 @@
+// The products of one element kind (ELEM_KIND, one object file each) and their launches.
+#include "product.h"
+
+namespace dpamd {
+
+namespace {
+
+// 16-bit kinds: 256 x 256 x 64 with eight waves of 128 x 64 (128 KB of LDS, one block
+// a compute unit) and 128 x 128 x 64 with four of 64 x 64 (64 KB, two). fp32, with
+// three planes to stage: 256 x 128 x 32 with eight of 64 x 64 and 128 x 64 x 32 with four of 64 x 32.
+template <int KIND>
+struct Shapes {
+  using Big = Shape<256, 256, 64, 2, 4>;
+  using Small = Shape<128, 128, 64, 2, 2>;
+};
+template <>
+struct Shapes<kF32> {
+  using Big = Shape<256, 128, 32, 4, 2>;
+  using Small = Shape<128, 64, 32, 2, 2>;
+};
+
+template <int KIND, int LA, int LB, int EPI, class S>
+void launch(hipStream_t st, ProductArgs& p) {
+  constexpr int SUB = EPI == kEpiGate ? 2 : 1;
+  p.tiles_m = (p.M + S::BM - 1) / S::BM;
+  p.tiles_n1 = (p.N + S::BN / SUB - 1) / (S::BN / SUB);
+  p.tiles_n = p.tiles_n1 * p.mats;
+  if ((long)p.tiles_m * p.tiles_n * p.split * (S::WM * S::WN * 64) >= 1L << 32)
+    throw HipError{hipErrorInvalidValue, "gated block: too many tiles for one launch"};
+  hipLaunchKernelGGL((k_product<KIND, LA, LB, EPI, S>), dim3(p.tiles_m * p.tiles_n, p.split),
+                     dim3(S::WM * S::WN * 64), 0, st, p);
+  DPAMD_LAUNCH_CHECK();
+  if (p.split > 1) {
+    const long rows = (long)p.M * (EPI == kEpiGate ? 1 : p.mats), quads = p.ldp / 4;
+    hipLaunchKernelGGL((k_join<KIND, EPI>), dim3((unsigned)((rows * quads + 255) / 256)), dim3(256), 0, st, p);
+    DPAMD_LAUNCH_CHECK();
+  }
+}
+
+template <int KIND, class S>
+void launch_kind(hipStream_t st, ProductKind what, ProductArgs& p) {
+  switch (what) {
+    case kProdGate: return launch<KIND, kRowK, kColK, kEpiGate, S>(st, p);
+    case kProdDown: return launch<KIND, kRowK, kColK, kEpiStore, S>(st, p);
+    case kProdGateGrad: return launch<KIND, kRowK, kRowK, kEpiGateGrad, S>(st, p);
+    case kProdInput: return launch<KIND, kRowK, kRowK, kEpiStore, S>(st, p);
+    case kProdWeight: return launch<KIND, kColK, kColK, kEpiStore, S>(st, p);
+  }
+}
+
+}  // namespace
+
+template <int KIND>
+void launch_product(hipStream_t st, ProductKind what, int shape, ProductArgs& p) {
+  if (shape == 0)
+    launch_kind<KIND, typename Shapes<KIND>::Big>(st, what, p);
+  else
+    launch_kind<KIND, typename Shapes<KIND>::Small>(st, what, p);
+}
+
+template void launch_product<ELEM_KIND>(hipStream_t, ProductKind, int, ProductArgs&);
+
+}  // namespace dpamd

@@ -342,6 +342,100 @@ int dp_stage_times(dp_model* model, int enable, double* times, int n, char* name
 /* Peak device bytes allocated by this handle so far (memory high-water mark). */
 size_t dp_device_bytes(const dp_model* model);
 
+/*
+ * Operators of trainable heads: what a per-atom (or per-token) net on top of
+ * descriptors or embeddings needs, forward and backward. No counterpart in the
+ * reference, whose nets are evaluated inside its model. Every array is device memory
+ * on the handle's GPU; work is ordered on `stream` (a hipStream_t, NULL = default
+ * stream) and the calls return without waiting for it. Matrices are row-major;
+ * a row length (ld_*) of 0 means packed rows. Inputs and outputs of one call must
+ * not overlap. Weights are [in][out], as in the model files.
+ *
+ * Types: DP_TYPE_F32, DP_TYPE_BF16 or DP_TYPE_F16 for every matrix of a call. Sums
+ * are held in fp32 and rounded once; the products of fp32 matrices are formed from
+ * three exact bf16 pieces an element on the matrix cores, to fp32 accuracy (an infinite
+ * input gives NaN there). Of the matrices between the products only h, dg and du are
+ * rounded to the type (and a value past the f16 range is infinite).
+ * Results do not depend on the order in which blocks run: a call repeated on the
+ * same inputs gives the same bits.
+ *
+ * A handle keeps one workspace for each stream it is used with, which grows to the largest call.
+ * Calls on several streams need no ordering by the caller beyond that of their own inputs
+ * and outputs. The calls can be captured into a HIP graph once the same call has run
+ * on that stream (so that the workspace is there; else DP_ERR_ARG); a workspace that a
+ * capture has seen is kept until dp_ops_destroy, and replays must not run beside
+ * other calls that use it. One handle per host thread; dp_ops_destroy waits for the
+ * handle's streams' work.
+ */
+typedef struct dp_ops dp_ops;
+enum { DP_TYPE_F32 = 0, DP_TYPE_BF16 = 1, DP_TYPE_F16 = 2 };
+/* activations; the first two have the codes of the DPA4C model files */
+enum { DP_ACT_TANH = 0, DP_ACT_SILU = 1, DP_ACT_GELU = 2 };
+
+int dp_ops_create(int gpu_rank, dp_ops** out);
+void dp_ops_destroy(dp_ops* ops);
+const char* dp_ops_last_error(const dp_ops* ops);
+/* Peak device bytes of the handle's workspaces. */
+size_t dp_ops_device_bytes(const dp_ops* ops);
+
+/*
+ * out[i] = scale * table[ids[i]], i < n: the rows of a table [vocab][width] that the
+ * ids name (atom types, tokens). An id outside 0 .. vocab - 1 (a virtual atom,
+ * padding) gives a row of zeros. One multiplication in fp32, rounded once. ld_table
+ * and ld_out: row lengths, so the rows can be columns of wider matrices (the type
+ * columns of a descriptor).
+ */
+int dp_embed(dp_ops* ops, int type, int64_t n, int vocab, int width, const int* d_ids,
+             const void* d_table, int64_t ld_table, float scale, void* d_out, int64_t ld_out,
+             void* stream);
+
+/*
+ * The gradient of dp_embed's table: dtable[v] = scale * sum of dout[i] over the i
+ * with ids[i] == v, every row of dtable written (zeros where no id names it).
+ * The ids are sorted and each row's sum is formed in fp32 in an order that depends on
+ * the ids alone, and rounded once.
+ */
+int dp_embed_grad(dp_ops* ops, int type, int64_t n, int vocab, int width, const int* d_ids,
+                  const void* d_dout, int64_t ld_dout, float scale, void* d_dtable,
+                  int64_t ld_dtable, void* stream);
+
+/*
+ * The gated feed-forward block y = h w_down, h = act(x w_gate) * (x w_up):
+ * x [rows][d_in], w_gate and w_up [d_in][d_hidden], w_down [d_hidden][d_out],
+ * y [rows][d_out]. ld_hidden is the row length of w_gate, w_up and of their gradients
+ * (2 d_hidden for the two stored side by side), ld_down that of w_down and its gradient.
+ */
+typedef struct {
+  int64_t rows;
+  int d_in, d_hidden, d_out;
+  int type, act;
+  int64_t ld_x;      /* x and dx */
+  int64_t ld_y;      /* y and dy */
+  int64_t ld_hidden; /* w_gate, w_up and their gradients */
+  int64_t ld_down;   /* w_down and its gradient */
+} dp_gated_shape;
+
+/* Bytes that dp_gated_forward keeps for dp_gated_backward: x w_gate and x w_up in fp32, 8 bytes
+ * for each of rows * d_hidden. 0 for a shape that the calls refuse. */
+size_t dp_gated_saved_bytes(const dp_gated_shape* shape);
+
+/* d_saved: NULL (no backward follows) or dp_gated_saved_bytes bytes, 16-byte aligned. */
+int dp_gated_forward(dp_ops* ops, const dp_gated_shape* shape, const void* d_x,
+                     const void* d_w_gate, const void* d_w_up, const void* d_w_down, void* d_y,
+                     void* d_saved, void* stream);
+
+/*
+ * From dy and what the forward kept: dx = dg w_gate^T + du w_up^T, dw_gate = x^T dg,
+ * dw_up = x^T du, dw_down = h^T dy, with dh = dy w_down^T, du = dh * act(g) and
+ * dg = dh * u * act'(g). An output that is NULL is not formed (dx of frozen descriptors;
+ * dw_gate and dw_up are both given or both NULL). With rows == 0 the weights'
+ * gradients are zeros.
+ */
+int dp_gated_backward(dp_ops* ops, const dp_gated_shape* shape, const void* d_x,
+                      const void* d_w_gate, const void* d_w_up, const void* d_w_down,
+                      const void* d_saved, const void* d_dy, void* d_dx, void* d_dw_gate,
+                      void* d_dw_up, void* d_dw_down, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
