@@ -73,10 +73,10 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
     int bm, bn, bk, per_cu;
     double us;  // one step of k of one block
   };
-  static const S shapes[2][2] = {{{256, 256, 64, 1, 2.1}, {128, 128, 64, 2, 1.5}},
-                                 {{256, 128, 32, 1, 2.0}, {128, 64, 32, 2, 1.2}}};
+  static const S shapes[2][2] = {{{256, 256, 64, 1, 1.9}, {128, 128, 64, 2, 1.4}},
+                                 {{256, 128, 32, 1, 1.8}, {128, 64, 32, 2, 1.1}}};
   const int sub = what == kProdGate ? 2 : 1;
-  ProductPlan best{1, 1, 0};
+  ProductPlan best{1, 1, ncu, 0};
   double best_us = 0;
   for (int k = 0; k < 2; ++k) {
     const S& s = shapes[elem == kF32][k];
@@ -89,7 +89,7 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
     const double us = (double)rounds * ((steps + split - 1) / split) * s.us + (split > 1 ? 3 + 2 * bytes / 4e6 : 0);
     if (k == 0 || us < best_us) {
       best_us = us;
-      best = ProductPlan{k, (int)split, (size_t)bytes};
+      best = ProductPlan{k, (int)split, (int)slots / 8 * 8, (size_t)bytes};
     }
   }
   return best;
@@ -97,6 +97,7 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
 
 void run_product(hipStream_t st, ProductKind what, int elem, const ProductPlan& plan, ProductArgs& p) {
   p.split = plan.split;
+  p.blocks = plan.blocks;
   p.ldp = (p.cols + 3) / 4 * 4;
   if (elem == kBf16)
     launch_product<kBf16>(st, what, plan.shape, p);

@@ -5,10 +5,16 @@
 // a row's chunks, four rows a thread so that their loads are under way together.
 //
 // Gradient: dE[v] = s sum_{id_i = v} dout_i, without atomics, so that the sums' order is
-// fixed by the ids alone. The row indices are sorted by id (stable radix sort, 8 bits a pass;
-// ids outside the table sort behind it); then each table row sums its run of the
-// sorted rows, and a long run, cut at every kWindow sorted positions, is summed window by
-// window first and the windows' sums in order.
+// fixed by the ids alone. It reads n rows, writes vocab rows. Two forms:
+//
+// Few ids (atom types): a block sums a contiguous share of the rows into tables of its own in
+// LDS, one for each row it has under way, so that every entry has one thread; the blocks'
+// tables are then added up in order.
+//
+// Many ids (tokens): the row indices are sorted by id (stable radix sort, 8 bits a pass;
+// ids outside the table sort behind it), each table row sums its run of the sorted rows, and
+// a long run, cut at every kWindow sorted positions, is summed window by window first and the
+// windows' sums in order.
 #include <algorithm>
 
 #include "kernels.h"
@@ -73,7 +79,7 @@ __global__ __launch_bounds__(256) void k_lookup(long n, int vocab, int chunks, i
 #pragma unroll
       for (int k = 0; k < kLookupRows; ++k) {
         if (id[k] >= 0) {
-          v[k] = *reinterpret_cast<const C*>(table + id[k] * ld_table + c * E);
+          v[k] = *reinterpret_cast<const C*>(table + id[k] * ld_table + (long)c * E);
 #pragma unroll
           for (int e = 0; e < E; ++e) v[k].v[e] = from_f32<KIND>(to_f32<KIND>(v[k].v[e]) * scale);
         } else {
@@ -83,7 +89,7 @@ __global__ __launch_bounds__(256) void k_lookup(long n, int vocab, int chunks, i
       }
 #pragma unroll
       for (int k = 0; k < kLookupRows; ++k)
-        if (r0 + k < n) *reinterpret_cast<C*>(out + (r0 + k) * ld_out + c * E) = v[k];
+        if (r0 + k < n) *reinterpret_cast<C*>(out + (r0 + k) * ld_out + (long)c * E) = v[k];
     }
   }
 }
@@ -99,13 +105,18 @@ int chunk_of(int width, const void* a, long lda, const void* b, long ldb) {
   return 1;
 }
 
+// lanes that read one row
+int row_lanes(int chunks) {
+  int lanes = 1;
+  while (lanes < chunks && lanes < 256) lanes *= 2;
+  return lanes;
+}
+
 template <int KIND, int E>
 void launch_lookup(hipStream_t st, long n, int vocab, int width, const int* ids, const void* table, long ld_table,
                    float scale, void* out, long ld_out) {
   using T = typename ElemOf<KIND>::T;
-  const int chunks = width / E;
-  int lanes = 1;
-  while (lanes < chunks && lanes < 256) lanes *= 2;
+  const int chunks = width / E, lanes = row_lanes(chunks);
   const long per = 256 / lanes * kLookupRows;
   const dim3 grid((unsigned)std::min((n + per - 1) / per, 1L << 20));
   hipLaunchKernelGGL((k_lookup<KIND, E>), grid, dim3(256), 0, st, n, vocab, chunks, lanes, ids,
@@ -139,11 +150,14 @@ __device__ __forceinline__ unsigned key_of(const int* ids, const unsigned* keys,
   return id >= 0 && id < vocab ? (unsigned)id : (unsigned)vocab;
 }
 
-// counts[digit][tile]
+// counts[digit][tile]; also clears `zeros` ints
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const int* ids, const unsigned* keys, long n, int vocab,
-                                                             int shift, int tiles, int* counts) {
+                                                             int shift, int tiles, int* counts, int* zero,
+                                                             long zeros) {
   __shared__ int hist[kDigits];
   hist[threadIdx.x] = 0;
+  for (long i = (long)blockIdx.x * kSortThreads + threadIdx.x; i < zeros; i += (long)gridDim.x * kSortThreads)
+    zero[i] = 0;
   __syncthreads();
   const long base = (long)blockIdx.x * kSortTile;
 #pragma unroll
@@ -155,13 +169,15 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const int* ids, con
   counts[(long)threadIdx.x * tiles + blockIdx.x] = hist[threadIdx.x];
 }
 
-// Places the tile's rows at starts[digit][tile] + rank among the tile's rows of that
-// digit, in row order: wave w takes a contiguous run of rows, 64 at a time; the lanes of
+// Places the tile's rows at starts[digit][tile] (the counts' exclusive sums; null: formed
+// here) + rank among the tile's rows of that digit, in row order: wave w takes a contiguous run of rows, 64 at a time; the lanes of
 // equal digits are found by one ballot a bit.
 __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, const unsigned* keys, const int* rows,
                                                              long n, int vocab, int shift, int tiles,
-                                                             const int* starts, unsigned* keys_out, int* rows_out) {
+                                                             const int* starts, const int* counts,
+                                                             unsigned* keys_out, int* rows_out) {
   __shared__ int count[kSortWaves][kDigits];
+  __shared__ int totals[kDigits];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   for (int w = 0; w < kSortWaves; ++w) count[w][threadIdx.x] = 0;
   __syncthreads();
@@ -189,7 +205,28 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, con
   }
   __syncthreads();
   {
-    int at = starts[(long)threadIdx.x * tiles + blockIdx.x];
+    int at;
+    if (starts) {
+      at = starts[(long)threadIdx.x * tiles + blockIdx.x];
+    } else {
+      // few tiles: this tile's starts from the counts themselves
+      int before = 0, total = 0;
+      for (int t = 0; t < tiles; ++t) {
+        const int c = counts[(long)threadIdx.x * tiles + t];
+        before += t < (int)blockIdx.x ? c : 0;
+        total += c;
+      }
+      int sum = total;  // inclusive over the wave's digits
+#pragma unroll
+      for (int off = 1; off < kWave; off *= 2) {
+        const int v = __shfl_up(sum, off, kWave);
+        if (lane >= off) sum += v;
+      }
+      totals[threadIdx.x] = sum;
+      __syncthreads();
+      at = before + sum - total;
+      for (int w = 0; w < wave; ++w) at += totals[w * kWave + kWave - 1];
+    }
     for (int w = 0; w < kSortWaves; ++w) {
       const int c = count[w][threadIdx.x];
       count[w][threadIdx.x] = at;
@@ -209,108 +246,216 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, con
 }
 
 // ---- sums of runs ---------------------------------------------------------------------
-constexpr int kWindow = 32;   // sorted positions of one window
-constexpr int kShort = 64;    // runs up to this length are summed by their table row itself
+constexpr int kWindow = 32;     // sorted positions of one window
+constexpr int kShort = 64;      // runs up to this length are summed by their table row itself
+constexpr int kScanTiles = 64;  // tiles up to which each block of the sort forms its starts itself
 
-// first position whose key is >= v
-__device__ __forceinline__ int lower_bound(const unsigned* keys, int n, unsigned v) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (keys[mid] < v)
-      lo = mid + 1;
-    else
-      hi = mid;
+// run[2 v], run[2 v + 1]: first position and end of id v's run (both 0 where there is none)
+__global__ __launch_bounds__(256) void k_runs(int n, int vocab, const unsigned* __restrict__ keys,
+                                              int* __restrict__ run) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const unsigned v = keys[i];
+  if (v >= (unsigned)vocab) return;
+  if (i == 0 || keys[i - 1] != v) run[2 * (long)v] = i;
+  if (i == n - 1 || keys[i + 1] != v) run[2 * (long)v + 1] = i + 1;
+}
+
+// acc += rows[from .. to) of this lane's chunk, four loads under way
+template <int KIND, int E>
+__device__ __forceinline__ void add_rows(float (&acc)[E], int from, int to, const int* __restrict__ rows,
+                                         const typename ElemOf<KIND>::T* __restrict__ dout, long ld, int c) {
+  using C = Chunk<KIND, E>;
+  int i = from;
+  for (; i + 4 <= to; i += 4) {
+    C x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = *reinterpret_cast<const C*>(dout + rows[i + q] * ld + (long)c * E);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int k = 0; k < E; ++k) acc[k] += to_f32<KIND>(x[q].v[k]);
   }
-  return lo;
+  for (; i < to; ++i) {
+    const C x = *reinterpret_cast<const C*>(dout + rows[i] * ld + (long)c * E);
+#pragma unroll
+    for (int k = 0; k < E; ++k) acc[k] += to_f32<KIND>(x.v[k]);
+  }
 }
 
 // partial[2 w + 0]: the window's part of the run that holds its first position;
 // partial[2 w + 1]: of a long run that starts inside it (there is at most one: a run
-// longer than a window reaches the window's end). Only for runs longer than kShort. One
-// lane sums E columns.
+// longer than a window reaches the window's end). Only for runs longer than kShort.
 template <int KIND, int E>
-__global__ __launch_bounds__(64) void k_grad_windows(int n, int vocab, int chunks, const unsigned* __restrict__ keys,
-                                                     const int* __restrict__ rows,
+__global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chunks, const unsigned* __restrict__ keys,
+                                                      const int* __restrict__ rows, const int* __restrict__ run,
+                                                      const typename ElemOf<KIND>::T* __restrict__ dout, long ld,
+                                                      float* __restrict__ partial) {
+  const int windows = (n + kWindow - 1) / kWindow, lane = threadIdx.x & 63;
+  for (int w = blockIdx.x * 4 + threadIdx.x / 64; w < windows; w += gridDim.x * 4) {
+    const int b = w * kWindow, e = min(n, b + kWindow);
+    const unsigned first = keys[b], last = keys[e - 1];
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const unsigned v = part ? last : first;
+      if (v >= (unsigned)vocab || (part && last == first)) continue;
+      const int lo = run[2 * (long)v], hi = run[2 * (long)v + 1];
+      if (hi - lo <= kShort) continue;
+      for (int c = lane; c < chunks; c += 64) {
+        float acc[E] = {};
+        add_rows<KIND, E>(acc, max(lo, b), min(hi, e), rows, dout, ld, c);
+        float* o = partial + ((long)(2 * (long)w + part) * chunks + c) * E;
+#pragma unroll
+        for (int k = 0; k < E; ++k) o[k] = acc[k];
+      }
+    }
+  }
+}
+
+// One wave a table row.
+template <int KIND, int E>
+__global__ __launch_bounds__(256) void k_grad_rows(int vocab, int chunks, const int* __restrict__ rows,
+                                                   const int* __restrict__ run,
+                                                   const typename ElemOf<KIND>::T* __restrict__ dout, long ld,
+                                                   const float* __restrict__ partial, float scale,
+                                                   typename ElemOf<KIND>::T* __restrict__ dtable, long ld_table) {
+  using C = Chunk<KIND, E>;
+  const int lane = threadIdx.x & 63;
+  for (long v = (long)blockIdx.x * 4 + threadIdx.x / 64; v < vocab; v += (long)gridDim.x * 4) {
+    const int lo = run[2 * v], hi = run[2 * v + 1];
+    for (int c = lane; c < chunks; c += 64) {
+      float acc[E] = {};
+      if (hi - lo <= kShort) {
+        add_rows<KIND, E>(acc, lo, hi, rows, dout, ld, c);
+      } else {
+        const int w0 = lo / kWindow, w1 = (hi - 1) / kWindow;
+        for (int w = w0; w <= w1; ++w) {
+          const float* p = partial + ((2 * (long)w + (lo > w * kWindow)) * chunks + c) * E;
+#pragma unroll
+          for (int k = 0; k < E; ++k) acc[k] += p[k];
+        }
+      }
+      C o;
+#pragma unroll
+      for (int k = 0; k < E; ++k) o.v[k] = from_f32<KIND>(acc[k] * scale);
+      *reinterpret_cast<C*>(dtable + v * ld_table + (long)c * E) = o;
+    }
+  }
+}
+
+// ---- few ids ----------------------------------------------------------------------------
+constexpr int kTableBytes = 64 << 10;  // LDS of a block's tables: two blocks a compute unit
+constexpr int kTableRows = 4;          // rows a thread has under way
+
+// The tables of one block: one for each of the 256 / lanes rows that it reads at a time.
+// A thread adds its chunks of its rows into its entries, which no other thread touches.
+template <int KIND, int E>
+__global__ __launch_bounds__(256) void k_grad_tables(long n, int vocab, int chunks, int lanes, long share,
+                                                     const int* __restrict__ ids,
                                                      const typename ElemOf<KIND>::T* __restrict__ dout, long ld,
                                                      float* __restrict__ partial) {
   using C = Chunk<KIND, E>;
-  const int w = blockIdx.x, c = blockIdx.y * 64 + threadIdx.x;
-  const int b = w * kWindow, e = min(n, b + kWindow);
-  const unsigned first = keys[b], last = keys[e - 1];
+  extern __shared__ __align__(16) float table[];
+  const int per = 256 / lanes, sub = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+  const int entries = vocab * chunks * E;
+  for (int k = threadIdx.x; k < per * entries; k += 256) table[k] = 0.0f;
+  __syncthreads();
+  float* mine = table + sub * entries;
+  const long from = blockIdx.x * share, to = min(n, from + share);
+  for (long r0 = from + sub; r0 < to; r0 += (long)per * kTableRows) {
+    int id[kTableRows];
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const unsigned v = part ? last : first;
-    if (v >= (unsigned)vocab || (part && last == first)) continue;
-    const int lo = lower_bound(keys, n, v), hi = lower_bound(keys, n, v + 1);
-    if (hi - lo <= kShort) continue;
-    const int from = max(lo, b), to = min(hi, e);
-    float acc[E] = {};
-    if (c < chunks) {
-      for (int i = from; i < to; ++i) {
-        const C x = *reinterpret_cast<const C*>(dout + rows[i] * ld + c * E);
-#pragma unroll
-        for (int k = 0; k < E; ++k) acc[k] += to_f32<KIND>(x.v[k]);
-      }
-      float* o = partial + ((long)(2 * w + part) * chunks + c) * E;
-#pragma unroll
-      for (int k = 0; k < E; ++k) o[k] = acc[k];
+    for (int k = 0; k < kTableRows; ++k) {
+      const long r = r0 + (long)k * per;
+      id[k] = r < to ? ids[r] : -1;
+      if (id[k] >= vocab) id[k] = -1;
     }
+    for (int c = lane; c < chunks; c += lanes) {
+      C x[kTableRows];
+#pragma unroll
+      for (int k = 0; k < kTableRows; ++k)
+        if (id[k] >= 0) x[k] = *reinterpret_cast<const C*>(dout + (r0 + (long)k * per) * ld + (long)c * E);
+#pragma unroll
+      for (int k = 0; k < kTableRows; ++k)
+        if (id[k] >= 0) {
+          float* t = mine + (id[k] * chunks + c) * E;
+#pragma unroll
+          for (int e = 0; e < E; ++e) t[e] += to_f32<KIND>(x[k].v[e]);
+        }
+    }
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < entries; k += 256) {
+    float acc = 0.0f;
+    for (int q = 0; q < per; ++q) acc += table[q * entries + k];
+    partial[(long)blockIdx.x * entries + k] = acc;
   }
 }
 
-// One wave a table row and 64 chunks of it.
-template <int KIND, int E>
-__global__ __launch_bounds__(64) void k_grad_rows(int n, int chunks, const unsigned* __restrict__ keys,
-                                                  const int* __restrict__ rows,
-                                                  const typename ElemOf<KIND>::T* __restrict__ dout, long ld,
-                                                  const float* __restrict__ partial, float scale,
-                                                  typename ElemOf<KIND>::T* __restrict__ dtable, long ld_table) {
-  using C = Chunk<KIND, E>;
-  const int v = blockIdx.x, c = blockIdx.y * 64 + threadIdx.x;
-  const int lo = lower_bound(keys, n, v), hi = lower_bound(keys, n, v + 1);
-  if (c >= chunks) return;
-  float acc[E] = {};
-  if (hi - lo <= kShort) {
-    for (int i = lo; i < hi; ++i) {
-      const C x = *reinterpret_cast<const C*>(dout + rows[i] * ld + c * E);
+// The blocks' tables added up: G threads an entry, each a contiguous share of the
+// blocks in order, the shares joined in order.
+template <int KIND>
+__global__ __launch_bounds__(256) void k_grad_join(int blocks, int entries, int width, int G,
+                                                   const float* __restrict__ partial, float scale,
+                                                   typename ElemOf<KIND>::T* __restrict__ dtable, long ld_table) {
+  __shared__ float part[256];
+  const int per = 256 / G, slot = threadIdx.x % per, share = threadIdx.x / per;
+  const int k = blockIdx.x * per + slot;
+  const int b0 = (int)((long)blocks * share / G), b1 = (int)((long)blocks * (share + 1) / G);
+  float acc = 0.0f;
+  if (k < entries) {
+    int b = b0;
+    for (; b + 8 <= b1; b += 8) {
+      float x[8];
 #pragma unroll
-      for (int k = 0; k < E; ++k) acc[k] += to_f32<KIND>(x.v[k]);
-    }
-  } else {
-    for (int w = lo / kWindow; w * kWindow < hi; ++w) {
-      const int part = lo > w * kWindow;
-      const float* p = partial + ((long)(2 * w + part) * chunks + c) * E;
+      for (int q = 0; q < 8; ++q) x[q] = partial[(long)(b + q) * entries + k];
 #pragma unroll
-      for (int k = 0; k < E; ++k) acc[k] += p[k];
+      for (int q = 0; q < 8; ++q) acc += x[q];
     }
+    for (; b < b1; ++b) acc += partial[(long)b * entries + k];
   }
-  C o;
-#pragma unroll
-  for (int k = 0; k < E; ++k) o.v[k] = from_f32<KIND>(acc[k] * scale);
-  *reinterpret_cast<C*>(dtable + v * ld_table + c * E) = o;
+  part[threadIdx.x] = acc;
+  __syncthreads();
+  if (share || k >= entries) return;
+  for (int q = 1; q < G; ++q) acc += part[q * per + slot];
+  dtable[k / width * ld_table + k % width] = from_f32<KIND>(acc * scale);
+}
+
+// Blocks of the form for few ids, 0 where its tables do not fit. A block has at least
+// 16 rows a thread, so that the tables written are few beside the rows read.
+int table_blocks(long n, int vocab, int width, int chunks) {
+  const long per = 256 / row_lanes(chunks), entries = (long)vocab * width;
+  if (per * entries * 4 > kTableBytes) return 0;
+  return (int)std::max(1L, std::min(1024L, n / (per * 16)));
 }
 
 struct GradPlan {
+  int blocks;  // of the form for few ids, or 0
   int passes, tiles;
-  size_t keys[2], rows[2], counts, starts, scan, partial, bytes;
+  size_t keys[2], rows[2], run, counts, starts, scan, partial, bytes;
 };
 
-GradPlan grad_plan(long n, int vocab, int width) {
+GradPlan grad_plan(long n, int vocab, int width, int chunks) {
   GradPlan g{};
-  int bits = 1;
-  while (bits < 31 && (1L << bits) <= vocab) ++bits;  // keys 0 .. vocab
-  g.passes = (bits + kBits - 1) / kBits;
-  g.tiles = (int)((n + kSortTile - 1) / kSortTile);
   auto take = [&](size_t b) {
     const size_t at = g.bytes;
     g.bytes += (b + 255) & ~size_t(255);
     return at;
   };
+  g.blocks = table_blocks(n, vocab, width, chunks);
+  if (g.blocks) {
+    g.partial = take(4 * (size_t)g.blocks * vocab * width);
+    return g;
+  }
+  int bits = 1;
+  while (bits < 31 && (1L << bits) <= vocab) ++bits;  // keys 0 .. vocab
+  g.passes = (bits + kBits - 1) / kBits;
+  g.tiles = (int)((n + kSortTile - 1) / kSortTile);
   for (int k = 0; k < 2; ++k) {
     g.keys[k] = take(4 * n);
     g.rows[k] = take(4 * n);
   }
+  g.run = take(8 * (size_t)vocab);
   const int m = kDigits * g.tiles;
   g.counts = take(4 * (size_t)m);
   g.starts = take(4 * (size_t)m);
@@ -319,29 +464,70 @@ GradPlan grad_plan(long n, int vocab, int width) {
   return g;
 }
 
+// a grid of `waves` waves in blocks of four, striding where there are more than a launch takes
+dim3 wave_blocks(long waves) { return dim3((unsigned)std::min((waves + 3) / 4, 1L << 20)); }
+
 template <int KIND, int E>
-void launch_grad(hipStream_t st, long n, int vocab, int width, const void* dout, long ld, float scale, void* dtable,
-                 long ld_table, const unsigned* keys, const int* rows, float* partial) {
+void launch_grad(hipStream_t st, long n, int vocab, int width, const int* ids, const void* dout_, long ld, float scale,
+                 void* dtable_, long ld_table, char* ws) {
   using T = typename ElemOf<KIND>::T;
-  const int chunks = width / E, cols = (chunks + 63) / 64;
-  hipLaunchKernelGGL((k_grad_windows<KIND, E>), dim3((unsigned)((n + kWindow - 1) / kWindow), cols), dim3(64), 0, st,
-                     (int)n, vocab, chunks, keys, rows, static_cast<const T*>(dout), ld, partial);
+  const T* dout = static_cast<const T*>(dout_);
+  T* dtable = static_cast<T*>(dtable_);
+  const int chunks = width / E;
+  const GradPlan g = grad_plan(n, vocab, width, chunks);
+  float* partial = reinterpret_cast<float*>(ws + g.partial);
+  if (g.blocks) {
+    const int lanes = row_lanes(chunks), entries = vocab * width;
+    const long share = (n + g.blocks - 1) / g.blocks;
+    hipLaunchKernelGGL((k_grad_tables<KIND, E>), dim3(g.blocks), dim3(256), 256 / lanes * entries * 4, st, n, vocab,
+                       chunks, lanes, share, ids, dout, ld, partial);
+    DPAMD_LAUNCH_CHECK();
+    int G = 1;
+    while (G < 256 && g.blocks > 8 * G) G *= 2;
+    hipLaunchKernelGGL((k_grad_join<KIND>), dim3((entries + 256 / G - 1) / (256 / G)), dim3(256), 0, st, g.blocks,
+                       entries, width, G, partial, scale, dtable, ld_table);
+    DPAMD_LAUNCH_CHECK();
+    return;
+  }
+  unsigned* keys[2] = {reinterpret_cast<unsigned*>(ws + g.keys[0]), reinterpret_cast<unsigned*>(ws + g.keys[1])};
+  int* rows[2] = {reinterpret_cast<int*>(ws + g.rows[0]), reinterpret_cast<int*>(ws + g.rows[1])};
+  int* run = reinterpret_cast<int*>(ws + g.run);
+  int* counts = reinterpret_cast<int*>(ws + g.counts);
+  int* starts = g.tiles > kScanTiles ? reinterpret_cast<int*>(ws + g.starts) : nullptr;
+  const int m = kDigits * g.tiles;
+  for (int p = 0; p < g.passes; ++p) {
+    const unsigned* kin = p ? keys[(p + 1) & 1] : nullptr;
+    const int* rin = p ? rows[(p + 1) & 1] : nullptr;
+    hipLaunchKernelGGL(k_sort_count, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, n, vocab, kBits * p, g.tiles,
+                       counts, run, p ? 0 : 2 * (long)vocab);
+    DPAMD_LAUNCH_CHECK();
+    if (starts) exclusive_scan_int(st, counts, starts, m, ws + g.scan, scan_temp_bytes(m));
+    hipLaunchKernelGGL(k_sort_place, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, rin, n, vocab, kBits * p,
+                       g.tiles, starts, counts, keys[p & 1], rows[p & 1]);
+    DPAMD_LAUNCH_CHECK();
+  }
+  const unsigned* key = keys[(g.passes - 1) & 1];
+  const int* row = rows[(g.passes - 1) & 1];
+  hipLaunchKernelGGL(k_runs, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (int)n, vocab, key, run);
   DPAMD_LAUNCH_CHECK();
-  hipLaunchKernelGGL((k_grad_rows<KIND, E>), dim3(vocab, cols), dim3(64), 0, st, (int)n, chunks, keys, rows,
-                     static_cast<const T*>(dout), ld, partial, scale, static_cast<T*>(dtable), ld_table);
+  hipLaunchKernelGGL((k_grad_windows<KIND, E>), wave_blocks((n + kWindow - 1) / kWindow), dim3(256), 0, st, (int)n,
+                     vocab, chunks, key, row, run, dout, ld, partial);
+  DPAMD_LAUNCH_CHECK();
+  hipLaunchKernelGGL((k_grad_rows<KIND, E>), wave_blocks(vocab), dim3(256), 0, st, vocab, chunks, row, run, dout, ld,
+                     partial, scale, dtable, ld_table);
   DPAMD_LAUNCH_CHECK();
 }
 
 template <int KIND>
-void grad_kind(hipStream_t st, long n, int vocab, int width, const void* dout, long ld, float scale, void* dtable,
-               long ld_table, const unsigned* keys, const int* rows, float* partial) {
+void grad_kind(hipStream_t st, long n, int vocab, int width, const int* ids, const void* dout, long ld, float scale,
+               void* dtable, long ld_table, char* ws) {
   switch (chunk_of<KIND>(width, dout, ld, dtable, ld_table)) {
     case 8:
       if constexpr (KIND != kF32)
-        return launch_grad<KIND, 8>(st, n, vocab, width, dout, ld, scale, dtable, ld_table, keys, rows, partial);
-    case 4: return launch_grad<KIND, 4>(st, n, vocab, width, dout, ld, scale, dtable, ld_table, keys, rows, partial);
-    case 2: return launch_grad<KIND, 2>(st, n, vocab, width, dout, ld, scale, dtable, ld_table, keys, rows, partial);
-    default: return launch_grad<KIND, 1>(st, n, vocab, width, dout, ld, scale, dtable, ld_table, keys, rows, partial);
+        return launch_grad<KIND, 8>(st, n, vocab, width, ids, dout, ld, scale, dtable, ld_table, ws);
+    case 4: return launch_grad<KIND, 4>(st, n, vocab, width, ids, dout, ld, scale, dtable, ld_table, ws);
+    case 2: return launch_grad<KIND, 2>(st, n, vocab, width, ids, dout, ld, scale, dtable, ld_table, ws);
+    default: return launch_grad<KIND, 1>(st, n, vocab, width, ids, dout, ld, scale, dtable, ld_table, ws);
   }
 }
 
@@ -357,35 +543,21 @@ void lookup_rows(hipStream_t st, int elem, long n, int vocab, int width, const i
     lookup_kind<kF32>(st, n, vocab, width, ids, table, ld_table, scale, out, ld_out);
 }
 
-size_t lookup_grad_bytes(long n, int vocab, int width) { return grad_plan(n, vocab, width).bytes; }
+size_t lookup_grad_bytes(int elem, long n, int vocab, int width, const void* dout, long ld, const void* dtable,
+                         long ld_table) {
+  const int e = elem == kF32 ? chunk_of<kF32>(width, dout, ld, dtable, ld_table)
+                             : chunk_of<kBf16>(width, dout, ld, dtable, ld_table);
+  return grad_plan(n, vocab, width, width / e).bytes;
+}
 
 void lookup_grad(hipStream_t st, int elem, long n, int vocab, int width, const int* ids, const void* dout, long ld,
                  float scale, void* dtable, long ld_table, char* ws) {
-  const GradPlan g = grad_plan(n, vocab, width);
-  unsigned* keys[2] = {reinterpret_cast<unsigned*>(ws + g.keys[0]), reinterpret_cast<unsigned*>(ws + g.keys[1])};
-  int* rows[2] = {reinterpret_cast<int*>(ws + g.rows[0]), reinterpret_cast<int*>(ws + g.rows[1])};
-  int* counts = reinterpret_cast<int*>(ws + g.counts);
-  int* starts = reinterpret_cast<int*>(ws + g.starts);
-  const int m = kDigits * g.tiles;
-  for (int p = 0; p < g.passes; ++p) {
-    const unsigned* kin = p ? keys[(p + 1) & 1] : nullptr;
-    const int* rin = p ? rows[(p + 1) & 1] : nullptr;
-    hipLaunchKernelGGL(k_sort_count, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, n, vocab, kBits * p, g.tiles,
-                       counts);
-    DPAMD_LAUNCH_CHECK();
-    exclusive_scan_int(st, counts, starts, m, ws + g.scan, scan_temp_bytes(m));
-    hipLaunchKernelGGL(k_sort_place, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, rin, n, vocab, kBits * p,
-                       g.tiles, starts, keys[p & 1], rows[p & 1]);
-    DPAMD_LAUNCH_CHECK();
-  }
-  const int last = (g.passes - 1) & 1;
-  float* partial = reinterpret_cast<float*>(ws + g.partial);
   if (elem == kBf16)
-    grad_kind<kBf16>(st, n, vocab, width, dout, ld, scale, dtable, ld_table, keys[last], rows[last], partial);
+    grad_kind<kBf16>(st, n, vocab, width, ids, dout, ld, scale, dtable, ld_table, ws);
   else if (elem == kF16)
-    grad_kind<kF16>(st, n, vocab, width, dout, ld, scale, dtable, ld_table, keys[last], rows[last], partial);
+    grad_kind<kF16>(st, n, vocab, width, ids, dout, ld, scale, dtable, ld_table, ws);
   else
-    grad_kind<kF32>(st, n, vocab, width, dout, ld, scale, dtable, ld_table, keys[last], rows[last], partial);
+    grad_kind<kF32>(st, n, vocab, width, ids, dout, ld, scale, dtable, ld_table, ws);
 }
 
 }  // namespace dpamd

@@ -378,7 +378,7 @@ int dp_embed_grad(dp_ops* O, int type, int64_t n, int vocab, int width, const in
       return;
     }
     const int elem = elem_of(type);
-    char* ws = workspace(O, st, lookup_grad_bytes(n, vocab, width));
+    char* ws = workspace(O, st, lookup_grad_bytes(elem, n, vocab, width, dout, li, dtable, lo));
     lookup_grad(st, elem, n, vocab, width, ids, dout, li, scale, dtable, lo, ws);
   });
 }

@@ -39,7 +39,9 @@ struct ProductArgs {
   int segs;     // 2: K runs over a[0], b[0] and then over a[1], b[1]
   int mats;     // 2: the columns of b[0] and then those of b[1], each to its own out
   int split;    // slices of K, each to its own part of `partial`
+  int join;     // threads that share the slices of one quad of columns (divides 256)
   int tiles_m, tiles_n, tiles_n1;  // tiles_n1: those of one matrix
+  int blocks;  // at most: those that the card holds at once
   int act;
   float* partial;
   long ldp;  // cols up to a multiple of 4
@@ -60,7 +62,7 @@ enum ProductKind {
 
 // How a product is cut: tile shape and slices of K, and the workspace its slices need.
 struct ProductPlan {
-  int shape, split;
+  int shape, split, blocks;
   size_t bytes;
 };
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu);
@@ -75,7 +77,8 @@ void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride
 // ---- lookup (lookup.hip) ----
 void lookup_rows(hipStream_t st, int elem, long n, int vocab, int width, const int* ids,
                  const void* table, long ld_table, float scale, void* out, long ld_out);
-size_t lookup_grad_bytes(long n, int vocab, int width);
+size_t lookup_grad_bytes(int elem, long n, int vocab, int width, const void* dout, long ld, const void* dtable,
+                         long ld_table);
 void lookup_grad(hipStream_t st, int elem, long n, int vocab, int width, const int* ids, const void* dout,
                  long ld, float scale, void* dtable, long ld_table, char* ws);
 

@@ -3,7 +3,10 @@
 // operands and for fp32 ones as three exact bf16 pieces (bf16x3.h).
 #pragma once
 
+#include <type_traits>
+
 #include "bf16x3.h"
+#include "fastmath.h"
 #include "ops.h"
 
 namespace dpamd {
@@ -65,14 +68,14 @@ __device__ __forceinline__ void put_operand4(unsigned short* p, long plane, cons
   for (int s = 0; s < pieces<KIND>(); ++s) *reinterpret_cast<us4*>(p + s * plane) = q[s];
 }
 
-// Columns n .. n + 3 of one row of an output of the kind's own type. `vec`: the
-// rows are aligned to four elements.
-template <int KIND>
-__device__ __forceinline__ void put_row4(void* out, long at, const float* v, int count, bool vec) {
+// Four columns of one row of an output of the kind's own type, `count` of them inside it; FULL:
+// all four, and aligned.
+template <int KIND, bool FULL>
+__device__ __forceinline__ void put_row4(void* out, long at, const f4& v, int count) {
   if constexpr (KIND == kF32) {
     float* o = static_cast<float*>(out) + at;
-    if (vec && count >= 4) {
-      *reinterpret_cast<f4*>(o) = f4{v[0], v[1], v[2], v[3]};
+    if constexpr (FULL) {
+      *reinterpret_cast<f4*>(o) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -81,7 +84,7 @@ __device__ __forceinline__ void put_row4(void* out, long at, const float* v, int
   } else {
     typedef unsigned short us4 __attribute__((ext_vector_type(4)));
     unsigned short* o = static_cast<unsigned short*>(out) + at;
-    if (vec && count >= 4) {
+    if constexpr (FULL) {
       *reinterpret_cast<us4*>(o) = us4{to16<KIND>(v[0]), to16<KIND>(v[1]), to16<KIND>(v[2]), to16<KIND>(v[3])};
     } else {
 #pragma unroll
@@ -91,84 +94,127 @@ __device__ __forceinline__ void put_row4(void* out, long at, const float* v, int
   }
 }
 
-// The activation a(g) and its derivative: tanh, silu g s(g), gelu g Phi(g).
-__device__ __forceinline__ void activation(int act, float g, float& a, float& da) {
-  if (act == kActTanh) {
-    a = tanhf(g);
+// The activation a(g) and its derivative: tanh, silu g s(g), gelu g Phi(g), on the hardware's
+// base-2 exponential and reciprocal (about 1 ulp each), to about 2e-7 of max(1, |g|). Phi
+// from erfc(z) = exp(-z^2) (a1 t + .. + a5 t^5), t = 1 / (1 + 0.3275911 z) (Abramowitz and
+// Stegun 7.1.26: 1.5e-7), which shares its exponential with the derivative. With the
+// library's expf, tanhf, erff and a division the epilogues below issued about four times the
+// instructions, and 8192 rows of 2048-8192-2048 took the forward 823 us (now 709) and dg, du 2031 (now 476).
+template <int ACT>
+__device__ __forceinline__ void activate(float g, float& a, float& da) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  if constexpr (ACT == kActTanh) {
+    a = tanh_f32(g);
     da = 1.0f - a * a;
-  } else if (act == kActSilu) {
-    const float p = 1.0f / (1.0f + expf(-g));
+  } else if constexpr (ACT == kActSilu) {
+    const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
     a = g * p;
     da = p * (1.0f + g * (1.0f - p));
   } else {
-    const float p = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    const float z = 0.70710678118654752f * fabsf(g);
+    const float e = __builtin_amdgcn_exp2f(-kLog2e * z * z);
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * z);
+    const float poly =
+        t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float q = 0.5f * poly * e;  // Phi(-|g|)
+    const float p = g < 0.0f ? q : 1.0f - q;
     a = g * p;
-    da = p + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+    da = p + g * e * 0.39894228040143268f;
   }
+}
+__device__ __forceinline__ void activate4(int act, const f4& g, f4& a, f4& da) {
+  auto all = [&](auto k) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x, y;
+      activate<decltype(k)::value>(g[r], x, y);
+      a[r] = x;
+      da[r] = y;
+    }
+  };
+  if (act == kActTanh)
+    all(std::integral_constant<int, kActTanh>{});
+  else if (act == kActSilu)
+    all(std::integral_constant<int, kActSilu>{});
+  else
+    all(std::integral_constant<int, kActGelu>{});
 }
 
 // ---- epilogues on four consecutive columns of one row, shared by the products and
 // by the sums over slices of K --------------------------------------------------------
 
-// h = a(g) u in operand form (columns N .. ldh - 1 are zeros), g and u kept for the
-// backward in 32 bits, so that what it forms from them is rounded once.
-template <int KIND>
-__device__ __forceinline__ void epi_gate(const EpiArgs& e, int act, long m, int n, int N, const float* g,
-                                         const float* u) {
-  float h[4];
+// The four columns are `count` of the output's (and the rest beyond it); FULL: all four, and
+// aligned.
+
+// h = a(g) u in operand form (zeros beyond the output), g and u kept for the backward in 32
+// bits, so that what it forms from them is rounded once. kept: pairs (g, u), or null.
+template <int KIND, bool FULL>
+__device__ __forceinline__ void put_gate(unsigned short* h, long plane, float* kept, int act, int count, const f4& g,
+                                         const f4& u) {
+  f4 a, da;
+  activate4(act, g, a, da);
+  float v[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    float a, da;
-    activation(act, g[r], a, da);
-    h[r] = n + r < N ? a * u[r] : 0.0f;
-  }
-  put_operand4<KIND>(e.h + m * e.ldh + n, e.plane_h, h);
-  if (e.saved) {
-    float* s = e.saved + 2 * (m * (long)N + n);
-    if ((N & 1) == 0 && n + 4 <= N) {  // (n is a multiple of 4, N even: 16-byte aligned)
-      *reinterpret_cast<f4*>(s) = f4{g[0], u[0], g[1], u[1]};
-      *reinterpret_cast<f4*>(s + 4) = f4{g[2], u[2], g[3], u[3]};
-    } else {
+  for (int r = 0; r < 4; ++r) v[r] = FULL || r < count ? a[r] * u[r] : 0.0f;
+  put_operand4<KIND>(h, plane, v);
+  if (!kept) return;
+  if constexpr (FULL) {
+    *reinterpret_cast<f4*>(kept) = f4{g[0], u[0], g[1], u[1]};
+    *reinterpret_cast<f4*>(kept + 4) = f4{g[2], u[2], g[3], u[3]};
+  } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < N) {
-          s[2 * r] = g[r];
-          s[2 * r + 1] = u[r];
-        }
-    }
+    for (int r = 0; r < 4; ++r)
+      if (r < count) {
+        kept[2 * r] = g[r];
+        kept[2 * r + 1] = u[r];
+      }
   }
 }
 
-// From dh and the kept g, u: dg = dh u a'(g), du = dh a(g) and h again, in operand form.
-template <int KIND>
-__device__ __forceinline__ void epi_gate_grad(const EpiArgs& e, int act, long m, int n, int N, const float* dh) {
-  const float* s = e.saved + 2 * (m * (long)N + n);
-  float g[4], u[4];
-  if ((N & 1) == 0 && n + 4 <= N) {
-    const f4 p = *reinterpret_cast<const f4*>(s), q = *reinterpret_cast<const f4*>(s + 4);
-    g[0] = p[0], u[0] = p[1], g[1] = p[2], u[1] = p[3];
-    g[2] = q[0], u[2] = q[1], g[3] = q[2], u[3] = q[3];
+// g and u of four columns as the forward kept them (zeros beyond the output)
+struct Kept {
+  f4 g, u;
+};
+template <bool FULL>
+__device__ __forceinline__ Kept load_kept(const float* kept, int count) {
+  Kept k;
+  if constexpr (FULL) {
+    const f4 p = *reinterpret_cast<const f4*>(kept), q = *reinterpret_cast<const f4*>(kept + 4);
+    k.g = f4{p[0], p[2], q[0], q[2]};
+    k.u = f4{p[1], p[3], q[1], q[3]};
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      g[r] = n + r < N ? s[2 * r] : 0.0f;
-      u[r] = n + r < N ? s[2 * r + 1] : 0.0f;
+      k.g[r] = r < count ? kept[2 * r] : 0.0f;
+      k.u[r] = r < count ? kept[2 * r + 1] : 0.0f;
     }
   }
+  return k;
+}
+
+// From dh and the kept g, u: dg = dh u a'(g), du = dh a(g) and h again.
+struct GateGrad {
   float h[4], dg[4], du[4];
+};
+template <bool FULL>
+__device__ __forceinline__ GateGrad gate_grad(int act, int count, const f4& dh, const Kept& k) {
+  GateGrad o;
+  f4 a, da;
+  activate4(act, k.g, a, da);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    float a, da;
-    activation(act, g[r], a, da);
-    const bool in = n + r < N;
-    h[r] = in ? a * u[r] : 0.0f;
-    du[r] = in ? dh[r] * a : 0.0f;
-    dg[r] = in ? dh[r] * u[r] * da : 0.0f;
+    const bool in = FULL || r < count;
+    o.h[r] = in ? a[r] * k.u[r] : 0.0f;
+    o.du[r] = in ? dh[r] * a[r] : 0.0f;
+    o.dg[r] = in ? dh[r] * k.u[r] * da[r] : 0.0f;
   }
-  const long at = m * e.ldh + n;
-  if (e.h) put_operand4<KIND>(e.h + at, e.plane_h, h);
-  put_operand4<KIND>(e.dg + at, e.plane_h, dg);
-  put_operand4<KIND>(e.du + at, e.plane_h, du);
+  return o;
+}
+template <int KIND>
+__device__ __forceinline__ void put_gate_grad(const EpiArgs& e, long at, const GateGrad& o) {
+  if (e.h) put_operand4<KIND>(e.h + at, e.plane_h, o.h);
+  put_operand4<KIND>(e.dg + at, e.plane_h, o.dg);
+  put_operand4<KIND>(e.du + at, e.plane_h, o.du);
 }
 
 // ---- the product ------------------------------------------------------------------------
@@ -177,11 +223,34 @@ __device__ __forceinline__ void epi_gate_grad(const EpiArgs& e, int act, long m,
 // contiguous (kRowMajorK: element (r, k) at k ld + r).
 enum Layout { kRowK = 0, kColK = 1 };
 
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
 typedef __attribute__((address_space(3))) s4v lds_s4;
 
-__device__ const unsigned g_zero16[4] = {0, 0, 0, 0};
+// 16 bytes a lane from base + offset straight into LDS: lane l's to the LDS address lds + 16 l
+// (base and lds are wave-uniform; tile_landed() is the wait). Written as an instruction,
+// which has no register result, because the compiler waits for every such load that it
+// knows of before any transposing LDS read, as it can not tell that they are of different tiles:
+// with the builtin each row of fragments waited for the loads issued just before it.
+// (m0 is a register that a statement may not name as changed; nothing else in these kernels uses it.)
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned offset, unsigned lds) {
+  // (both in scalar registers, whatever the compiler knows of them)
+  lds = __builtin_amdgcn_readfirstlane(lds);
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)(size_t)base);
+  const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((size_t)base >> 32));
+  const size_t at = ((size_t)hi << 32) | lo;
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(offset), "s"(at), "s"(lds)
+      : "memory");
+}
+// Every load_to_lds of this wave has landed, and after the barrier every wave's; all
+// LDS reads before it are done.
+__device__ __forceinline__ void tile_landed() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 
 // One operand's tile in LDS: `ROWS` rows by BK of k, in SUB side-by-side parts of
 // ROWS / SUB rows that come from as many matrices.
@@ -204,7 +273,9 @@ struct TileOf {
   static constexpr int kUnits = kPart / 16;
 
   static __device__ __forceinline__ int swz_row(int row) {
-    return (row / (256 / (BK * 2))) & (kChunks - 1);
+    // (a 16-byte LDS read takes its lanes in the groups 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31
+    // of each half of the wave: eight rows at each of two neighbouring chunks)
+    return (BK == 32 ? (row / 8) & 1 : (row / 2) & 3) << 1;
   }
   static __device__ __forceinline__ int swz_k(int k) {
     return ((k & 3) | (((k >> 3) & 3) << 2)) & (kUnits - 1);
@@ -225,13 +296,22 @@ struct TileOf {
       chunk = ((w / 16) % (kPart / 8)) ^ (swz_k(row) << 1);
     }
   }
-  // byte offset of this lane's 16 bytes of load q from the part's origin at the step's k
+  // Byte offset of this lane's 16 bytes of load q from the part's origin at the step's k:
+  // offset(kind(q)) + moved(q) rows of ld, the former in a register for each of kOffsets
+  // kinds. (Rows, or k rows 32 apart, have one permutation, and differ by the uniform part alone.)
+  static constexpr int kRows = LAYOUT == kRowK ? WAVES * 512 / BK : WAVES * 512 / kPart;  // of one load of all waves
+  static_assert(LAYOUT == kColK || (SUB == 1 && kRows % (512 / BK) == 0), "whole permutations a load");
+  static constexpr int kOffsets =
+      LAYOUT == kRowK || kRows >= 32 ? 1 : (32 / kRows < kLoads ? 32 / kRows : kLoads);
+  static constexpr __device__ int kind(int q) { return q % kOffsets; }
+  static constexpr __device__ long moved(int q) {
+    return LAYOUT == kRowK ? q * kRows : (q * kRows) % BK / 32 * 32;
+  }
   static __device__ __forceinline__ unsigned offset(int q, int wave, int lane, long ld, int rows_left) {
     int part, row, chunk;
     place(q, wave, lane, part, row, chunk);
     if constexpr (LAYOUT == kRowK) {
-      // rows past the end repeat the last one: their sums are not stored
-      return (unsigned)(min(row, rows_left - 1) * ld * 2 + chunk * 16);
+      return (unsigned)(row * ld * 2 + chunk * 16);
     } else {
       const int left = ((rows_left + 7) & ~7) - 8;
       return (unsigned)(row * ld * 2 + min(chunk * 8, left) * 2);
@@ -242,6 +322,17 @@ struct TileOf {
     int part, row, chunk;
     place(q, wave, lane, part, row, chunk);
     return (LAYOUT == kRowK ? chunk * 8 : row) >= k_left;
+  }
+  // or in a row past the operand's last (whose sums are not stored, whatever its tile row holds)
+  static __device__ __forceinline__ bool outside(int q, int wave, int lane, int k_left, int rows_left) {
+    int part, row, chunk;
+    if constexpr (LAYOUT == kRowK) {
+      place(0, wave, lane, part, row, chunk);
+      return chunk * 8 >= k_left || row >= rows_left - q * kRows;
+    } else {
+      place(q, wave, lane, part, row, chunk);
+      return row >= k_left;
+    }
   }
   // the fragment of rows r0 .. r0 + 15 (of part `part`) and k kk * 32 .. + 31
   static __device__ __forceinline__ s8v frag(const char* tile, int part, int r0, int kk, int lane) {
@@ -288,8 +379,9 @@ struct Shape {
 };
 
 // EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad.
-// Two stages of LDS: the loads of step t + 1 are issued after the barrier that ends
-// step t - 1 and land while step t's fragments are multiplied.
+//
+// A block takes tiles (and slices of K) one after another; the first two steps of the next one are
+// loaded before the epilogue of the last, so that they arrive under it. Two stages of LDS.
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
   constexpr int P = pieces<KIND>(), SUB = EPI == kEpiGate ? 2 : 1;
@@ -299,152 +391,374 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
   using TB = TileOf<LB, S::BN, S::BK, SUB, WAVES>;
   constexpr int kStage = P * (TA::kBytes + TB::kBytes);
   __shared__ __align__(1024) char lds[2 * kStage];
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)lds);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / S::WN, wn = wave % S::WN;
-  // blocks in groups of eight row tiles by all column tiles, consecutive ones on one XCD
-  const int3 id = xcd_swizzle();
-  const int group = 8 * p.tiles_n, q = id.x / group, in = id.x % group;
-  const int gm = min(8, p.tiles_m - 8 * q);
-  const int tm = 8 * q + in % gm, tn_all = in / gm;
-  const int mat = tn_all / p.tiles_n1, tn = tn_all % p.tiles_n1;
-  const int m0 = tm * S::BM, n0 = tn * (S::BN / SUB);
-  const int per_seg = (p.K + S::BK - 1) / S::BK, steps = per_seg * p.segs;
-  const int t0 = (int)((long)steps * id.y / p.split), t1 = (int)((long)steps * (id.y + 1) / p.split);
+  const int wm = wave / S::WN, wn = wave % S::WN, g = lane >> 4, c = lane & 15;
+  const int K = p.K, per_seg = (K + S::BK - 1) / S::BK, steps = per_seg * p.segs;
+  const long lda2 = 2 * p.a[0].ld, ldb2 = 2 * p.b[0].ld, pla = 2 * p.a[0].plane, plb = 2 * p.b[0].plane;
+  const long da = LA == kRowK ? 2 * S::BK : S::BK * lda2, db = LB == kRowK ? 2 * S::BK : S::BK * ldb2;
 
-  unsigned oa[TA::kLoads], ob[TB::kLoads];
-#pragma unroll
-  for (int l = 0; l < TA::kLoads; ++l) oa[l] = TA::offset(l, wave, lane, p.a[0].ld, p.M - m0);
-#pragma unroll
-  for (int l = 0; l < TB::kLoads; ++l) ob[l] = TB::offset(l, wave, lane, p.b[mat].ld, p.N - n0);
+  // ---- a tile and its steps ----
+  struct Item {
+    int m0, n0, mat, slice, t0, t1;
+  };
+  // items in the order slice by slice, tiles in groups of eight row tiles by all column
+  // tiles, so that the tiles under way on one XCD share rows and columns
+  // (readfirstlane: quotients are formed on vector registers, and what is computed from them would be too)
+  auto item_of = [&](int id) {
+    Item it;
+    const int tiles = p.tiles_m * p.tiles_n;
+    it.slice = __builtin_amdgcn_readfirstlane(id / tiles);
+    const int tile = id - it.slice * tiles, group = 8 * p.tiles_n;
+    const int q = __builtin_amdgcn_readfirstlane(tile / group), in = tile - q * group;
+    const int gm = min(8, p.tiles_m - 8 * q);
+    const int tn = __builtin_amdgcn_readfirstlane(in / gm);
+    it.mat = p.mats == 2 && tn >= p.tiles_n1;
+    it.m0 = (8 * q + in - tn * gm) * S::BM;
+    it.n0 = (tn - (it.mat ? p.tiles_n1 : 0)) * (S::BN / SUB);
+    it.t0 = __builtin_amdgcn_readfirstlane((int)((long)steps * it.slice / p.split));
+    it.t1 = __builtin_amdgcn_readfirstlane((int)((long)steps * (it.slice + 1) / p.split));
+    return it;
+  };
+  const int items = p.tiles_m * p.tiles_n * p.split;
+  int walk, walk_step = 1, walk_end = 0;
+  if ((int)gridDim.x == items) {
+    walk = __builtin_amdgcn_readfirstlane(xcd_swizzle().x);
+  } else {
+    const ChunkWalk w = xcd_chunks(items);
+    walk = w.first, walk_step = w.step, walk_end = w.end;
+  }
+  if ((int)gridDim.x != items && walk >= walk_end) return;
 
-  auto load = [&](int t, char* to) {
-    const int seg = t >= per_seg, k0 = (t - seg * per_seg) * S::BK;
-    const Operand& A = p.a[seg];
-    const char* pa = reinterpret_cast<const char*>(A.p) +
-                     2 * (LA == kRowK ? (long)m0 * A.ld + k0 : (long)k0 * A.ld + m0);
-    const char* pb[SUB];
-    long bplane = 0;
+  Item it = item_of(walk);
+  unsigned oa[TA::kOffsets], ob[TB::kOffsets];
+  const char *a0, *a1, *b0, *b1;
+  auto aim = [&]() {
 #pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      const Operand& B = p.b[SUB == 2 ? s : p.segs == 2 ? seg : mat];
-      pb[s] = reinterpret_cast<const char*>(B.p) +
-              2 * (LB == kRowK ? (long)n0 * B.ld + k0 : (long)k0 * B.ld + n0);
-      bplane = B.plane;
-    }
-    const int k_left = p.K - k0;
-    const bool tail = k_left < S::BK;
+    for (int l = 0; l < TA::kOffsets; ++l) oa[l] = TA::offset(l, wave, lane, p.a[0].ld, p.M - it.m0);
 #pragma unroll
-    for (int s = 0; s < P; ++s) {
-#pragma unroll
-      for (int l = 0; l < TA::kLoads; ++l) {
-        const char* src = pa + 2 * s * A.plane + oa[l];
-        if (tail && TA::past(l, wave, lane, k_left)) src = reinterpret_cast<const char*>(g_zero16);
-        __builtin_amdgcn_global_load_lds((global_void*)src,
-                                         (lds_void*)(to + s * TA::kBytes + (l * WAVES + wave) * 1024), 16, 0, 0);
-      }
-#pragma unroll
-      for (int l = 0; l < TB::kLoads; ++l) {
-        // (every lane of one load lies in one part: a part is whole loads)
-        const int part = SUB == 1 ? 0 : (l * WAVES + wave) * 1024 / (TB::kBytes / SUB);
-        const char* src = (part ? pb[SUB - 1] : pb[0]) + 2 * s * bplane + ob[l];
-        if (tail && TB::past(l, wave, lane, k_left)) src = reinterpret_cast<const char*>(g_zero16);
-        __builtin_amdgcn_global_load_lds(
-            (global_void*)src, (lds_void*)(to + P * TA::kBytes + s * TB::kBytes + (l * WAVES + wave) * 1024), 16, 0, 0);
-      }
-    }
+    for (int l = 0; l < TB::kOffsets; ++l) ob[l] = TB::offset(l, wave, lane, p.b[0].ld, p.N - it.n0);
+    const long ra = LA == kRowK ? it.m0 * lda2 : 2l * it.m0, rb = LB == kRowK ? it.n0 * ldb2 : 2l * it.n0;
+    const bool pair = SUB == 2 || p.segs == 2;
+    a0 = reinterpret_cast<const char*>(p.a[0].p) + ra;
+    a1 = reinterpret_cast<const char*>(p.a[1].p) + ra;
+    b0 = reinterpret_cast<const char*>(p.b[pair ? 0 : it.mat].p) + rb;
+    b1 = reinterpret_cast<const char*>(p.b[pair ? 1 : it.mat].p) + rb;
   };
 
-  f4 acc[MI][NJ];
+  // where a step's loads come from (wave-uniform); none of them past the slice's end
+  // (the products then read on in a tile of which no one uses what they read)
+  struct Cursor {
+    const char *pa, *pb, *pb_second;
+    int k_left;
+  };
+  auto cursor = [&](int t) {
+    const bool seg = t >= per_seg;
+    const int step = seg ? t - per_seg : t;
+    return Cursor{(seg ? a1 : a0) + step * da, (SUB == 1 && seg ? b1 : b0) + step * db, b1 + step * db,
+                  t < it.t1 ? K - step * S::BK : 0};
+  };
+  // One of a step's kLoads loads of this wave, by the lanes whose row and k are before the ends;
+  // the 16 bytes past the end of k are zeroed by fill() (in the last step of a segment).
+  constexpr int kLoads = P * (TA::kLoads + TB::kLoads);
+  auto slot = [&](int q) {
+    if (q < P * TA::kLoads) return q / TA::kLoads * TA::kBytes + (q % TA::kLoads * WAVES + wave) * 1024;
+    const int r = q - P * TA::kLoads;
+    return P * TA::kBytes + r / TB::kLoads * TB::kBytes + (r % TB::kLoads * WAVES + wave) * 1024;
+  };
+  auto past = [&](int q, int k_left) {
+    return q < P * TA::kLoads ? TA::past(q % TA::kLoads, wave, lane, k_left)
+                              : TB::past((q - P * TA::kLoads) % TB::kLoads, wave, lane, k_left);
+  };
+  auto issue = [&](int q, const Cursor& u, int to) {
+    if (q < P * TA::kLoads) {
+      const int l = q % TA::kLoads;
+      if (TA::outside(l, wave, lane, u.k_left, p.M - it.m0)) return;
+      load_to_lds(u.pa + q / TA::kLoads * pla + TA::moved(l) * lda2, oa[TA::kind(l)], lds0 + to + slot(q));
+    } else {
+      const int r = q - P * TA::kLoads, s = r / TB::kLoads, l = r % TB::kLoads;
+      if (TB::outside(l, wave, lane, u.k_left, p.N - it.n0)) return;
+      // (every lane of one load lies in one part: a part is whole loads)
+      const bool part = SUB == 2 && (l * WAVES + wave) * 1024 >= TB::kBytes / 2;
+      load_to_lds((part ? u.pb_second : u.pb) + s * plb + TB::moved(l) * ldb2, ob[TB::kind(l)], lds0 + to + slot(q));
+    }
+  };
+  auto fill = [&](const Cursor& u, int to) {
+    if (u.k_left <= 0 || u.k_left >= S::BK) return;
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+    for (int q = 0; q < kLoads; ++q)
+      if (past(q, u.k_left)) *reinterpret_cast<f4*>(lds + to + slot(q) + lane * 16) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  };
+  auto load = [&](int t, int to) {
+    const Cursor u = cursor(t);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < kLoads; ++q) issue(q, u, to);
+    fill(u, to);
+  };
+  auto frag_a = [&](const char* tile, int s, int i, int kk) {
+    return TA::frag(tile + s * TA::kBytes, 0, wm * TM + i * 16, kk, lane);
+  };
+  auto frag_b = [&](const char* tile, int s, int j, int kk) {
+    return TB::frag(tile + P * TA::kBytes + s * TB::kBytes, SUB == 2 ? j / (NJ / 2) : 0,
+                    SUB == 2 ? wn * (TN / 2) + (j % (NJ / 2)) * 16 : wn * TN + j * 16, kk, lane);
+  };
 
-  if (t0 < t1) load(t0, lds);
-  for (int t = t0; t < t1; ++t) {
-    char* cur = lds + ((t - t0) & 1) * kStage;
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of step t are in LDS
-    __syncthreads();                     // and so are the other waves'; step t - 1 is read
-    if (t + 1 < t1) load(t + 1, lds + ((t + 1 - t0) & 1) * kStage);
+  aim();
+  load(it.t0, 0);
+  load(it.t0 + 1, kStage);
+  for (;;) {
+    f4 acc[MI][NJ];
 #pragma unroll
-    for (int kk = 0; kk < S::BK / 32; ++kk) {
-      s8v b[NJ][P];
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    tile_landed();
+    if constexpr (P == 1) {
+      // Two halves of 32 of k a step: a half's fragments are multiplied while the next half's
+      // are read. A row's fragments are read again, for the next half, as soon as its products are
+      // issued, and so have the other rows' products of time to arrive; the columns' fragments,
+      // which every row needs, and the last rows', whose registers come free too late, have two sets of
+      // registers. (Two sets of all spilled.) A step's loads go into the tile that all waves
+      // have just read, once the step before it has landed: one barrier a step, in its middle.
+      static_assert(S::BK == 64, "a step is two halves");
+      constexpr int LATE = MI >= 4 ? 2 : 0, EARLY = MI - LATE;
+      s8v fa[EARLY], fl[2][LATE + 1], fb[2][NJ];
+      auto half = [&](auto h_, const char* next, bool loads, const Cursor& u, int to) {
+        constexpr int h = decltype(h_)::value, o = h ^ 1;
 #pragma unroll
-        for (int s = 0; s < P; ++s)
-          b[j][s] = TB::frag(cur + P * TA::kBytes + s * TB::kBytes, SUB == 2 ? j / (NJ / 2) : 0,
-                             SUB == 2 ? wn * (TN / 2) + (j % (NJ / 2)) * 16 : wn * TN + j * 16, kk, lane);
+        for (int j = 0; j < NJ; ++j) fb[o][j] = frag_b(next, 0, j, o);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        s8v a[P];
+        for (int i = 0; i < MI; ++i) {
+          // the operands change places: a lane then holds four consecutive columns of one row
 #pragma unroll
-        for (int s = 0; s < P; ++s) a[s] = TA::frag(cur + s * TA::kBytes, 0, wm * TM + i * 16, kk, lane);
-        // the operands change places: a lane then holds four consecutive columns of one row
+          for (int j = 0; j < NJ; ++j)
+            acc[i][j] = mfma16<KIND>(fb[h][j], i < EARLY ? fa[i < EARLY ? i : 0] : fl[h][i < EARLY ? 0 : i - EARLY],
+                                     acc[i][j]);
+          if (i < EARLY) fa[i < EARLY ? i : 0] = frag_a(next, 0, i, o);
+          if (i < EARLY && i >= EARLY - LATE) fl[o][i - EARLY + LATE] = frag_a(next, 0, i + LATE, o);
+          if (loads) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = mfma_all<KIND>(b[j], a, acc[i][j]);
+            for (int q = 0; q < kLoads; ++q)
+              if (q * MI / kLoads == i) issue(q, u, to);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // the reads have landed (a compiler-placed wait would come after the next reads and be for those too)
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+      };
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) fb[0][j] = frag_b(lds, 0, j, 0);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        (i < EARLY ? fa[i < EARLY ? i : 0] : fl[0][i < EARLY ? 0 : i - EARLY]) = frag_a(lds, 0, i, 0);
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+      __builtin_amdgcn_sched_barrier(0);
+      for (int t = it.t0; t < it.t1; ++t) {
+        const int cur = ((t - it.t0) & 1) * kStage;
+        const Cursor u = cursor(t + 2);
+        half(std::integral_constant<int, 0>{}, lds + cur, false, u, cur);
+        tile_landed();
+        fill(u, cur);
+        half(std::integral_constant<int, 1>{}, lds + (kStage - cur), true, u, cur);
+      }
+    } else {
+      // (three pieces: a row's products take six times as long, and the compiler's order of
+      // reads and products within a step is as fast as the above, with fewer registers)
+      for (int t = it.t0; t < it.t1; ++t) {
+        const char* cur = lds + ((t - it.t0) & 1) * kStage;
+        if (t > it.t0) {
+          tile_landed();  // this step's loads are in LDS, and the last step's tile is read
+          load(t + 1, ((t + 1 - it.t0) & 1) * kStage);
+        }
+#pragma unroll
+        for (int kk = 0; kk < S::BK / 32; ++kk) {
+          s8v b[NJ][P];
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int s = 0; s < P; ++s) b[j][s] = frag_b(cur, s, j, kk);
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            s8v a[P];
+#pragma unroll
+            for (int s = 0; s < P; ++s) a[s] = frag_a(cur, s, i, kk);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = mfma_all<KIND>(b[j], a, acc[i][j]);
+          }
+        }
       }
     }
-  }
 
-  const int g = lane >> 4, c = lane & 15;
+    // the next item's first loads, then this one's epilogue
+    const Item done = it;
+    walk += walk_step;
+    const bool more = walk < walk_end;
+    if (more) {
+      it = item_of(walk);
+      aim();
+      __syncthreads();  // every wave has read its last
+      load(it.t0, 0);
+      load(it.t0 + 1, kStage);
+    }
+    // One test a wave for what lies inside the output, and one address a row where all does:
+    // with tests, products of 64 bits and branches for every four columns the epilogue issued
+    // several thousand instructions a wave, and took longer than eight steps of products.
+    const int m0 = done.m0 + wm * TM + c, n0 = done.n0 + wn * (TN / SUB) + 4 * g;
+    const bool inside = done.m0 + (wm + 1) * TM <= p.M && done.n0 + (wn + 1) * (TN / SUB) <= p.N;
+    if (p.split > 1) {
+      // a slice's sums, columns in rows of ldp (a multiple of 4)
+      const int sub = SUB == 2 ? 2 : p.mats;
+      float* o = p.partial + (((long)done.slice * sub + done.mat) * p.M + m0) * p.ldp + n0;
+      const long second = (long)p.M * p.ldp, row = 16 * p.ldp;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int m = m0 + wm * TM + i * 16 + c;
-    if (m >= p.M) continue;
+      for (int i = 0; i < MI; ++i, o += row)
 #pragma unroll
-    for (int j = 0; j < NJ / SUB; ++j) {
-      const int n = n0 + wn * (TN / SUB) + j * 16 + 4 * g;
-      if (n >= p.cols) continue;
-      float v[4], w[4];
+        for (int j = 0; j < NJ / SUB; ++j)
+          if (inside || (m0 + i * 16 < p.M && n0 + j * 16 < p.cols)) {
+            *reinterpret_cast<f4*>(o + j * 16) = acc[i][j];
+            if constexpr (SUB == 2) *reinterpret_cast<f4*>(o + second + j * 16) = acc[i][j + NJ / 2];
+          }
+    } else if constexpr (EPI == kEpiStore) {
+      const long row = 16 * p.ldo[done.mat];
+      long at = m0 * p.ldo[done.mat] + n0;
+      void* out = p.out[done.mat];
+      if (inside && p.vec[done.mat]) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[r] = acc[i][j][r];
-        w[r] = acc[i][SUB == 2 ? j + NJ / 2 : j][r];
-      }
-      if (p.split > 1) {
-        // a slice's sums, columns in rows of ldp (a multiple of 4)
-        const int sub = SUB == 2 ? 2 : p.mats;
-        float* o = p.partial + (((long)id.y * sub + mat) * p.M + m) * p.ldp + n;
-        *reinterpret_cast<f4*>(o) = f4{v[0], v[1], v[2], v[3]};
-        if constexpr (SUB == 2) *reinterpret_cast<f4*>(o + (long)p.M * p.ldp) = f4{w[0], w[1], w[2], w[3]};
-      } else if constexpr (EPI == kEpiGate) {
-        epi_gate<KIND>(p.epi, p.act, m, n, p.N, v, w);
-      } else if constexpr (EPI == kEpiGateGrad) {
-        epi_gate_grad<KIND>(p.epi, p.act, m, n, p.N, v);
+        for (int i = 0; i < MI; ++i, at += row)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) put_row4<KIND, true>(out, at + j * 16, acc[i][j], 4);
       } else {
-        put_row4<KIND>(p.out[mat], (long)m * p.ldo[mat] + n, v, p.N - n, p.vec[mat]);
+#pragma unroll
+        for (int i = 0; i < MI; ++i, at += row)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            if (m0 + i * 16 < p.M && n0 + j * 16 < p.N)
+              put_row4<KIND, false>(out, at + j * 16, acc[i][j], p.N - n0 - j * 16);
       }
+    } else if constexpr (EPI == kEpiGate) {
+      unsigned short* h = p.epi.h + m0 * p.epi.ldh + n0;
+      float* kept = p.epi.saved ? p.epi.saved + 2 * ((long)m0 * p.N + n0) : nullptr;
+      const long hrow = 16 * p.epi.ldh, krow = p.epi.saved ? 32l * p.N : 0;
+      if (inside && (p.N & 1) == 0) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i, h += hrow, kept += krow)
+#pragma unroll
+          for (int j = 0; j < NJ / SUB; ++j)
+            put_gate<KIND, true>(h + j * 16, p.epi.plane_h, p.epi.saved ? kept + j * 32 : nullptr, p.act, 4, acc[i][j],
+                                 acc[i][j + NJ / 2]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < MI; ++i, h += hrow, kept += krow)
+#pragma unroll
+          for (int j = 0; j < NJ / SUB; ++j)
+            if (m0 + i * 16 < p.M && n0 + j * 16 < p.cols)
+              put_gate<KIND, false>(h + j * 16, p.epi.plane_h, p.epi.saved ? kept + j * 32 : nullptr, p.act,
+                                    p.N - n0 - j * 16, acc[i][j], acc[i][j + NJ / 2]);
+      }
+    } else {
+      // The kept g, u of the next sixteen rows are under way while these rows' values are
+      // computed, and are waited for before the stores that follow them are issued (a wait
+      // for a load issued before stores would be a wait for those too).
+      auto rows = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const float* kept_at = p.epi.saved + 2 * ((long)m0 * p.N + n0);
+        long at = m0 * p.epi.ldh + n0;
+        auto fetch = [&](int i, Kept* k) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            k[j] = FULL || (m0 + i * 16 < p.M && n0 + j * 16 < p.N)
+                       ? load_kept<FULL>(kept_at + i * 32l * p.N + j * 32, p.N - n0 - j * 16)
+                       : Kept{};
+        };
+        Kept kept[2][NJ];
+        fetch(0, kept[0]);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          if (i + 1 < MI) fetch(i + 1, kept[(i + 1) & 1]);
+          GateGrad o[NJ];
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            o[j] = gate_grad<FULL>(p.act, p.N - n0 - j * 16, acc[i][j], kept[i & 1][j]);
+          vmem_wait_all();
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            if (FULL || (m0 + i * 16 < p.M && n0 + j * 16 < p.cols))
+              put_gate_grad<KIND>(p.epi, at + i * 16 * p.epi.ldh + j * 16, o[j]);
+        }
+      };
+      if (inside && (p.N & 1) == 0)
+        rows(std::true_type{});
+      else
+        rows(std::false_type{});
     }
+    if (!more) return;
   }
 }
 
-// The slices' sums added up in order, and the epilogue.
+// The slices' sums added up, and the epilogue: a block takes 256 / G quads of columns, G
+// threads each, every thread a contiguous share of the slices in order, the shares
+// joined in order through LDS. With one thread a quad the 249 slices of a 96 x 1 sum took
+// 62 us, a chain of loads.
 template <int KIND, int EPI>
 __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
+  constexpr int SUB = EPI == kEpiGate ? 2 : 1;
+  __shared__ f4 part[SUB][256];
+  const int G = p.join, per = 256 / G;
   const int quads = p.ldp / 4, sub = EPI == kEpiGate ? 2 : p.mats;
   const long rows = EPI == kEpiGate ? p.M : (long)p.M * p.mats;
-  const long at = (long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= rows * quads) return;
-  const long row = at / quads;
-  const int n = (int)(at % quads) * 4;
-  const int mat = EPI == kEpiGate ? 0 : (int)(row / p.M);
-  const long m = EPI == kEpiGate ? row : row % p.M;
+  const int slot = threadIdx.x % per, share = threadIdx.x / per;
+  const long at = (long)blockIdx.x * per + slot;
+  const bool in = at < rows * quads;
+  const long row = in ? at / quads : 0;
+  const int n = in ? (int)(at % quads) * 4 : 0;
   const long slice = (long)sub * p.M * p.ldp;
   const float* s = p.partial + row * p.ldp + n;
+  const int z0 = p.split * share / G, z1 = p.split * (share + 1) / G;
   f4 v = {0, 0, 0, 0}, w = v;
-  for (int z = 0; z < p.split; ++z) {
-    v += *reinterpret_cast<const f4*>(s + z * slice);
-    if constexpr (EPI == kEpiGate) w += *reinterpret_cast<const f4*>(s + z * slice + (long)p.M * p.ldp);
+  int z = z0;
+  for (; z + 4 <= z1; z += 4) {
+    f4 q[4], r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      q[k] = *reinterpret_cast<const f4*>(s + (z + k) * slice);
+      if constexpr (SUB == 2) r[k] = *reinterpret_cast<const f4*>(s + (z + k) * slice + (long)p.M * p.ldp);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v += q[k];
+      if constexpr (SUB == 2) w += r[k];
+    }
   }
-  float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {w[0], w[1], w[2], w[3]};
+  for (; z < z1; ++z) {
+    v += *reinterpret_cast<const f4*>(s + z * slice);
+    if constexpr (SUB == 2) w += *reinterpret_cast<const f4*>(s + z * slice + (long)p.M * p.ldp);
+  }
+  if (G > 1) {
+    part[0][threadIdx.x] = v;
+    if constexpr (SUB == 2) part[SUB - 1][threadIdx.x] = w;
+    __syncthreads();
+    if (share) return;
+    for (int k = 1; k < G; ++k) {
+      v += part[0][k * per + slot];
+      if constexpr (SUB == 2) w += part[SUB - 1][k * per + slot];
+    }
+  }
+  if (!in) return;
+  const int mat = EPI == kEpiGate ? 0 : (int)(row / p.M);
+  const long m = EPI == kEpiGate ? row : row % p.M;
   if constexpr (EPI == kEpiGate)
-    epi_gate<KIND>(p.epi, p.act, m, n, p.N, a, b);
+    put_gate<KIND, false>(p.epi.h + m * p.epi.ldh + n, p.epi.plane_h,
+                          p.epi.saved ? p.epi.saved + 2 * (m * p.N + n) : nullptr, p.act, p.N - n, v, w);
   else if constexpr (EPI == kEpiGateGrad)
-    epi_gate_grad<KIND>(p.epi, p.act, m, n, p.N, a);
+    put_gate_grad<KIND>(p.epi, m * p.epi.ldh + n,
+                        gate_grad<false>(p.act, p.N - n, v, load_kept<false>(p.epi.saved + 2 * (m * p.N + n), p.N - n)));
+  else if (p.vec[mat] && n + 4 <= p.N)
+    put_row4<KIND, true>(p.out[mat], m * p.ldo[mat] + n, v, 4);
   else
-    put_row4<KIND>(p.out[mat], m * p.ldo[mat] + n, a, p.N - n, p.vec[mat]);
+    put_row4<KIND, false>(p.out[mat], m * p.ldo[mat] + n, v, p.N - n);
 }
 
 }  // namespace dpamd

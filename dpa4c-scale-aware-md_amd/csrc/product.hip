@@ -1,4 +1,6 @@
 // The products of one element kind (ELEM_KIND, one object file each) and their launches.
+#include <algorithm>
+
 #include "product.h"
 
 namespace dpamd {
@@ -7,7 +9,8 @@ namespace {
 
 // 16-bit kinds: 256 x 256 x 64 with eight waves of 128 x 64 (128 KB of LDS, one block
 // a compute unit) and 128 x 128 x 64 with four of 64 x 64 (64 KB, two). fp32, with
-// three planes to stage: 256 x 128 x 32 with eight of 64 x 64 and 128 x 64 x 32 with four of 64 x 32.
+// three planes to stage: 256 x 128 x 32 with eight of 64 x 64 (144 KB) and 128 x 64 x 32 with
+// four of 64 x 32 (72 KB, two).
 template <int KIND>
 struct Shapes {
   using Big = Shape<256, 256, 64, 2, 4>;
@@ -25,14 +28,18 @@ void launch(hipStream_t st, ProductArgs& p) {
   p.tiles_m = (p.M + S::BM - 1) / S::BM;
   p.tiles_n1 = (p.N + S::BN / SUB - 1) / (S::BN / SUB);
   p.tiles_n = p.tiles_n1 * p.mats;
-  if ((long)p.tiles_m * p.tiles_n * p.split * (S::WM * S::WN * 64) >= 1L << 32)
-    throw HipError{hipErrorInvalidValue, "gated block: too many tiles for one launch"};
-  hipLaunchKernelGGL((k_product<KIND, LA, LB, EPI, S>), dim3(p.tiles_m * p.tiles_n, p.split),
+  const long items = (long)p.tiles_m * p.tiles_n * p.split;
+  if (items >= 1L << 31) throw HipError{hipErrorInvalidValue, "gated block: too many tiles"};
+  hipLaunchKernelGGL((k_product<KIND, LA, LB, EPI, S>), dim3((unsigned)std::min(items, (long)p.blocks)),
                      dim3(S::WM * S::WN * 64), 0, st, p);
   DPAMD_LAUNCH_CHECK();
   if (p.split > 1) {
     const long rows = (long)p.M * (EPI == kEpiGate ? 1 : p.mats), quads = p.ldp / 4;
-    hipLaunchKernelGGL((k_join<KIND, EPI>), dim3((unsigned)((rows * quads + 255) / 256)), dim3(256), 0, st, p);
+    // threads that share a quad's slices: up to 8 slices each, more where the quads fill the card
+    p.join = 1;
+    while (p.join < 64 && p.split > 8 * p.join && rows * quads * p.join < 1L << 18) p.join *= 2;
+    const long per = 256 / p.join;
+    hipLaunchKernelGGL((k_join<KIND, EPI>), dim3((unsigned)((rows * quads + per - 1) / per)), dim3(256), 0, st, p);
     DPAMD_LAUNCH_CHECK();
   }
 }
