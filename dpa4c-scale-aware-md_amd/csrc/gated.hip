@@ -14,28 +14,41 @@ extern template void launch_product<kF32>(hipStream_t, ProductKind, int, Product
 
 namespace {
 
-// Eight elements a thread: rows of any stride into rows of ld, zeros from cols to ld.
+// Rows of any stride into rows of ld, zeros from cols to ld: eight elements a thread,
+// the matrices of one call one after another in one launch (a launch for each costs more
+// than the work of small ones: 17 launches of a training step of 31,920 rows through 70-96-1 took 139
+// us, 11 take 106).
 template <int KIND>
-__global__ __launch_bounds__(256) void k_pack(const void* src, long ld_src, long rows, int cols, unsigned short* dst,
-                                              long ld, long plane) {
-  const int per = (int)(ld / 8);
-  for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < rows * per; at += (long)gridDim.x * 256) {
-    const long row = at / per;
-    const int c0 = (int)(at % per) * 8;
-    unsigned short* d = dst + row * ld + c0;
+__global__ __launch_bounds__(256) void k_pack(const PackList list) {
+  for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < list.end[list.count - 1]; at += (long)gridDim.x * 256) {
+    int m = 0;
+    while (at >= list.end[m]) ++m;
+    const PackItem& it = list.item[m];
+    const long k = at - (m ? list.end[m - 1] : 0);
+    const int per = (int)(it.ld / 8);
+    const long row = k / per;
+    const int c0 = (int)(k % per) * 8;
+    unsigned short* d = it.dst + row * it.ld + c0;
     if constexpr (KIND == kF32) {
-      const float* s = static_cast<const float*>(src) + row * ld_src + c0;
+      const float* s = static_cast<const float*>(it.src) + row * it.ld_src + c0;
       float v[8];
+      if (c0 + 8 <= it.cols) {
+        __builtin_memcpy(v, s, sizeof(v));  // (the hardware takes addresses of any alignment)
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c0 + e < cols ? s[e] : 0.0f;
-      put_operand4<KIND>(d, plane, v);
-      put_operand4<KIND>(d + 4, plane, v + 4);
+        for (int e = 0; e < 8; ++e) v[e] = c0 + e < it.cols ? s[e] : 0.0f;
+      }
+      put_operand8<KIND>(d, it.plane, v);
     } else {
-      const unsigned short* s = static_cast<const unsigned short*>(src) + row * ld_src + c0;
+      const unsigned short* s = static_cast<const unsigned short*>(it.src) + row * it.ld_src + c0;
       typedef unsigned short us8 __attribute__((ext_vector_type(8)));
       us8 v;
+      if (c0 + 8 <= it.cols) {
+        __builtin_memcpy(&v, s, sizeof(v));  // (the hardware takes addresses of any alignment)
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c0 + e < cols ? s[e] : (unsigned short)0;
+        for (int e = 0; e < 8; ++e) v[e] = c0 + e < it.cols ? s[e] : (unsigned short)0;
+      }
       *reinterpret_cast<us8*>(d) = v;
     }
   }
@@ -51,13 +64,13 @@ unsigned blocks_for(long threads) { return (unsigned)std::min((threads + 255) / 
 
 }  // namespace
 
-void pack_operand(hipStream_t st, int elem, const void* src, long ld_src, long rows, long cols, unsigned short* dst,
-                  long ld, long plane) {
-  const dim3 grid(blocks_for(rows * (ld / 8)));
+void pack_operands(hipStream_t st, int elem, const PackList& list) {
+  if (!list.count) return;
+  const dim3 grid(blocks_for(list.end[list.count - 1]));
   if (elem == kF32)
-    hipLaunchKernelGGL((k_pack<kF32>), grid, dim3(256), 0, st, src, ld_src, rows, (int)cols, dst, ld, plane);
+    hipLaunchKernelGGL((k_pack<kF32>), grid, dim3(256), 0, st, list);
   else
-    hipLaunchKernelGGL((k_pack<kBf16>), grid, dim3(256), 0, st, src, ld_src, rows, (int)cols, dst, ld, plane);
+    hipLaunchKernelGGL((k_pack<kBf16>), grid, dim3(256), 0, st, list);
   DPAMD_LAUNCH_CHECK();
 }
 
@@ -73,21 +86,23 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
     int bm, bn, bk, per_cu;
     double us;  // one step of k of one block
   };
-  static const S shapes[2][2] = {{{256, 256, 64, 1, 1.9}, {128, 128, 64, 2, 1.4}},
-                                 {{256, 128, 32, 1, 1.8}, {128, 64, 32, 2, 1.1}}};
+  static const S shapes[2][3] = {{{256, 256, 64, 1, 1.9}, {128, 128, 64, 2, 1.4}, {64, 128, 64, 3, 1.2}},
+                                 {{256, 128, 32, 1, 1.8}, {128, 64, 32, 2, 1.1}, {64, 64, 32, 3, 0.9}}};
+  const char* fs = getenv("DPAMD_SHAPE");
+  const char* fz = getenv("DPAMD_SPLIT");
   const int sub = what == kProdGate ? 2 : 1;
   ProductPlan best{1, 1, ncu, 0};
   double best_us = 0;
-  for (int k = 0; k < 2; ++k) {
+  for (int k = fs ? atoi(fs) : 0; k < (fs ? atoi(fs) + 1 : 3); ++k) {
     const S& s = shapes[elem == kF32][k];
     const long tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn / sub - 1) / (s.bn / sub)) * mats;
     const long steps = (K + s.bk - 1) / s.bk * segs, slots = (long)ncu * s.per_cu;
     long split = 1;
-    if (tiles < slots) split = std::max(1L, std::min(slots / tiles, steps / 4));
+    if (fz) split = std::min(steps, atol(fz)); else if (tiles < slots) split = std::max(1L, std::min(slots / tiles, steps / 4));
     const long rounds = (tiles * split + slots - 1) / slots;
     const double bytes = split > 1 ? 4.0 * split * sub * mats * M * ((N + 7) / 8 * 8) : 0;
     const double us = (double)rounds * ((steps + split - 1) / split) * s.us + (split > 1 ? 3 + 2 * bytes / 4e6 : 0);
-    if (k == 0 || us < best_us) {
+    if (best_us == 0 || us < best_us) {
       best_us = us;
       best = ProductPlan{k, (int)split, (int)slots / 8 * 8, (size_t)bytes};
     }

@@ -168,10 +168,14 @@ Source source_of(int type, const void* p, int64_t ld, int64_t rows, int64_t cols
   return s;
 }
 
-Operand operand_of(hipStream_t st, int elem, const Source& s, char* ws) {
+// The operand's place, and what packs it there.
+Operand operand_of(const Source& s, char* ws, PackList& list) {
   if (s.direct) return Operand{static_cast<const unsigned short*>(s.src), s.ld, 0};
   auto* dst = reinterpret_cast<unsigned short*>(ws + s.at);
-  pack_operand(st, elem, s.src, s.ld_src, s.rows, s.cols, dst, s.ld, s.rows * s.ld);
+  PackItem& it = list.item[list.count];
+  it = PackItem{s.src, s.ld_src, s.ld, s.rows * s.ld, (int)s.cols, dst};
+  list.end[list.count] = (list.count ? list.end[list.count - 1] : 0) + s.rows * (s.ld / 8);
+  ++list.count;
   return Operand{dst, s.ld, s.rows * s.ld};
 }
 
@@ -207,6 +211,17 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
                    void* y, void* saved, hipStream_t st) {
   const int elem = elem_of(s.type);
   const int64_t n = s.rows, f8 = (s.d_hidden + 7) / 8 * 8;
+  if (n <= kFewRows) {
+    RowsArgs p{};
+    p.rows = (int)n;
+    p.d = s.d_in, p.f = s.d_hidden, p.o = s.d_out, p.act = s.act;
+    p.ld_x = s.ld_x, p.ld_hidden = s.ld_hidden, p.ld_down = s.ld_down, p.ld_y = s.ld_y;
+    p.x = x, p.wg = wg, p.wu = wu, p.wd = wd, p.y = y;
+    p.saved = static_cast<float*>(saved);
+    p.partial1 = reinterpret_cast<float*>(workspace(O, st, plan_rows(elem, O->ncu, p)));
+    run_rows(st, elem, p);
+    return;
+  }
   Regions r;
   const Source sx = source_of(s.type, x, s.ld_x, n, s.d_in, r);
   const bool both = pair_direct(s, wg, wu);
@@ -220,8 +235,10 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   const size_t at_part = r.take(std::max(p1.bytes, p2.bytes));
   char* ws = workspace(O, st, r.used);
 
-  const Operand ox = operand_of(st, elem, sx, ws);
-  const Operand og = operand_of(st, elem, sg, ws), ou = operand_of(st, elem, su, ws);
+  PackList list{};
+  const Operand ox = operand_of(sx, ws, list), og = operand_of(sg, ws, list), ou = operand_of(su, ws, list);
+  const Operand od = operand_of(sd, ws, list);
+  pack_operands(st, elem, list);
   ProductArgs a = product(ox, og, n, s.d_hidden, s.d_in);
   a.b[1] = ou;
   a.cols = (int)f8;
@@ -233,7 +250,7 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   a.partial = reinterpret_cast<float*>(ws + at_part);
   run_product(st, kProdGate, elem, p1, a);
 
-  const Operand oh{a.epi.h, (long)f8, plane_h}, od = operand_of(st, elem, sd, ws);
+  const Operand oh{a.epi.h, (long)f8, plane_h};
   ProductArgs b = product(oh, od, n, s.d_out, s.d_hidden);
   output(b, 0, y, s.ld_y, s.type);
   b.partial = a.partial;
@@ -266,7 +283,15 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
   char* ws = workspace(O, st, r.used);
   float* part = reinterpret_cast<float*>(ws + at_part);
 
-  const Operand ody = operand_of(st, elem, sdy, ws), od = operand_of(st, elem, sd, ws);
+  PackList list{};
+  const Operand ody = operand_of(sdy, ws, list), od = operand_of(sd, ws, list);
+  Operand ox{}, og{}, ou{};
+  if (dwg) ox = operand_of(sx, ws, list);
+  if (dx) {
+    og = operand_of(sg, ws, list);
+    ou = operand_of(su, ws, list);
+  }
+  pack_operands(st, elem, list);
   ProductArgs a = product(ody, od, n, f, s.d_out);
   a.cols = (int)f8;
   a.act = s.act;
@@ -281,16 +306,16 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
   const Operand odg{a.epi.dg, (long)f8, plane_h}, odu{a.epi.du, (long)f8, plane_h};
 
   if (dx) {
-    ProductArgs b = product(odg, operand_of(st, elem, sg, ws), n, s.d_in, f);
+    ProductArgs b = product(odg, og, n, s.d_in, f);
     b.a[1] = odu;
-    b.b[1] = operand_of(st, elem, su, ws);
+    b.b[1] = ou;
     b.segs = 2;
     output(b, 0, dx, s.ld_x, s.type);
     b.partial = part;
     run_product(st, kProdInput, elem, p2, b);
   }
   if (dwg) {
-    ProductArgs b = product(operand_of(st, elem, sx, ws), odg, s.d_in, f, n);
+    ProductArgs b = product(ox, odg, s.d_in, f, n);
     b.b[1] = odu;
     b.mats = 2;
     output(b, 0, dwg, s.ld_hidden, s.type);

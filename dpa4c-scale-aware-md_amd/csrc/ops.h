@@ -68,9 +68,34 @@ struct ProductPlan {
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu);
 void run_product(hipStream_t st, ProductKind what, int elem, const ProductPlan& plan, ProductArgs& args);
 
-// [rows][cols] of the caller's type into operand form, zeros up to ld.
-void pack_operand(hipStream_t st, int elem, const void* src, long ld_src, long rows, long cols, unsigned short* dst,
-                  long ld, long plane);
+// ---- the block for a few rows (gated_rows.hip) ----
+constexpr int kFewRows = 8;
+struct RowsArgs {
+  int rows, d, f, o, act;
+  long ld_x, ld_hidden, ld_down, ld_y;
+  const void *x, *wg, *wu, *wd;
+  void* y;
+  float* saved;
+  float *partial1, *partial2;  // [slices][rows][2][f], [slices][rows][o]
+  int slice1, slices1, slice2, slices2;
+};
+size_t plan_rows(int elem, int ncu, RowsArgs& args);  // bytes of the partial sums
+void run_rows(hipStream_t st, int elem, RowsArgs& args);
+
+// Matrices [rows][cols] of the caller's type to be brought into operand form, zeros up to ld.
+struct PackItem {
+  const void* src;
+  long ld_src, ld, plane;
+  int cols;
+  unsigned short* dst;
+};
+constexpr int kMaxPack = 5;
+struct PackList {
+  PackItem item[kMaxPack];
+  long end[kMaxPack];  // running sums of the items' groups of eight elements
+  int count;
+};
+void pack_operands(hipStream_t st, int elem, const PackList& list);
 // rows x row_bytes of zeros, rows `stride` bytes apart (a kernel: may be captured)
 void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride);
 

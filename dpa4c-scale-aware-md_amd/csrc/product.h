@@ -31,28 +31,13 @@ __device__ __forceinline__ unsigned short to16(float v) {
     return __builtin_bit_cast(unsigned short, (__bf16)v);
 }
 
-// One element of an operand: its 16 bits, or its three pieces a plane apart.
-template <int KIND>
-__device__ __forceinline__ void put_operand(unsigned short* p, long plane, float v) {
-  if constexpr (KIND == kF32) {
-    const __bf16 h = (__bf16)v;
-    const float r1 = v - (float)h;
-    const __bf16 m = (__bf16)r1;
-    p[0] = __builtin_bit_cast(unsigned short, h);
-    p[plane] = __builtin_bit_cast(unsigned short, m);
-    p[2 * plane] = __builtin_bit_cast(unsigned short, (__bf16)(r1 - (float)m));
-  } else {
-    p[0] = to16<KIND>(v);
-  }
-}
-
-// Four consecutive elements (p 8-byte aligned, plane a multiple of 4).
-template <int KIND>
-__device__ __forceinline__ void put_operand4(unsigned short* p, long plane, const float* v) {
-  typedef unsigned short us4 __attribute__((ext_vector_type(4)));
-  us4 q[3];
+// N consecutive elements (p aligned to them, plane a multiple of N).
+template <int KIND, int N>
+__device__ __forceinline__ void put_operands(unsigned short* p, long plane, const float* v) {
+  typedef unsigned short us __attribute__((ext_vector_type(N)));
+  us q[3];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < N; ++e) {
     if constexpr (KIND == kF32) {
       const __bf16 h = (__bf16)v[e];
       const float r1 = v[e] - (float)h;
@@ -65,7 +50,15 @@ __device__ __forceinline__ void put_operand4(unsigned short* p, long plane, cons
     }
   }
 #pragma unroll
-  for (int s = 0; s < pieces<KIND>(); ++s) *reinterpret_cast<us4*>(p + s * plane) = q[s];
+  for (int s = 0; s < pieces<KIND>(); ++s) *reinterpret_cast<us*>(p + s * plane) = q[s];
+}
+template <int KIND>
+__device__ __forceinline__ void put_operand4(unsigned short* p, long plane, const float* v) {
+  put_operands<KIND, 4>(p, plane, v);
+}
+template <int KIND>
+__device__ __forceinline__ void put_operand8(unsigned short* p, long plane, const float* v) {
+  put_operands<KIND, 8>(p, plane, v);
 }
 
 // Four columns of one row of an output of the kind's own type, `count` of them inside it; FULL:
@@ -359,19 +352,6 @@ __device__ __forceinline__ f4 mfma16(s8v a, s8v b, f4 c) {
     return mfma_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c);
 }
 
-// acc += the products of all pieces (the six down to 2^-18, smallest first)
-template <int KIND>
-__device__ __forceinline__ f4 mfma_all(const s8v* a, const s8v* b, f4 c) {
-  if constexpr (KIND == kF32) {
-    c = mfma16<KIND>(a[1], b[1], c);
-    c = mfma16<KIND>(a[2], b[0], c);
-    c = mfma16<KIND>(a[0], b[2], c);
-    c = mfma16<KIND>(a[1], b[0], c);
-    c = mfma16<KIND>(a[0], b[1], c);
-  }
-  return mfma16<KIND>(a[0], b[0], c);
-}
-
 // Shape of a block's tile: BM rows by BN columns by BK of k, WM by WN waves.
 template <int BM_, int BN_, int BK_, int WM_, int WN_>
 struct Shape {
@@ -471,14 +451,14 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
     return q < P * TA::kLoads ? TA::past(q % TA::kLoads, wave, lane, k_left)
                               : TB::past((q - P * TA::kLoads) % TB::kLoads, wave, lane, k_left);
   };
-  auto issue = [&](int q, const Cursor& u, int to) {
+  auto issue = [&](int q, const Cursor& u, int to, bool whole = false) {
     if (q < P * TA::kLoads) {
       const int l = q % TA::kLoads;
-      if (TA::outside(l, wave, lane, u.k_left, p.M - it.m0)) return;
+      if (!whole && TA::outside(l, wave, lane, u.k_left, p.M - it.m0)) return;
       load_to_lds(u.pa + q / TA::kLoads * pla + TA::moved(l) * lda2, oa[TA::kind(l)], lds0 + to + slot(q));
     } else {
       const int r = q - P * TA::kLoads, s = r / TB::kLoads, l = r % TB::kLoads;
-      if (TB::outside(l, wave, lane, u.k_left, p.N - it.n0)) return;
+      if (!whole && TB::outside(l, wave, lane, u.k_left, p.N - it.n0)) return;
       // (every lane of one load lies in one part: a part is whole loads)
       const bool part = SUB == 2 && (l * WAVES + wave) * 1024 >= TB::kBytes / 2;
       load_to_lds((part ? u.pb_second : u.pb) + s * plb + TB::moved(l) * ldb2, ob[TB::kind(l)], lds0 + to + slot(q));
@@ -492,9 +472,14 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
   };
   auto load = [&](int t, int to) {
     const Cursor u = cursor(t);
+    if (u.k_left >= S::BK && it.m0 + S::BM <= p.M && it.n0 + S::BN / SUB <= p.N) {
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) issue(q, u, to);
-    fill(u, to);
+      for (int q = 0; q < kLoads; ++q) issue(q, u, to, true);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) issue(q, u, to);
+      fill(u, to);
+    }
   };
   auto frag_a = [&](const char* tile, int s, int i, int kk) {
     return TA::frag(tile + s * TA::kBytes, 0, wm * TM + i * 16, kk, lane);
@@ -575,18 +560,23 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
         }
 #pragma unroll
         for (int kk = 0; kk < S::BK / 32; ++kk) {
-          s8v b[NJ][P];
+          // the pieces' products that reach 2^-18 of the leading one, in the order in which
+          // the pieces are read
+          constexpr int kPairs = 6, kRow[kPairs] = {0, 0, 1, 1, 0, 2}, kCol[kPairs] = {0, 1, 0, 1, 2, 0};
+          s8v b[P][NJ];
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+          for (int s = 0; s < P; ++s)
 #pragma unroll
-            for (int s = 0; s < P; ++s) b[j][s] = frag_b(cur, s, j, kk);
+            for (int j = 0; j < NJ; ++j) b[s][j] = frag_b(cur, s, j, kk);
 #pragma unroll
           for (int i = 0; i < MI; ++i) {
             s8v a[P];
 #pragma unroll
             for (int s = 0; s < P; ++s) a[s] = frag_a(cur, s, i, kk);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[i][j] = mfma_all<KIND>(b[j], a, acc[i][j]);
+            for (int q = 0; q < kPairs; ++q)
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) acc[i][j] = mfma16<KIND>(b[kCol[q]][j], a[kRow[q]], acc[i][j]);
           }
         }
       }
