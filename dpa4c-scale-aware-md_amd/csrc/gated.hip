@@ -16,9 +16,8 @@ namespace {
 
 // Rows of any stride into rows of ld, zeros from cols to ld: eight elements a thread,
 // the matrices of one call one after another in one launch (a launch for each costs more
-// than the work of small ones: 17 launches of a training step of 31,920 rows through 70-96-1 took 139
-// us, 11 take 106).
-template <int KIND>
+// than the work of small ones).
+template <class T>
 __global__ __launch_bounds__(256) void k_pack(const PackList list) {
   for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < list.end[list.count - 1]; at += (long)gridDim.x * 256) {
     int m = 0;
@@ -28,29 +27,17 @@ __global__ __launch_bounds__(256) void k_pack(const PackList list) {
     const int per = (int)(it.ld / 8);
     const long row = k / per;
     const int c0 = (int)(k % per) * 8;
-    unsigned short* d = it.dst + row * it.ld + c0;
-    if constexpr (KIND == kF32) {
-      const float* s = static_cast<const float*>(it.src) + row * it.ld_src + c0;
-      float v[8];
-      if (c0 + 8 <= it.cols) {
-        __builtin_memcpy(v, s, sizeof(v));  // (the hardware takes addresses of any alignment)
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c0 + e < it.cols ? s[e] : 0.0f;
-      }
-      put_operand8<KIND>(d, it.plane, v);
+    const T* s = static_cast<const T*>(it.src) + row * it.ld_src + c0;
+    struct alignas(16) Eight {
+      T v[8];
+    } v;
+    if (c0 + 8 <= it.cols) {
+      __builtin_memcpy(&v, s, sizeof(v));  // (the hardware takes addresses of any alignment)
     } else {
-      const unsigned short* s = static_cast<const unsigned short*>(it.src) + row * it.ld_src + c0;
-      typedef unsigned short us8 __attribute__((ext_vector_type(8)));
-      us8 v;
-      if (c0 + 8 <= it.cols) {
-        __builtin_memcpy(&v, s, sizeof(v));  // (the hardware takes addresses of any alignment)
-      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c0 + e < it.cols ? s[e] : (unsigned short)0;
-      }
-      *reinterpret_cast<us8*>(d) = v;
+      for (int e = 0; e < 8; ++e) v.v[e] = c0 + e < it.cols ? s[e] : T(0);
     }
+    *reinterpret_cast<Eight*>(static_cast<T*>(it.dst) + row * it.ld + c0) = v;
   }
 }
 
@@ -68,9 +55,9 @@ void pack_operands(hipStream_t st, int elem, const PackList& list) {
   if (!list.count) return;
   const dim3 grid(blocks_for(list.end[list.count - 1]));
   if (elem == kF32)
-    hipLaunchKernelGGL((k_pack<kF32>), grid, dim3(256), 0, st, list);
+    hipLaunchKernelGGL((k_pack<float>), grid, dim3(256), 0, st, list);
   else
-    hipLaunchKernelGGL((k_pack<kBf16>), grid, dim3(256), 0, st, list);
+    hipLaunchKernelGGL((k_pack<unsigned short>), grid, dim3(256), 0, st, list);
   DPAMD_LAUNCH_CHECK();
 }
 
@@ -82,29 +69,33 @@ void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride
 }
 
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu) {
+  // One step (128 bytes of k) of one block, measured: its share of a compute unit's time
+  // among others, and its time alone; and the blocks that a compute unit holds. (fp32: the matrix cores
+  // are slow enough that 256 x 256 tiles gain nothing over 128 x 128.)
   struct S {
-    int bm, bn, bk, per_cu;
-    double us;  // one step of k of one block
+    int bm, bn, per_cu;
+    double share_us, alone_us;
   };
-  static const S shapes[2][3] = {{{256, 256, 64, 1, 1.9}, {128, 128, 64, 2, 1.4}, {64, 128, 64, 3, 1.2}},
-                                 {{256, 128, 32, 1, 1.8}, {128, 64, 32, 2, 1.1}, {64, 64, 32, 3, 0.9}}};
-  const char* fs = getenv("DPAMD_SHAPE");
-  const char* fz = getenv("DPAMD_SPLIT");
-  const int sub = what == kProdGate ? 2 : 1;
-  ProductPlan best{1, 1, ncu, 0};
+  static const S shapes[2][3] = {{{256, 256, 1, 1.8, 1.8}, {128, 128, 2, 0.62, 1.0}, {64, 128, 3, 0.40, 0.9}},
+                                 {{256, 256, 1, 8.1, 8.1}, {128, 128, 2, 2.05, 2.26}, {64, 128, 3, 1.05, 1.27}}};
+  const int sub = what == kProdGate ? 2 : 1, bk = elem == kF32 ? 32 : 64;
+  ProductPlan best{};
   double best_us = 0;
-  for (int k = fs ? atoi(fs) : 0; k < (fs ? atoi(fs) + 1 : 3); ++k) {
+  const long steps = (K + bk - 1) / bk * segs;
+  for (int k = elem == kF32 ? 1 : 0; k < 3; ++k) {
     const S& s = shapes[elem == kF32][k];
     const long tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn / sub - 1) / (s.bn / sub)) * mats;
-    const long steps = (K + s.bk - 1) / s.bk * segs, slots = (long)ncu * s.per_cu;
-    long split = 1;
-    if (fz) split = std::min(steps, atol(fz)); else if (tiles < slots) split = std::max(1L, std::min(slots / tiles, steps / 4));
-    const long rounds = (tiles * split + slots - 1) / slots;
-    const double bytes = split > 1 ? 4.0 * split * sub * mats * M * ((N + 7) / 8 * 8) : 0;
-    const double us = (double)rounds * ((steps + split - 1) / split) * s.us + (split > 1 ? 3 + 2 * bytes / 4e6 : 0);
-    if (best_us == 0 || us < best_us) {
-      best_us = us;
-      best = ProductPlan{k, (int)split, (int)slots / 8 * 8, (size_t)bytes};
+    const long slots = (long)ncu * s.per_cu;
+    const long most = std::max(1L, std::min(steps / 4, 2 * slots / tiles));
+    for (long split = 1; split <= most; split = split < 4 ? split + 1 : split + split / 4) {
+      const long items = tiles * split, a_cu = (items + ncu - 1) / ncu, rounds = (items + slots - 1) / slots;
+      const double bytes = split > 1 ? 4.0 * split * sub * mats * M * ((N + 7) / 8 * 8) : 0;
+      const double us = (double)((steps + split - 1) / split) * std::max(a_cu * s.share_us, rounds * s.alone_us) +
+                        2.0 * rounds + (split > 1 ? 4 + 2 * bytes / 4e6 : 0);
+      if (best_us == 0 || us < best_us) {
+        best_us = us;
+        best = ProductPlan{k, (int)split, (int)slots / 8 * 8, (size_t)bytes};
+      }
     }
   }
   return best;

@@ -24,24 +24,10 @@ namespace {
 constexpr int kThreads = 256, kColLanes = 8, kRowLanes = kThreads / kColLanes;
 constexpr int kMaxSlice = 1024;  // rows of weights a slice: rows * 4 KB of LDS
 
+// elements of 16 bytes
 template <int KIND>
-struct NativeOf {
-  using T = unsigned short;
-  static constexpr int E = 8;
-};
-template <>
-struct NativeOf<kF32> {
-  using T = float;
-  static constexpr int E = 4;
-};
-template <int KIND>
-__device__ __forceinline__ float widen(typename NativeOf<KIND>::T v) {
-  if constexpr (KIND == kF32)
-    return v;
-  else if constexpr (KIND == kF16)
-    return (float)__builtin_bit_cast(_Float16, v);
-  else
-    return __builtin_bit_cast(float, (unsigned)v << 16);
+constexpr int chunk_of() {
+  return KIND == kF32 ? 4 : 8;
 }
 
 // N elements at any alignment of the element (the hardware takes unaligned addresses)
@@ -59,8 +45,8 @@ __device__ __forceinline__ Some<T, N> load_some(const T* p) {
 // acc[r][m][e] += sum over the slice's k of x[r][k] w_m[k][c + e]; x in LDS, rows `slice` apart
 template <int KIND, int R, int MATS, int E>
 __device__ __forceinline__ void sweep(float (&acc)[R][MATS][E], const float* x, int slice, int count,
-                                      const typename NativeOf<KIND>::T* const (&w)[MATS], long ld) {
-  using T = typename NativeOf<KIND>::T;
+                                      const typename ElemOf<KIND>::T* const (&w)[MATS], long ld) {
+  using T = typename ElemOf<KIND>::T;
   constexpr int U = 4;  // rows of weights under way
   const int first = threadIdx.x / kColLanes;
   int k = first;
@@ -78,7 +64,7 @@ __device__ __forceinline__ void sweep(float (&acc)[R][MATS][E], const float* x, 
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[r][m][e] += a * widen<KIND>(v[u][m].v[e]);
+          for (int e = 0; e < E; ++e) acc[r][m][e] += a * to_f32<KIND>(v[u][m].v[e]);
       }
   }
   for (; k < count; k += kRowLanes) {
@@ -90,7 +76,7 @@ __device__ __forceinline__ void sweep(float (&acc)[R][MATS][E], const float* x, 
 #pragma unroll
       for (int m = 0; m < MATS; ++m)
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[r][m][e] += x[r * slice + k] * widen<KIND>(v[m].v[e]);
+        for (int e = 0; e < E; ++e) acc[r][m][e] += x[r * slice + k] * to_f32<KIND>(v[m].v[e]);
   }
 }
 
@@ -140,13 +126,13 @@ __device__ __forceinline__ int column(int block0, int E, int cols) {
 
 template <int KIND, int R, int E>
 __global__ __launch_bounds__(kThreads) void k_rows_gate(RowsArgs p) {
-  using T = typename NativeOf<KIND>::T;
+  using T = typename ElemOf<KIND>::T;
   extern __shared__ __align__(16) float lds[];
   const int slice = p.slice1, k0 = blockIdx.y * slice, count = min(slice, p.d - k0);
   const T* x = static_cast<const T*>(p.x);
   for (int q = threadIdx.x; q < R * count; q += kThreads) {
     const int r = q / count, k = q % count;
-    lds[r * slice + k] = r < p.rows ? widen<KIND>(x[r * p.ld_x + k0 + k]) : 0.0f;
+    lds[r * slice + k] = r < p.rows ? to_f32<KIND>(x[r * p.ld_x + k0 + k]) : 0.0f;
   }
   __syncthreads();
   const int block0 = blockIdx.x * kColLanes * E, c = column(block0, E, p.f);
@@ -159,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void k_rows_gate(RowsArgs p) {
 
 template <int KIND, int R, int E>
 __global__ __launch_bounds__(kThreads) void k_rows_down(RowsArgs p) {
-  using T = typename NativeOf<KIND>::T;
+  using T = typename ElemOf<KIND>::T;
   extern __shared__ __align__(16) float lds[];
   const int slice = p.slice2, k0 = blockIdx.y * slice, count = min(slice, p.f - k0);
   for (int q = threadIdx.x; q < R * count; q += kThreads) {
@@ -212,10 +198,7 @@ __global__ __launch_bounds__(kThreads) void k_rows_join(RowsArgs p) {
   if (share || at >= all) return;
   for (int k = 1; k < G; ++k) v += part[k * per + slot];
   const long to = at / p.o * p.ld_y + at % p.o;
-  if constexpr (KIND == kF32)
-    static_cast<float*>(p.y)[to] = v;
-  else
-    static_cast<unsigned short*>(p.y)[to] = to16<KIND>(v);
+  static_cast<typename ElemOf<KIND>::T*>(p.y)[to] = from_f32<KIND>(v);
 }
 
 template <int KIND, int R, int E>
@@ -245,7 +228,7 @@ void rows_by_count(hipStream_t st, const RowsArgs& p) {
 
 template <int KIND>
 void rows_kind(hipStream_t st, const RowsArgs& p) {
-  constexpr int E = NativeOf<KIND>::E;
+  constexpr int E = chunk_of<KIND>();
   if (p.f >= E && p.o >= E)
     rows_by_count<KIND, E>(st, p);
   else

@@ -24,33 +24,6 @@ namespace dpamd {
 
 namespace {
 
-// ---- elements -------------------------------------------------------------------------
-template <int KIND>
-struct ElemOf {
-  using T = unsigned short;
-};
-template <>
-struct ElemOf<kF32> {
-  using T = float;
-};
-
-template <int KIND>
-__device__ __forceinline__ float to_f32(typename ElemOf<KIND>::T v) {
-  if constexpr (KIND == kF32)
-    return v;
-  else if constexpr (KIND == kF16)
-    return (float)__builtin_bit_cast(_Float16, v);
-  else
-    return __builtin_bit_cast(float, (unsigned)v << 16);
-}
-template <int KIND>
-__device__ __forceinline__ typename ElemOf<KIND>::T from_f32(float v) {
-  if constexpr (KIND == kF32)
-    return v;
-  else
-    return to16<KIND>(v);
-}
-
 // E consecutive elements, loaded and stored as one
 template <int KIND, int E>
 struct alignas(sizeof(typename ElemOf<KIND>::T) * E) Chunk {

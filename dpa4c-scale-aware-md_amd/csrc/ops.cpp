@@ -144,8 +144,8 @@ dp_gated_shape checked(const dp_gated_shape* s) {
   return t;
 }
 
-// An operand of the products: the caller's matrix where it has the operand form (16
-// bits, rows of whole 16-byte chunks), and else a region that it is packed into.
+// An operand of the products: the caller's matrix where it is one (rows of whole 16-byte
+// chunks, aligned), and else a region that it is copied into.
 struct Source {
   const void* src;
   long ld_src, rows, cols;
@@ -154,34 +154,33 @@ struct Source {
   long ld;
 };
 
-bool has_operand_form(int type, const void* p, int64_t ld, int64_t cols) {
-  return type != DP_TYPE_F32 && cols % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+bool is_operand(int type, const void* p, int64_t ld, int64_t cols) {
+  const int64_t chunk = 16 / (int64_t)bytes_of(type);
+  return cols % chunk == 0 && ld % chunk == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 }
 
 Source source_of(int type, const void* p, int64_t ld, int64_t rows, int64_t cols, Regions& r, bool direct = true) {
   Source s{p, (long)ld, (long)rows, (long)cols, false, 0, (long)ld};
-  s.direct = direct && has_operand_form(type, p, ld, cols);
+  s.direct = direct && is_operand(type, p, ld, cols);
   if (!s.direct) {
     s.ld = (s.cols + 7) / 8 * 8;
-    s.at = r.take((type == DP_TYPE_F32 ? 6 : 2) * (size_t)s.rows * s.ld);
+    s.at = r.take(bytes_of(type) * (size_t)s.rows * s.ld);
   }
   return s;
 }
 
-// The operand's place, and what packs it there.
+// The operand's place, and what copies it there.
 Operand operand_of(const Source& s, char* ws, PackList& list) {
-  if (s.direct) return Operand{static_cast<const unsigned short*>(s.src), s.ld, 0};
-  auto* dst = reinterpret_cast<unsigned short*>(ws + s.at);
-  PackItem& it = list.item[list.count];
-  it = PackItem{s.src, s.ld_src, s.ld, s.rows * s.ld, (int)s.cols, dst};
+  if (s.direct) return Operand{s.src, s.ld};
+  list.item[list.count] = PackItem{s.src, s.ld_src, s.ld, (int)s.cols, ws + s.at};
   list.end[list.count] = (list.count ? list.end[list.count - 1] : 0) + s.rows * (s.ld / 8);
   ++list.count;
-  return Operand{dst, s.ld, s.rows * s.ld};
+  return Operand{ws + s.at, s.ld};
 }
 
-// gate and up are packed both or neither: the products take one row length for the two
+// gate and up are copied both or neither: the products take one row length for the two
 bool pair_direct(const dp_gated_shape& s, const void* wg, const void* wu) {
-  return has_operand_form(s.type, wg, s.ld_hidden, s.d_hidden) && has_operand_form(s.type, wu, s.ld_hidden, s.d_hidden);
+  return is_operand(s.type, wg, s.ld_hidden, s.d_hidden) && is_operand(s.type, wu, s.ld_hidden, s.d_hidden);
 }
 
 // whether rows of four elements of `out` can be stored whole
@@ -228,8 +227,7 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   const Source sg = source_of(s.type, wg, s.ld_hidden, s.d_in, s.d_hidden, r, both);
   const Source su = source_of(s.type, wu, s.ld_hidden, s.d_in, s.d_hidden, r, both);
   const Source sd = source_of(s.type, wd, s.ld_down, s.d_hidden, s.d_out, r);
-  const long plane_h = n * f8;
-  const size_t at_h = r.take((s.type == DP_TYPE_F32 ? 6 : 2) * (size_t)plane_h);
+  const size_t at_h = r.take(bytes_of(s.type) * (size_t)n * f8);
   const ProductPlan p1 = plan_product(kProdGate, elem, n, s.d_hidden, s.d_in, 1, 1, O->ncu);
   const ProductPlan p2 = plan_product(kProdDown, elem, n, s.d_out, s.d_hidden, 1, 1, O->ncu);
   const size_t at_part = r.take(std::max(p1.bytes, p2.bytes));
@@ -243,14 +241,13 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   a.b[1] = ou;
   a.cols = (int)f8;
   a.act = s.act;
-  a.epi.h = reinterpret_cast<unsigned short*>(ws + at_h);
+  a.epi.h = ws + at_h;
   a.epi.ldh = f8;
-  a.epi.plane_h = plane_h;
   a.epi.saved = static_cast<float*>(saved);
   a.partial = reinterpret_cast<float*>(ws + at_part);
   run_product(st, kProdGate, elem, p1, a);
 
-  const Operand oh{a.epi.h, (long)f8, plane_h};
+  const Operand oh{a.epi.h, (long)f8};
   ProductArgs b = product(oh, od, n, s.d_out, s.d_hidden);
   output(b, 0, y, s.ld_y, s.type);
   b.partial = a.partial;
@@ -271,8 +268,7 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     sg = source_of(s.type, wg, s.ld_hidden, s.d_in, f, r, both);
     su = source_of(s.type, wu, s.ld_hidden, s.d_in, f, r, both);
   }
-  const long plane_h = n * f8;
-  const size_t hb = (s.type == DP_TYPE_F32 ? 6 : 2) * (size_t)plane_h;
+  const size_t hb = bytes_of(s.type) * (size_t)n * f8;
   const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd ? r.take(hb) : 0;
   const ProductPlan p1 = plan_product(kProdGateGrad, elem, n, f, s.d_out, 1, 1, O->ncu);
   const ProductPlan p2 = plan_product(kProdInput, elem, n, s.d_in, f, 2, 1, O->ncu);
@@ -295,15 +291,14 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
   ProductArgs a = product(ody, od, n, f, s.d_out);
   a.cols = (int)f8;
   a.act = s.act;
-  a.epi.h = dwd ? reinterpret_cast<unsigned short*>(ws + at_h) : nullptr;
-  a.epi.dg = reinterpret_cast<unsigned short*>(ws + at_dg);
-  a.epi.du = reinterpret_cast<unsigned short*>(ws + at_du);
+  a.epi.h = dwd ? ws + at_h : nullptr;
+  a.epi.dg = ws + at_dg;
+  a.epi.du = ws + at_du;
   a.epi.ldh = f8;
-  a.epi.plane_h = plane_h;
   a.epi.saved = static_cast<float*>(const_cast<void*>(saved));
   a.partial = part;
   run_product(st, kProdGateGrad, elem, p1, a);
-  const Operand odg{a.epi.dg, (long)f8, plane_h}, odu{a.epi.du, (long)f8, plane_h};
+  const Operand odg{a.epi.dg, (long)f8}, odu{a.epi.du, (long)f8};
 
   if (dx) {
     ProductArgs b = product(odg, og, n, s.d_in, f);
@@ -324,7 +319,7 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     run_product(st, kProdWeight, elem, p3, b);
   }
   if (dwd) {
-    ProductArgs b = product(Operand{a.epi.h, (long)f8, plane_h}, ody, f, s.d_out, n);
+    ProductArgs b = product(Operand{a.epi.h, (long)f8}, ody, f, s.d_out, n);
     output(b, 0, dwd, s.ld_down, s.type);
     b.partial = part;
     run_product(st, kProdWeight, elem, p4, b);

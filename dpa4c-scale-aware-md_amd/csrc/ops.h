@@ -15,20 +15,17 @@ enum { kActTanh = 0, kActSilu = 1, kActGelu = 2 };
 // ---- tile products (product.h) ----
 enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2 };
 
-// A 16-bit operand: row length in elements; elements between its pieces (fp32 only).
-// 16-byte aligned, ld a multiple of 8, and the contiguous side ends at a multiple of 8
-// or is followed by zeros up to one.
+// An operand of the products, of the call's type: 16-byte aligned, rows of whole 16-byte
+// chunks (ld elements), and the contiguous side ends with a chunk or is followed by zeros up to one.
 struct Operand {
-  const unsigned short* p;
+  const void* p;
   long ld;
-  long plane;
 };
 
-// h, dg and du in operand form: [M][ldh], pieces plane_h apart; saved: [M][N] pairs (g, u).
+// h, dg and du as operands [M][ldh]; saved: [M][N] pairs (g, u).
 struct EpiArgs {
-  unsigned short* h;
-  unsigned short *dg, *du;
-  long ldh, plane_h;
+  void *h, *dg, *du;
+  long ldh;
   float* saved;
 };
 
@@ -82,12 +79,12 @@ struct RowsArgs {
 size_t plan_rows(int elem, int ncu, RowsArgs& args);  // bytes of the partial sums
 void run_rows(hipStream_t st, int elem, RowsArgs& args);
 
-// Matrices [rows][cols] of the caller's type to be brought into operand form, zeros up to ld.
+// Matrices [rows][cols] to be copied into rows of ld (a multiple of 8), with zeros past cols.
 struct PackItem {
   const void* src;
-  long ld_src, ld, plane;
+  long ld_src, ld;
   int cols;
-  unsigned short* dst;
+  void* dst;
 };
 constexpr int kMaxPack = 5;
 struct PackList {

@@ -1,26 +1,30 @@
-// Tile products on the 16-bit matrix cores: C[m][n] = sum_k A(m, k) B(n, k), with an
-// epilogue on the fp32 sums. The products of the gated block (gated.hip), for 16-bit
-// operands and for fp32 ones as three exact bf16 pieces (bf16x3.h).
+// Tile products on the matrix cores: C[m][n] = sum_k A(m, k) B(n, k), with an
+// epilogue on the fp32 sums. The products of the gated block (gated.hip), for bf16, f16 and
+// fp32 operands (v_mfma_f32_16x16x32_bf16 / _f16, v_mfma_f32_16x16x4_f32).
 #pragma once
 
 #include <type_traits>
 
-#include "bf16x3.h"
+#include "common.h"
 #include "fastmath.h"
 #include "ops.h"
 
 namespace dpamd {
 
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 typedef short s8v __attribute__((ext_vector_type(8)));
 
-// Element kinds: kBf16, kF16, and kF32 whose operands are three bf16 planes.
 enum ElemKind { kBf16 = 0, kF16 = 1, kF32 = 2 };
 template <int KIND>
-constexpr int pieces() {
-  return KIND == kF32 ? 3 : 1;
-}
+struct ElemOf {
+  using T = unsigned short;
+};
+template <>
+struct ElemOf<kF32> {
+  using T = float;
+};
 
 // v rounded to the kind's 16 bits (to nearest, ties to even)
 template <int KIND>
@@ -30,60 +34,44 @@ __device__ __forceinline__ unsigned short to16(float v) {
   else
     return __builtin_bit_cast(unsigned short, (__bf16)v);
 }
-
-// N consecutive elements (p aligned to them, plane a multiple of N).
-template <int KIND, int N>
-__device__ __forceinline__ void put_operands(unsigned short* p, long plane, const float* v) {
-  typedef unsigned short us __attribute__((ext_vector_type(N)));
-  us q[3];
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    if constexpr (KIND == kF32) {
-      const __bf16 h = (__bf16)v[e];
-      const float r1 = v[e] - (float)h;
-      const __bf16 m = (__bf16)r1;
-      q[0][e] = __builtin_bit_cast(unsigned short, h);
-      q[1][e] = __builtin_bit_cast(unsigned short, m);
-      q[2][e] = __builtin_bit_cast(unsigned short, (__bf16)(r1 - (float)m));
-    } else {
-      q[0][e] = to16<KIND>(v[e]);
-    }
-  }
-#pragma unroll
-  for (int s = 0; s < pieces<KIND>(); ++s) *reinterpret_cast<us*>(p + s * plane) = q[s];
+template <int KIND>
+__device__ __forceinline__ float to_f32(typename ElemOf<KIND>::T v) {
+  if constexpr (KIND == kF32)
+    return v;
+  else if constexpr (KIND == kF16)
+    return (float)__builtin_bit_cast(_Float16, v);
+  else
+    return __builtin_bit_cast(float, (unsigned)v << 16);
 }
 template <int KIND>
-__device__ __forceinline__ void put_operand4(unsigned short* p, long plane, const float* v) {
-  put_operands<KIND, 4>(p, plane, v);
-}
-template <int KIND>
-__device__ __forceinline__ void put_operand8(unsigned short* p, long plane, const float* v) {
-  put_operands<KIND, 8>(p, plane, v);
+__device__ __forceinline__ typename ElemOf<KIND>::T from_f32(float v) {
+  if constexpr (KIND == kF32)
+    return v;
+  else
+    return to16<KIND>(v);
 }
 
-// Four columns of one row of an output of the kind's own type, `count` of them inside it; FULL:
-// all four, and aligned.
-template <int KIND, bool FULL>
-__device__ __forceinline__ void put_row4(void* out, long at, const f4& v, int count) {
+// Four consecutive elements, aligned to them.
+template <int KIND>
+__device__ __forceinline__ void put4(typename ElemOf<KIND>::T* p, const f4& v) {
   if constexpr (KIND == kF32) {
-    float* o = static_cast<float*>(out) + at;
-    if constexpr (FULL) {
-      *reinterpret_cast<f4*>(o) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < count) o[e] = v[e];
-    }
+    *reinterpret_cast<f4*>(p) = v;
   } else {
     typedef unsigned short us4 __attribute__((ext_vector_type(4)));
-    unsigned short* o = static_cast<unsigned short*>(out) + at;
-    if constexpr (FULL) {
-      *reinterpret_cast<us4*>(o) = us4{to16<KIND>(v[0]), to16<KIND>(v[1]), to16<KIND>(v[2]), to16<KIND>(v[3])};
-    } else {
+    *reinterpret_cast<us4*>(p) = us4{to16<KIND>(v[0]), to16<KIND>(v[1]), to16<KIND>(v[2]), to16<KIND>(v[3])};
+  }
+}
+
+// Four columns of one row of an output, `count` of them inside it; FULL: all four, and aligned.
+template <int KIND, bool FULL>
+__device__ __forceinline__ void put_row4(void* out, long at, const f4& v, int count) {
+  auto* o = static_cast<typename ElemOf<KIND>::T*>(out) + at;
+  if constexpr (FULL) {
+    put4<KIND>(o, v);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < count) o[e] = to16<KIND>(v[e]);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (e < count) o[e] = from_f32<KIND>(v[e]);
   }
 }
 
@@ -139,17 +127,16 @@ __device__ __forceinline__ void activate4(int act, const f4& g, f4& a, f4& da) {
 // The four columns are `count` of the output's (and the rest beyond it); FULL: all four, and
 // aligned.
 
-// h = a(g) u in operand form (zeros beyond the output), g and u kept for the backward in 32
+// h = a(g) u (zeros beyond the output), g and u kept for the backward in 32
 // bits, so that what it forms from them is rounded once. kept: pairs (g, u), or null.
 template <int KIND, bool FULL>
-__device__ __forceinline__ void put_gate(unsigned short* h, long plane, float* kept, int act, int count, const f4& g,
+__device__ __forceinline__ void put_gate(void* h, long at, float* kept, int act, int count, const f4& g,
                                          const f4& u) {
-  f4 a, da;
+  f4 a, da, v;
   activate4(act, g, a, da);
-  float v[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) v[r] = FULL || r < count ? a[r] * u[r] : 0.0f;
-  put_operand4<KIND>(h, plane, v);
+  put4<KIND>(static_cast<typename ElemOf<KIND>::T*>(h) + at, v);
   if (!kept) return;
   if constexpr (FULL) {
     *reinterpret_cast<f4*>(kept) = f4{g[0], u[0], g[1], u[1]};
@@ -187,7 +174,7 @@ __device__ __forceinline__ Kept load_kept(const float* kept, int count) {
 
 // From dh and the kept g, u: dg = dh u a'(g), du = dh a(g) and h again.
 struct GateGrad {
-  float h[4], dg[4], du[4];
+  f4 h, dg, du;
 };
 template <bool FULL>
 __device__ __forceinline__ GateGrad gate_grad(int act, int count, const f4& dh, const Kept& k) {
@@ -205,9 +192,10 @@ __device__ __forceinline__ GateGrad gate_grad(int act, int count, const f4& dh, 
 }
 template <int KIND>
 __device__ __forceinline__ void put_gate_grad(const EpiArgs& e, long at, const GateGrad& o) {
-  if (e.h) put_operand4<KIND>(e.h + at, e.plane_h, o.h);
-  put_operand4<KIND>(e.dg + at, e.plane_h, o.dg);
-  put_operand4<KIND>(e.du + at, e.plane_h, o.du);
+  using T = typename ElemOf<KIND>::T;
+  if (e.h) put4<KIND>(static_cast<T*>(e.h) + at, o.h);
+  put4<KIND>(static_cast<T*>(e.dg) + at, o.dg);
+  put4<KIND>(static_cast<T*>(e.du) + at, o.du);
 }
 
 // ---- the product ------------------------------------------------------------------------
@@ -245,117 +233,142 @@ __device__ __forceinline__ void tile_landed() {
   __syncthreads();
 }
 
-// One operand's tile in LDS: `ROWS` rows by BK of k, in SUB side-by-side parts of
-// ROWS / SUB rows that come from as many matrices.
+// One operand's tile in LDS: ROWS rows by 128 bytes of k (BK = 64 or 32 elements of EB bytes), in
+// SUB side-by-side parts of ROWS / SUB rows that come from as many matrices.
 //
-// kRowK: rows of BK elements; the row's 16-byte chunks are permuted by xor with
-// the row's index among the rows that share the 64 banks' 256 bytes, so that the
-// sixteen rows a fragment read takes at one chunk lie in different banks.
-// kColK: per part, BK rows of ROWS / SUB elements, read by the transposing LDS load; 32-byte
-// units permuted by xor with (k & 3) + 4 ((k >> 3) & 3): the 4 k rows of each of the four lane
-// groups of one read fall in different banks.
+// kRowK: rows of 128 bytes, whose 16-byte chunks are permuted by pairs, so that the sixteen
+// rows that a fragment read takes at one chunk lie in different banks (a read takes its lanes
+// in the groups 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of each half of the wave: eight rows
+// at each of two neighbouring chunks).
+// kColK: per part, BK rows of ROWS / SUB elements. 16 bits: read by the transposing LDS load, 32-byte
+// units permuted by xor with (k & 3) + 4 ((k >> 3) & 3), so that the 4 k rows of each of the four lane
+// groups of one read fall in different banks. 32 bits: read element by element, 64-byte
+// units permuted by xor with (k >> 2) & 3 for the same.
 // The tile is written by the direct global-to-LDS load, whose lanes fill 1 KB in lane
 // order; the permutation is on the side of the global addresses.
-template <int LAYOUT, int ROWS, int BK, int SUB, int WAVES>
+template <int LAYOUT, int ROWS, int EB, int SUB, int WAVES>
 struct TileOf {
-  static constexpr int kBytes = ROWS * BK * 2;
+  static constexpr int BK = 128 / EB, VE = 16 / EB;  // k of a tile, elements of a chunk
+  static constexpr int kBytes = ROWS * 128;
   static constexpr int kPart = ROWS / SUB;
   static constexpr int kLoads = kBytes / 1024 / WAVES;  // per wave
   static_assert(kLoads * 1024 * WAVES == kBytes, "a tile is whole 1 KB loads of every wave");
-  static constexpr int kChunks = BK / 8;
-  static constexpr int kUnits = kPart / 16;
+  static constexpr int kKRow = kPart * EB;               // bytes of one k row of a part (kColK)
+  static constexpr int kUnits = kKRow / (EB == 2 ? 32 : 64);
+  static constexpr int kPeriod = EB == 2 ? 32 : 16;      // k rows of one permutation
 
-  static __device__ __forceinline__ int swz_row(int row) {
-    // (a 16-byte LDS read takes its lanes in the groups 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31
-    // of each half of the wave: eight rows at each of two neighbouring chunks)
-    return (BK == 32 ? (row / 8) & 1 : (row / 2) & 3) << 1;
+  static __device__ __forceinline__ int swz_row(int row) { return ((row / 2) & 3) << 1; }
+  static __device__ __forceinline__ int swz_k(int k) {  // in chunks
+    if constexpr (EB == 2)
+      return (((k & 3) | (((k >> 3) & 3) << 2)) & (kUnits - 1)) << 1;
+    else
+      return (((k >> 2) & 3) & (kUnits - 1)) << 2;
   }
-  static __device__ __forceinline__ int swz_k(int k) {
-    return ((k & 3) | (((k >> 3) & 3) << 2)) & (kUnits - 1);
-  }
-  // place of this lane in load q: part, row or k row, chunk of eight elements
+  // place of this lane in load q: part, row or k row, chunk
   static __device__ __forceinline__ void place(int q, int wave, int lane, int& part, int& row, int& chunk) {
     const int b = (q * WAVES + wave) * 1024 + lane * 16;
     if constexpr (LAYOUT == kRowK) {
-      row = b / (BK * 2);
-      chunk = ((b / 16) % kChunks) ^ swz_row(row);
-      part = row / kPart;
-      row %= kPart;
+      row = b / 128;
+      chunk = ((b / 16) % 8) ^ swz_row(row);
+      part = 0;
     } else {
-      constexpr int kPartBytes = kPart * BK * 2;
-      part = b / kPartBytes;
-      const int w = b % kPartBytes;
-      row = w / (kPart * 2);
-      chunk = ((w / 16) % (kPart / 8)) ^ (swz_k(row) << 1);
+      part = b / (kPart * 128);
+      const int w = b % (kPart * 128);
+      row = w / kKRow;
+      chunk = ((w / 16) % (kKRow / 16)) ^ swz_k(row);
     }
   }
   // Byte offset of this lane's 16 bytes of load q from the part's origin at the step's k:
   // offset(kind(q)) + moved(q) rows of ld, the former in a register for each of kOffsets
-  // kinds. (Rows, or k rows 32 apart, have one permutation, and differ by the uniform part alone.)
-  static constexpr int kRows = LAYOUT == kRowK ? WAVES * 512 / BK : WAVES * 512 / kPart;  // of one load of all waves
-  static_assert(LAYOUT == kColK || (SUB == 1 && kRows % (512 / BK) == 0), "whole permutations a load");
+  // kinds. (Rows, or k rows a period apart, differ by the uniform part alone.)
+  static constexpr int kRows = LAYOUT == kRowK ? WAVES * 8 : WAVES * 1024 / kKRow;  // of one load of all waves
+  static_assert(LAYOUT == kColK || (SUB == 1 && kRows % 8 == 0), "whole permutations a load");
   static constexpr int kOffsets =
-      LAYOUT == kRowK || kRows >= 32 ? 1 : (32 / kRows < kLoads ? 32 / kRows : kLoads);
+      LAYOUT == kRowK || kRows >= kPeriod ? 1 : (kPeriod / kRows < kLoads ? kPeriod / kRows : kLoads);
   static constexpr __device__ int kind(int q) { return q % kOffsets; }
   static constexpr __device__ long moved(int q) {
-    return LAYOUT == kRowK ? q * kRows : (q * kRows) % BK / 32 * 32;
+    return LAYOUT == kRowK ? q * kRows : (q * kRows) % BK / kPeriod * kPeriod;
   }
   static __device__ __forceinline__ unsigned offset(int q, int wave, int lane, long ld, int rows_left) {
     int part, row, chunk;
     place(q, wave, lane, part, row, chunk);
     if constexpr (LAYOUT == kRowK) {
-      return (unsigned)(row * ld * 2 + chunk * 16);
+      return (unsigned)(row * ld * EB + chunk * 16);
     } else {
-      const int left = ((rows_left + 7) & ~7) - 8;
-      return (unsigned)(row * ld * 2 + min(chunk * 8, left) * 2);
+      const int left = (rows_left + VE - 1) / VE - 1;  // the last chunk of the row
+      return (unsigned)(row * ld * EB + min(chunk, left) * 16);
     }
   }
   // whether the lane's 16 bytes of load q lie at or past the end of k
   static __device__ __forceinline__ bool past(int q, int wave, int lane, int k_left) {
     int part, row, chunk;
     place(q, wave, lane, part, row, chunk);
-    return (LAYOUT == kRowK ? chunk * 8 : row) >= k_left;
+    return (LAYOUT == kRowK ? chunk * VE : row) >= k_left;
   }
   // or in a row past the operand's last (whose sums are not stored, whatever its tile row holds)
   static __device__ __forceinline__ bool outside(int q, int wave, int lane, int k_left, int rows_left) {
     int part, row, chunk;
     if constexpr (LAYOUT == kRowK) {
       place(0, wave, lane, part, row, chunk);
-      return chunk * 8 >= k_left || row >= rows_left - q * kRows;
+      return chunk * VE >= k_left || row >= rows_left - q * kRows;
     } else {
       place(q, wave, lane, part, row, chunk);
       return row >= k_left;
     }
   }
-  // the fragment of rows r0 .. r0 + 15 (of part `part`) and k kk * 32 .. + 31
+  // The fragment of rows r0 .. r0 + 15 (of part `part`) and half `kk` of the tile's k: lane
+  // (g, c) holds row c. 16 bits: k 8 g .. 8 g + 7 of the 32. 32 bits: k 4 g .. 4 g + 3 of the
+  // 16, of which element q is the operand of the q-th of four products.
   static __device__ __forceinline__ s8v frag(const char* tile, int part, int r0, int kk, int lane) {
     const int g = lane >> 4, c = lane & 15;
     if constexpr (LAYOUT == kRowK) {
-      const int row = part * kPart + r0 + c;
-      return *reinterpret_cast<const s8v*>(tile + row * (BK * 2) + (((kk * 4 + g) ^ swz_row(c)) * 16));
-    } else {
+      return *reinterpret_cast<const s8v*>(tile + (r0 + c) * 128 + (((kk * 4 + g) ^ swz_row(c)) * 16));
+    } else if constexpr (EB == 2) {
       const int k = kk * 32 + 8 * g + (c >> 2);
       const int s = (((c >> 2) | (g << 2)) & (kUnits - 1)) ^ (r0 / 16);
-      const char* p = tile + part * (kPart * BK * 2) + k * (kPart * 2) + s * 32 + (c & 3) * 8;
+      const char* p = tile + part * (kPart * 128) + k * kKRow + s * 32 + (c & 3) * 8;
       const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
-      const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * kPart * 2));
+      const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * kKRow));
       return s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    } else {
+      const char* p = tile + part * (kPart * 128) + (kk * 16 + 4 * g) * kKRow +
+                      (((g & (kUnits - 1)) ^ (r0 / 16)) * 64) + c * 4;
+      f4 v;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const float*>(p + q * kKRow);
+      return __builtin_bit_cast(s8v, v);
     }
   }
 };
 
-template <int KIND>
-__device__ __forceinline__ f4 mfma16(s8v a, s8v b, f4 c) {
-  if constexpr (KIND == kF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-  else
-    return mfma_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c);
+// acc[j] += the products of one row fragment and NJ column fragments (whose places are
+// exchanged: a lane then holds four consecutive columns of one row). fp32: the four products
+// of each j apart from each other, as one that waits for the last one's sum is issued late.
+template <int KIND, int NJ>
+__device__ __forceinline__ void multiply_row(f4 (&acc)[NJ], const s8v (&b)[NJ], s8v a) {
+  if constexpr (KIND == kF32) {
+    const f4 y = __builtin_bit_cast(f4, a);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] = mfma_f32(__builtin_bit_cast(f4, b[j])[q], y[q], acc[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if constexpr (KIND == kBf16)
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, b[j]), __builtin_bit_cast(bf8, a),
+                                                         acc[j], 0, 0, 0);
+      else
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, b[j]), __builtin_bit_cast(h8, a),
+                                                        acc[j], 0, 0, 0);
+    }
+  }
 }
 
-// Shape of a block's tile: BM rows by BN columns by BK of k, WM by WN waves.
-template <int BM_, int BN_, int BK_, int WM_, int WN_>
+// Shape of a block's tile: BM rows by BN columns, WM by WN waves.
+template <int BM_, int BN_, int WM_, int WN_>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
 };
 
 // EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad.
@@ -364,20 +377,20 @@ struct Shape {
 // loaded before the epilogue of the last, so that they arrive under it. Two stages of LDS.
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
-  constexpr int P = pieces<KIND>(), SUB = EPI == kEpiGate ? 2 : 1;
+  constexpr int SUB = EPI == kEpiGate ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
   constexpr int WAVES = S::WM * S::WN, TM = S::BM / S::WM, TN = S::BN / S::WN;
   constexpr int MI = TM / 16, NJ = TN / 16;
-  using TA = TileOf<LA, S::BM, S::BK, 1, WAVES>;
-  using TB = TileOf<LB, S::BN, S::BK, SUB, WAVES>;
-  constexpr int kStage = P * (TA::kBytes + TB::kBytes);
+  using TA = TileOf<LA, S::BM, EB, 1, WAVES>;
+  using TB = TileOf<LB, S::BN, EB, SUB, WAVES>;
+  constexpr int kStage = TA::kBytes + TB::kBytes;
   __shared__ __align__(1024) char lds[2 * kStage];
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)lds);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / S::WN, wn = wave % S::WN, g = lane >> 4, c = lane & 15;
-  const int K = p.K, per_seg = (K + S::BK - 1) / S::BK, steps = per_seg * p.segs;
-  const long lda2 = 2 * p.a[0].ld, ldb2 = 2 * p.b[0].ld, pla = 2 * p.a[0].plane, plb = 2 * p.b[0].plane;
-  const long da = LA == kRowK ? 2 * S::BK : S::BK * lda2, db = LB == kRowK ? 2 * S::BK : S::BK * ldb2;
+  const int K = p.K, per_seg = (K + BK - 1) / BK, steps = per_seg * p.segs;
+  const long lda = EB * p.a[0].ld, ldb = EB * p.b[0].ld;  // bytes
+  const long da = LA == kRowK ? 128 : BK * lda, db = LB == kRowK ? 128 : BK * ldb;
 
   // ---- a tile and its steps ----
   struct Item {
@@ -419,7 +432,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
     for (int l = 0; l < TA::kOffsets; ++l) oa[l] = TA::offset(l, wave, lane, p.a[0].ld, p.M - it.m0);
 #pragma unroll
     for (int l = 0; l < TB::kOffsets; ++l) ob[l] = TB::offset(l, wave, lane, p.b[0].ld, p.N - it.n0);
-    const long ra = LA == kRowK ? it.m0 * lda2 : 2l * it.m0, rb = LB == kRowK ? it.n0 * ldb2 : 2l * it.n0;
+    const long ra = LA == kRowK ? it.m0 * lda : (long)EB * it.m0, rb = LB == kRowK ? it.n0 * ldb : (long)EB * it.n0;
     const bool pair = SUB == 2 || p.segs == 2;
     a0 = reinterpret_cast<const char*>(p.a[0].p) + ra;
     a1 = reinterpret_cast<const char*>(p.a[1].p) + ra;
@@ -437,55 +450,40 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
     const bool seg = t >= per_seg;
     const int step = seg ? t - per_seg : t;
     return Cursor{(seg ? a1 : a0) + step * da, (SUB == 1 && seg ? b1 : b0) + step * db, b1 + step * db,
-                  t < it.t1 ? K - step * S::BK : 0};
+                  t < it.t1 ? K - step * BK : 0};
   };
   // One of a step's kLoads loads of this wave, by the lanes whose row and k are before the ends;
   // the 16 bytes past the end of k are zeroed by fill() (in the last step of a segment).
-  constexpr int kLoads = P * (TA::kLoads + TB::kLoads);
-  auto slot = [&](int q) {
-    if (q < P * TA::kLoads) return q / TA::kLoads * TA::kBytes + (q % TA::kLoads * WAVES + wave) * 1024;
-    const int r = q - P * TA::kLoads;
-    return P * TA::kBytes + r / TB::kLoads * TB::kBytes + (r % TB::kLoads * WAVES + wave) * 1024;
-  };
-  auto past = [&](int q, int k_left) {
-    return q < P * TA::kLoads ? TA::past(q % TA::kLoads, wave, lane, k_left)
-                              : TB::past((q - P * TA::kLoads) % TB::kLoads, wave, lane, k_left);
-  };
-  auto issue = [&](int q, const Cursor& u, int to, bool whole = false) {
-    if (q < P * TA::kLoads) {
-      const int l = q % TA::kLoads;
-      if (!whole && TA::outside(l, wave, lane, u.k_left, p.M - it.m0)) return;
-      load_to_lds(u.pa + q / TA::kLoads * pla + TA::moved(l) * lda2, oa[TA::kind(l)], lds0 + to + slot(q));
+  constexpr int kLoads = TA::kLoads + TB::kLoads;
+  auto slot = [&](int q) { return (q * WAVES + wave) * 1024; };
+  auto issue = [&](int q, const Cursor& u, int to) {
+    if (q < TA::kLoads) {
+      if (TA::outside(q, wave, lane, u.k_left, p.M - it.m0)) return;
+      load_to_lds(u.pa + TA::moved(q) * lda, oa[TA::kind(q)], lds0 + to + slot(q));
     } else {
-      const int r = q - P * TA::kLoads, s = r / TB::kLoads, l = r % TB::kLoads;
-      if (!whole && TB::outside(l, wave, lane, u.k_left, p.N - it.n0)) return;
+      const int l = q - TA::kLoads;
+      if (TB::outside(l, wave, lane, u.k_left, p.N - it.n0)) return;
       // (every lane of one load lies in one part: a part is whole loads)
-      const bool part = SUB == 2 && (l * WAVES + wave) * 1024 >= TB::kBytes / 2;
-      load_to_lds((part ? u.pb_second : u.pb) + s * plb + TB::moved(l) * ldb2, ob[TB::kind(l)], lds0 + to + slot(q));
+      const bool part = SUB == 2 && slot(l) >= TB::kBytes / 2;
+      load_to_lds((part ? u.pb_second : u.pb) + TB::moved(l) * ldb, ob[TB::kind(l)], lds0 + to + slot(q));
     }
   };
   auto fill = [&](const Cursor& u, int to) {
-    if (u.k_left <= 0 || u.k_left >= S::BK) return;
+    if (u.k_left <= 0 || u.k_left >= BK) return;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q)
-      if (past(q, u.k_left)) *reinterpret_cast<f4*>(lds + to + slot(q) + lane * 16) = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (q < TA::kLoads ? TA::past(q, wave, lane, u.k_left) : TB::past(q - TA::kLoads, wave, lane, u.k_left))
+        *reinterpret_cast<f4*>(lds + to + slot(q) + lane * 16) = f4{0.0f, 0.0f, 0.0f, 0.0f};
   };
   auto load = [&](int t, int to) {
     const Cursor u = cursor(t);
-    if (u.k_left >= S::BK && it.m0 + S::BM <= p.M && it.n0 + S::BN / SUB <= p.N) {
 #pragma unroll
-      for (int q = 0; q < kLoads; ++q) issue(q, u, to, true);
-    } else {
-#pragma unroll
-      for (int q = 0; q < kLoads; ++q) issue(q, u, to);
-      fill(u, to);
-    }
+    for (int q = 0; q < kLoads; ++q) issue(q, u, to);
+    fill(u, to);
   };
-  auto frag_a = [&](const char* tile, int s, int i, int kk) {
-    return TA::frag(tile + s * TA::kBytes, 0, wm * TM + i * 16, kk, lane);
-  };
-  auto frag_b = [&](const char* tile, int s, int j, int kk) {
-    return TB::frag(tile + P * TA::kBytes + s * TB::kBytes, SUB == 2 ? j / (NJ / 2) : 0,
+  auto frag_a = [&](const char* tile, int i, int kk) { return TA::frag(tile, 0, wm * TM + i * 16, kk, lane); };
+  auto frag_b = [&](const char* tile, int j, int kk) {
+    return TB::frag(tile + TA::kBytes, SUB == 2 ? j / (NJ / 2) : 0,
                     SUB == 2 ? wn * (TN / 2) + (j % (NJ / 2)) * 16 : wn * TN + j * 16, kk, lane);
   };
 
@@ -499,87 +497,49 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     tile_landed();
-    if constexpr (P == 1) {
-      // Two halves of 32 of k a step: a half's fragments are multiplied while the next half's
-      // are read. A row's fragments are read again, for the next half, as soon as its products are
-      // issued, and so have the other rows' products of time to arrive; the columns' fragments,
-      // which every row needs, and the last rows', whose registers come free too late, have two sets of
-      // registers. (Two sets of all spilled.) A step's loads go into the tile that all waves
-      // have just read, once the step before it has landed: one barrier a step, in its middle.
-      static_assert(S::BK == 64, "a step is two halves");
-      constexpr int LATE = MI >= 4 ? 2 : 0, EARLY = MI - LATE;
-      s8v fa[EARLY], fl[2][LATE + 1], fb[2][NJ];
-      auto half = [&](auto h_, const char* next, bool loads, const Cursor& u, int to) {
-        constexpr int h = decltype(h_)::value, o = h ^ 1;
+    // Two halves of 64 bytes of k a step: a half's fragments are multiplied while the next half's
+    // are read. A row's fragments are read again, for the next half, as soon as its products are
+    // issued, and so have the other rows' products of time to arrive; the columns' fragments,
+    // which every row needs, and the last rows', whose registers come free too late, have two sets of
+    // registers. (Two sets of all spilled.) A step's loads go into the tile that all waves
+    // have just read, once the step before it has landed: one barrier a step, in its middle.
+    constexpr int LATE = MI >= 4 ? 2 : 0, EARLY = MI - LATE;
+    s8v fa[EARLY], fl[2][LATE + 1], fb[2][NJ];
+    auto half = [&](auto h_, const char* next, bool loads, const Cursor& u, int to) {
+      constexpr int h = decltype(h_)::value, o = h ^ 1;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[o][j] = frag_b(next, 0, j, o);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < NJ; ++j) fb[o][j] = frag_b(next, j, o);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          // the operands change places: a lane then holds four consecutive columns of one row
+      for (int i = 0; i < MI; ++i) {
+        multiply_row<KIND, NJ>(acc[i], fb[h], i < EARLY ? fa[i < EARLY ? i : 0] : fl[h][i < EARLY ? 0 : i - EARLY]);
+        if (i < EARLY) fa[i < EARLY ? i : 0] = frag_a(next, i, o);
+        if (i < EARLY && i >= EARLY - LATE) fl[o][i - EARLY + LATE] = frag_a(next, i + LATE, o);
+        if (loads) {
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            acc[i][j] = mfma16<KIND>(fb[h][j], i < EARLY ? fa[i < EARLY ? i : 0] : fl[h][i < EARLY ? 0 : i - EARLY],
-                                     acc[i][j]);
-          if (i < EARLY) fa[i < EARLY ? i : 0] = frag_a(next, 0, i, o);
-          if (i < EARLY && i >= EARLY - LATE) fl[o][i - EARLY + LATE] = frag_a(next, 0, i + LATE, o);
-          if (loads) {
-#pragma unroll
-            for (int q = 0; q < kLoads; ++q)
-              if (q * MI / kLoads == i) issue(q, u, to);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+          for (int q = 0; q < kLoads; ++q)
+            if (q * MI / kLoads == i) issue(q, u, to);
         }
-        // the reads have landed (a compiler-placed wait would come after the next reads and be for those too)
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
         __builtin_amdgcn_sched_barrier(0);
-      };
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) fb[0][j] = frag_b(lds, 0, j, 0);
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-        (i < EARLY ? fa[i < EARLY ? i : 0] : fl[0][i < EARLY ? 0 : i - EARLY]) = frag_a(lds, 0, i, 0);
+      }
+      // the reads have landed (a compiler-placed wait would come after the next reads and be for those too)
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
       __builtin_amdgcn_sched_barrier(0);
-      for (int t = it.t0; t < it.t1; ++t) {
-        const int cur = ((t - it.t0) & 1) * kStage;
-        const Cursor u = cursor(t + 2);
-        half(std::integral_constant<int, 0>{}, lds + cur, false, u, cur);
-        tile_landed();
-        fill(u, cur);
-        half(std::integral_constant<int, 1>{}, lds + (kStage - cur), true, u, cur);
-      }
-    } else {
-      // (three pieces: a row's products take six times as long, and the compiler's order of
-      // reads and products within a step is as fast as the above, with fewer registers)
-      for (int t = it.t0; t < it.t1; ++t) {
-        const char* cur = lds + ((t - it.t0) & 1) * kStage;
-        if (t > it.t0) {
-          tile_landed();  // this step's loads are in LDS, and the last step's tile is read
-          load(t + 1, ((t + 1 - it.t0) & 1) * kStage);
-        }
+    };
 #pragma unroll
-        for (int kk = 0; kk < S::BK / 32; ++kk) {
-          // the pieces' products that reach 2^-18 of the leading one, in the order in which
-          // the pieces are read
-          constexpr int kPairs = 6, kRow[kPairs] = {0, 0, 1, 1, 0, 2}, kCol[kPairs] = {0, 1, 0, 1, 2, 0};
-          s8v b[P][NJ];
+    for (int j = 0; j < NJ; ++j) fb[0][j] = frag_b(lds, j, 0);
 #pragma unroll
-          for (int s = 0; s < P; ++s)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) b[s][j] = frag_b(cur, s, j, kk);
-#pragma unroll
-          for (int i = 0; i < MI; ++i) {
-            s8v a[P];
-#pragma unroll
-            for (int s = 0; s < P; ++s) a[s] = frag_a(cur, s, i, kk);
-#pragma unroll
-            for (int q = 0; q < kPairs; ++q)
-#pragma unroll
-              for (int j = 0; j < NJ; ++j) acc[i][j] = mfma16<KIND>(b[kCol[q]][j], a[kRow[q]], acc[i][j]);
-          }
-        }
-      }
+    for (int i = 0; i < MI; ++i)
+      (i < EARLY ? fa[i < EARLY ? i : 0] : fl[0][i < EARLY ? 0 : i - EARLY]) = frag_a(lds, i, 0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+    for (int t = it.t0; t < it.t1; ++t) {
+      const int cur = ((t - it.t0) & 1) * kStage;
+      const Cursor u = cursor(t + 2);
+      half(std::integral_constant<int, 0>{}, lds + cur, false, u, cur);
+      tile_landed();
+      fill(u, cur);
+      half(std::integral_constant<int, 1>{}, lds + (kStage - cur), true, u, cur);
     }
 
     // the next item's first loads, then this one's epilogue
@@ -629,7 +589,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
               put_row4<KIND, false>(out, at + j * 16, acc[i][j], p.N - n0 - j * 16);
       }
     } else if constexpr (EPI == kEpiGate) {
-      unsigned short* h = p.epi.h + m0 * p.epi.ldh + n0;
+      long h = m0 * p.epi.ldh + n0;
       float* kept = p.epi.saved ? p.epi.saved + 2 * ((long)m0 * p.N + n0) : nullptr;
       const long hrow = 16 * p.epi.ldh, krow = p.epi.saved ? 32l * p.N : 0;
       if (inside && (p.N & 1) == 0) {
@@ -637,7 +597,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
         for (int i = 0; i < MI; ++i, h += hrow, kept += krow)
 #pragma unroll
           for (int j = 0; j < NJ / SUB; ++j)
-            put_gate<KIND, true>(h + j * 16, p.epi.plane_h, p.epi.saved ? kept + j * 32 : nullptr, p.act, 4, acc[i][j],
+            put_gate<KIND, true>(p.epi.h, h + j * 16, p.epi.saved ? kept + j * 32 : nullptr, p.act, 4, acc[i][j],
                                  acc[i][j + NJ / 2]);
       } else {
 #pragma unroll
@@ -645,7 +605,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 #pragma unroll
           for (int j = 0; j < NJ / SUB; ++j)
             if (m0 + i * 16 < p.M && n0 + j * 16 < p.cols)
-              put_gate<KIND, false>(h + j * 16, p.epi.plane_h, p.epi.saved ? kept + j * 32 : nullptr, p.act,
+              put_gate<KIND, false>(p.epi.h, h + j * 16, p.epi.saved ? kept + j * 32 : nullptr, p.act,
                                     p.N - n0 - j * 16, acc[i][j], acc[i][j + NJ / 2]);
       }
     } else {
@@ -740,7 +700,7 @@ __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
   const int mat = EPI == kEpiGate ? 0 : (int)(row / p.M);
   const long m = EPI == kEpiGate ? row : row % p.M;
   if constexpr (EPI == kEpiGate)
-    put_gate<KIND, false>(p.epi.h + m * p.epi.ldh + n, p.epi.plane_h,
+    put_gate<KIND, false>(p.epi.h, m * p.epi.ldh + n,
                           p.epi.saved ? p.epi.saved + 2 * (m * p.N + n) : nullptr, p.act, p.N - n, v, w);
   else if constexpr (EPI == kEpiGateGrad)
     put_gate_grad<KIND>(p.epi, m * p.epi.ldh + n,

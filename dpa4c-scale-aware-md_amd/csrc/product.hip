@@ -7,22 +7,12 @@ namespace dpamd {
 
 namespace {
 
-// 16-bit kinds: 256 x 256 x 64 with eight waves of 128 x 64 (128 KB of LDS, one block
-// a compute unit) and 128 x 128 x 64 with four of 64 x 64 (64 KB, two). fp32, with
-// three planes to stage: 256 x 128 x 32 with eight of 64 x 64 (144 KB) and 128 x 64 x 32 with
-// four of 64 x 32 (72 KB, two). For few rows 64 x 128 x 64 (48 KB, three), fp32 64 x 64 x 32.
-template <int KIND>
-struct Shapes {
-  using Big = Shape<256, 256, 64, 2, 4>;
-  using Small = Shape<128, 128, 64, 2, 2>;
-  using Thin = Shape<64, 128, 64, 1, 4>;
-};
-template <>
-struct Shapes<kF32> {
-  using Big = Shape<256, 128, 32, 4, 2>;
-  using Small = Shape<128, 64, 32, 2, 2>;
-  using Thin = Shape<64, 64, 32, 2, 2>;
-};
+// 256 x 256 with eight waves of 128 x 64 (128 KB of LDS, one block a compute unit), 128 x 128
+// with four of 64 x 64 (64 KB, two), and for few rows 64 x 128 with four of 64 x 32 (48 KB,
+// three). fp32 has the two smaller ones.
+using Big = Shape<256, 256, 2, 4>;
+using Small = Shape<128, 128, 2, 2>;
+using Thin = Shape<64, 128, 1, 4>;
 
 template <int KIND, int LA, int LB, int EPI, class S>
 void launch(hipStream_t st, ProductArgs& p) {
@@ -61,12 +51,12 @@ void launch_kind(hipStream_t st, ProductKind what, ProductArgs& p) {
 
 template <int KIND>
 void launch_product(hipStream_t st, ProductKind what, int shape, ProductArgs& p) {
-  if (shape == 0)
-    launch_kind<KIND, typename Shapes<KIND>::Big>(st, what, p);
-  else if (shape == 1)
-    launch_kind<KIND, typename Shapes<KIND>::Small>(st, what, p);
+  if constexpr (KIND != kF32)
+    if (shape == 0) return launch_kind<KIND, Big>(st, what, p);
+  if (shape <= 1)
+    launch_kind<KIND, Small>(st, what, p);
   else
-    launch_kind<KIND, typename Shapes<KIND>::Thin>(st, what, p);
+    launch_kind<KIND, Thin>(st, what, p);
 }
 
 template void launch_product<ELEM_KIND>(hipStream_t, ProductKind, int, ProductArgs&);
