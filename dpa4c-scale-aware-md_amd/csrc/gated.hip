@@ -1,5 +1,5 @@
-// The gated block's products: how each is cut into tiles and slices, and the operand
-// form of what is not in it already.
+// The gated block's products: how each is cut into tiles and slices, and the copies of
+// matrices whose rows are not whole aligned 16-byte chunks.
 #include <algorithm>
 
 #include "product.h"

@@ -123,14 +123,11 @@ __device__ __forceinline__ unsigned key_of(const int* ids, const unsigned* keys,
   return id >= 0 && id < vocab ? (unsigned)id : (unsigned)vocab;
 }
 
-// counts[digit][tile]; also clears `zeros` ints
+// counts[digit][tile]
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const int* ids, const unsigned* keys, long n, int vocab,
-                                                             int shift, int tiles, int* counts, int* zero,
-                                                             long zeros) {
+                                                             int shift, int tiles, int* counts) {
   __shared__ int hist[kDigits];
   hist[threadIdx.x] = 0;
-  for (long i = (long)blockIdx.x * kSortThreads + threadIdx.x; i < zeros; i += (long)gridDim.x * kSortThreads)
-    zero[i] = 0;
   __syncthreads();
   const long base = (long)blockIdx.x * kSortTile;
 #pragma unroll
@@ -221,17 +218,113 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, con
 // ---- sums of runs ---------------------------------------------------------------------
 constexpr int kWindow = 32;     // sorted positions of one window
 constexpr int kShort = 64;      // runs up to this length are summed by their table row itself
+// Rows up to which one block sorts them all. Random ids among 30,000, width 1024, us, one block /
+// tiles: 4,000 29 / 44, 16,000 57 / 47; they cross near 10,000.
+constexpr int kOneMost = 8192;
 constexpr int kScanTiles = 64;  // tiles up to which each block of the sort forms its starts itself
 
-// run[2 v], run[2 v + 1]: first position and end of id v's run (both 0 where there is none)
-__global__ __launch_bounds__(256) void k_runs(int n, int vocab, const unsigned* __restrict__ keys,
-                                              int* __restrict__ run) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+// run[2 v], run[2 v + 1]: first position and end of id v's run. Those of ids without rows are
+// not written (run_of() tells by the key at the first position).
+__device__ __forceinline__ void put_run(const unsigned* keys, int i, int n, int vocab, int* run) {
   const unsigned v = keys[i];
   if (v >= (unsigned)vocab) return;
   if (i == 0 || keys[i - 1] != v) run[2 * (long)v] = i;
   if (i == n - 1 || keys[i + 1] != v) run[2 * (long)v + 1] = i + 1;
+}
+__device__ __forceinline__ int2 run_of(const unsigned* keys, const int* run, int n, long v) {
+  const int lo = run[2 * v];
+  if ((unsigned)lo >= (unsigned)n || keys[lo] != (unsigned)v) return int2{0, 0};
+  return int2{lo, run[2 * v + 1]};
+}
+__global__ __launch_bounds__(256) void k_runs(int n, int vocab, const unsigned* __restrict__ keys,
+                                              int* __restrict__ run) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) put_run(keys, i, n, vocab, run);
+}
+
+// The whole sort and the runs in one block, for up to 1024 ITEMS rows (a launch costs more than
+// the work of a pass): as k_sort_place, with the rows in LDS and sixteen waves.
+constexpr int kOneWaves = 16, kOneThreads = kOneWaves * kWave;
+template <int ITEMS>
+__global__ __launch_bounds__(kOneThreads) void k_sort_one(const int* __restrict__ ids, int n, int vocab, int passes,
+                                                          unsigned* __restrict__ keys_out, int* __restrict__ rows_out,
+                                                          int* __restrict__ run) {
+  __shared__ unsigned keys[kOneThreads * ITEMS];
+  __shared__ unsigned short rows[kOneThreads * ITEMS];
+  __shared__ int count[kOneWaves][kDigits];
+  __shared__ int totals[kDigits / kWave];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  for (int i = threadIdx.x; i < n; i += kOneThreads) {
+    keys[i] = key_of(ids, nullptr, i, vocab);
+    rows[i] = (unsigned short)i;
+  }
+  for (int p = 0; p < passes; ++p) {
+    for (int k = threadIdx.x; k < kOneWaves * kDigits; k += kOneThreads) count[k / kDigits][k % kDigits] = 0;
+    __syncthreads();
+    unsigned key[ITEMS];
+    unsigned short row[ITEMS];
+    int rank[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int i = (wave * ITEMS + k) * kWave + lane;
+      const bool in = i < n;
+      key[k] = in ? keys[i] : 0u;
+      row[k] = in ? rows[i] : (unsigned short)0;
+      rank[k] = 0;
+      const int digit = (key[k] >> (kBits * p)) & (kDigits - 1);
+      unsigned long long same = __ballot(in);
+      if (!same) continue;  // (of the whole wave)
+#pragma unroll
+      for (int b = 0; b < kBits; ++b) {
+        const bool bit = (digit >> b) & 1;
+        const unsigned long long set = __ballot(bit);
+        same &= bit ? set : ~set;
+      }
+      const int below = __popcll(same & ((1ull << lane) - 1));
+      if (in) rank[k] = count[wave][digit] + below;
+      wave_lds_sync();
+      if (in && below == 0) count[wave][digit] += __popcll(same);
+      wave_lds_sync();
+    }
+    __syncthreads();
+    int total = 0, sum = 0;
+    if (threadIdx.x < kDigits) {
+      for (int w = 0; w < kOneWaves; ++w) total += count[w][threadIdx.x];
+      sum = total;
+#pragma unroll
+      for (int off = 1; off < kWave; off *= 2) {
+        const int v = __shfl_up(sum, off, kWave);
+        if (lane >= off) sum += v;
+      }
+      if (lane == kWave - 1) totals[wave] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+      int at = sum - total;
+      for (int w = 0; w < wave; ++w) at += totals[w];
+      for (int w = 0; w < kOneWaves; ++w) {
+        const int c = count[w][threadIdx.x];
+        count[w][threadIdx.x] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int i = (wave * ITEMS + k) * kWave + lane;
+      if (i < n) {
+        const int to = count[wave][(key[k] >> (kBits * p)) & (kDigits - 1)] + rank[k];
+        keys[to] = key[k];
+        rows[to] = row[k];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < n; i += kOneThreads) {
+    keys_out[i] = keys[i];
+    rows_out[i] = rows[i];
+    put_run(keys, i, n, vocab, run);
+  }
 }
 
 // acc += rows[from .. to) of this lane's chunk, four loads under way
@@ -272,7 +365,7 @@ __global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chun
     for (int part = 0; part < 2; ++part) {
       const unsigned v = part ? last : first;
       if (v >= (unsigned)vocab || (part && last == first)) continue;
-      const int lo = run[2 * (long)v], hi = run[2 * (long)v + 1];
+      const int lo = run[2 * (long)v], hi = run[2 * (long)v + 1];  // (v has rows)
       if (hi - lo <= kShort) continue;
       for (int c = lane; c < chunks; c += 64) {
         float acc[E] = {};
@@ -285,33 +378,57 @@ __global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chun
   }
 }
 
-// One wave a table row.
+// One wave `each` table rows, whose runs its lanes look up together: eight of a large table, most of
+// whose rows have none (a wave a row then spends its time on two loads that wait for each other:
+// 45 us, now 33, of 32,768 tokens among 50,000), one of a small table, whose rows are long.
 template <int KIND, int E>
-__global__ __launch_bounds__(256) void k_grad_rows(int vocab, int chunks, const int* __restrict__ rows,
-                                                   const int* __restrict__ run,
+__global__ __launch_bounds__(256) void k_grad_rows(int n, int vocab, int chunks, int each,
+                                                   const unsigned* __restrict__ keys,
+                                                   const int* __restrict__ rows, const int* __restrict__ run,
                                                    const typename ElemOf<KIND>::T* __restrict__ dout, long ld,
                                                    const float* __restrict__ partial, float scale,
                                                    typename ElemOf<KIND>::T* __restrict__ dtable, long ld_table) {
   using C = Chunk<KIND, E>;
   const int lane = threadIdx.x & 63;
-  for (long v = (long)blockIdx.x * 4 + threadIdx.x / 64; v < vocab; v += (long)gridDim.x * 4) {
-    const int lo = run[2 * v], hi = run[2 * v + 1];
-    for (int c = lane; c < chunks; c += 64) {
-      float acc[E] = {};
-      if (hi - lo <= kShort) {
-        add_rows<KIND, E>(acc, lo, hi, rows, dout, ld, c);
-      } else {
-        const int w0 = lo / kWindow, w1 = (hi - 1) / kWindow;
-        for (int w = w0; w <= w1; ++w) {
-          const float* p = partial + ((2 * (long)w + (lo > w * kWindow)) * chunks + c) * E;
+  const long stride = (long)gridDim.x * 4 * each;
+  for (long v0 = ((long)blockIdx.x * 4 + threadIdx.x / 64) * each; v0 < vocab; v0 += stride) {
+    const int2 mine =
+        lane < each && v0 + lane < vocab ? run_of(keys, run, n, v0 + lane) : int2{0, 0};
+    for (int k = 0; k < each && v0 + k < vocab; ++k) {
+      const int lo = __builtin_amdgcn_readlane(mine.x, k), hi = __builtin_amdgcn_readlane(mine.y, k);
+      for (int c = lane; c < chunks; c += 64) {
+        float acc[E] = {};
+        if (hi - lo <= kShort) {
+          add_rows<KIND, E>(acc, lo, hi, rows, dout, ld, c);
+        } else {
+          const int w0 = lo / kWindow, w1 = (hi - 1) / kWindow;
+          // the first window's part is the second of that window where the run starts inside it
+          const long step = 2 * (long)chunks * E;
+          const float* p = partial + ((2 * (long)w0 + (lo > w0 * kWindow)) * chunks + c) * E;
 #pragma unroll
-          for (int k = 0; k < E; ++k) acc[k] += p[k];
+          for (int e = 0; e < E; ++e) acc[e] += p[e];
+          p = partial + (2 * (long)(w0 + 1) * chunks + c) * E;
+          int w = w0 + 1;
+          for (; w + 8 <= w1 + 1; w += 8, p += 8 * step) {
+            float y[8][E];  // (eight loads under way: a frequent token's run has a hundred windows)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+              for (int e = 0; e < E; ++e) y[q][e] = p[q * step + e];
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[e] += y[q][e];
+          }
+          for (; w <= w1; ++w, p += step)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += p[e];
         }
-      }
-      C o;
+        C o;
 #pragma unroll
-      for (int k = 0; k < E; ++k) o.v[k] = from_f32<KIND>(acc[k] * scale);
-      *reinterpret_cast<C*>(dtable + v * ld_table + (long)c * E) = o;
+        for (int e = 0; e < E; ++e) o.v[e] = from_f32<KIND>(acc[e] * scale);
+        *reinterpret_cast<C*>(dtable + (v0 + k) * ld_table + (long)c * E) = o;
+      }
     }
   }
 }
@@ -440,6 +557,28 @@ GradPlan grad_plan(long n, int vocab, int width, int chunks) {
 // a grid of `waves` waves in blocks of four, striding where there are more than a launch takes
 dim3 wave_blocks(long waves) { return dim3((unsigned)std::min((waves + 3) / 4, 1L << 20)); }
 
+// The rows sorted by id and the ids' runs, in launches over tiles.
+void sort_rows(hipStream_t st, const GradPlan& g, long n, int vocab, const int* ids, unsigned* const* keys,
+               int* const* rows, int* run, char* ws) {
+  int* counts = reinterpret_cast<int*>(ws + g.counts);
+  int* starts = g.tiles > kScanTiles ? reinterpret_cast<int*>(ws + g.starts) : nullptr;
+  const int m = kDigits * g.tiles;
+  for (int p = 0; p < g.passes; ++p) {
+    const unsigned* kin = p ? keys[(p + 1) & 1] : nullptr;
+    const int* rin = p ? rows[(p + 1) & 1] : nullptr;
+    hipLaunchKernelGGL(k_sort_count, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, n, vocab, kBits * p, g.tiles,
+                       counts);
+    DPAMD_LAUNCH_CHECK();
+    if (starts) exclusive_scan_int(st, counts, starts, m, ws + g.scan, scan_temp_bytes(m));
+    hipLaunchKernelGGL(k_sort_place, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, rin, n, vocab, kBits * p,
+                       g.tiles, starts, counts, keys[p & 1], rows[p & 1]);
+    DPAMD_LAUNCH_CHECK();
+  }
+  hipLaunchKernelGGL(k_runs, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (int)n, vocab,
+                     keys[(g.passes - 1) & 1], run);
+  DPAMD_LAUNCH_CHECK();
+}
+
 template <int KIND, int E>
 void launch_grad(hipStream_t st, long n, int vocab, int width, const int* ids, const void* dout_, long ld, float scale,
                  void* dtable_, long ld_table, char* ws) {
@@ -465,29 +604,24 @@ void launch_grad(hipStream_t st, long n, int vocab, int width, const int* ids, c
   unsigned* keys[2] = {reinterpret_cast<unsigned*>(ws + g.keys[0]), reinterpret_cast<unsigned*>(ws + g.keys[1])};
   int* rows[2] = {reinterpret_cast<int*>(ws + g.rows[0]), reinterpret_cast<int*>(ws + g.rows[1])};
   int* run = reinterpret_cast<int*>(ws + g.run);
-  int* counts = reinterpret_cast<int*>(ws + g.counts);
-  int* starts = g.tiles > kScanTiles ? reinterpret_cast<int*>(ws + g.starts) : nullptr;
-  const int m = kDigits * g.tiles;
-  for (int p = 0; p < g.passes; ++p) {
-    const unsigned* kin = p ? keys[(p + 1) & 1] : nullptr;
-    const int* rin = p ? rows[(p + 1) & 1] : nullptr;
-    hipLaunchKernelGGL(k_sort_count, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, n, vocab, kBits * p, g.tiles,
-                       counts, run, p ? 0 : 2 * (long)vocab);
-    DPAMD_LAUNCH_CHECK();
-    if (starts) exclusive_scan_int(st, counts, starts, m, ws + g.scan, scan_temp_bytes(m));
-    hipLaunchKernelGGL(k_sort_place, dim3(g.tiles), dim3(kSortThreads), 0, st, ids, kin, rin, n, vocab, kBits * p,
-                       g.tiles, starts, counts, keys[p & 1], rows[p & 1]);
-    DPAMD_LAUNCH_CHECK();
-  }
   const unsigned* key = keys[(g.passes - 1) & 1];
   const int* row = rows[(g.passes - 1) & 1];
-  hipLaunchKernelGGL(k_runs, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (int)n, vocab, key, run);
-  DPAMD_LAUNCH_CHECK();
-  hipLaunchKernelGGL((k_grad_windows<KIND, E>), wave_blocks((n + kWindow - 1) / kWindow), dim3(256), 0, st, (int)n,
-                     vocab, chunks, key, row, run, dout, ld, partial);
-  DPAMD_LAUNCH_CHECK();
-  hipLaunchKernelGGL((k_grad_rows<KIND, E>), wave_blocks(vocab), dim3(256), 0, st, vocab, chunks, row, run, dout, ld,
-                     partial, scale, dtable, ld_table);
+  if (n <= kOneMost) {
+    auto* kernel = n <= kOneThreads ? k_sort_one<1> : n <= 4 * kOneThreads ? k_sort_one<4> : k_sort_one<8>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(kOneThreads), 0, st, ids, (int)n, vocab, g.passes,
+                       keys[(g.passes - 1) & 1], rows[(g.passes - 1) & 1], run);
+    DPAMD_LAUNCH_CHECK();
+  } else {
+    sort_rows(st, g, n, vocab, ids, keys, rows, run, ws);
+  }
+  if (n > kShort) {  // (else no run is long)
+    hipLaunchKernelGGL((k_grad_windows<KIND, E>), wave_blocks((n + kWindow - 1) / kWindow), dim3(256), 0, st, (int)n,
+                       vocab, chunks, key, row, run, dout, ld, partial);
+    DPAMD_LAUNCH_CHECK();
+  }
+  const int each = vocab >= 16384 ? 8 : 1;
+  hipLaunchKernelGGL((k_grad_rows<KIND, E>), wave_blocks((vocab + each - 1) / each), dim3(256), 0, st, (int)n, vocab,
+                     chunks, each, key, row, run, dout, ld, partial, scale, dtable, ld_table);
   DPAMD_LAUNCH_CHECK();
 }
 

@@ -78,9 +78,8 @@ __device__ __forceinline__ void put_row4(void* out, long at, const f4& v, int co
 // The activation a(g) and its derivative: tanh, silu g s(g), gelu g Phi(g), on the hardware's
 // base-2 exponential and reciprocal (about 1 ulp each), to about 2e-7 of max(1, |g|). Phi
 // from erfc(z) = exp(-z^2) (a1 t + .. + a5 t^5), t = 1 / (1 + 0.3275911 z) (Abramowitz and
-// Stegun 7.1.26: 1.5e-7), which shares its exponential with the derivative. With the
-// library's expf, tanhf, erff and a division the epilogues below issued about four times the
-// instructions, and 8192 rows of 2048-8192-2048 took the forward 823 us (now 709) and dg, du 2031 (now 476).
+// Stegun 7.1.26: 1.5e-7), which shares its exponential with the derivative. With the library's
+// expf, tanhf, erff and a division the epilogues below issued about four times the instructions.
 template <int ACT>
 __device__ __forceinline__ void activate(float g, float& a, float& da) {
   constexpr float kLog2e = 1.4426950408889634f;
@@ -210,7 +209,7 @@ typedef __attribute__((address_space(3))) s4v lds_s4;
 // (base and lds are wave-uniform; tile_landed() is the wait). Written as an instruction,
 // which has no register result, because the compiler waits for every such load that it
 // knows of before any transposing LDS read, as it can not tell that they are of different tiles:
-// with the builtin each row of fragments waited for the loads issued just before it.
+// with the builtin each row of k-strided fragments waited for the loads issued just before it.
 // (m0 is a register that a statement may not name as changed; nothing else in these kernels uses it.)
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned offset, unsigned lds) {
   // (both in scalar registers, whatever the compiler knows of them)
@@ -375,6 +374,14 @@ struct Shape {
 //
 // A block takes tiles (and slices of K) one after another; the first two steps of the next one are
 // loaded before the epilogue of the last, so that they arrive under it. Two stages of LDS.
+//
+// 16 bits, large products: bound by what the matrix cores reach while LDS is read beside them
+// (0.6 of their cycles, 1130 to 1200 TFLOP/s; a large library product 1130 to 1180). Steps on the
+// way, training step of 8192 rows through 2048-8192-2048 in bf16: fragments read where they are
+// used, operations of the library in the epilogues 4578 us; hardware exponentials, the kept g, u fetched
+// a row ahead 3171; fragments read a half ahead, loads spread over the products 2676;
+// one address and one test a row of the epilogue 2614 (queued 2370). fp32: bound by the fp32 matrix cores (0.8 of their
+// cycles). Few rows or columns: by the loads' latency, which slices of K share out.
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
   constexpr int SUB = EPI == kEpiGate ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;

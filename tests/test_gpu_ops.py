@@ -93,6 +93,21 @@ def test_gated_sizes(ops, dp, dtype, n, d, f, o):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 7, 8, 9])
+@pytest.mark.parametrize("d,f,o", [(200, 300, 100), (1100, 65, 72), (64, 2100, 9)])
+def test_gated_few_rows(ops, dp, dtype, n, d, f, o):
+    """Up to eight rows (kernels of their own) and nine: several slices, columns that end inside a
+    chunk, slices longer than one block's."""
+    gated_case(ops, dp, dtype, "gelu", n, d, f, o, seed=n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("pad,skip", [(8, 8), (3, 1)])
+def test_gated_few_rows_strides(ops, dp, dtype, pad, skip):
+    gated_case(ops, dp, dtype, "silu", 3, 130, 203, 77, pad=pad, skip=skip)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("act", ["tanh", "gelu"])
 def test_gated_activations(ops, dp, dtype, act):
     gated_case(ops, dp, dtype, act, 70, 48, 80, 24, seed=5, size=3.0)
@@ -325,6 +340,25 @@ EMBED = [(1, 1, 1), (5, 2, 8), (192, 2, 8), (33, 300, 7), (257, 118, 64), (1000,
          (4100, 257, 33), (3000, 50, 520)]
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,vocab,width", [(8192, 70001, 12), (8193, 70001, 12), (20000, 300, 40),
+                                           (140000, 20000, 5), (65, 20000, 9)])
+def test_embed_gradient_forms(ops, dtype, n, vocab, width):
+    """Rows on both sides of each form of the sort: one block, tiles with their own starts,
+    tiles with scanned ones; ids of more than 16 bits; a table of few and of many rows."""
+    gen = torch.Generator().manual_seed(n)
+    ids = ids_of(gen, n, vocab, "skewed")
+    dout = rand(gen, dtype, n, width)
+    dt = Mat(shape=(vocab, width), dtype=dtype, fill=7.0)
+    d_ids, d_dout = ids.cuda(), dout.cuda()
+    for _ in range(2):  # (the second finds what the first left in the workspace)
+        ops.embed_grad(d_ids.data_ptr(), d_dout.data_ptr(), dt.ptr, n, vocab, width, dtype, stream=stream())
+        torch.cuda.synchronize()
+        check(dt.view, ref.embed_grad(dtype, ids, dout.double(), vocab, 1.0), "embed_grad")
+        ids = ids.flip(0)
+        d_ids = ids.cuda()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,vocab,width", EMBED)
 @pytest.mark.parametrize("kind", ["even", "skewed", "one"])
@@ -387,6 +421,47 @@ def test_embed_nothing(ops):
     ops.embed_grad(ids.data_ptr(), g.data_ptr(), dt.data_ptr(), 70, 5, 8, ld_dtable=9, stream=stream())
     torch.cuda.synchronize()
     assert not dt[:, :8].any()
+
+
+# ---- offsets past 32 bits ----------------------------------------------------------------
+def test_offsets_past_32_bits(ops, dp):
+    """Rows that lie more than 2^32 elements into a matrix."""
+    gen = torch.Generator().manual_seed(12)
+    n, ld, d, f, o = (1 << 20) + 300, 4112, 16, 24, 8
+    x = torch.zeros(n, ld, dtype=torch.bfloat16, device="cuda")
+    last = rand(gen, "bf16", 300, d)
+    x[-300:, :d] = last.cuda()
+    w = [rand(gen, "bf16", d, f, .25), rand(gen, "bf16", d, f, .25), rand(gen, "bf16", f, o, .2)]
+    y = torch.full((n, o), 7.0, dtype=torch.bfloat16, device="cuda")
+    shape = dp.ops.GatedShape(n, d, f, o, dtype="bf16", ld_x=ld)
+    dw = [t.cuda() for t in w]
+    ops.gated_forward(shape, x.data_ptr(), *(t.data_ptr() for t in dw), y.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    check(y[-300:], ref.gated("bf16", "silu", last.double(), *(t.double() for t in w))["y"], "y")
+    assert not y[:-300].any()
+    # the same matrix as a table: its last rows, and their gradient
+    ids = torch.arange(n - 300, n, dtype=torch.int32)
+    out = torch.empty(300, d, dtype=torch.bfloat16, device="cuda")
+    d_ids = ids.cuda()
+    ops.embed(d_ids.data_ptr(), x.data_ptr(), out.data_ptr(), 300, n, d, "bf16", ld_table=ld, stream=stream())
+    assert torch.equal(out.cpu(), last)
+    x[-300:, :d] = 0
+    ops.embed_grad(d_ids.data_ptr(), out.data_ptr(), x.data_ptr(), 300, n, d, "bf16", ld_dtable=ld, stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(x[-300:, :d].cpu(), last)
+
+
+def test_example_learns(dp):
+    """The head of examples/train_head.py learns its targets: half of their variance within 30 steps."""
+    import importlib.util
+    import os
+
+    from _pkg import ROOT
+    spec = importlib.util.spec_from_file_location("train_head", os.path.join(ROOT, "examples", "train_head.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    losses = mod.train(dp, steps=30, cells=2)
+    assert all(math.isfinite(v) for v in losses) and losses[-1] < 0.5 * losses[0]
 
 
 # ---- refusals ---------------------------------------------------------------------------
