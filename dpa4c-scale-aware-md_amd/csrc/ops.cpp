@@ -59,10 +59,14 @@ int guarded(dp_ops* O, F&& f) {
     O->err = e.msg;
     return e.code;
   } catch (const HipError& e) {
+    (void)hipGetLastError();  // (else the next call's launch check finds it)
     O->err = std::string("HIP error ") + hipGetErrorString(e.code) + " in " + e.where;
     return DP_ERR_HIP;
   } catch (const std::exception& e) {
     O->err = e.what();
+    return DP_ERR_ARG;
+  } catch (...) {
+    O->err = "unknown error";
     return DP_ERR_ARG;
   }
 }

@@ -500,6 +500,18 @@ def test_refusals(ops, dp):
             ops.embed_grad(*(0 if q == k else p for q in range(3)), 4, 4, 8)
 
 
+def test_no_memory_is_an_error(dp):
+    """A workspace that no card holds is an error before anything is launched, and the next call works."""
+    one = dp.ops.Operators()
+    p = torch.zeros(4096, device="cuda").data_ptr()
+    with pytest.raises(dp.DeepmdException, match="HIP error"):
+        one.gated_forward(dp.ops.GatedShape(2 ** 30, 8, 2 ** 20, 8), p, p, p, p, p)
+    with pytest.raises(dp.DeepmdException, match="HIP error"):
+        one.embed_grad(p, p, p, 2 ** 30, 2 ** 30, 2 ** 20)
+    gated_case(one, dp, "f32", "silu", 20, 8, 16, 8)
+    assert one.device_bytes() > 0
+
+
 def test_capture_needs_a_workspace(dp):
     """A call whose workspace would have to grow inside a capture is refused, and the capture lives on."""
     one = dp.ops.Operators()
