@@ -70,28 +70,44 @@ void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride
 
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu) {
   // One step (128 bytes of k) of one block, measured: its share of a compute unit's time
-  // among others, and its time alone; and the blocks that a compute unit holds. (fp32: the matrix cores
-  // are slow enough that 256 x 256 tiles gain nothing over 128 x 128.)
+  // among others, and its time alone; what a tile's epilogue adds (a plain store, the gate, the gate's
+  // gradient); and the blocks that a compute unit holds. Measured with each shape forced, every
+  // product of training steps of ten sizes, 33 to 131,072 rows: the one picked here took within 6 % of
+  // the best one's time but for eleven of 108, of which the worst took 24 % more. (fp32: the
+  // matrix cores are slow enough that 256 x 256 tiles gain nothing over 128 x 128. 16 bits: 128 x 32
+  // was nowhere ahead of both neighbours.)
   struct S {
     int bm, bn, per_cu;
-    double share_us, alone_us;
+    double share_us, alone_us, end_us[3];
   };
-  static const S shapes[2][3] = {{{256, 256, 1, 1.8, 1.8}, {128, 128, 2, 0.62, 1.0}, {64, 128, 3, 0.40, 0.9}},
-                                 {{256, 256, 1, 8.1, 8.1}, {128, 128, 2, 2.05, 2.26}, {64, 128, 3, 1.05, 1.27}}};
+  static const S shapes[2][5] = {{{256, 256, 1, 1.8, 1.8, {14, 24, 66}},
+                                  {128, 128, 2, 0.62, 1.0, {5, 8, 23}},
+                                  {64, 128, 3, 0.40, 0.9, {2.2, 3.2, 7}},
+                                  {},
+                                  {64, 32, 6, 0.22, 0.55, {0.7, 1, 1.5}}},
+                                 {{},
+                                  {128, 128, 2, 2.05, 2.26, {5, 8, 23}},
+                                  {64, 128, 3, 1.05, 1.27, {2.2, 3.2, 7}},
+                                  {128, 32, 4, 0.575, 0.75, {1.5, 1.5, 3.5}},
+                                  {64, 32, 6, 0.33, 0.5, {0.7, 1, 1.5}}}};
   const int sub = what == kProdGate ? 2 : 1, bk = elem == kF32 ? 32 : 64;
   ProductPlan best{};
   double best_us = 0;
   const long steps = (K + bk - 1) / bk * segs;
-  for (int k = elem == kF32 ? 1 : 0; k < 3; ++k) {
+  for (int k = 0; k < 5; ++k) {
     const S& s = shapes[elem == kF32][k];
+    if (!s.bm) continue;
+    // (k-strided tiles of 32 columns have too few banks apart)
+    const double share = s.share_us * (what == kProdWeight && s.bn == 32 ? 1.3 : 1.0);
     const long tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn / sub - 1) / (s.bn / sub)) * mats;
     const long slots = (long)ncu * s.per_cu;
     const long most = std::max(1L, std::min(steps / 4, 2 * slots / tiles));
     for (long split = 1; split <= most; split = split < 4 ? split + 1 : split + split / 4) {
       const long items = tiles * split, a_cu = (items + ncu - 1) / ncu, rounds = (items + slots - 1) / slots;
       const double bytes = split > 1 ? 4.0 * split * sub * mats * M * ((N + 7) / 8 * 8) : 0;
-      const double us = (double)((steps + split - 1) / split) * std::max(a_cu * s.share_us, rounds * s.alone_us) +
-                        2.0 * rounds + (split > 1 ? 4 + 2 * bytes / 4e6 : 0);
+      const double end = s.end_us[split > 1 ? 0 : what == kProdGate ? 1 : what == kProdGateGrad ? 2 : 0];
+      const double us = (double)((steps + split - 1) / split) * std::max(a_cu * share, rounds * s.alone_us) +
+                        a_cu * end + 2.0 + (split > 1 ? 4 + 2 * bytes / 4e6 : 0);
       if (best_us == 0 || us < best_us) {
         best_us = us;
         best = ProductPlan{k, (int)split, (int)slots / 8 * 8, (size_t)bytes};

@@ -210,6 +210,15 @@ void output(ProductArgs& p, int k, void* out, int64_t ld, int type) {
   p.vec[k] = four_aligned(out, ld, type);
 }
 
+OutsArgs outs_of(const dp_gated_shape& s, const void* wd) {
+  OutsArgs q{};
+  q.rows = (long)s.rows;
+  q.f = s.d_hidden, q.o = s.d_out, q.act = s.act;
+  q.wd = wd;
+  q.ldh = (s.d_hidden + 7) / 8 * 8, q.ld_down = (long)s.ld_down, q.ld_y = (long)s.ld_y;
+  return q;
+}
+
 void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void* wg, const void* wu, const void* wd,
                    void* y, void* saved, hipStream_t st) {
   const int elem = elem_of(s.type);
@@ -230,16 +239,18 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   const bool both = pair_direct(s, wg, wu);
   const Source sg = source_of(s.type, wg, s.ld_hidden, s.d_in, s.d_hidden, r, both);
   const Source su = source_of(s.type, wu, s.ld_hidden, s.d_in, s.d_hidden, r, both);
-  const Source sd = source_of(s.type, wd, s.ld_down, s.d_hidden, s.d_out, r);
+  const bool few = few_outputs(s.d_hidden, s.d_out);
+  Source sd{};
+  if (!few) sd = source_of(s.type, wd, s.ld_down, s.d_hidden, s.d_out, r);
   const size_t at_h = r.take(bytes_of(s.type) * (size_t)n * f8);
   const ProductPlan p1 = plan_product(kProdGate, elem, n, s.d_hidden, s.d_in, 1, 1, O->ncu);
-  const ProductPlan p2 = plan_product(kProdDown, elem, n, s.d_out, s.d_hidden, 1, 1, O->ncu);
+  const ProductPlan p2 = few ? ProductPlan{} : plan_product(kProdDown, elem, n, s.d_out, s.d_hidden, 1, 1, O->ncu);
   const size_t at_part = r.take(std::max(p1.bytes, p2.bytes));
   char* ws = workspace(O, st, r.used);
 
   PackList list{};
   const Operand ox = operand_of(sx, ws, list), og = operand_of(sg, ws, list), ou = operand_of(su, ws, list);
-  const Operand od = operand_of(sd, ws, list);
+  const Operand od = few ? Operand{} : operand_of(sd, ws, list);
   pack_operands(st, elem, list);
   ProductArgs a = product(ox, og, n, s.d_hidden, s.d_in);
   a.b[1] = ou;
@@ -251,6 +262,12 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   a.partial = reinterpret_cast<float*>(ws + at_part);
   run_product(st, kProdGate, elem, p1, a);
 
+  if (few) {
+    OutsArgs q = outs_of(s, wd);
+    q.h = a.epi.h;
+    q.y = y;
+    return run_outs_down(st, elem, O->ncu, q);
+  }
   const Operand oh{a.epi.h, (long)f8};
   ProductArgs b = product(oh, od, n, s.d_out, s.d_hidden);
   output(b, 0, y, s.ld_y, s.type);
@@ -262,10 +279,13 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
                     const void* saved, const void* dy, void* dx, void* dwg, void* dwu, void* dwd, hipStream_t st) {
   const int elem = elem_of(s.type);
   const int64_t n = s.rows, f = s.d_hidden, f8 = (f + 7) / 8 * 8;
+  const bool few = few_outputs(s.d_hidden, s.d_out);
   Regions r;
-  const Source sdy = source_of(s.type, dy, s.ld_y, n, s.d_out, r);
-  const Source sd = source_of(s.type, wd, s.ld_down, f, s.d_out, r);
-  Source sx{}, sg{}, su{};
+  Source sdy{}, sd{}, sx{}, sg{}, su{};
+  if (!few) {
+    sdy = source_of(s.type, dy, s.ld_y, n, s.d_out, r);
+    sd = source_of(s.type, wd, s.ld_down, f, s.d_out, r);
+  }
   if (dwg) sx = source_of(s.type, x, s.ld_x, n, s.d_in, r);
   if (dx) {
     const bool both = pair_direct(s, wg, wu);
@@ -273,36 +293,51 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     su = source_of(s.type, wu, s.ld_hidden, s.d_in, f, r, both);
   }
   const size_t hb = bytes_of(s.type) * (size_t)n * f8;
-  const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd ? r.take(hb) : 0;
-  const ProductPlan p1 = plan_product(kProdGateGrad, elem, n, f, s.d_out, 1, 1, O->ncu);
+  const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd && !few ? r.take(hb) : 0;
+  const ProductPlan p1 = few ? ProductPlan{} : plan_product(kProdGateGrad, elem, n, f, s.d_out, 1, 1, O->ncu);
   const ProductPlan p2 = plan_product(kProdInput, elem, n, s.d_in, f, 2, 1, O->ncu);
   const ProductPlan p3 = plan_product(kProdWeight, elem, s.d_in, f, n, 1, 2, O->ncu);
-  const ProductPlan p4 = plan_product(kProdWeight, elem, f, s.d_out, n, 1, 1, O->ncu);
+  const ProductPlan p4 = few ? ProductPlan{} : plan_product(kProdWeight, elem, f, s.d_out, n, 1, 1, O->ncu);
+  OutsArgs q = outs_of(s, wd);
+  const size_t down_bytes = few ? plan_outs_grad(O->ncu, q) : p4.bytes;
   const size_t at_part = r.take(
-      std::max(std::max(p1.bytes, dx ? p2.bytes : 0), std::max(dwg ? p3.bytes : 0, dwd ? p4.bytes : 0)));
+      std::max(std::max(p1.bytes, dx ? p2.bytes : 0), std::max(dwg ? p3.bytes : 0, dwd ? down_bytes : 0)));
   char* ws = workspace(O, st, r.used);
   float* part = reinterpret_cast<float*>(ws + at_part);
 
   PackList list{};
-  const Operand ody = operand_of(sdy, ws, list), od = operand_of(sd, ws, list);
-  Operand ox{}, og{}, ou{};
+  Operand ody{}, od{}, ox{}, og{}, ou{};
+  if (!few) {
+    ody = operand_of(sdy, ws, list);
+    od = operand_of(sd, ws, list);
+  }
   if (dwg) ox = operand_of(sx, ws, list);
   if (dx) {
     og = operand_of(sg, ws, list);
     ou = operand_of(su, ws, list);
   }
   pack_operands(st, elem, list);
-  ProductArgs a = product(ody, od, n, f, s.d_out);
-  a.cols = (int)f8;
-  a.act = s.act;
-  a.epi.h = dwd ? ws + at_h : nullptr;
-  a.epi.dg = ws + at_dg;
-  a.epi.du = ws + at_du;
-  a.epi.ldh = f8;
-  a.epi.saved = static_cast<float*>(const_cast<void*>(saved));
-  a.partial = part;
-  run_product(st, kProdGateGrad, elem, p1, a);
-  const Operand odg{a.epi.dg, (long)f8}, odu{a.epi.du, (long)f8};
+  if (few) {
+    q.dy = dy;
+    q.saved = static_cast<const float*>(saved);
+    q.dg = ws + at_dg;
+    q.du = ws + at_du;
+    q.dwd = dwd;
+    q.partial = dwd ? part : nullptr;
+    run_outs_grad(st, elem, q);
+  } else {
+    ProductArgs a = product(ody, od, n, f, s.d_out);
+    a.cols = (int)f8;
+    a.act = s.act;
+    a.epi.h = dwd ? ws + at_h : nullptr;
+    a.epi.dg = ws + at_dg;
+    a.epi.du = ws + at_du;
+    a.epi.ldh = f8;
+    a.epi.saved = static_cast<float*>(const_cast<void*>(saved));
+    a.partial = part;
+    run_product(st, kProdGateGrad, elem, p1, a);
+  }
+  const Operand odg{ws + at_dg, (long)f8}, odu{ws + at_du, (long)f8};
 
   if (dx) {
     ProductArgs b = product(odg, og, n, s.d_in, f);
@@ -322,8 +357,8 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     b.partial = part;
     run_product(st, kProdWeight, elem, p3, b);
   }
-  if (dwd) {
-    ProductArgs b = product(Operand{a.epi.h, (long)f8}, ody, f, s.d_out, n);
+  if (dwd && !few) {
+    ProductArgs b = product(Operand{ws + at_h, (long)f8}, ody, f, s.d_out, n);
     output(b, 0, dwd, s.ld_down, s.type);
     b.partial = part;
     run_product(st, kProdWeight, elem, p4, b);

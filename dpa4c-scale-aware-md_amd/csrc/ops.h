@@ -79,6 +79,23 @@ struct RowsArgs {
 size_t plan_rows(int elem, int ncu, RowsArgs& args);  // bytes of the partial sums
 void run_rows(hipStream_t st, int elem, RowsArgs& args);
 
+// ---- the block's down side for few outputs (gated_outs.hip) ----
+constexpr int kFewOutputs = 4;
+struct OutsArgs {
+  long rows;
+  int f, o, act;
+  const void *h, *wd, *dy;  // h: rows of ldh, zeros from f on
+  const float* saved;
+  long ldh, ld_down, ld_y;
+  void *y, *dg, *du, *dwd;
+  float* partial;  // [slices][f][o], or null: no d w_down
+  int quads, groups, slices;
+};
+bool few_outputs(int d_hidden, int d_out);
+void run_outs_down(hipStream_t st, int elem, int ncu, const OutsArgs& args);
+size_t plan_outs_grad(int ncu, OutsArgs& args);  // bytes of the partial sums
+void run_outs_grad(hipStream_t st, int elem, const OutsArgs& args);
+
 // Matrices [rows][cols] to be copied into rows of ld (a multiple of 8), with zeros past cols.
 struct PackItem {
   const void* src;

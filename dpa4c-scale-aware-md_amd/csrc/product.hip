@@ -8,11 +8,14 @@ namespace dpamd {
 namespace {
 
 // 256 x 256 with eight waves of 128 x 64 (128 KB of LDS, one block a compute unit), 128 x 128
-// with four of 64 x 64 (64 KB, two), and for few rows 64 x 128 with four of 64 x 32 (48 KB,
-// three). fp32 has the two smaller ones.
+// with four of 64 x 64 (64 KB, two), for few rows 64 x 128 with four of 64 x 32 (48 KB, three),
+// and for small products 64 x 32 with four of 16 x 32 (24 KB, six). fp32 has 128 x 32 (40 KB,
+// four) for narrow ones in place of the first.
 using Big = Shape<256, 256, 2, 4>;
 using Small = Shape<128, 128, 2, 2>;
 using Thin = Shape<64, 128, 1, 4>;
+using Slim = Shape<128, 32, 4, 1>;
+using Tiny = Shape<64, 32, 4, 1>;
 
 template <int KIND, int LA, int LB, int EPI, class S>
 void launch(hipStream_t st, ProductArgs& p) {
@@ -53,10 +56,14 @@ template <int KIND>
 void launch_product(hipStream_t st, ProductKind what, int shape, ProductArgs& p) {
   if constexpr (KIND != kF32)
     if (shape == 0) return launch_kind<KIND, Big>(st, what, p);
-  if (shape <= 1)
-    launch_kind<KIND, Small>(st, what, p);
-  else
+  if constexpr (KIND == kF32)
+    if (shape == 3) return launch_kind<KIND, Slim>(st, what, p);
+  if (shape == 4)
+    launch_kind<KIND, Tiny>(st, what, p);
+  else if (shape == 2)
     launch_kind<KIND, Thin>(st, what, p);
+  else
+    launch_kind<KIND, Small>(st, what, p);
 }
 
 template void launch_product<ELEM_KIND>(hipStream_t, ProductKind, int, ProductArgs&);

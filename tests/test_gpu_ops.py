@@ -108,6 +108,21 @@ def test_gated_few_rows_strides(ops, dp, dtype, pad, skip):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,d,f,o", [(9, 24, 8185, 1), (9, 24, 8193, 1), (13, 40, 4100, 2), (300, 40, 2043, 4),
+                                     (300, 40, 2056, 3), (3000, 33, 97, 3), (1, 16, 260, 4), (4111, 16, 260, 5)])
+def test_gated_few_outputs(ops, dp, dtype, n, d, f, o):
+    """Up to four outputs (kernels of their own), five, and where the hidden side is too wide for them:
+    odd widths, several groups of columns, slices of one row and of many."""
+    gated_case(ops, dp, dtype, "tanh", n, d, f, o, seed=n + o)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("pad,skip", [(8, 8), (3, 1)])
+def test_gated_few_outputs_strides(ops, dp, dtype, pad, skip):
+    gated_case(ops, dp, dtype, "silu", 70, 33, 131, 3, pad=pad, skip=skip)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("act", ["tanh", "gelu"])
 def test_gated_activations(ops, dp, dtype, act):
     gated_case(ops, dp, dtype, act, 70, 48, 80, 24, seed=5, size=3.0)
