@@ -112,7 +112,7 @@ void lookup_kind(hipStream_t st, long n, int vocab, int width, const int* ids, c
 
 // ---- sort -----------------------------------------------------------------------------
 constexpr int kSortThreads = 256, kSortWaves = kSortThreads / kWave;
-constexpr int kSortItems = 8;                         // a thread
+constexpr int kSortItems = 4;                         // a thread (8: place 10 to 12 us of 32,768 rows, 4: 7)
 constexpr int kSortTile = kSortThreads * kSortItems;  // a block
 constexpr int kBits = 8, kDigits = 1 << kBits;
 
@@ -140,8 +140,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const int* ids, con
 }
 
 // Places the tile's rows at starts[digit][tile] (the counts' exclusive sums; null: formed
-// here) + rank among the tile's rows of that digit, in row order: wave w takes a contiguous run of rows, 64 at a time; the lanes of
-// equal digits are found by one ballot a bit.
+// here) + rank among the tile's rows of that digit, in row order: wave w takes a contiguous
+// run of rows, 64 at a time; the lanes of equal digits are found by one ballot a bit.
 __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, const unsigned* keys, const int* rows,
                                                              long n, int vocab, int shift, int tiles,
                                                              const int* starts, const int* counts,
@@ -181,6 +181,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, con
     } else {
       // few tiles: this tile's starts from the counts themselves
       int before = 0, total = 0;
+#pragma unroll 8
       for (int t = 0; t < tiles; ++t) {
         const int c = counts[(long)threadIdx.x * tiles + t];
         before += t < (int)blockIdx.x ? c : 0;
@@ -218,10 +219,10 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, con
 // ---- sums of runs ---------------------------------------------------------------------
 constexpr int kWindow = 32;     // sorted positions of one window
 constexpr int kShort = 64;      // runs up to this length are summed by their table row itself
-// Rows up to which one block sorts them all. Random ids among 30,000, width 1024, us, one block /
-// tiles: 4,000 29 / 44, 16,000 57 / 47; they cross near 10,000.
+// Rows up to which one block sorts them all. The whole gradient, tokens among 30,000, 1024 wide in
+// bf16, us, one block / tiles: 1,500 39 / 48, 4,000 45 / 51, 8,000 55 / 55.
 constexpr int kOneMost = 8192;
-constexpr int kScanTiles = 64;  // tiles up to which each block of the sort forms its starts itself
+constexpr int kScanTiles = 128; // tiles up to which each block of the sort forms its starts itself
 
 // run[2 v], run[2 v + 1]: first position and end of id v's run. Those of ids without rows are
 // not written (run_of() tells by the key at the first position).
@@ -327,18 +328,18 @@ __global__ __launch_bounds__(kOneThreads) void k_sort_one(const int* __restrict_
   }
 }
 
-// acc += rows[from .. to) of this lane's chunk, four loads under way
-template <int KIND, int E>
+// acc += rows[from .. to) of this lane's chunk, U loads under way
+template <int KIND, int E, int U>
 __device__ __forceinline__ void add_rows(float (&acc)[E], int from, int to, const int* __restrict__ rows,
                                          const typename ElemOf<KIND>::T* __restrict__ dout, long ld, int c) {
   using C = Chunk<KIND, E>;
   int i = from;
-  for (; i + 4 <= to; i += 4) {
-    C x[4];
+  for (; i + U <= to; i += U) {
+    C x[U];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = *reinterpret_cast<const C*>(dout + rows[i + q] * ld + (long)c * E);
+    for (int q = 0; q < U; ++q) x[q] = *reinterpret_cast<const C*>(dout + rows[i + q] * ld + (long)c * E);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < U; ++q)
 #pragma unroll
       for (int k = 0; k < E; ++k) acc[k] += to_f32<KIND>(x[q].v[k]);
   }
@@ -357,8 +358,10 @@ __global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chun
                                                       const int* __restrict__ rows, const int* __restrict__ run,
                                                       const typename ElemOf<KIND>::T* __restrict__ dout, long ld,
                                                       float* __restrict__ partial) {
-  const int windows = (n + kWindow - 1) / kWindow, lane = threadIdx.x & 63;
-  for (int w = blockIdx.x * 4 + threadIdx.x / 64; w < windows; w += gridDim.x * 4) {
+  const int windows = (n + kWindow - 1) / kWindow, lane = threadIdx.x & 63, groups = (chunks + 63) / 64;
+  // a wave 64 chunks of a window
+  for (long at = (long)blockIdx.x * 4 + threadIdx.x / 64; at < (long)windows * groups; at += (long)gridDim.x * 4) {
+    const int w = (int)(at / groups), c = (int)(at % groups) * 64 + lane;
     const int b = w * kWindow, e = min(n, b + kWindow);
     const unsigned first = keys[b], last = keys[e - 1];
 #pragma unroll
@@ -366,14 +369,12 @@ __global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chun
       const unsigned v = part ? last : first;
       if (v >= (unsigned)vocab || (part && last == first)) continue;
       const int lo = run[2 * (long)v], hi = run[2 * (long)v + 1];  // (v has rows)
-      if (hi - lo <= kShort) continue;
-      for (int c = lane; c < chunks; c += 64) {
-        float acc[E] = {};
-        add_rows<KIND, E>(acc, max(lo, b), min(hi, e), rows, dout, ld, c);
-        float* o = partial + ((long)(2 * (long)w + part) * chunks + c) * E;
+      if (hi - lo <= kShort || c >= chunks) continue;
+      float acc[E] = {};
+      add_rows<KIND, E, 8>(acc, max(lo, b), min(hi, e), rows, dout, ld, c);
+      float* o = partial + ((long)(2 * (long)w + part) * chunks + c) * E;
 #pragma unroll
-        for (int k = 0; k < E; ++k) o[k] = acc[k];
-      }
+      for (int k = 0; k < E; ++k) o[k] = acc[k];
     }
   }
 }
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(256) void k_grad_rows(int n, int vocab, int chunks,
       for (int c = lane; c < chunks; c += 64) {
         float acc[E] = {};
         if (hi - lo <= kShort) {
-          add_rows<KIND, E>(acc, lo, hi, rows, dout, ld, c);
+          add_rows<KIND, E, 4>(acc, lo, hi, rows, dout, ld, c);
         } else {
           const int w0 = lo / kWindow, w1 = (hi - 1) / kWindow;
           // the first window's part is the second of that window where the run starts inside it
@@ -615,7 +616,7 @@ void launch_grad(hipStream_t st, long n, int vocab, int width, const int* ids, c
     sort_rows(st, g, n, vocab, ids, keys, rows, run, ws);
   }
   if (n > kShort) {  // (else no run is long)
-    hipLaunchKernelGGL((k_grad_windows<KIND, E>), wave_blocks((n + kWindow - 1) / kWindow), dim3(256), 0, st, (int)n,
+    hipLaunchKernelGGL((k_grad_windows<KIND, E>), wave_blocks((n + kWindow - 1) / kWindow * ((chunks + 63) / 64)), dim3(256), 0, st, (int)n,
                        vocab, chunks, key, row, run, dout, ld, partial);
     DPAMD_LAUNCH_CHECK();
   }

@@ -71,9 +71,11 @@ def gated_case(ops, dp, dtype, act, n, d, f, o, pad=0, skip=0, seed=0, size=1.0)
     ops.gated_backward(shape, p["x"], p["wg"], p["wu"], p["wd"], saved.data_ptr(), p["dy"], p["dx"], p["dwg"],
                        p["dwu"], p["dwd"], stream=stream())
     torch.cuda.synchronize()
-    want = ref.gated(dtype, act, *(host[k].double() for k in ("x", "wg", "wu", "wd", "dy")))
-    for k, w in want.items():
-        check(m[k].view, w, (k, dtype, act, n, d, f, o))
+    # (large ones' 64-bit products on the GPU: plain matrix products of torch)
+    at = "cuda" if n * f * max(d, o) > 2e9 else "cpu"
+    want = ref.gated(dtype, act, *(host[k].double().to(at) for k in ("x", "wg", "wu", "wd", "dy")))
+    for k, (v, b) in want.items():
+        check(m[k].view, (v.cpu(), b.cpu()), (k, dtype, act, n, d, f, o))
         assert m[k].untouched(7.0), k
     # (with a workspace grown by the backward or not, kept or not: the same bits)
     assert torch.equal(y0.view, m["y"].view)
@@ -141,6 +143,14 @@ def test_gated_strides(ops, dp, dtype, pad, skip):
                                      (2100, 300, 520, 264)])
 def test_gated_long_axes(ops, dp, dtype, n, d, f, o):
     """Sums over many rows or columns (cut into slices), several tiles each way."""
+    gated_case(ops, dp, dtype, "silu", n, d, f, o, seed=n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,d,f,o", [(9001, 515, 1031, 520), (12300, 1601, 242, 250), (8201, 1031, 4105, 2060),
+                                     (4101, 64, 8201, 4100)])
+def test_gated_large_tiles(ops, dp, dtype, n, d, f, o):
+    """Each tile shape in every product that takes it, with edges inside its tiles."""
     gated_case(ops, dp, dtype, "silu", n, d, f, o, seed=n)
 
 
