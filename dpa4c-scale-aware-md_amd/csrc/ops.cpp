@@ -187,10 +187,9 @@ bool pair_direct(const dp_gated_shape& s, const void* wg, const void* wu) {
   return is_operand(s.type, wg, s.ld_hidden, s.d_hidden) && is_operand(s.type, wu, s.ld_hidden, s.d_hidden);
 }
 
-// whether rows of four elements of `out` can be stored whole
-bool four_aligned(const void* out, int64_t ld, int type) {
-  const size_t b = 4 * bytes_of(type);
-  return reinterpret_cast<uintptr_t>(out) % b == 0 && ld % 4 == 0;
+// whether `many` elements of a row of `out`, from a multiple of it on, can be stored whole
+bool aligned(const void* out, int64_t ld, int type, int many) {
+  return reinterpret_cast<uintptr_t>(out) % (many * bytes_of(type)) == 0 && ld % many == 0;
 }
 
 ProductArgs product(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K) {
@@ -207,7 +206,8 @@ ProductArgs product(const Operand& a, const Operand& b, int64_t M, int64_t N, in
 void output(ProductArgs& p, int k, void* out, int64_t ld, int type) {
   p.out[k] = out;
   p.ldo[k] = ld;
-  p.vec[k] = four_aligned(out, ld, type);
+  p.vec[k] = aligned(out, ld, type, 4);
+  p.wide[k] = type != DP_TYPE_F32 && aligned(out, ld, type, 8);
 }
 
 OutsArgs outs_of(const dp_gated_shape& s, const void* wd) {

@@ -44,7 +44,7 @@ struct ProductArgs {
   long ldp;  // cols up to a multiple of 4
   void* out[2];
   long ldo[2];
-  bool vec[2];
+  bool vec[2], wide[2];  // whether four, and eight, columns of a row can be stored whole
   EpiArgs epi;
 };
 

@@ -62,6 +62,15 @@ __device__ __forceinline__ void put4(typename ElemOf<KIND>::T* p, const f4& v) {
   }
 }
 
+// Eight, of 16 bits each.
+template <int KIND>
+__device__ __forceinline__ void put8(typename ElemOf<KIND>::T* p, const f4& v, const f4& w) {
+  static_assert(KIND != kF32, "four of 32 bits are 16 bytes already");
+  typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+  *reinterpret_cast<us8*>(p) = us8{to16<KIND>(v[0]), to16<KIND>(v[1]), to16<KIND>(v[2]), to16<KIND>(v[3]),
+                                   to16<KIND>(w[0]), to16<KIND>(w[1]), to16<KIND>(w[2]), to16<KIND>(w[3])};
+}
+
 // Four columns of one row of an output, `count` of them inside it; FULL: all four, and aligned.
 template <int KIND, bool FULL>
 __device__ __forceinline__ void put_row4(void* out, long at, const f4& v, int count) {
@@ -195,6 +204,21 @@ __device__ __forceinline__ void put_gate_grad(const EpiArgs& e, long at, const G
   if (e.h) put4<KIND>(static_cast<T*>(e.h) + at, o.h);
   put4<KIND>(static_cast<T*>(e.dg) + at, o.dg);
   put4<KIND>(static_cast<T*>(e.du) + at, o.du);
+}
+
+// Of two neighbouring fragments of 16 columns, of which lane group g holds columns 4 g .. 4 g + 3
+// each: afterwards g holds eight consecutive ones, 8 (g >> 1) .. of fragment g & 1, in v and w.
+__device__ __forceinline__ void join_quads(f4& v, f4& w) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    // (in scalars of their own: a bit cast of a vector's element has been compiled as one of element 0)
+    const float x = v[e], y = w[e];
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y),
+                                                    true, false);
+    const unsigned a = r[0], b = r[1];
+    v[e] = __builtin_bit_cast(float, a);
+    w[e] = __builtin_bit_cast(float, b);
+  }
 }
 
 // ---- the product ------------------------------------------------------------------------
@@ -564,6 +588,9 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
     // with tests, products of 64 bits and branches for every four columns the epilogue issued
     // several thousand instructions a wave, and took longer than eight steps of products.
     const int m0 = done.m0 + wm * TM + c, n0 = done.n0 + wn * (TN / SUB) + 4 * g;
+    // (16 bits: 16 bytes a lane, the columns of pairs of fragments exchanged between lanes)
+    constexpr bool WIDE = KIND != kF32;
+    const int wide_at = 16 * (g & 1) + 8 * (g >> 1) - 4 * g;
     const bool inside = done.m0 + (wm + 1) * TM <= p.M && done.n0 + (wn + 1) * (TN / SUB) <= p.N;
     if (p.split > 1) {
       // a slice's sums, columns in rows of ldp (a multiple of 4)
@@ -582,7 +609,22 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
       const long row = 16 * p.ldo[done.mat];
       long at = m0 * p.ldo[done.mat] + n0;
       void* out = p.out[done.mat];
-      if (inside && p.vec[done.mat]) {
+      bool stored = false;
+      if constexpr (WIDE && NJ % 2 == 0) {
+        if (inside && p.wide[done.mat]) {
+          stored = true;
+          long w = at + wide_at;
+#pragma unroll
+          for (int i = 0; i < MI; ++i, w += row)
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2) {
+              join_quads(acc[i][j], acc[i][j + 1]);
+              put8<KIND>(static_cast<typename ElemOf<KIND>::T*>(out) + w + j * 16, acc[i][j], acc[i][j + 1]);
+            }
+        }
+      }
+      if (stored) {
+      } else if (inside && p.vec[done.mat]) {
 #pragma unroll
         for (int i = 0; i < MI; ++i, at += row)
 #pragma unroll
