@@ -61,15 +61,6 @@ __global__ __launch_bounds__(256) void k_outs_down(const OutsArgs p) {
   }
 }
 
-// g and u of four columns, `count` of them inside, at any row length
-__device__ __forceinline__ Kept kept_at(const float* p, int count) {
-  if (count < 4) return load_kept<false>(p, count);
-  f4 a, b;
-  __builtin_memcpy(&a, p, sizeof(a));  // (the hardware takes unaligned addresses)
-  __builtin_memcpy(&b, p + 4, sizeof(b));
-  return Kept{f4{a[0], a[2], b[0], b[2]}, f4{a[1], a[3], b[1], b[3]}};
-}
-
 // Blocks: slices of the rows by groups of p.quads quads of columns; 256 / p.quads rows at a time.
 template <int KIND, int O>
 __global__ __launch_bounds__(256) void k_outs_grad(const OutsArgs p) {
@@ -78,6 +69,7 @@ __global__ __launch_bounds__(256) void k_outs_grad(const OutsArgs p) {
   const int at_once = 256 / p.quads, slot = threadIdx.x / p.quads, quad = threadIdx.x % p.quads;
   const int c = (blockIdx.y * p.quads + quad) * 4, count = p.f - c;
   const long r0 = p.rows * blockIdx.x / gridDim.x, r1 = p.rows * (blockIdx.x + 1) / gridDim.x;
+  const long plane = p.rows * p.f;
   float w[4][O], acc[4][O] = {};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -91,7 +83,8 @@ __global__ __launch_bounds__(256) void k_outs_grad(const OutsArgs p) {
     };
     auto fetch = [&](long r) {
       Row x;
-      x.kept = kept_at(p.saved + 2 * (r * p.f + c), count);
+      const float* kept = p.saved + (r * p.f + c);
+      x.kept = count >= 4 ? load_kept<true>(kept, plane, 4) : load_kept<false>(kept, plane, count);
 #pragma unroll
       for (int k = 0; k < O; ++k)
         x.dy[k] = k < p.o ? to_f32<KIND>(static_cast<const T*>(p.dy)[r * p.ld_y + k]) : 0.0f;

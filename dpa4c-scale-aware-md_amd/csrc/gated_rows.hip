@@ -169,8 +169,8 @@ __global__ __launch_bounds__(kThreads) void k_rows_down(RowsArgs p) {
       activate4(p.act, f4{g, g, g, g}, a, da);
       h = a[0] * u;
       if (p.saved && blockIdx.x == 0) {
-        p.saved[2 * ((long)r * p.f + k0 + k)] = g;
-        p.saved[2 * ((long)r * p.f + k0 + k) + 1] = u;
+        p.saved[(long)r * p.f + k0 + k] = g;
+        p.saved[(long)(p.rows + r) * p.f + k0 + k] = u;
       }
     }
     lds[r * slice + k] = h;

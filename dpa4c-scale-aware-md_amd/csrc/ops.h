@@ -22,7 +22,7 @@ struct Operand {
   long ld;
 };
 
-// h, dg and du as operands [M][ldh]; saved: [M][N] pairs (g, u).
+// h, dg and du as operands [M][ldh]; saved: g and then u, [M][N] each.
 struct EpiArgs {
   void *h, *dg, *du;
   long ldh;

@@ -62,15 +62,6 @@ __device__ __forceinline__ void put4(typename ElemOf<KIND>::T* p, const f4& v) {
   }
 }
 
-// Eight, of 16 bits each.
-template <int KIND>
-__device__ __forceinline__ void put8(typename ElemOf<KIND>::T* p, const f4& v, const f4& w) {
-  static_assert(KIND != kF32, "four of 32 bits are 16 bytes already");
-  typedef unsigned short us8 __attribute__((ext_vector_type(8)));
-  *reinterpret_cast<us8*>(p) = us8{to16<KIND>(v[0]), to16<KIND>(v[1]), to16<KIND>(v[2]), to16<KIND>(v[3]),
-                                   to16<KIND>(w[0]), to16<KIND>(w[1]), to16<KIND>(w[2]), to16<KIND>(w[3])};
-}
-
 // Four columns of one row of an output, `count` of them inside it; FULL: all four, and aligned.
 template <int KIND, bool FULL>
 __device__ __forceinline__ void put_row4(void* out, long at, const f4& v, int count) {
@@ -135,46 +126,49 @@ __device__ __forceinline__ void activate4(int act, const f4& g, f4& a, f4& da) {
 // The four columns are `count` of the output's (and the rest beyond it); FULL: all four, and
 // aligned.
 
-// h = a(g) u (zeros beyond the output), g and u kept for the backward in 32
-// bits, so that what it forms from them is rounded once. kept: pairs (g, u), or null.
-template <int KIND, bool FULL>
-__device__ __forceinline__ void put_gate(void* h, long at, float* kept, int act, int count, const f4& g,
-                                         const f4& u) {
+// h = a(g) u (zeros beyond the output)
+template <bool FULL>
+__device__ __forceinline__ f4 gate_value(int act, int count, const f4& g, const f4& u) {
   f4 a, da, v;
   activate4(act, g, a, da);
 #pragma unroll
   for (int r = 0; r < 4; ++r) v[r] = FULL || r < count ? a[r] * u[r] : 0.0f;
-  put4<KIND>(static_cast<typename ElemOf<KIND>::T*>(h) + at, v);
-  if (!kept) return;
-  if constexpr (FULL) {
-    *reinterpret_cast<f4*>(kept) = f4{g[0], u[0], g[1], u[1]};
-    *reinterpret_cast<f4*>(kept + 4) = f4{g[2], u[2], g[3], u[3]};
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r < count) {
-        kept[2 * r] = g[r];
-        kept[2 * r + 1] = u[r];
-      }
-  }
+  return v;
 }
 
-// g and u of four columns as the forward kept them (zeros beyond the output)
+// g and u of four columns are kept for the backward in 32 bits, so that what it forms from
+// them is rounded once: all of g, and all of u `plane` floats on. (As pairs the lanes' 16 bytes of
+// one instruction lay 32 apart.)
 struct Kept {
   f4 g, u;
 };
 template <bool FULL>
-__device__ __forceinline__ Kept load_kept(const float* kept, int count) {
+__device__ __forceinline__ void put_kept(float* kept, long plane, int count, const f4& g, const f4& u) {
+  if constexpr (FULL) {
+    // (the hardware takes unaligned addresses)
+    __builtin_memcpy(kept, &g, sizeof(g));
+    __builtin_memcpy(kept + plane, &u, sizeof(u));
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < count) {
+        kept[r] = g[r];
+        kept[plane + r] = u[r];
+      }
+  }
+}
+// as the forward kept them (zeros beyond the output)
+template <bool FULL>
+__device__ __forceinline__ Kept load_kept(const float* kept, long plane, int count) {
   Kept k;
   if constexpr (FULL) {
-    const f4 p = *reinterpret_cast<const f4*>(kept), q = *reinterpret_cast<const f4*>(kept + 4);
-    k.g = f4{p[0], p[2], q[0], q[2]};
-    k.u = f4{p[1], p[3], q[1], q[3]};
+    __builtin_memcpy(&k.g, kept, sizeof(k.g));
+    __builtin_memcpy(&k.u, kept + plane, sizeof(k.u));
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      k.g[r] = r < count ? kept[2 * r] : 0.0f;
-      k.u[r] = r < count ? kept[2 * r + 1] : 0.0f;
+      k.g[r] = r < count ? kept[r] : 0.0f;
+      k.u[r] = r < count ? kept[plane + r] : 0.0f;
     }
   }
   return k;
@@ -206,19 +200,28 @@ __device__ __forceinline__ void put_gate_grad(const EpiArgs& e, long at, const G
   put4<KIND>(static_cast<T*>(e.du) + at, o.du);
 }
 
-// Of two neighbouring fragments of 16 columns, of which lane group g holds columns 4 g .. 4 g + 3
-// each: afterwards g holds eight consecutive ones, 8 (g >> 1) .. of fragment g & 1, in v and w.
-__device__ __forceinline__ void join_quads(f4& v, f4& w) {
+// Where a lane of group g (at column 4 g of a fragment of 16) puts the eight columns that put_pair
+// gives it.
+__device__ __forceinline__ int pair_at(int g) { return 16 * (g & 1) + 8 * (g >> 1) - 4 * g; }
+// v and w are columns 4 g .. 4 g + 3 of two neighbouring fragments: rounded to 16 bits and traded
+// between lane groups, so that each has eight consecutive columns, 8 (g >> 1) .. of fragment g & 1, and
+// stores 16 bytes (whose rows are then whole 64-byte pieces: with 8 bytes a lane dx of 131,072 x 2048
+// took 411 us, so 370).
+template <int KIND>
+__device__ __forceinline__ void put_pair(typename ElemOf<KIND>::T* p, const f4& v, const f4& w) {
+  static_assert(KIND != kF32, "four of 32 bits are 16 bytes already");
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  unsigned out[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    // (in scalars of their own: a bit cast of a vector's element has been compiled as one of element 0)
-    const float x = v[e], y = w[e];
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y),
-                                                    true, false);
-    const unsigned a = r[0], b = r[1];
-    v[e] = __builtin_bit_cast(float, a);
-    w[e] = __builtin_bit_cast(float, b);
+  for (int e = 0; e < 2; ++e) {
+    const unsigned x = __builtin_bit_cast(unsigned, us2{to16<KIND>(v[2 * e]), to16<KIND>(v[2 * e + 1])});
+    const unsigned y = __builtin_bit_cast(unsigned, us2{to16<KIND>(w[2 * e]), to16<KIND>(w[2 * e + 1])});
+    const auto r = __builtin_amdgcn_permlane16_swap(x, y, true, false);
+    out[e] = r[0];
+    out[2 + e] = r[1];
   }
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<u4*>(p) = u4{out[0], out[1], out[2], out[3]};
 }
 
 // ---- the product ------------------------------------------------------------------------
@@ -409,6 +412,7 @@ struct Shape {
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
   constexpr int SUB = EPI == kEpiGate ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
+  using T = typename ElemOf<KIND>::T;
   constexpr int WAVES = S::WM * S::WN, TM = S::BM / S::WM, TN = S::BN / S::WN;
   constexpr int MI = TM / 16, NJ = TN / 16;
   using TA = TileOf<LA, S::BM, EB, 1, WAVES>;
@@ -588,9 +592,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
     // with tests, products of 64 bits and branches for every four columns the epilogue issued
     // several thousand instructions a wave, and took longer than eight steps of products.
     const int m0 = done.m0 + wm * TM + c, n0 = done.n0 + wn * (TN / SUB) + 4 * g;
-    // (16 bits: 16 bytes a lane, the columns of pairs of fragments exchanged between lanes)
-    constexpr bool WIDE = KIND != kF32;
-    const int wide_at = 16 * (g & 1) + 8 * (g >> 1) - 4 * g;
+    constexpr bool WIDE = KIND != kF32;  // pairs of fragments are stored together
     const bool inside = done.m0 + (wm + 1) * TM <= p.M && done.n0 + (wn + 1) * (TN / SUB) <= p.N;
     if (p.split > 1) {
       // a slice's sums, columns in rows of ldp (a multiple of 4)
@@ -613,14 +615,12 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
       if constexpr (WIDE && NJ % 2 == 0) {
         if (inside && p.wide[done.mat]) {
           stored = true;
-          long w = at + wide_at;
+          long w = at + pair_at(g);
 #pragma unroll
           for (int i = 0; i < MI; ++i, w += row)
 #pragma unroll
-            for (int j = 0; j < NJ; j += 2) {
-              join_quads(acc[i][j], acc[i][j + 1]);
-              put8<KIND>(static_cast<typename ElemOf<KIND>::T*>(out) + w + j * 16, acc[i][j], acc[i][j + 1]);
-            }
+            for (int j = 0; j < NJ; j += 2)
+              put_pair<KIND>(static_cast<T*>(out) + w + j * 16, acc[i][j], acc[i][j + 1]);
         }
       }
       if (stored) {
@@ -639,23 +639,37 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
       }
     } else if constexpr (EPI == kEpiGate) {
       long h = m0 * p.epi.ldh + n0;
-      float* kept = p.epi.saved ? p.epi.saved + 2 * ((long)m0 * p.N + n0) : nullptr;
-      const long hrow = 16 * p.epi.ldh, krow = p.epi.saved ? 32l * p.N : 0;
-      if (inside && (p.N & 1) == 0) {
+      float* kept = p.epi.saved ? p.epi.saved + ((long)m0 * p.N + n0) : nullptr;
+      const long hrow = 16 * p.epi.ldh, krow = p.epi.saved ? 16l * p.N : 0, plane = (long)p.M * p.N;
+      T* to = static_cast<T*>(p.epi.h);
+      constexpr int NG = NJ / SUB;  // fragments of g, and as many of u
+      if (inside) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i, h += hrow, kept += krow)
+        for (int i = 0; i < MI; ++i, h += hrow, kept += krow) {
+          f4 v[NG];
 #pragma unroll
-          for (int j = 0; j < NJ / SUB; ++j)
-            put_gate<KIND, true>(p.epi.h, h + j * 16, p.epi.saved ? kept + j * 32 : nullptr, p.act, 4, acc[i][j],
-                                 acc[i][j + NJ / 2]);
+          for (int j = 0; j < NG; ++j) {
+            v[j] = gate_value<true>(p.act, 4, acc[i][j], acc[i][j + NG]);
+            if (p.epi.saved) put_kept<true>(kept + j * 16, plane, 4, acc[i][j], acc[i][j + NG]);
+          }
+          if constexpr (WIDE && NG % 2 == 0) {
+#pragma unroll
+            for (int j = 0; j < NG; j += 2) put_pair<KIND>(to + h + pair_at(g) + j * 16, v[j], v[j + 1]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NG; ++j) put4<KIND>(to + h + j * 16, v[j]);
+          }
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < MI; ++i, h += hrow, kept += krow)
 #pragma unroll
-          for (int j = 0; j < NJ / SUB; ++j)
-            if (m0 + i * 16 < p.M && n0 + j * 16 < p.cols)
-              put_gate<KIND, false>(p.epi.h, h + j * 16, p.epi.saved ? kept + j * 32 : nullptr, p.act,
-                                    p.N - n0 - j * 16, acc[i][j], acc[i][j + NJ / 2]);
+          for (int j = 0; j < NG; ++j)
+            if (m0 + i * 16 < p.M && n0 + j * 16 < p.cols) {
+              const int count = p.N - n0 - j * 16;
+              put4<KIND>(to + h + j * 16, gate_value<false>(p.act, count, acc[i][j], acc[i][j + NG]));
+              if (p.epi.saved) put_kept<false>(kept + j * 16, plane, count, acc[i][j], acc[i][j + NG]);
+            }
       }
     } else {
       // The kept g, u of the next sixteen rows are under way while these rows' values are
@@ -663,13 +677,14 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
       // for a load issued before stores would be a wait for those too).
       auto rows = [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
-        const float* kept_at = p.epi.saved + 2 * ((long)m0 * p.N + n0);
+        const float* kept_at = p.epi.saved + ((long)m0 * p.N + n0);
+        const long plane = (long)p.M * p.N;
         long at = m0 * p.epi.ldh + n0;
         auto fetch = [&](int i, Kept* k) {
 #pragma unroll
           for (int j = 0; j < NJ; ++j)
             k[j] = FULL || (m0 + i * 16 < p.M && n0 + j * 16 < p.N)
-                       ? load_kept<FULL>(kept_at + i * 32l * p.N + j * 32, p.N - n0 - j * 16)
+                       ? load_kept<FULL>(kept_at + i * 16l * p.N + j * 16, plane, p.N - n0 - j * 16)
                        : Kept{};
         };
         Kept kept[2][NJ];
@@ -682,13 +697,24 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
           for (int j = 0; j < NJ; ++j)
             o[j] = gate_grad<FULL>(p.act, p.N - n0 - j * 16, acc[i][j], kept[i & 1][j]);
           vmem_wait_all();
+          const long row = at + i * 16 * p.epi.ldh;
+          if constexpr (FULL && WIDE) {
+            auto store = [&](void* out, auto member) {
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            if (FULL || (m0 + i * 16 < p.M && n0 + j * 16 < p.cols))
-              put_gate_grad<KIND>(p.epi, at + i * 16 * p.epi.ldh + j * 16, o[j]);
+              for (int j = 0; j < NJ; j += 2)
+                put_pair<KIND>(static_cast<T*>(out) + row + pair_at(g) + j * 16, o[j].*member, o[j + 1].*member);
+            };
+            if (p.epi.h) store(p.epi.h, &GateGrad::h);
+            store(p.epi.dg, &GateGrad::dg);
+            store(p.epi.du, &GateGrad::du);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+              if (FULL || (m0 + i * 16 < p.M && n0 + j * 16 < p.cols)) put_gate_grad<KIND>(p.epi, row + j * 16, o[j]);
+          }
         }
       };
-      if (inside && (p.N & 1) == 0)
+      if (inside)
         rows(std::true_type{});
       else
         rows(std::false_type{});
@@ -748,13 +774,15 @@ __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
   if (!in) return;
   const int mat = EPI == kEpiGate ? 0 : (int)(row / p.M);
   const long m = EPI == kEpiGate ? row : row % p.M;
-  if constexpr (EPI == kEpiGate)
-    put_gate<KIND, false>(p.epi.h, m * p.epi.ldh + n,
-                          p.epi.saved ? p.epi.saved + 2 * (m * p.N + n) : nullptr, p.act, p.N - n, v, w);
-  else if constexpr (EPI == kEpiGateGrad)
-    put_gate_grad<KIND>(p.epi, m * p.epi.ldh + n,
-                        gate_grad<false>(p.act, p.N - n, v, load_kept<false>(p.epi.saved + 2 * (m * p.N + n), p.N - n)));
-  else if (p.vec[mat] && n + 4 <= p.N)
+  const long plane = (long)p.M * p.N;
+  if constexpr (EPI == kEpiGate) {
+    put4<KIND>(static_cast<typename ElemOf<KIND>::T*>(p.epi.h) + m * p.epi.ldh + n,
+               gate_value<false>(p.act, p.N - n, v, w));
+    if (p.epi.saved) put_kept<false>(p.epi.saved + (m * p.N + n), plane, p.N - n, v, w);
+  } else if constexpr (EPI == kEpiGateGrad) {
+    const Kept k = load_kept<false>(p.epi.saved + (m * p.N + n), plane, p.N - n);
+    put_gate_grad<KIND>(p.epi, m * p.epi.ldh + n, gate_grad<false>(p.act, p.N - n, v, k));
+  } else if (p.vec[mat] && n + 4 <= p.N)
     put_row4<KIND, true>(p.out[mat], m * p.ldo[mat] + n, v, 4);
   else
     put_row4<KIND, false>(p.out[mat], m * p.ldo[mat] + n, v, p.N - n);
