@@ -403,12 +403,16 @@ struct Shape {
 // loaded before the epilogue of the last, so that they arrive under it. Two stages of LDS.
 //
 // 16 bits, large products: bound by what the matrix cores reach while LDS is read beside them
-// (0.6 of their cycles, 1130 to 1200 TFLOP/s; a large library product 1130 to 1180). Steps on the
-// way, training step of 8192 rows through 2048-8192-2048 in bf16: fragments read where they are
-// used, operations of the library in the epilogues 4578 us; hardware exponentials, the kept g, u fetched
-// a row ahead 3171; fragments read a half ahead, loads spread over the products 2676;
-// one address and one test a row of the epilogue 2614 (queued 2370). fp32: bound by the fp32 matrix cores (0.8 of their
-// cycles). Few rows or columns: by the loads' latency, which slices of K share out.
+// (0.6 of their cycles, 1130 to 1200 TFLOP/s; a large library product 1130 to 1180), and the
+// epilogues with much to load and store by the bytes (one block a compute unit holds the large
+// tiles, so that they do not run beside products). Steps on the way, training step of 8192 rows
+// through 2048-8192-2048 in bf16 (kernels in turn): fragments read where they are used, operations of the
+// library in the epilogues 4578 us; hardware exponentials, the kept g, u fetched a row ahead 3171;
+// fragments read a half ahead, loads spread over the products 2676; one address and one test a
+// row of the epilogue 2614; queued, 2373; 16 bytes a lane stored, g and u apart 2307. fp32: bound by
+// the fp32 matrix cores (0.8 of their cycles). Few rows or columns: by a step's own chain of barrier,
+// LDS reads and products, which slices of K and small tiles share out (four steps in LDS
+// instead of two changed nothing).
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
   constexpr int SUB = EPI == kEpiGate ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;

@@ -354,8 +354,8 @@ size_t dp_device_bytes(const dp_model* model);
  * Types: DP_TYPE_F32, DP_TYPE_BF16 or DP_TYPE_F16 for every matrix of a call. Products
  * run on the matrix cores of that type; sums are held in fp32 and rounded once. Of
  * the matrices between the products only h, dg and du are rounded to the type (a value
- * past the f16 range is then infinite; with up to eight rows h is not rounded). The
- * activations are evaluated to about 2e-7 of max(1, |g|).
+ * past the f16 range is then infinite; with up to eight rows, and in dw_down with up to
+ * four outputs, h is not rounded). The activations are evaluated to about 2e-7 of max(1, |g|).
  * Results do not depend on the order in which blocks run: a call repeated on the
  * same inputs gives the same bits.
  *
