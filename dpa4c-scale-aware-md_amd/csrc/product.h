@@ -403,7 +403,7 @@ struct Shape {
 // loaded before the epilogue of the last, so that they arrive under it. Two stages of LDS.
 //
 // 16 bits, large products: bound by what the matrix cores reach while LDS is read beside them
-// (0.6 of their cycles, 1130 to 1200 TFLOP/s; a large library product 1130 to 1180), and the
+// (0.6 of their cycles, 1090 to 1300 TFLOP/s; a large library product 1130 to 1600), and the
 // epilogues with much to load and store by the bytes (one block a compute unit holds the large
 // tiles, so that they do not run beside products). Steps on the way, training step of 8192 rows
 // through 2048-8192-2048 in bf16 (kernels in turn): fragments read where they are used, operations of the
