@@ -549,6 +549,8 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 #pragma unroll
       for (int j = 0; j < NJ; ++j) fb[o][j] = frag_b(next, j, o);
       __builtin_amdgcn_sched_barrier(0);
+      // (a wave in its products is served before one at its reads and barriers)
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         multiply_row<KIND, NJ>(acc[i], fb[h], i < EARLY ? fa[i < EARLY ? i : 0] : fl[h][i < EARLY ? 0 : i - EARLY]);
@@ -561,6 +563,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       // the reads have landed (a compiler-placed wait would come after the next reads and be for those too)
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
       __builtin_amdgcn_sched_barrier(0);
