@@ -421,6 +421,27 @@ def test_embed_gradient_repeats_and_order(ops):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("repeat", [1, 9])
+@pytest.mark.parametrize("width", [3, 520])
+def test_embed_gradient_lengths_of_runs(ops, repeat, width):
+    """Runs around one window and the length from which windows sum them, at every offset to
+    the windows (lead), up to the last position; exact, on small whole numbers. In one block of the sort and in
+    tiles."""
+    gen = torch.Generator().manual_seed(11)
+    lengths = [31, 32, 33, 63, 64, 65, 1, 66, 0, 95, 96, 97, 2, 127, 128, 129, 64, 65] * repeat
+    vocab = 3 * len(lengths) + 20000
+    for lead in (0, 1, 30, 31, 32, 33):
+        counts = torch.tensor([lead] + lengths)
+        ids = torch.repeat_interleave(3 * torch.arange(len(counts)), counts)
+        ids = ids[torch.randperm(len(ids), generator=gen)].int().cuda()
+        dout = torch.randint(-8, 9, (len(ids), width), generator=gen).float().cuda()
+        dt = torch.full((vocab, width), 7.0, device="cuda")
+        ops.embed_grad(ids.data_ptr(), dout.data_ptr(), dt.data_ptr(), len(ids), vocab, width, stream=stream())
+        want = torch.zeros(vocab, width, dtype=torch.float64).index_add_(0, ids.cpu().long(), dout.double().cpu())
+        torch.cuda.synchronize()
+        assert torch.equal(dt.double().cpu(), want), lead
+
+
 def test_embed_gradient_is_the_lookup_transposed(ops):
     """<lookup(table), w> = <table, gradient(w)>, exactly, on small whole numbers."""
     gen = torch.Generator().manual_seed(9)
