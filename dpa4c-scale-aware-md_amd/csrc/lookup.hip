@@ -379,9 +379,12 @@ __global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chun
   }
 }
 
-// One wave `each` table rows, whose runs its lanes look up together: eight of a large table, most of
-// whose rows have none (a wave a row then spends its time on two loads that wait for each other:
-// 45 us, now 33, of 32,768 tokens among 50,000), one of a small table, whose rows are long.
+// One wave 64 chunks of `each` table rows, whose runs its lanes look up together: eight of a large
+// table, most of whose rows have none (a wave a row then spends its time on two loads that wait for each
+// other: 45 us, now 33, of 32,768 tokens among 50,000), one of a small table, whose rows are long. The runs follow
+// one another in the sorted order; where they hold few rows in all, these are loaded before any table row is
+// stored, as a wait for a load is one for the stores before it too.
+constexpr int kTogether = 8;
 template <int KIND, int E>
 __global__ __launch_bounds__(256) void k_grad_rows(int n, int vocab, int chunks, int each,
                                                    const unsigned* __restrict__ keys,
@@ -390,46 +393,89 @@ __global__ __launch_bounds__(256) void k_grad_rows(int n, int vocab, int chunks,
                                                    const float* __restrict__ partial, float scale,
                                                    typename ElemOf<KIND>::T* __restrict__ dtable, long ld_table) {
   using C = Chunk<KIND, E>;
-  const int lane = threadIdx.x & 63;
-  const long stride = (long)gridDim.x * 4 * each;
-  for (long v0 = ((long)blockIdx.x * 4 + threadIdx.x / 64) * each; v0 < vocab; v0 += stride) {
-    const int2 mine =
-        lane < each && v0 + lane < vocab ? run_of(keys, run, n, v0 + lane) : int2{0, 0};
-    for (int k = 0; k < each && v0 + k < vocab; ++k) {
-      const int lo = __builtin_amdgcn_readlane(mine.x, k), hi = __builtin_amdgcn_readlane(mine.y, k);
-      for (int c = lane; c < chunks; c += 64) {
+  const int lane = threadIdx.x & 63, groups = (chunks + 63) / 64;
+  const long parts = (((long)vocab + each - 1) / each) * groups;
+  for (long at = (long)blockIdx.x * 4 + threadIdx.x / 64; at < parts; at += (long)gridDim.x * 4) {
+    const long v0 = at / groups * each;
+    const int c = (int)(at % groups) * 64 + lane, many = (int)min((long)each, vocab - v0);
+    const int2 mine = lane < many ? run_of(keys, run, n, v0 + lane) : int2{0, 0};
+    auto put = [&](long v, const float (&acc)[E]) {
+      C o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.v[e] = from_f32<KIND>(acc[e] * scale);
+      *reinterpret_cast<C*>(dtable + v * ld_table + (long)c * E) = o;
+    };
+    const unsigned long long with = __ballot(mine.y > mine.x);
+    int base = 0, count = 0;
+    if (with) {
+      base = __builtin_amdgcn_readlane(mine.x, __builtin_ctzll(with));
+      count = __builtin_amdgcn_readlane(mine.y, 63 - __builtin_clzll(with)) - base;
+    }
+    if (count <= kTogether) {
+      const int row = lane < count ? rows[base + lane] : 0;
+      const int v = lane < count ? (int)keys[base + lane] : -1;
+      // (read from the lanes while all of them are under way: those past the chunks hold some of them)
+      int from[kTogether], id[kTogether + 1];
+#pragma unroll
+      for (int q = 0; q < kTogether; ++q) {
+        from[q] = __builtin_amdgcn_readlane(row, q);
+        id[q] = __builtin_amdgcn_readlane(v, q);
+      }
+      id[kTogether] = -1;
+      if (c < chunks) {
+        C x[kTogether];
+#pragma unroll
+        for (int q = 0; q < kTogether; ++q)
+          if (q < count)
+            x[q] = *reinterpret_cast<const C*>(dout + from[q] * ld + (long)c * E);
         float acc[E] = {};
-        if (hi - lo <= kShort) {
-          add_rows<KIND, E, 4>(acc, lo, hi, rows, dout, ld, c);
-        } else {
-          const int w0 = lo / kWindow, w1 = (hi - 1) / kWindow;
-          // the first window's part is the second of that window where the run starts inside it
-          const long step = 2 * (long)chunks * E;
-          const float* p = partial + ((2 * (long)w0 + (lo > w0 * kWindow)) * chunks + c) * E;
+        for (int k = 0; k < many; ++k)
+          if (!((with >> k) & 1)) put(v0 + k, acc);
+#pragma unroll
+        for (int q = 0; q < kTogether; ++q)
+          if (q < count) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += to_f32<KIND>(x[q].v[e]);
+            if (id[q + 1] != id[q]) {
+              put(id[q], acc);
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+            }
+          }
+      }
+      continue;
+    }
+    for (int k = 0; k < many; ++k) {
+      const int lo = __builtin_amdgcn_readlane(mine.x, k), hi = __builtin_amdgcn_readlane(mine.y, k);
+      if (c >= chunks) continue;
+      float acc[E] = {};
+      if (hi - lo <= kShort) {
+        add_rows<KIND, E, 4>(acc, lo, hi, rows, dout, ld, c);
+      } else {
+        const int w0 = lo / kWindow, w1 = (hi - 1) / kWindow;
+        // the first window's part is the second of that window where the run starts inside it
+        const long step = 2 * (long)chunks * E;
+        const float* p = partial + ((2 * (long)w0 + (lo > w0 * kWindow)) * chunks + c) * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += p[e];
+        p = partial + (2 * (long)(w0 + 1) * chunks + c) * E;
+        int w = w0 + 1;
+        for (; w + 8 <= w1 + 1; w += 8, p += 8 * step) {
+          float y[8][E];  // (eight loads under way: a frequent token's run has a hundred windows)
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[q][e] = p[q * step + e];
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += y[q][e];
+        }
+        for (; w <= w1; ++w, p += step)
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] += p[e];
-          p = partial + (2 * (long)(w0 + 1) * chunks + c) * E;
-          int w = w0 + 1;
-          for (; w + 8 <= w1 + 1; w += 8, p += 8 * step) {
-            float y[8][E];  // (eight loads under way: a frequent token's run has a hundred windows)
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-#pragma unroll
-              for (int e = 0; e < E; ++e) y[q][e] = p[q * step + e];
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-#pragma unroll
-              for (int e = 0; e < E; ++e) acc[e] += y[q][e];
-          }
-          for (; w <= w1; ++w, p += step)
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += p[e];
-        }
-        C o;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o.v[e] = from_f32<KIND>(acc[e] * scale);
-        *reinterpret_cast<C*>(dtable + (v0 + k) * ld_table + (long)c * E) = o;
       }
+      put(v0 + k, acc);
     }
   }
 }
@@ -621,8 +667,9 @@ void launch_grad(hipStream_t st, long n, int vocab, int width, const int* ids, c
     DPAMD_LAUNCH_CHECK();
   }
   const int each = vocab >= 16384 ? 8 : 1;
-  hipLaunchKernelGGL((k_grad_rows<KIND, E>), wave_blocks((vocab + each - 1) / each), dim3(256), 0, st, (int)n, vocab,
-                     chunks, each, key, row, run, dout, ld, partial, scale, dtable, ld_table);
+  hipLaunchKernelGGL((k_grad_rows<KIND, E>), wave_blocks(((long)vocab + each - 1) / each * ((chunks + 63) / 64)),
+                     dim3(256), 0, st, (int)n, vocab, chunks, each, key, row, run, dout, ld, partial, scale, dtable,
+                     ld_table);
   DPAMD_LAUNCH_CHECK();
 }
 
