@@ -381,9 +381,10 @@ __global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chun
 
 // One wave 64 chunks of `each` table rows, whose runs its lanes look up together: eight of a large
 // table, most of whose rows have none (a wave a row then spends its time on two loads that wait for each
-// other: 45 us, now 33, of 32,768 tokens among 50,000), one of a small table, whose rows are long. The runs follow
-// one another in the sorted order; where they hold few rows in all, these are loaded before any table row is
-// stored, as a wait for a load is one for the stores before it too.
+// other: 45 us, with eight 34, of 32,768 tokens among 50,000, 1024 wide in bf16), one of a small table, whose
+// rows are long. The runs follow one another in the sorted order; where they hold few rows in all, these are
+// loaded before any table row is stored, as a wait for a load is one for the stores before it too: 26 us, for
+// 143 MB (with four table rows a wave, and with sixteen rows loaded together, no faster).
 constexpr int kTogether = 8;
 template <int KIND, int E>
 __global__ __launch_bounds__(256) void k_grad_rows(int n, int vocab, int chunks, int each,

@@ -409,7 +409,8 @@ struct Shape {
 // through 2048-8192-2048 in bf16 (kernels in turn): fragments read where they are used, operations of the
 // library in the epilogues 4578 us; hardware exponentials, the kept g, u fetched a row ahead 3171;
 // fragments read a half ahead, loads spread over the products 2676; one address and one test a
-// row of the epilogue 2614; queued, 2373; 16 bytes a lane stored, g and u apart 2307. fp32: bound by
+// row of the epilogue 2614; queued, 2373; 16 bytes a lane stored, g and u apart 2307; waves in
+// their products at raised priority 2286. fp32: bound by
 // the fp32 matrix cores (0.8 of their cycles). Few rows or columns: by a step's own chain of barrier,
 // LDS reads and products, which slices of K and small tiles share out (four steps in LDS
 // instead of two changed nothing).
