@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_place(const int* ids, con
 constexpr int kWindow = 32;     // sorted positions of one window
 constexpr int kShort = 64;      // runs up to this length are summed by their table row itself
 // Rows up to which one block sorts them all. The whole gradient, tokens among 30,000, 1024 wide in
-// bf16, us, one block / tiles: 1,500 39 / 48, 4,000 45 / 51, 8,000 55 / 55.
+// bf16, us, one block / tiles: 1,500 43 / 53, 4,000 51 / 58, 8,000 63 / 62.
 constexpr int kOneMost = 8192;
 constexpr int kScanTiles = 128; // tiles up to which each block of the sort forms its starts itself
 
@@ -379,12 +379,13 @@ __global__ __launch_bounds__(256) void k_grad_windows(int n, int vocab, int chun
   }
 }
 
-// One wave 64 chunks of `each` table rows, whose runs its lanes look up together: eight of a large
+// One wave 64 chunks of `each` table rows, whose runs its lanes look up together: several of a large
 // table, most of whose rows have none (a wave a row then spends its time on two loads that wait for each
 // other: 45 us, with eight 34, of 32,768 tokens among 50,000, 1024 wide in bf16), one of a small table, whose
 // rows are long. The runs follow one another in the sorted order; where they hold few rows in all, these are
 // loaded before any table row is stored, as a wait for a load is one for the stores before it too: 26 us, for
-// 143 MB (with four table rows a wave, and with sixteen rows loaded together, no faster).
+// 143 MB (with sixteen rows loaded together no faster; a wave for all chunks of its rows instead
+// of 64: the gradient of 16,000 tokens among 12,000, 1001 wide, 176 us, so 98).
 constexpr int kTogether = 8;
 template <int KIND, int E>
 __global__ __launch_bounds__(256) void k_grad_rows(int n, int vocab, int chunks, int each,
@@ -667,7 +668,10 @@ void launch_grad(hipStream_t st, long n, int vocab, int width, const int* ids, c
                        vocab, chunks, key, row, run, dout, ld, partial);
     DPAMD_LAUNCH_CHECK();
   }
-  const int each = vocab >= 16384 ? 8 : 1;
+  // Of n tokens among vocab, the gradient in us with 1 / 4 / 8 table rows a wave: 16,000 among 12,000, 1001 wide,
+  // 98 / 67 / 64, 1,000 among 12,000, 512 wide, 20 / 18 / 19; 8,000 among 6,000, 1024 wide, 43 / 42 / 42,
+  // 20,000 among 2,500, 1024 wide, 50 / 53 / 58; 32,768 among 50,000, 1024 wide, - / 84 / 81.
+  const int each = vocab >= 16384 ? 8 : vocab >= 8192 ? 4 : 1;
   hipLaunchKernelGGL((k_grad_rows<KIND, E>), wave_blocks(((long)vocab + each - 1) / each * ((chunks + 63) / 64)),
                      dim3(256), 0, st, (int)n, vocab, chunks, each, key, row, run, dout, ld, partial, scale, dtable,
                      ld_table);

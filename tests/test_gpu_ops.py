@@ -423,13 +423,14 @@ def test_embed_gradient_repeats_and_order(ops):
 
 @pytest.mark.parametrize("repeat", [1, 9])
 @pytest.mark.parametrize("width", [3, 520])
-def test_embed_gradient_lengths_of_runs(ops, repeat, width):
+@pytest.mark.parametrize("empty", [2500, 9000, 20000])
+def test_embed_gradient_lengths_of_runs(ops, repeat, width, empty):
     """Runs around one window and the length from which windows sum them, at every offset to
     the windows (lead), up to the last position; exact, on small whole numbers. In one block of the sort and in
-    tiles."""
+    tiles, with one table row a wave, four and eight."""
     gen = torch.Generator().manual_seed(11)
     lengths = [31, 32, 33, 63, 64, 65, 1, 66, 0, 95, 96, 97, 2, 127, 128, 129, 64, 65] * repeat
-    vocab = 3 * len(lengths) + 20000
+    vocab = 3 * len(lengths) + empty
     for lead in (0, 1, 30, 31, 32, 33):
         counts = torch.tensor([lead] + lengths)
         ids = torch.repeat_interleave(3 * torch.arange(len(counts)), counts)
