@@ -6,7 +6,6 @@
 #include <type_traits>
 
 #include "common.h"
-#include "fastmath.h"
 #include "ops.h"
 
 namespace dpamd {
@@ -76,7 +75,10 @@ __device__ __forceinline__ void put_row4(void* out, long at, const f4& v, int co
 }
 
 // The activation a(g) and its derivative: tanh, silu g s(g), gelu g Phi(g), on the hardware's
-// base-2 exponential and reciprocal (about 1 ulp each), to about 2e-7 of max(1, |g|). Phi
+// base-2 exponential and reciprocal (about 1 ulp each). tanh from q = 2 / (exp(2 |g|) + 1): 1 - q, which
+// cancels where g is small, and there (below 0.625) an odd polynomial, fitted to 4e-9 of tanh;
+// the derivative 1 - tanh^2 = q (2 - q) at any g. Relative errors in 32 bits: tanh 1.8e-7, the derivative
+// 6e-7 up to |g| = 3 and 1e-6 at 9 (the exponent's rounding). silu to about 2e-7 of max(1, |g|). Phi
 // from erfc(z) = exp(-z^2) (a1 t + .. + a5 t^5), t = 1 / (1 + 0.3275911 z) (Abramowitz and
 // Stegun 7.1.26: 1.5e-7), which shares its exponential with the derivative. With the library's
 // expf, tanhf, erff and a division the epilogues below issued about four times the instructions.
@@ -84,8 +86,13 @@ template <int ACT>
 __device__ __forceinline__ void activate(float g, float& a, float& da) {
   constexpr float kLog2e = 1.4426950408889634f;
   if constexpr (ACT == kActTanh) {
-    a = tanh_f32(g);
-    da = 1.0f - a * a;
+    const float z = fabsf(g), s = g * g;
+    const float e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * z);
+    const float q = 2.0f * e * __builtin_amdgcn_rcpf(1.0f + e);
+    const float odd =
+        -0.33333282f + s * (0.13331442f + s * (-0.05373971f + s * (0.02063909f + s * -0.00570499f)));
+    a = z < 0.625f ? g + g * s * odd : copysignf(1.0f - q, g);
+    da = q * (2.0f - q);
   } else if constexpr (ACT == kActSilu) {
     const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
     a = g * p;
