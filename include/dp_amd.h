@@ -355,7 +355,9 @@ size_t dp_device_bytes(const dp_model* model);
  * run on the matrix cores of that type; sums are held in fp32 and rounded once. Of
  * the matrices between the products only h, dg and du are rounded to the type (a value
  * past the f16 range is then infinite; with up to eight rows, and in dw_down with up to
- * four outputs, h is not rounded). The activations are evaluated to about 2e-7 of max(1, |g|).
+ * four outputs, h is not rounded). tanh and gelu are evaluated to about
+ * 2e-7 of themselves (4e-6 where gelu is about to vanish), silu and the derivatives of silu and gelu, which have
+ * zeros, to about 2e-7 of max(1, |g|).
  * Results do not depend on the order in which blocks run: a call repeated on the
  * same inputs gives the same bits.
  *

@@ -45,7 +45,7 @@ def values(n, dtype):
 # (eight rows and more, and one output, have kernels of their own)
 @pytest.mark.parametrize("n,o", [(8, 8), (1001, 8), (1001, 1)])
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
-@pytest.mark.parametrize("act", ["tanh", "silu"])
+@pytest.mark.parametrize("act", ["tanh", "silu", "gelu"])
 def test_activation(dp, act, dtype, n, o):
     t, d, f = TORCH[dtype], 8, 8
     v = values(n, dtype)
