@@ -365,12 +365,11 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
   }
 }
 
-void check_embed(int type, int64_t n, int vocab, int width, const void* ids, const void* in, const void* out) {
+void check_embed(int type, int64_t n, int vocab, int width) {
   require(type == DP_TYPE_F32 || type == DP_TYPE_BF16 || type == DP_TYPE_F16, "unknown type");
   require(n >= 0 && n <= kMaxRows, "n out of range");
   require(vocab >= 1 && vocab <= (1 << 30), "vocab must be 1 .. 2^30");
   require(width >= 1 && width <= kMaxDim, "width must be 1 .. 2^20");
-  require(out && (n == 0 || (ids && in)), "null pointer");
 }
 
 }  // namespace
@@ -415,10 +414,11 @@ size_t dp_ops_device_bytes(const dp_ops* O) { return O ? O->bytes_peak : 0; }
 int dp_embed(dp_ops* O, int type, int64_t n, int vocab, int width, const int* ids, const void* table, int64_t ld_table,
              float scale, void* out, int64_t ld_out, void* stream) {
   return guarded(O, [&]() {
-    check_embed(type, n, vocab, width, ids, table, out);
+    check_embed(type, n, vocab, width);
     const int64_t lt = row_length(ld_table, width, "ld_table is shorter than width, or too long");
     const int64_t lo = row_length(ld_out, width, "ld_out is shorter than width, or too long");
-    if (n == 0) return;
+    if (n == 0) return;  // (arrays without rows may have no address)
+    require(ids && table && out, "null pointer");
     DPAMD_HIP(hipSetDevice(O->device));
     lookup_rows(static_cast<hipStream_t>(stream), elem_of(type), n, vocab, width, ids, table, lt, scale, out, lo);
   });
@@ -427,7 +427,8 @@ int dp_embed(dp_ops* O, int type, int64_t n, int vocab, int width, const int* id
 int dp_embed_grad(dp_ops* O, int type, int64_t n, int vocab, int width, const int* ids, const void* dout,
                   int64_t ld_dout, float scale, void* dtable, int64_t ld_dtable, void* stream) {
   return guarded(O, [&]() {
-    check_embed(type, n, vocab, width, ids, dout, dtable);
+    check_embed(type, n, vocab, width);
+    require(dtable && (n == 0 || (ids && dout)), "null pointer");
     const int64_t li = row_length(ld_dout, width, "ld_dout is shorter than width, or too long");
     const int64_t lo = row_length(ld_dtable, width, "ld_dtable is shorter than width, or too long");
     DPAMD_HIP(hipSetDevice(O->device));

@@ -385,7 +385,7 @@ size_t dp_ops_device_bytes(const dp_ops* ops);
  * ids name (atom types, tokens). An id outside 0 .. vocab - 1 (a virtual atom,
  * padding) gives a row of zeros. One multiplication in fp32, rounded once. ld_table
  * and ld_out: row lengths, so the rows can be columns of wider matrices (the type
- * columns of a descriptor).
+ * columns of a descriptor). With n == 0 nothing is done and the arrays may be NULL.
  */
 int dp_embed(dp_ops* ops, int type, int64_t n, int vocab, int width, const int* d_ids,
              const void* d_table, int64_t ld_table, float scale, void* d_out, int64_t ld_out,
@@ -393,7 +393,8 @@ int dp_embed(dp_ops* ops, int type, int64_t n, int vocab, int width, const int* 
 
 /*
  * The gradient of dp_embed's table: dtable[v] = scale * sum of dout[i] over the i
- * with ids[i] == v, every row of dtable written (zeros where no id names it).
+ * with ids[i] == v, every row of dtable written (zeros where no id names it; with n == 0,
+ * where ids and dout may be NULL, all of it).
  * The ids are sorted and each row's sum is formed in fp32 in an order that depends on
  * the ids alone, and rounded once.
  */
