@@ -46,6 +46,28 @@ __global__ __launch_bounds__(256) void k_zero(unsigned char* dst, long rows, lon
     dst[at / row_bytes * stride + at % row_bytes] = 0;
 }
 
+// One step (128 bytes of k) of one block, measured: its share of a compute unit's time
+// among others, and its time alone; what a tile's epilogue adds (a plain store, the gate, the gate's
+// gradient); and the blocks that a compute unit holds. Measured with each shape forced, every
+// product of training steps of ten sizes, 33 to 131,072 rows: the one picked here took within 6 % of
+// the best one's time but for eleven of 108, of which the worst took 24 % more. (fp32: the
+// matrix cores are slow enough that 256 x 256 tiles gain nothing over 128 x 128. 16 bits: 128 x 32
+// was nowhere ahead of both neighbours.)
+struct TileShape {
+  int bm, bn, per_cu;
+  double share_us, alone_us, end_us[3];
+};
+const TileShape kShapes[2][5] = {{{256, 256, 1, 1.8, 1.8, {14, 24, 66}},
+                                {128, 128, 2, 0.62, 1.0, {5, 8, 23}},
+                                {64, 128, 3, 0.40, 0.9, {2.2, 3.2, 7}},
+                                {},
+                                {64, 32, 6, 0.22, 0.55, {0.7, 1, 1.5}}},
+                               {{},
+                                {128, 128, 2, 2.05, 2.26, {5, 8, 23}},
+                                {64, 128, 3, 1.05, 1.27, {2.2, 3.2, 7}},
+                                {128, 32, 4, 0.575, 0.75, {1.5, 1.5, 3.5}},
+                                {64, 32, 6, 0.33, 0.5, {0.7, 1, 1.5}}}};
+
 // (a grid holds fewer than 2^32 threads: the kernels stride over what is beyond)
 unsigned blocks_for(long threads) { return (unsigned)std::min((threads + 255) / 256, 1L << 20); }
 
@@ -69,33 +91,12 @@ void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride
 }
 
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu) {
-  // One step (128 bytes of k) of one block, measured: its share of a compute unit's time
-  // among others, and its time alone; what a tile's epilogue adds (a plain store, the gate, the gate's
-  // gradient); and the blocks that a compute unit holds. Measured with each shape forced, every
-  // product of training steps of ten sizes, 33 to 131,072 rows: the one picked here took within 6 % of
-  // the best one's time but for eleven of 108, of which the worst took 24 % more. (fp32: the
-  // matrix cores are slow enough that 256 x 256 tiles gain nothing over 128 x 128. 16 bits: 128 x 32
-  // was nowhere ahead of both neighbours.)
-  struct S {
-    int bm, bn, per_cu;
-    double share_us, alone_us, end_us[3];
-  };
-  static const S shapes[2][5] = {{{256, 256, 1, 1.8, 1.8, {14, 24, 66}},
-                                  {128, 128, 2, 0.62, 1.0, {5, 8, 23}},
-                                  {64, 128, 3, 0.40, 0.9, {2.2, 3.2, 7}},
-                                  {},
-                                  {64, 32, 6, 0.22, 0.55, {0.7, 1, 1.5}}},
-                                 {{},
-                                  {128, 128, 2, 2.05, 2.26, {5, 8, 23}},
-                                  {64, 128, 3, 1.05, 1.27, {2.2, 3.2, 7}},
-                                  {128, 32, 4, 0.575, 0.75, {1.5, 1.5, 3.5}},
-                                  {64, 32, 6, 0.33, 0.5, {0.7, 1, 1.5}}}};
   const int sub = what == kProdGate ? 2 : 1, bk = elem == kF32 ? 32 : 64;
   ProductPlan best{};
   double best_us = 0;
   const long steps = (K + bk - 1) / bk * segs;
   for (int k = 0; k < 5; ++k) {
-    const S& s = shapes[elem == kF32][k];
+    const TileShape& s = kShapes[elem == kF32][k];
     if (!s.bm) continue;
     // (k-strided tiles of 32 columns have too few banks apart)
     const double share = s.share_us * (what == kProdWeight && s.bn == 32 ? 1.3 : 1.0);
@@ -115,6 +116,11 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
     }
   }
   return best;
+}
+
+void tile_of(int shape, int elem, int& rows, int& cols) {
+  rows = kShapes[elem == kF32][shape].bm;
+  cols = kShapes[elem == kF32][shape].bn;
 }
 
 void run_product(hipStream_t st, ProductKind what, int elem, const ProductPlan& plan, ProductArgs& p) {

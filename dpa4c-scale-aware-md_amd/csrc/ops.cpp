@@ -219,6 +219,26 @@ OutsArgs outs_of(const dp_gated_shape& s, const void* wd) {
   return q;
 }
 
+// How each product of the block is cut.
+ProductPlan plan_gate(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdGate, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
+}
+ProductPlan plan_down(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdDown, elem_of(s.type), s.rows, s.d_out, s.d_hidden, 1, 1, ncu);
+}
+ProductPlan plan_gate_grad(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdGateGrad, elem_of(s.type), s.rows, s.d_hidden, s.d_out, 1, 1, ncu);
+}
+ProductPlan plan_input(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdInput, elem_of(s.type), s.rows, s.d_in, s.d_hidden, 2, 1, ncu);
+}
+ProductPlan plan_weights(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdWeight, elem_of(s.type), s.d_in, s.d_hidden, s.rows, 1, 2, ncu);
+}
+ProductPlan plan_down_weight(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdWeight, elem_of(s.type), s.d_hidden, s.d_out, s.rows, 1, 1, ncu);
+}
+
 void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void* wg, const void* wu, const void* wd,
                    void* y, void* saved, hipStream_t st) {
   const int elem = elem_of(s.type);
@@ -243,8 +263,8 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   Source sd{};
   if (!few) sd = source_of(s.type, wd, s.ld_down, s.d_hidden, s.d_out, r);
   const size_t at_h = r.take(bytes_of(s.type) * (size_t)n * f8);
-  const ProductPlan p1 = plan_product(kProdGate, elem, n, s.d_hidden, s.d_in, 1, 1, O->ncu);
-  const ProductPlan p2 = few ? ProductPlan{} : plan_product(kProdDown, elem, n, s.d_out, s.d_hidden, 1, 1, O->ncu);
+  const ProductPlan p1 = plan_gate(s, O->ncu);
+  const ProductPlan p2 = few ? ProductPlan{} : plan_down(s, O->ncu);
   const size_t at_part = r.take(std::max(p1.bytes, p2.bytes));
   char* ws = workspace(O, st, r.used);
 
@@ -294,10 +314,10 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
   }
   const size_t hb = bytes_of(s.type) * (size_t)n * f8;
   const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd && !few ? r.take(hb) : 0;
-  const ProductPlan p1 = few ? ProductPlan{} : plan_product(kProdGateGrad, elem, n, f, s.d_out, 1, 1, O->ncu);
-  const ProductPlan p2 = plan_product(kProdInput, elem, n, s.d_in, f, 2, 1, O->ncu);
-  const ProductPlan p3 = plan_product(kProdWeight, elem, s.d_in, f, n, 1, 2, O->ncu);
-  const ProductPlan p4 = few ? ProductPlan{} : plan_product(kProdWeight, elem, f, s.d_out, n, 1, 1, O->ncu);
+  const ProductPlan p1 = few ? ProductPlan{} : plan_gate_grad(s, O->ncu);
+  const ProductPlan p2 = plan_input(s, O->ncu);
+  const ProductPlan p3 = plan_weights(s, O->ncu);
+  const ProductPlan p4 = few ? ProductPlan{} : plan_down_weight(s, O->ncu);
   OutsArgs q = outs_of(s, wd);
   const size_t down_bytes = few ? plan_outs_grad(O->ncu, q) : p4.bytes;
   const size_t at_part = r.take(
@@ -449,6 +469,29 @@ size_t dp_gated_saved_bytes(const dp_gated_shape* shape) {
     return 8 * (size_t)s.rows * (size_t)s.d_hidden;
   } catch (...) {
     return 0;
+  }
+}
+
+int dp_debug_gated_plan(const dp_gated_shape* shape, int compute_units, int* plan) {
+  if (!plan || compute_units < 1) return DP_ERR_ARG;
+  try {
+    const dp_gated_shape s = checked(shape);
+    std::fill(plan, plan + 3 * DP_GATED_PRODUCTS, 0);
+    if (s.rows == 0) return DP_OK;
+    auto put = [&](int k, const ProductPlan& p) {
+      tile_of(p.shape, elem_of(s.type), plan[3 * k], plan[3 * k + 1]);
+      plan[3 * k + 2] = p.split;
+    };
+    const bool few = few_outputs(s.d_hidden, s.d_out);
+    if (s.rows > kFewRows) put(0, plan_gate(s, compute_units));
+    if (s.rows > kFewRows && !few) put(1, plan_down(s, compute_units));
+    if (!few) put(2, plan_gate_grad(s, compute_units));
+    put(3, plan_input(s, compute_units));
+    put(4, plan_weights(s, compute_units));
+    if (!few) put(5, plan_down_weight(s, compute_units));
+    return DP_OK;
+  } catch (...) {
+    return DP_ERR_ARG;
   }
 }
 

@@ -63,6 +63,7 @@ struct ProductPlan {
   size_t bytes;
 };
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu);
+void tile_of(int shape, int elem, int& rows, int& cols);  // of a plan's shape
 void run_product(hipStream_t st, ProductKind what, int elem, const ProductPlan& plan, ProductArgs& args);
 
 // ---- the block for a few rows (gated_rows.hip) ----

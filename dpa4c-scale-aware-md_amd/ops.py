@@ -15,7 +15,8 @@ TYPES = {"f32": TYPE_F32, "bf16": TYPE_BF16, "f16": TYPE_F16}
 ACTS = {"tanh": ACT_TANH, "silu": ACT_SILU, "gelu": ACT_GELU}
 
 EXPORTED = ("dp_ops_create", "dp_ops_destroy", "dp_ops_last_error", "dp_ops_device_bytes", "dp_embed",
-            "dp_embed_grad", "dp_gated_saved_bytes", "dp_gated_forward", "dp_gated_backward")
+            "dp_embed_grad", "dp_gated_saved_bytes", "dp_gated_forward", "dp_gated_backward", "dp_debug_gated_plan")
+PRODUCTS = ("gate", "down", "gate_grad", "dx", "dw", "dw_down")
 
 
 class _Shape(C.Structure):
@@ -39,6 +40,7 @@ def bind(L):
     L.dp_embed_grad.argtypes = [P, I, N, I, I, P, P, N, C.c_float, P, N, P]
     L.dp_gated_saved_bytes.argtypes = [S]
     L.dp_gated_saved_bytes.restype = C.c_size_t
+    L.dp_debug_gated_plan.argtypes = [S, I, C.POINTER(C.c_int)]
     L.dp_gated_forward.argtypes = [P, S, P, P, P, P, P, P, P]
     L.dp_gated_backward.argtypes = [P, S, P, P, P, P, P, P, P, P, P, P, P]
 
@@ -68,6 +70,14 @@ class GatedShape:
         """Bytes that gated_forward keeps for gated_backward (dp_gated_saved_bytes)."""
         from . import lib
         return int(lib().dp_gated_saved_bytes(C.byref(self.c)))
+
+    def plan(self, compute_units: int = 256) -> dict:
+        """{product: (tile rows, tile columns, slices)} of those that run as tiles (dp_debug_gated_plan)."""
+        from . import DeepmdException, lib
+        p = (C.c_int * (3 * len(PRODUCTS)))()
+        if lib().dp_debug_gated_plan(C.byref(self.c), compute_units, p) != 0:
+            raise DeepmdException("dp_debug_gated_plan: a shape that the calls refuse")
+        return {k: tuple(p[3 * i:3 * i + 3]) for i, k in enumerate(PRODUCTS) if p[3 * i]}
 
 
 class Operators:

@@ -422,6 +422,13 @@ typedef struct {
  * for each of rows * d_hidden. 0 for a shape that the calls refuse. */
 size_t dp_gated_saved_bytes(const dp_gated_shape* shape);
 
+/* How the block's tile products are cut on a GPU of `compute_units`: rows and columns of a tile, and slices
+ * of the summed axis, three integers for each of the products x w_gate and x w_up, h w_down, dh, dx, dw_gate and
+ * dw_up, dw_down; zeros for those that other kernels form (up to eight rows, up to four outputs). A test hook, so
+ * that each tile and its sliced form are known to be tested. */
+enum { DP_GATED_PRODUCTS = 6 };
+int dp_debug_gated_plan(const dp_gated_shape* shape, int compute_units, int* plan);
+
 /* d_saved: NULL (no backward follows) or dp_gated_saved_bytes bytes, 16-byte aligned. */
 int dp_gated_forward(dp_ops* ops, const dp_gated_shape* shape, const void* d_x,
                      const void* d_w_gate, const void* d_w_up, const void* d_w_down, void* d_y,
