@@ -253,7 +253,11 @@ typedef __attribute__((address_space(3))) s4v lds_s4;
 // which has no register result, because the compiler waits for every such load that it
 // knows of before any transposing LDS read, as it can not tell that they are of different tiles:
 // with the builtin each row of k-strided fragments waited for the loads issued just before it.
-// (m0 is a register that a statement may not name as changed; nothing else in these kernels uses it.)
+// (m0 is a register that a statement may not name as changed; nothing else in these kernels uses it.
+// The s_nop is the wait state between m0's move and the load. The compiler inserts none for what a
+// statement reads: had a vector instruction written the address, the load would need five after it. In
+// all kernels built the address comes from scalar instructions, which need none, and
+// tests/test_ops_listing.py holds the build to it; five states in the statement cost 1 % of the large products.)
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned offset, unsigned lds) {
   // (both in scalar registers, whatever the compiler knows of them)
   lds = __builtin_amdgcn_readfirstlane(lds);
