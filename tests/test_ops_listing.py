@@ -36,8 +36,8 @@ def too_early(lines):
             for o, a in reversed(before):
                 if states >= STATES:
                     break
-                # (the second operand of an addition with carry is written too)
-                if o.startswith("v_") and (scalars(a[0]) | (scalars(a[1]) if len(a) > 2 else set())) & address:
+                written = a[:2] if "_co_" in o or "div_scale" in o else a[:1]  # (the former two write a mask too)
+                if o.startswith("v_") and address & set().union(*map(scalars, written)):
                     bad.append(line.strip())
                     break
                 states += int(a[0], 0) + 1 if o == "s_nop" else 1
@@ -51,6 +51,7 @@ def test_reader():
     assert too_early((head + "\ts_mov_b32 m0, s9\n\ts_nop 0\n" + load).split("\n")) == (1, [load.strip().split("\n")[0]])
     assert too_early((head + "\ts_mov_b32 m0, s9\n\ts_nop 3\n" + load).split("\n")) == (1, [])
     assert too_early(("\ts_add_u32 s4, s6, s7\n\ts_mov_b32 m0, s9\n\ts_nop 0\n" + load).split("\n")) == (1, [])
+    assert too_early(("\tv_add_u32_e32 v1, s4, v1\n" + load).split("\n")) == (1, [])
     assert too_early((head.replace("s5", "s6") + load).split("\n")) == (1, [])
 
 
