@@ -7,7 +7,6 @@ the calls return without waiting. Failures raise DeepmdException.
 from __future__ import annotations
 
 import ctypes as C
-import operator
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 ACT_TANH, ACT_SILU, ACT_GELU = 0, 1, 2
@@ -45,15 +44,10 @@ def bind(L):
     L.dp_gated_backward.argtypes = [P, S, P, P, P, P, P, P, P, P, P, P, P]
 
 
-def _size(v, bits=32):
-    """v, or -1, which every call refuses, where a C integer does not hold it (ctypes drops
-    its upper bits)."""
-    v = operator.index(v)
-    return v if -2 ** (bits - 1) <= v < 2 ** (bits - 1) else -1
-
-
+# ctypes drops the upper bits of what a C integer does not hold: such sizes are passed on as -1, which every
+# call refuses (one test of several together: a call on few rows takes as long as its Python).
 def _code(names, v):
-    return names.get(v, -1) if isinstance(v, str) else _size(v)
+    return names.get(v, -1) if isinstance(v, str) else -1 if v >> 31 else int(v)
 
 
 class GatedShape:
@@ -62,9 +56,12 @@ class GatedShape:
 
     def __init__(self, rows, d_in, d_hidden, d_out, dtype="f32", act="silu", ld_x=0, ld_y=0, ld_hidden=0,
                  ld_down=0):
-        lds = (_size(v, 64) for v in (ld_x, ld_y, ld_hidden, ld_down))
-        self.c = _Shape(_size(rows, 64), _size(d_in), _size(d_hidden), _size(d_out), _code(TYPES, dtype),
-                        _code(ACTS, act), *lds)
+        if (d_in | d_hidden | d_out) >> 31:
+            d_in = -1
+        if (rows | ld_x | ld_y | ld_hidden | ld_down) >> 63:
+            rows = -1
+        self.c = _Shape(rows, d_in, d_hidden, d_out, _code(TYPES, dtype), _code(ACTS, act), ld_x, ld_y, ld_hidden,
+                        ld_down)
 
     def saved_bytes(self) -> int:
         """Bytes that gated_forward keeps for gated_backward (dp_gated_saved_bytes)."""
@@ -107,16 +104,19 @@ class Operators:
     def embed(self, d_ids: int, d_table: int, d_out: int, n: int, vocab: int, width: int, dtype="f32",
               scale: float = 1.0, ld_table: int = 0, ld_out: int = 0, stream: int = 0):
         """out[i] = scale * table[ids[i]]; zeros for an id outside the table (dp_embed)."""
-        self._check(self._lib.dp_embed(self._h, _code(TYPES, dtype), _size(n, 64), _size(vocab), _size(width),
-                                       d_ids or None, d_table or None, _size(ld_table, 64), scale, d_out or None,
-                                       _size(ld_out, 64), stream or None))
+        if (vocab | width) >> 31 or (n | ld_table | ld_out) >> 63:
+            n = -1
+        self._check(self._lib.dp_embed(self._h, _code(TYPES, dtype), n, vocab, width, d_ids or None, d_table or None,
+                                       ld_table, scale, d_out or None, ld_out, stream or None))
 
     def embed_grad(self, d_ids: int, d_dout: int, d_dtable: int, n: int, vocab: int, width: int, dtype="f32",
                    scale: float = 1.0, ld_dout: int = 0, ld_dtable: int = 0, stream: int = 0):
         """dtable[v] = scale * sum of dout[i] over ids[i] == v, every row written (dp_embed_grad)."""
-        self._check(self._lib.dp_embed_grad(self._h, _code(TYPES, dtype), _size(n, 64), _size(vocab), _size(width),
-                                            d_ids or None, d_dout or None, _size(ld_dout, 64), scale,
-                                            d_dtable or None, _size(ld_dtable, 64), stream or None))
+        if (vocab | width) >> 31 or (n | ld_dout | ld_dtable) >> 63:
+            n = -1
+        self._check(self._lib.dp_embed_grad(self._h, _code(TYPES, dtype), n, vocab, width, d_ids or None,
+                                            d_dout or None, ld_dout, scale, d_dtable or None, ld_dtable,
+                                            stream or None))
 
     def gated_forward(self, shape: GatedShape, d_x: int, d_w_gate: int, d_w_up: int, d_w_down: int, d_y: int,
                       saved: int = 0, stream: int = 0):

@@ -34,10 +34,11 @@ def test_lookup(dp, call):
     try:
         run(16, 16, 16, 4, 5, 8)
         assert ops._lib.args[1:5] == (0, 4, 5, 8)
-        for at, args in ((2, (2 ** 64 + 4, 5, 8)), (3, (4, 2 ** 32 + 5, 8)), (4, (4, 5, 2 ** 32 + 8))):
+        for args in ((2 ** 64 + 4, 5, 8), (4, 2 ** 32 + 5, 8), (4, 5, 2 ** 32 + 8), (4, -5, 8),
+                     (4, 5, 8, "f32", 1.0, 2 ** 64 + 8), (4, 5, 8, "f32", 1.0, 0, 2 ** 64 + 8)):
             run(16, 16, 16, *args)
-            assert ops._lib.args[at] == -1
-        run(16, 16, 16, 4, 5, 8, "f32", 1.0, 2 ** 64 + 8, 2 ** 64 + 8)
-        assert ops._lib.args.count(-1) == 2
+            assert ops._lib.args[2] == -1  # (n, which the library refuses)
+        run(16, 16, 16, 4, 5, 8, 2 ** 32)
+        assert ops._lib.args[1] == -1
     finally:
         ops._h = None
