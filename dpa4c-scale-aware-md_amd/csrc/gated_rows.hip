@@ -1,6 +1,7 @@
 // The gated block for a few rows (single tokens, single atoms): the weights are read once and
 // each element meets up to eight rows, so the bytes bound it; vector units, fp32
-// throughout (h is not rounded), matrices of any alignment.
+// throughout (h is not rounded, as it is from nine rows on; the backward is the same for any number
+// of rows, and rounds it), matrices of any alignment.
 //
 //   k_rows_gate: a block takes 16 bytes by eight lanes of columns (one 128-byte line a
 //     row of weights) and a slice of K, 32 rows of weights at a time in 32 lane groups; their sums
@@ -82,7 +83,7 @@ __device__ __forceinline__ void sweep(float (&acc)[R][MATS][E], const float* x, 
 }
 
 // The 32 lane groups' sums joined (always in the same order) and written: out[r][m][column]
-// of this slice. `own`: the lane's columns are not also a neighbour's.
+// of this slice; c is the block's first column.
 template <int R, int MATS, int E>
 __device__ __forceinline__ void join_groups(float (&acc)[R][MATS][E], float* lds, float* out, int rows, int cols,
                                             int c) {

@@ -4,8 +4,10 @@
 // written. A row is cut into chunks as wide as its alignment allows (16 bytes at most), lanes side by side on
 // a row's chunks, four rows a thread so that their loads are under way together.
 //
-// Gradient: dE[v] = s sum_{id_i = v} dout_i, without atomics, so that the sums' order is
-// fixed by the ids alone. It reads n rows, writes vocab rows. Two forms:
+// Gradient: dE[v] = s sum_{id_i = v} dout_i, without floating-point atomics, so that the sums'
+// order does not depend on which block runs first: it is fixed by the ids, the sizes, and the
+// alignment of the rows (which sets the chunks, and with them the lanes of a row, the tables of a block and,
+// near its limit, the form). It reads n rows, writes vocab rows. Two forms:
 //
 // Few ids (atom types): a block sums a contiguous share of the rows into tables of its own in
 // LDS, one for each row it has under way, so that every entry has one thread; the blocks'
@@ -670,7 +672,9 @@ void launch_grad(hipStream_t st, long n, int vocab, int width, const int* ids, c
   }
   // Of n tokens among vocab, the gradient in us with 1 / 4 / 8 table rows a wave: 16,000 among 12,000, 1001 wide,
   // 98 / 67 / 64, 1,000 among 12,000, 512 wide, 20 / 18 / 19; 8,000 among 6,000, 1024 wide, 43 / 42 / 42,
-  // 20,000 among 2,500, 1024 wide, 50 / 53 / 58; 32,768 among 50,000, 1024 wide, - / 84 / 81.
+  // 20,000 among 2,500, 1024 wide, 50 / 53 / 58; 32,768 among 50,000, 1024 wide, 111 / 85 / 81. (The table's size
+  // stands for few rows a table row. Where a large table has many, one is ahead: 500,000 among 20,000, 64
+  // wide in fp32, 136 / 142 / 147, 256 wide in bf16, 164 / 171 / 177; 100,000 among them, 60 / 55 / 56.)
   const int each = vocab >= 16384 ? 8 : vocab >= 8192 ? 4 : 1;
   hipLaunchKernelGGL((k_grad_rows<KIND, E>), wave_blocks(((long)vocab + each - 1) / each * ((chunks + 63) / 64)),
                      dim3(256), 0, st, (int)n, vocab, chunks, each, key, row, run, dout, ld, partial, scale, dtable,

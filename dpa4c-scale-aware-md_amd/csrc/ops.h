@@ -23,6 +23,15 @@ struct Operand {
 };
 
 // h, dg and du as operands [M][ldh]; saved: g and then u, [M][N] each.
+//
+// h, dg and du are rounded to the call's type, once, because they are operands of the next products, whose matrix
+// cores take that type. It costs about half a bit: errors against 64 bits, relative to the outputs' size, of
+// 0.0023 in bf16 training steps (0.0017 with all of it in 32 bits and only the outputs rounded) and
+// 0.00029 in fp16 forwards (0.00021). As two numbers of 16 bits each they would keep 16 bits or more, for twice the
+// operations of h w_down, dx and the weights' gradients: of the 2.3 ms of a step of 8,192 rows
+// through 2048-8192-2048 in bf16 these take 1.3. Who needs the digits calls with fp32.
+// In f16 their range matters too: beyond 65,504 they are infinite; dg and du below 6e-5 have fewer
+// bits, and below 3e-8 they are zero.
 struct EpiArgs {
   void *h, *dg, *du;
   long ldh;

@@ -243,7 +243,7 @@ __device__ __forceinline__ void put_pair(typename ElemOf<KIND>::T* p, const f4& 
 // ---- the product ------------------------------------------------------------------------
 
 // Operand layouts: rows with k contiguous (kRowK), or k rows with the operand's rows
-// contiguous (kRowMajorK: element (r, k) at k ld + r).
+// contiguous (kColK: element (r, k) at k ld + r).
 enum Layout { kRowK = 0, kColK = 1 };
 
 typedef __attribute__((address_space(3))) s4v lds_s4;

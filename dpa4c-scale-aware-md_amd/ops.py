@@ -2,7 +2,8 @@
 the gated feed-forward block, forward and backward (the dp_ops part of
 include/dp_amd.h). As the device entry points of `DeepPot`, every array is a raw
 device pointer (an int), and work is ordered on `stream`; unlike the synchronous ones
-the calls return without waiting. Failures raise DeepmdException.
+the calls return without waiting. Failures raise DeepmdException. Ids are 32-bit integers (int32): a
+pointer to torch's int64 indices is read as pairs of them.
 """
 from __future__ import annotations
 

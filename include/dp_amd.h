@@ -352,16 +352,22 @@ size_t dp_device_bytes(const dp_model* model);
  * not overlap. Weights are [in][out], as in the model files.
  *
  * Types: DP_TYPE_F32, DP_TYPE_BF16 or DP_TYPE_F16 for every matrix of a call. Products
- * run on the matrix cores of that type; sums are held in fp32 and rounded once. Of
- * the matrices between the products only h, dg and du are rounded to the type (a value
- * past the f16 range is then infinite; with up to eight rows, and in dw_down with up to
- * four outputs, h is not rounded). tanh and gelu are evaluated to about
+ * run on the matrix cores of that type (a forward of up to eight rows, and the products with w_down
+ * of up to four outputs, on the vector units, in fp32); sums are held in fp32 and rounded once. Of
+ * the matrices between the products only h, dg and du are rounded to the type; h is not
+ * in a forward of up to eight rows, and in dw_down with up to four outputs. In f16 a value
+ * of theirs past 65,504 is then infinite (of h: y from nine rows on, and dw_down from any number of
+ * rows with more than four outputs), and dg and du lose bits below 6e-5 and are zero below 3e-8: the backward
+ * is linear in dy, so a caller whose dy is small scales it by a power of two, and the
+ * gradients back. tanh and gelu are evaluated to about
  * 2e-7 of themselves (4e-6 where gelu is about to vanish), silu and the derivatives of silu and gelu, which have
  * zeros, to about 2e-7 of max(1, |g|).
  * Results do not depend on the order in which blocks run: a call repeated on the
- * same inputs gives the same bits.
+ * same inputs at the same alignment gives the same bits.
  *
- * A handle keeps one workspace for each stream it is used with, which grows to the largest call.
+ * A handle keeps one workspace for each stream it is used with, which grows to the largest call and
+ * is released by dp_ops_destroy. It knows a stream by its address: destroy a stream only once its
+ * work has ended, as one created later may have the same address and takes over the workspace.
  * Calls on several streams need no ordering by the caller beyond that of their own inputs
  * and outputs. The calls can be captured into a HIP graph once the same call has run
  * on that stream (so that the workspace is there; else DP_ERR_ARG); a workspace that a
@@ -382,7 +388,7 @@ size_t dp_ops_device_bytes(const dp_ops* ops);
 
 /*
  * out[i] = scale * table[ids[i]], i < n: the rows of a table [vocab][width] that the
- * ids name (atom types, tokens). An id outside 0 .. vocab - 1 (a virtual atom,
+ * ids name (atom types, tokens), 32-bit integers. An id outside 0 .. vocab - 1 (a virtual atom,
  * padding) gives a row of zeros. One multiplication in fp32, rounded once. ld_table
  * and ld_out: row lengths, so the rows can be columns of wider matrices (the type
  * columns of a descriptor). With n == 0 nothing is done and the arrays may be NULL.
@@ -395,8 +401,8 @@ int dp_embed(dp_ops* ops, int type, int64_t n, int vocab, int width, const int* 
  * The gradient of dp_embed's table: dtable[v] = scale * sum of dout[i] over the i
  * with ids[i] == v, every row of dtable written (zeros where no id names it; with n == 0,
  * where ids and dout may be NULL, all of it).
- * The ids are sorted and each row's sum is formed in fp32 in an order that depends on
- * the ids alone, and rounded once.
+ * Each row's sum is formed in fp32 and rounded once. Its order depends on the ids, the sizes, and the
+ * alignment and row lengths of dout and dtable, not on the order in which blocks run.
  */
 int dp_embed_grad(dp_ops* ops, int type, int64_t n, int vocab, int width, const int* d_ids,
                   const void* d_dout, int64_t ld_dout, float scale, void* d_dtable,
