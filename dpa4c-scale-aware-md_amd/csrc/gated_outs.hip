@@ -2,7 +2,8 @@
 // columns fill a thirtieth of a tile, so these run on the vector units, where the bytes of
 // h, and of the kept g and u, bound them.
 //
-//   k_outs_down: y = h w_down; a group of lanes a row of h, w_down in LDS.
+//   k_outs_down: y = h w_down; a group of lanes a row of h, w_down in LDS. h comes in fp32 whatever the
+//     type: it is rounded for the matrix cores alone.
 //   k_outs_grad: from dy and the kept g, u a thread forms dh = dy w_down^T of four columns,
 //     then dg, du and h, row after row of its block's slice, and keeps its sums of h dy in registers: h is
 //     neither rounded nor stored.
@@ -19,7 +20,7 @@ namespace {
 template <int KIND, int O, int LANES>
 __global__ __launch_bounds__(256) void k_outs_down(const OutsArgs p) {
   using T = typename ElemOf<KIND>::T;
-  constexpr int V = 16 / sizeof(T), U = 4;
+  constexpr int V = 4, U = 4;
   extern __shared__ __align__(16) float w[];  // [O][ldh], zeros beyond w_down
   const int ldh = (int)p.ldh;
 #pragma unroll 4
@@ -31,26 +32,23 @@ __global__ __launch_bounds__(256) void k_outs_down(const OutsArgs p) {
   const int lane = threadIdx.x % LANES, chunks = ldh / V;
   for (long r0 = (long)blockIdx.x * (256 / LANES); r0 < p.rows; r0 += (long)gridDim.x * (256 / LANES)) {
     const long row = r0 + threadIdx.x / LANES;
-    const T* h = static_cast<const T*>(p.h) + std::min(row, p.rows - 1) * p.ldh;
+    const float* h = p.h + std::min(row, p.rows - 1) * p.ldh;
     float acc[O] = {};
-    struct alignas(16) Chunk {
-      T v[V];
-    };
-    auto add = [&](const Chunk& a, int q) {
+    auto add = [&](const f4& a, int q) {
 #pragma unroll
       for (int e = 0; e < V; ++e)
 #pragma unroll
-        for (int k = 0; k < O; ++k) acc[k] += to_f32<KIND>(a.v[e]) * w[k * ldh + q * V + e];
+        for (int k = 0; k < O; ++k) acc[k] += a[e] * w[k * ldh + q * V + e];
     };
     int q = lane;
     for (; q + (U - 1) * LANES < chunks; q += U * LANES) {
-      Chunk a[U];
+      f4 a[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) a[u] = *reinterpret_cast<const Chunk*>(h + (q + u * LANES) * V);
+      for (int u = 0; u < U; ++u) a[u] = *reinterpret_cast<const f4*>(h + (q + u * LANES) * V);
 #pragma unroll
       for (int u = 0; u < U; ++u) add(a[u], q + u * LANES);
     }
-    for (; q < chunks; q += LANES) add(*reinterpret_cast<const Chunk*>(h + q * V), q);
+    for (; q < chunks; q += LANES) add(*reinterpret_cast<const f4*>(h + q * V), q);
 #pragma unroll
     for (int k = 0; k < O; ++k) {
 #pragma unroll
@@ -182,9 +180,11 @@ void with_kind(int elem, F&& f) {
 
 }  // namespace
 
-// (w_down in LDS: up to 32 KB.) A training step of 31,920 rows through 70-96-o in fp32, of 12,288 through
-// 512-240-o and of 8,192 through 512-1024-o in bf16, us, these kernels / tiles, o = 1: 114 / 145 and
-// 78 / 99; o = 4: 83 / 97 and 138 / 156; eight outputs were behind in 16 bits: 99 / 92 and 178 / 153
+// (w_down in LDS: up to 32 KB.) A training step, us, these kernels / tiles: 31,920 rows through 70-96-1 in fp32 101 / 116,
+// in bf16 70 / 80; 70-96-4 in fp32 105 / 116; in bf16 12,288 rows through 512-240-1 74 / 89, 512-240-4 82 / 89;
+// 8,192 through 512-1024-1 136 / 152, 512-1024-4 150 / 152; 131,072 through 2048-240-1 1,086 / 1,170. A
+// forward alone in bf16 takes longer, as h is 4 bytes here and 2 as an operand: 26 / 21, 23 / 23, 24 / 23, 35 / 35,
+// 37 / 35 and 300 / 288 of these, and has one rounding fewer. Eight outputs were behind in 16 bits
 // (w_down's eight reads of LDS an element of h).
 bool few_outputs(int d_hidden, int d_out) {
   return d_out <= kFewOutputs && (long)(d_hidden + 7) / 8 * 8 * outs_of(d_out) <= 8192;
@@ -192,7 +192,7 @@ bool few_outputs(int d_hidden, int d_out) {
 
 void run_outs_down(hipStream_t st, int elem, int ncu, const OutsArgs& p) {
   // a row's chunks four a lane where sixteen lanes do for that
-  const bool wide = p.ldh * (elem == kF32 ? 4 : 2) > 16 * 16 * 16;
+  const bool wide = p.ldh * 4 > 16 * 16 * 16;
   const long each = 256 / (wide ? 64 : 16);
   const dim3 grid((unsigned)std::min((p.rows + each - 1) / each, 4l * ncu));
   with_kind(elem, [&](auto kind) {

@@ -262,7 +262,7 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   const bool few = few_outputs(s.d_hidden, s.d_out);
   Source sd{};
   if (!few) sd = source_of(s.type, wd, s.ld_down, s.d_hidden, s.d_out, r);
-  const size_t at_h = r.take(bytes_of(s.type) * (size_t)n * f8);
+  const size_t at_h = r.take((few ? sizeof(float) : bytes_of(s.type)) * (size_t)n * f8);
   const ProductPlan p1 = plan_gate(s, O->ncu);
   const ProductPlan p2 = few ? ProductPlan{} : plan_down(s, O->ncu);
   const size_t at_part = r.take(std::max(p1.bytes, p2.bytes));
@@ -276,7 +276,11 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   a.b[1] = ou;
   a.cols = (int)f8;
   a.act = s.act;
-  a.epi.h = ws + at_h;
+  // (with few outputs h is no operand of the matrix cores, so that nothing asks for its rounding)
+  if (few)
+    a.epi.h32 = reinterpret_cast<float*>(ws + at_h);
+  else
+    a.epi.h = ws + at_h;
   a.epi.ldh = f8;
   a.epi.saved = static_cast<float*>(saved);
   a.partial = reinterpret_cast<float*>(ws + at_part);
@@ -284,7 +288,7 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
 
   if (few) {
     OutsArgs q = outs_of(s, wd);
-    q.h = a.epi.h;
+    q.h = a.epi.h32;
     q.y = y;
     return run_outs_down(st, elem, O->ncu, q);
   }

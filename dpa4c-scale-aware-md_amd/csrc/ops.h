@@ -24,8 +24,8 @@ struct Operand {
 
 // h, dg and du as operands [M][ldh]; saved: g and then u, [M][N] each.
 //
-// h, dg and du are rounded to the call's type, once, because they are operands of the next products, whose matrix
-// cores take that type. It costs about half a bit: errors against 64 bits, relative to the outputs' size, of
+// h, dg and du are rounded to the call's type, once, where they are operands of the next products, whose matrix
+// cores take that type (h of few rows or few outputs meets none, and stays in fp32). It costs about half a bit: errors against 64 bits, relative to the outputs' size, of
 // 0.0023 in bf16 training steps (0.0017 with all of it in 32 bits and only the outputs rounded) and
 // 0.00029 in fp16 forwards (0.00021). As two numbers of 16 bits each they would keep 16 bits or more, for twice the
 // operations of h w_down, dx and the weights' gradients: of the 2.3 ms of a step of 8,192 rows
@@ -34,6 +34,7 @@ struct Operand {
 // bits, and below 3e-8 they are zero.
 struct EpiArgs {
   void *h, *dg, *du;
+  float* h32;  // h, not rounded, in place of `h` where no product follows (of a gate), or null
   long ldh;
   float* saved;
 };
@@ -94,7 +95,8 @@ constexpr int kFewOutputs = 4;
 struct OutsArgs {
   long rows;
   int f, o, act;
-  const void *h, *wd, *dy;  // h: rows of ldh, zeros from f on
+  const float* h;  // rows of ldh, zeros from f on
+  const void *wd, *dy;
   const float* saved;
   long ldh, ld_down, ld_y;
   void *y, *dg, *du, *dwd;

@@ -670,6 +670,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
       float* kept = p.epi.saved ? p.epi.saved + ((long)m0 * p.N + n0) : nullptr;
       const long hrow = 16 * p.epi.ldh, krow = p.epi.saved ? 16l * p.N : 0, plane = (long)p.M * p.N;
       T* to = static_cast<T*>(p.epi.h);
+      float* h32 = p.epi.h32;
       constexpr int NG = NJ / SUB;  // fragments of g, and as many of u
       if (inside) {
 #pragma unroll
@@ -680,7 +681,10 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
             v[j] = gate_value<true>(p.act, 4, acc[i][j], acc[i][j + NG]);
             if (p.epi.saved) put_kept<true>(kept + j * 16, plane, 4, acc[i][j], acc[i][j + NG]);
           }
-          if constexpr (WIDE && NG % 2 == 0) {
+          if (h32) {
+#pragma unroll
+            for (int j = 0; j < NG; ++j) *reinterpret_cast<f4*>(h32 + h + j * 16) = v[j];
+          } else if constexpr (WIDE && NG % 2 == 0) {
 #pragma unroll
             for (int j = 0; j < NG; j += 2) put_pair<KIND>(to + h + pair_at(g) + j * 16, v[j], v[j + 1]);
           } else {
@@ -695,7 +699,11 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
           for (int j = 0; j < NG; ++j)
             if (m0 + i * 16 < p.M && n0 + j * 16 < p.cols) {
               const int count = p.N - n0 - j * 16;
-              put4<KIND>(to + h + j * 16, gate_value<false>(p.act, count, acc[i][j], acc[i][j + NG]));
+              const f4 v = gate_value<false>(p.act, count, acc[i][j], acc[i][j + NG]);
+              if (h32)
+                *reinterpret_cast<f4*>(h32 + h + j * 16) = v;
+              else
+                put4<KIND>(to + h + j * 16, v);
               if (p.epi.saved) put_kept<false>(kept + j * 16, plane, count, acc[i][j], acc[i][j + NG]);
             }
       }
@@ -804,8 +812,11 @@ __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
   const long m = EPI == kEpiGate ? row : row % p.M;
   const long plane = (long)p.M * p.N;
   if constexpr (EPI == kEpiGate) {
-    put4<KIND>(static_cast<typename ElemOf<KIND>::T*>(p.epi.h) + m * p.epi.ldh + n,
-               gate_value<false>(p.act, p.N - n, v, w));
+    const f4 h = gate_value<false>(p.act, p.N - n, v, w);
+    if (p.epi.h32)
+      *reinterpret_cast<f4*>(p.epi.h32 + m * p.epi.ldh + n) = h;
+    else
+      put4<KIND>(static_cast<typename ElemOf<KIND>::T*>(p.epi.h) + m * p.epi.ldh + n, h);
     if (p.epi.saved) put_kept<false>(p.epi.saved + (m * p.N + n), plane, p.N - n, v, w);
   } else if constexpr (EPI == kEpiGateGrad) {
     const Kept k = load_kept<false>(p.epi.saved + (m * p.N + n), plane, p.N - n);

@@ -355,9 +355,10 @@ size_t dp_device_bytes(const dp_model* model);
  * run on the matrix cores of that type (a forward of up to eight rows, and the products with w_down
  * of up to four outputs, on the vector units, in fp32); sums are held in fp32 and rounded once. Of
  * the matrices between the products only h, dg and du are rounded to the type; h is not
- * in a forward of up to eight rows, and in dw_down with up to four outputs. In f16 a value
- * of theirs past 65,504 is then infinite (of h: y from nine rows on, and dw_down from any number of
- * rows with more than four outputs), and dg and du lose bits below 6e-5 and are zero below 3e-8: the backward
+ * in a forward of up to eight rows, and with up to four outputs (to 8,192 hidden columns of one
+ * output, 4,096 of two, 2,048 of three and four) in y and dw_down. In f16 a value
+ * of theirs past 65,504 is then infinite (of h: with more outputs, y from nine rows on, and dw_down from any
+ * number of rows), and dg and du lose bits below 6e-5 and are zero below 3e-8: the backward
  * is linear in dy, so a caller whose dy is small scales it by a power of two, and the
  * gradients back. tanh and gelu are evaluated to about
  * 2e-7 of themselves (4e-6 where gelu is about to vanish), silu and the derivatives of silu and gelu, which have
