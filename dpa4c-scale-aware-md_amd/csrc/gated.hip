@@ -91,7 +91,7 @@ void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride
 }
 
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu) {
-  const int sub = what == kProdGate ? 2 : 1, bk = elem == kF32 ? 32 : 64;
+  const int sub = what == kProdGate ? 2 : 1, bk = elem == kF32 ? 32 : elem == kI8 ? 128 : 64;
   ProductPlan best{};
   double best_us = 0;
   const long steps = (K + bk - 1) / bk * segs;

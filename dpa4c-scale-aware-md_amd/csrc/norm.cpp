@@ -1,0 +1,180 @@
+// C ABI of the group norm: argument checks, the choice of a form, workspaces.
+#include <hip/hip_runtime.h>
+
+#include "norm.h"
+#include "ops_host.h"
+
+namespace dpamd {
+
+template <>
+void norm_launch<0>(hipStream_t, const NormArgs&);
+template <>
+void norm_launch<1>(hipStream_t, const NormArgs&);
+template <>
+void norm_launch<2>(hipStream_t, const NormArgs&);
+template <>
+void norm_grad_launch<0>(hipStream_t, const NormArgs&);
+template <>
+void norm_grad_launch<1>(hipStream_t, const NormArgs&);
+template <>
+void norm_grad_launch<2>(hipStream_t, const NormArgs&);
+
+namespace {
+
+// lanes that sum the `entries` parts of each of `groups`, of `threads` in all
+int lanes_of(int groups, int entries, int threads) {
+  int lanes = 0;
+  while (lanes < 6 && (2 << lanes) <= entries && ((long)groups << (lanes + 1)) <= threads) ++lanes;
+  return lanes;
+}
+
+}  // namespace
+
+NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
+  const int most = elem == 2 ? 4 : 8;  // 16 bytes
+  p.per = p.channels / p.groups;
+  p.vec = p.per % most == 0 ? most : p.per % 2 == 0 ? 2 : 1;
+  p.chunks = p.channels / p.vec;
+  p.chunks_per = p.per / p.vec;
+  const long length = std::max(1L, p.rows / p.frames);
+  const bool affine = grad && (p.dgamma || p.dbeta);
+  NormNeeds need{};
+  p.slices = 1;
+  if (!p.starts && p.frames == p.rows && p.chunks <= 1024) {
+    p.form = kNormRows;
+    const int T = p.chunks <= 16 ? 16 : p.chunks <= 256 ? 64 : 256;
+    p.lanes = lanes_of(p.groups, p.chunks_per, T);
+    p.blocks = (int)std::min((p.rows + 256 / T - 1) / (256 / T), 2L * ncu);
+    if (affine) need.partial = 8 * (size_t)p.blocks * p.channels;
+  } else {
+    // whole groups a block, at least 16 chunks (256 bytes of a row) where that leaves no compute unit idle
+    int gp = std::max(1, std::min(p.groups, 256 / p.chunks_per));
+    auto blocks = [&](int g) { return (long)p.frames * ((p.groups + g - 1) / g); };
+    while (gp > 1 && (gp + 1) / 2 * p.chunks_per >= 4 &&
+           (blocks(gp) < ncu || (blocks(gp) < 4 * ncu && (gp + 1) / 2 * p.chunks_per >= 16)) &&
+           256 / ((gp + 1) / 2 * p.chunks_per) <= 2 * length)
+      gp = (gp + 1) / 2;
+    const double bytes = 4.0 * p.rows * p.channels;
+    const double each = 4.0 * length * gp * p.per * ((blocks(gp) + ncu - 1) / ncu);
+    // us: a block's own pace, and three launches with all compute units at work
+    const bool slices = p.chunks_per > 256 || each / 15e3 > 10.0 + bytes / 2e6;
+    if (!slices) {
+      p.form = kNormFrames;
+      p.part = gp * p.chunks_per;
+      p.parts = (p.chunks + p.part - 1) / p.part;
+      p.lanes = lanes_of(gp, 256 / p.part * p.chunks_per, 256);
+      p.blocks = grad ? std::max(1, 8 * ncu / p.parts) : 65535;
+      if (affine) need.partial = 8 * (size_t)std::min(p.frames, p.blocks) * p.channels;
+    } else {
+      p.form = kNormSlices;
+      p.part = std::min(256, p.chunks);
+      p.parts = (p.chunks + p.part - 1) / p.part;
+      const long want = std::max(1L, 8L * ncu / ((long)p.parts * p.frames));
+      const int rows_block = 256 / p.part * 4;
+      p.slices = (int)std::min(want, std::max(1L, length / rows_block));
+      p.blocks = (int)std::min((long)p.frames, std::max(1L, 8L * ncu / ((long)p.parts * p.slices)));
+      if (!grad || p.dx) need.pairs = 8 * (size_t)p.frames * p.slices * p.chunks;
+      if (grad && p.dx) need.sums = 8 * (size_t)p.frames * p.groups;
+      if (affine) need.partial = 8 * (size_t)p.blocks * p.slices * p.channels;
+      if (!grad && !p.stats) need.stats = 8 * (size_t)p.frames * p.groups;
+    }
+  }
+  return need;
+}
+
+namespace {
+
+template <class F>
+void by_elem(int elem, F&& f) {
+  if (elem == 0)
+    f(std::integral_constant<int, 0>{});
+  else if (elem == 1)
+    f(std::integral_constant<int, 1>{});
+  else
+    f(std::integral_constant<int, 2>{});
+}
+
+// The arguments that forward and backward share, checked.
+NormArgs norm_args(const dp_norm_shape* shape, const void* starts) {
+  require(shape != nullptr, "no shape");
+  const dp_norm_shape& s = *shape;
+  require(s.type == DP_TYPE_F32 || s.type == DP_TYPE_BF16 || s.type == DP_TYPE_F16, "unknown type");
+  require(s.act == DP_ACT_TANH || s.act == DP_ACT_SILU || s.act == DP_ACT_GELU || s.act == DP_ACT_NONE,
+          "unknown activation");
+  require(s.rows >= 0 && s.rows <= kMaxRows, "rows out of range");
+  require(s.channels >= 1 && s.channels <= kMaxDim, "channels must be 1 .. 2^20");
+  require(s.groups >= 1 && s.groups <= s.channels && s.channels % s.groups == 0, "groups must divide channels");
+  require(s.frames >= 1 && s.frames <= kMaxRows, "frames must be 1 .. 2^30");
+  require(starts || s.rows % s.frames == 0, "rows are not the same number for each frame, and there are no starts");
+  require(s.eps >= 0.0f && s.eps < 1e30f, "eps must be a number from 0 on");
+  NormArgs p{};
+  p.rows = (long)s.rows;
+  p.ld_x = (long)row_length(s.ld_x, s.channels, "ld_x is shorter than channels, or too long");
+  p.ld_y = (long)row_length(s.ld_y, s.channels, "ld_y is shorter than channels, or too long");
+  p.channels = s.channels, p.groups = s.groups, p.frames = s.frames, p.act = s.act, p.eps = s.eps;
+  p.starts = static_cast<const int*>(starts);
+  return p;
+}
+
+void buffers(dp_ops* O, hipStream_t st, const NormNeeds& need, NormArgs& p) {
+  Regions r;
+  const size_t a = r.take(need.stats), b = r.take(need.sums), c = r.take(need.pairs), d = r.take(need.partial);
+  if (!r.used) return;
+  char* ws = workspace(O, st, r.used);
+  if (need.stats) p.stats = reinterpret_cast<float*>(ws + a);
+  if (need.sums) p.sums = reinterpret_cast<float*>(ws + b);
+  if (need.pairs) p.pairs = reinterpret_cast<float*>(ws + c);
+  if (need.partial) p.partial = reinterpret_cast<float*>(ws + d);
+}
+
+}  // namespace
+}  // namespace dpamd
+
+using namespace dpamd;
+
+extern "C" {
+
+int dp_group_norm(dp_ops* O, const dp_norm_shape* shape, const void* x, const int* starts, const void* gamma,
+                  const void* beta, void* y, float* stats, void* stream) {
+  return guarded(O, [&]() {
+    NormArgs p = norm_args(shape, starts);
+    require(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "stats must be 8-byte aligned");
+    if (p.rows == 0) return;
+    require(x && y, "null pointer");
+    p.x = x, p.gamma = gamma, p.beta = beta, p.y = y, p.stats = stats;
+    DPAMD_HIP(hipSetDevice(O->device));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int elem = elem_of(shape->type);
+    buffers(O, st, plan_norm(elem, O->ncu, false, p), p);
+    by_elem(elem, [&](auto k) { norm_launch<decltype(k)::value>(st, p); });
+  });
+}
+
+int dp_group_norm_grad(dp_ops* O, const dp_norm_shape* shape, const void* x, const void* kept, const int* starts,
+                       const void* gamma, const void* beta, const float* stats, const void* dy, void* dx, void* dgamma,
+                       void* dbeta, void* stream) {
+  return guarded(O, [&]() {
+    NormArgs p = norm_args(shape, starts);
+    require(!x || !kept, "x and its checkpoint are not both given");
+    require(reinterpret_cast<uintptr_t>(kept) % 16 == 0, "kept must be 16-byte aligned");
+    require(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "stats must be 8-byte aligned");
+    if (!dx && !dgamma && !dbeta) return;
+    DPAMD_HIP(hipSetDevice(O->device));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (p.rows == 0) {
+      const long b = p.channels * (long)bytes_of(shape->type);
+      for (void* d : {dgamma, dbeta})
+        if (d) fill_zero(st, d, 1, b, b);
+      return;
+    }
+    require((x || kept) && stats && dy, "null pointer");
+    p.x = x, p.kept = static_cast<const unsigned char*>(kept), p.wide = kept8_wide(p.channels);
+    p.gamma = gamma, p.beta = beta, p.stats = const_cast<float*>(stats), p.dy = dy;
+    p.dx = dx, p.dgamma = dgamma, p.dbeta = dbeta;
+    const int elem = elem_of(shape->type);
+    buffers(O, st, plan_norm(elem, O->ncu, true, p), p);
+    by_elem(elem, [&](auto k) { norm_grad_launch<decltype(k)::value>(st, p); });
+  });
+}
+
+}  // extern "C"

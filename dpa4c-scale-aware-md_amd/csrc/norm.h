@@ -1,0 +1,49 @@
+// Group norm with an activation: arguments of its kernels (norm.hip).
+#pragma once
+
+#include "ops.h"
+
+namespace dpamd {
+
+struct NormArgs {
+  long rows, ld_x, ld_y;
+  int channels, groups, per;  // per: channels of a group
+  int frames, act;
+  float eps;
+  const int* starts;  // [frames + 1], or null: equal frames
+  const void *x, *gamma, *beta, *dy;
+  const unsigned char* kept;  // the checkpoint in place of x (gradients), or null
+  int wide;                   // its row length
+  void *y, *dx, *dgamma, *dbeta;
+  float* stats;  // [frames][groups][2]: mean, 1 / deviation
+
+  // how it is cut
+  int vec;     // channels a thread takes at once; `chunks` of them a row, `chunks_per` a group
+  int chunks, chunks_per;
+  int form;    // NormForm
+  int lanes;   // log2 of the lanes that sum one group's chunks
+  int part;    // chunks of a block's columns (whole groups with kNormFrames), `parts` of them
+  int parts, slices;
+  int blocks;  // of the persistent kernels
+  float* partial;  // dgamma and dbeta of blocks or slices, or null: none
+  float* pairs;    // two sums of each chunk of a slice
+  float* sums;     // [frames][groups][2]: means of gamma dz and gamma dz v
+};
+
+// kNormRows: every row a frame of its own, a wave or a block a row, in registers.
+// kNormFrames: a block takes whole frames over a part of the groups, and reads them twice.
+// kNormSlices: frames cut into slices of rows, whose sums meet in memory.
+enum NormForm { kNormRows = 0, kNormFrames = 1, kNormSlices = 2 };
+
+// Chooses the form; the bytes that its buffers take.
+struct NormNeeds {
+  size_t stats, sums, pairs, partial;
+};
+NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& args);
+
+template <int KIND>
+void norm_launch(hipStream_t st, const NormArgs& args);
+template <int KIND>
+void norm_grad_launch(hipStream_t st, const NormArgs& args);
+
+}  // namespace dpamd

@@ -6,132 +6,12 @@
 #include <cstring>
 #include <new>
 #include <string>
-#include <vector>
 
-#include "../../include/dp_amd.h"
-#include "common.h"
-#include "ops.h"
+#include "ops_host.h"
 
 using namespace dpamd;
 
 namespace {
-
-struct OpsError {
-  int code;
-  std::string msg;
-};
-
-// The workspace of one stream. Calls on one stream run in order, so they share it.
-struct Workspace {
-  hipStream_t stream = nullptr;
-  char* p = nullptr;
-  size_t cap = 0;
-  bool captured = false;  // a graph holds its address
-};
-
-// Longest side of a matrix and row length: a tile's byte offsets, up to 256 rows of the
-// longest, stay below 2^32.
-constexpr int64_t kMaxDim = 1 << 20;
-constexpr int64_t kMaxLd = 1 << 22;
-constexpr int64_t kMaxRows = 1 << 30;
-
-}  // namespace
-
-struct dp_ops {
-  int device = 0;
-  int ncu = 256;
-  std::string err;
-  std::vector<Workspace> ws;
-  std::vector<void*> retired;  // outgrown workspaces that graphs still name
-  size_t bytes_now = 0, bytes_peak = 0;
-};
-
-namespace {
-
-template <class F>
-int guarded(dp_ops* O, F&& f) {
-  if (!O) return DP_ERR_ARG;
-  try {
-    O->err.clear();
-    f();
-    return DP_OK;
-  } catch (const OpsError& e) {
-    O->err = e.msg;
-    return e.code;
-  } catch (const HipError& e) {
-    (void)hipGetLastError();  // (else the next call's launch check finds it)
-    O->err = std::string("HIP error ") + hipGetErrorString(e.code) + " in " + e.where;
-    return DP_ERR_HIP;
-  } catch (const std::exception& e) {
-    O->err = e.what();
-    return DP_ERR_ARG;
-  } catch (...) {
-    O->err = "unknown error";
-    return DP_ERR_ARG;
-  }
-}
-
-void require(bool ok, const char* what) {
-  if (!ok) throw OpsError{DP_ERR_ARG, what};
-}
-
-char* workspace(dp_ops* O, hipStream_t st, size_t bytes) {
-  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  DPAMD_HIP(hipStreamIsCapturing(st, &cs));
-  const bool capturing = cs != hipStreamCaptureStatusNone;
-  Workspace* w = nullptr;
-  for (Workspace& k : O->ws)
-    if (k.stream == st) w = &k;
-  if (!w) {
-    O->ws.emplace_back();
-    w = &O->ws.back();
-    w->stream = st;
-  }
-  if (bytes > w->cap) {
-    require(!capturing,
-            "the workspace of a stream under capture cannot grow: run the same call once on it first");
-    const size_t want = bytes + bytes / 8;
-    if (w->p && w->captured) {
-      O->retired.push_back(w->p);
-    } else if (w->p) {
-      DPAMD_HIP(hipStreamSynchronize(st));
-      DPAMD_HIP(hipFree(w->p));
-      O->bytes_now -= w->cap;
-    }
-    w->p = nullptr;
-    w->cap = 0;
-    w->captured = false;
-    void* p = nullptr;
-    DPAMD_HIP(hipMalloc(&p, want));
-    w->p = static_cast<char*>(p);
-    w->cap = want;
-    O->bytes_now += want;
-    O->bytes_peak = std::max(O->bytes_peak, O->bytes_now);
-  }
-  w->captured = w->captured || capturing;
-  return w->p;
-}
-
-// Regions of a workspace, 256-byte aligned, laid out before its size is known.
-struct Regions {
-  size_t used = 0;
-  size_t take(size_t bytes) {
-    const size_t at = used;
-    used += (bytes + 255) & ~size_t(255);
-    return at;
-  }
-};
-
-int elem_of(int type) {
-  return type == DP_TYPE_BF16 ? 0 : type == DP_TYPE_F16 ? 1 : 2;  // ElemKind
-}
-size_t bytes_of(int type) { return type == DP_TYPE_F32 ? 4 : 2; }
-
-int64_t row_length(int64_t ld, int64_t cols, const char* what) {
-  if (ld == 0) return cols;
-  require(ld >= cols && ld <= kMaxLd, what);
-  return ld;
-}
 
 dp_gated_shape checked(const dp_gated_shape* s) {
   require(s != nullptr, "no shape");
@@ -148,66 +28,9 @@ dp_gated_shape checked(const dp_gated_shape* s) {
   return t;
 }
 
-// An operand of the products: the caller's matrix where it is one (rows of whole 16-byte
-// chunks, aligned), and else a region that it is copied into.
-struct Source {
-  const void* src;
-  long ld_src, rows, cols;
-  bool direct;
-  size_t at;
-  long ld;
-};
-
-bool is_operand(int type, const void* p, int64_t ld, int64_t cols) {
-  const int64_t chunk = 16 / (int64_t)bytes_of(type);
-  return cols % chunk == 0 && ld % chunk == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-}
-
-Source source_of(int type, const void* p, int64_t ld, int64_t rows, int64_t cols, Regions& r, bool direct = true) {
-  Source s{p, (long)ld, (long)rows, (long)cols, false, 0, (long)ld};
-  s.direct = direct && is_operand(type, p, ld, cols);
-  if (!s.direct) {
-    s.ld = (s.cols + 7) / 8 * 8;
-    s.at = r.take(bytes_of(type) * (size_t)s.rows * s.ld);
-  }
-  return s;
-}
-
-// The operand's place, and what copies it there.
-Operand operand_of(const Source& s, char* ws, PackList& list) {
-  if (s.direct) return Operand{s.src, s.ld};
-  list.item[list.count] = PackItem{s.src, s.ld_src, s.ld, (int)s.cols, ws + s.at};
-  list.end[list.count] = (list.count ? list.end[list.count - 1] : 0) + s.rows * (s.ld / 8);
-  ++list.count;
-  return Operand{ws + s.at, s.ld};
-}
-
 // gate and up are copied both or neither: the products take one row length for the two
 bool pair_direct(const dp_gated_shape& s, const void* wg, const void* wu) {
   return is_operand(s.type, wg, s.ld_hidden, s.d_hidden) && is_operand(s.type, wu, s.ld_hidden, s.d_hidden);
-}
-
-// whether `many` elements of a row of `out`, from a multiple of it on, can be stored whole
-bool aligned(const void* out, int64_t ld, int type, int many) {
-  return reinterpret_cast<uintptr_t>(out) % (many * bytes_of(type)) == 0 && ld % many == 0;
-}
-
-ProductArgs product(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K) {
-  ProductArgs p{};
-  p.a[0] = p.a[1] = a;
-  p.b[0] = p.b[1] = b;
-  p.M = (int)M;
-  p.N = p.cols = (int)N;
-  p.K = (int)K;
-  p.segs = p.mats = 1;
-  return p;
-}
-
-void output(ProductArgs& p, int k, void* out, int64_t ld, int type) {
-  p.out[k] = out;
-  p.ldo[k] = ld;
-  p.vec[k] = aligned(out, ld, type, 4);
-  p.wide[k] = type != DP_TYPE_F32 && aligned(out, ld, type, 8);
 }
 
 OutsArgs outs_of(const dp_gated_shape& s, const void* wd) {
@@ -299,8 +122,11 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
   run_product(st, kProdDown, elem, p2, b);
 }
 
-void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const void* wg, const void* wu, const void* wd,
-                    const void* saved, const void* dy, void* dx, void* dwg, void* dwu, void* dwd, hipStream_t st) {
+// The backward from x and the kept g and u (saved), or from the 8-bit checkpoint of x alone (kept): its values
+// are restored into an operand and x w_gate, x w_up are formed again, into the workspace.
+void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const unsigned char* kept, const void* wg,
+                    const void* wu, const void* wd, const void* saved, const void* dy, void* dx, void* dwg, void* dwu,
+                    void* dwd, hipStream_t st) {
   const int elem = elem_of(s.type);
   const int64_t n = s.rows, f = s.d_hidden, f8 = (f + 7) / 8 * 8;
   const bool few = few_outputs(s.d_hidden, s.d_out);
@@ -310,22 +136,26 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     sdy = source_of(s.type, dy, s.ld_y, n, s.d_out, r);
     sd = source_of(s.type, wd, s.ld_down, f, s.d_out, r);
   }
-  if (dwg) sx = source_of(s.type, x, s.ld_x, n, s.d_in, r);
-  if (dx) {
+  if (dwg && !kept) sx = source_of(s.type, x, s.ld_x, n, s.d_in, r);
+  if (dx || kept) {
     const bool both = pair_direct(s, wg, wu);
     sg = source_of(s.type, wg, s.ld_hidden, s.d_in, f, r, both);
     su = source_of(s.type, wu, s.ld_hidden, s.d_in, f, r, both);
   }
   const size_t hb = bytes_of(s.type) * (size_t)n * f8;
-  const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd && !few ? r.take(hb) : 0;
+  const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = kept || (dwd && !few) ? r.take(hb) : 0;
+  const long ldx = (s.d_in + 7) / 8 * 8;
+  const size_t at_x = kept ? r.take(bytes_of(s.type) * (size_t)n * ldx) : 0;
+  const size_t at_saved = kept ? r.take(8 * (size_t)n * f) : 0;
+  const ProductPlan p0 = kept ? plan_gate(s, O->ncu) : ProductPlan{};
   const ProductPlan p1 = few ? ProductPlan{} : plan_gate_grad(s, O->ncu);
   const ProductPlan p2 = plan_input(s, O->ncu);
   const ProductPlan p3 = plan_weights(s, O->ncu);
   const ProductPlan p4 = few ? ProductPlan{} : plan_down_weight(s, O->ncu);
   OutsArgs q = outs_of(s, wd);
   const size_t down_bytes = few ? plan_outs_grad(O->ncu, q) : p4.bytes;
-  const size_t at_part = r.take(
-      std::max(std::max(p1.bytes, dx ? p2.bytes : 0), std::max(dwg ? p3.bytes : 0, dwd ? down_bytes : 0)));
+  const size_t at_part = r.take(std::max({p0.bytes, p1.bytes, dx ? p2.bytes : 0, dwg ? p3.bytes : 0,
+                                          dwd ? down_bytes : 0}));
   char* ws = workspace(O, st, r.used);
   float* part = reinterpret_cast<float*>(ws + at_part);
 
@@ -335,12 +165,31 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     ody = operand_of(sdy, ws, list);
     od = operand_of(sd, ws, list);
   }
-  if (dwg) ox = operand_of(sx, ws, list);
-  if (dx) {
+  if (dwg && !kept) ox = operand_of(sx, ws, list);
+  if (dx || kept) {
     og = operand_of(sg, ws, list);
     ou = operand_of(su, ws, list);
   }
   pack_operands(st, elem, list);
+  if (kept) {
+    KeepArgs k{};
+    k.rows = (long)n, k.cols = s.d_in, k.wide = kept8_wide(s.d_in);
+    k.kept = const_cast<unsigned char*>(kept);
+    k.out = ws + at_x;
+    k.ld = ldx, k.cols_out = (int)ldx;
+    restore8(st, elem, k);
+    ox = Operand{ws + at_x, ldx};
+    ProductArgs a = product(ox, og, n, f, s.d_in);
+    a.b[1] = ou;
+    a.cols = (int)f8;
+    a.act = s.act;
+    a.epi.h = ws + at_h;
+    a.epi.ldh = f8;
+    a.epi.saved = reinterpret_cast<float*>(ws + at_saved);
+    a.partial = part;
+    run_product(st, kProdGate, elem, p0, a);
+    saved = ws + at_saved;
+  }
   if (few) {
     q.dy = dy;
     q.saved = static_cast<const float*>(saved);
@@ -353,7 +202,7 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     ProductArgs a = product(ody, od, n, f, s.d_out);
     a.cols = (int)f8;
     a.act = s.act;
-    a.epi.h = dwd ? ws + at_h : nullptr;
+    a.epi.h = dwd && !kept ? ws + at_h : nullptr;
     a.epi.dg = ws + at_dg;
     a.epi.du = ws + at_du;
     a.epi.ldh = f8;
@@ -387,6 +236,14 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const voi
     b.partial = part;
     run_product(st, kProdWeight, elem, p4, b);
   }
+}
+
+// The weights' gradients of a batch without rows.
+void no_rows(const dp_gated_shape& s, void* dwg, void* dwu, void* dwd, hipStream_t st) {
+  const long b = (long)bytes_of(s.type);
+  for (void* d : {dwg, dwu})
+    if (d) fill_zero(st, d, s.d_in, s.d_hidden * b, s.ld_hidden * b);
+  if (dwd) fill_zero(st, dwd, s.d_hidden, s.d_out * b, s.ld_down * b);
 }
 
 void check_embed(int type, int64_t n, int vocab, int width) {
@@ -520,16 +377,27 @@ int dp_gated_backward(dp_ops* O, const dp_gated_shape* shape, const void* x, con
     if (!dx && !dw_gate && !dw_down) return;
     DPAMD_HIP(hipSetDevice(O->device));
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (s.rows == 0) {
-      const long b = (long)bytes_of(s.type);
-      for (void* d : {dw_gate, dw_up})
-        if (d) fill_zero(st, d, s.d_in, s.d_hidden * b, s.ld_hidden * b);
-      if (dw_down) fill_zero(st, dw_down, s.d_hidden, s.d_out * b, s.ld_down * b);
-      return;
-    }
+    if (s.rows == 0) return no_rows(s, dw_gate, dw_up, dw_down, st);
     require(x && w_gate && w_up && w_down && saved && dy, "null pointer");
     require(reinterpret_cast<uintptr_t>(saved) % 16 == 0, "saved must be 16-byte aligned");
-    gated_backward(O, s, x, w_gate, w_up, w_down, saved, dy, dx, dw_gate, dw_up, dw_down, st);
+    gated_backward(O, s, x, nullptr, w_gate, w_up, w_down, saved, dy, dx, dw_gate, dw_up, dw_down, st);
+  });
+}
+
+int dp_gated_backward8(dp_ops* O, const dp_gated_shape* shape, const void* kept, const void* w_gate, const void* w_up,
+                       const void* w_down, const void* dy, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                       void* stream) {
+  return guarded(O, [&]() {
+    const dp_gated_shape s = checked(shape);
+    require(!dw_gate == !dw_up, "dw_gate and dw_up are both given or both NULL");
+    if (!dx && !dw_gate && !dw_down) return;
+    DPAMD_HIP(hipSetDevice(O->device));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (s.rows == 0) return no_rows(s, dw_gate, dw_up, dw_down, st);
+    require(kept && w_gate && w_up && w_down && dy, "null pointer");
+    require(reinterpret_cast<uintptr_t>(kept) % 16 == 0, "kept must be 16-byte aligned");
+    gated_backward(O, s, nullptr, static_cast<const unsigned char*>(kept), w_gate, w_up, w_down, nullptr, dy, dx,
+                   dw_gate, dw_up, dw_down, st);
   });
 }
 

@@ -10,10 +10,10 @@
 namespace dpamd {
 
 // activations, with the codes of the model files
-enum { kActTanh = 0, kActSilu = 1, kActGelu = 2 };
+enum { kActTanh = 0, kActSilu = 1, kActGelu = 2, kActNone = 3 };
 
 // ---- tile products (product.h) ----
-enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2 };
+enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2, kEpiScale = 3, kEpiScaleGate = 4 };
 
 // An operand of the products, of the call's type: 16-byte aligned, rows of whole 16-byte
 // chunks (ld elements), and the contiguous side ends with a chunk or is followed by zeros up to one.
@@ -56,6 +56,9 @@ struct ProductArgs {
   long ldo[2];
   bool vec[2], wide[2];  // whether four, and eight, columns of a row can be stored whole
   EpiArgs epi;
+  // products of 8-bit integers: scales of the rows and of each B matrix's columns, element kind of out[0]
+  const float *row_scale, *col_scale[2];
+  int out_elem;
 };
 
 // What a product is: which layouts and epilogue.
@@ -107,6 +110,37 @@ bool few_outputs(int d_hidden, int d_out);
 void run_outs_down(hipStream_t st, int elem, int ncu, const OutsArgs& args);
 size_t plan_outs_grad(int ncu, OutsArgs& args);  // bytes of the partial sums
 void run_outs_grad(hipStream_t st, int elem, const OutsArgs& args);
+
+// ---- 8-bit forms (quant8.hip) and products (product8.hip) ----
+// Checkpoint of [rows][cols]: q [rows][wide] (wide: cols up to a multiple of 32), then a byte for each 32.
+struct KeepArgs {
+  long rows, ld;
+  int cols, wide, cols_out;
+  const void* x;
+  unsigned char* kept;
+  void* out;  // of restore8: [rows][ld], zeros from cols to cols_out
+};
+inline int kept8_wide(int cols) { return (cols + 31) / 32 * 32; }
+void keep8(hipStream_t st, int elem, const KeepArgs& args);
+void restore8(hipStream_t st, int elem, const KeepArgs& args);
+struct Rows8Args {
+  long rows, ld, ld_q;
+  int cols;
+  const void* x;
+  signed char* q;
+  float* scale;
+};
+void rows8(hipStream_t st, int elem, const Rows8Args& args);
+struct Weights8Args {
+  int d_in, d_out;
+  long ld_w, ld_q;
+  const void* w;
+  signed char* q;
+  float* scale;
+};
+void weights8(hipStream_t st, int elem, const Weights8Args& args);
+// x [M][K] and weights [N][K] of integers, k contiguous; two weight matrices with `gate`
+void run_product8(hipStream_t st, bool gate, const ProductPlan& plan, ProductArgs& args);
 
 // Matrices [rows][cols] to be copied into rows of ld (a multiple of 8), with zeros past cols.
 struct PackItem {

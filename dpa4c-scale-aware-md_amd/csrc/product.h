@@ -14,8 +14,9 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 typedef short s8v __attribute__((ext_vector_type(8)));
+typedef int i4 __attribute__((ext_vector_type(4)));
 
-enum ElemKind { kBf16 = 0, kF16 = 1, kF32 = 2 };
+enum ElemKind { kBf16 = 0, kF16 = 1, kF32 = 2, kI8 = 3 };
 template <int KIND>
 struct ElemOf {
   using T = unsigned short;
@@ -23,6 +24,10 @@ struct ElemOf {
 template <>
 struct ElemOf<kF32> {
   using T = float;
+};
+template <>
+struct ElemOf<kI8> {
+  using T = signed char;
 };
 
 // v rounded to the kind's 16 bits (to nearest, ties to even)
@@ -240,6 +245,103 @@ __device__ __forceinline__ void put_pair(typename ElemOf<KIND>::T* p, const f4& 
   *reinterpret_cast<u4*>(p) = u4{out[0], out[1], out[2], out[3]};
 }
 
+// ---- products of 8-bit integers -----------------------------------------------------------
+
+// act(g), or g itself
+__device__ __forceinline__ f4 activated4(int act, const f4& g) {
+  if (act == kActNone) return g;
+  f4 a, da;
+  activate4(act, g, a, da);
+  return a;
+}
+// A row's scale as two factors: with that of rows beyond 2^90 a sum (below 2^31) could leave fp32's range
+// before the column's scale brings it back.
+struct RowFactor {
+  float first, last;
+};
+__device__ __forceinline__ RowFactor row_factor(float scale) {
+  return scale >= 0x1p90f ? RowFactor{scale * 0x1p-32f, 0x1p32f} : RowFactor{scale, 1.0f};
+}
+// Four columns of a row from the integer sums: act(g), or act(g) u; each sum in fp32 times the row's scale
+// and then the column's.
+template <bool GATE>
+__device__ __forceinline__ f4 scaled4(int act, const f4& sums, const f4& other, const RowFactor& row, const f4& col,
+                                      const f4& col_other) {
+  const i4 s = __builtin_bit_cast(i4, sums), o = __builtin_bit_cast(i4, other);
+  f4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (float)s[e] * row.first * col[e] * row.last;
+  v = activated4(act, v);
+  if constexpr (GATE) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= (float)o[e] * row.first * col_other[e] * row.last;
+  }
+  return v;
+}
+// Scales of four columns, `count` of them there.
+__device__ __forceinline__ f4 scales4(const float* s, int count) {
+  f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (count >= 4) {
+    __builtin_memcpy(&v, s, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < count) v[e] = s[e];
+  }
+  return v;
+}
+// A wave's sums: rows m0 + 16 i, columns n0 + 16 j .. + 3 of its lanes; acc[i][NG + j] the second matrix's.
+template <int MI, int NG, bool GATE, int NJ>
+__device__ __forceinline__ void scaled_out(const ProductArgs& p, const f4 (&acc)[MI][NJ], int m0, int n0, int g,
+                                           bool inside) {
+  f4 col[NG], other[NG];
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    col[j] = scales4(p.col_scale[0] + n0 + j * 16, p.N - n0 - j * 16);
+    other[j] = GATE ? scales4(p.col_scale[1] + n0 + j * 16, p.N - n0 - j * 16) : f4{};
+  }
+  float scale[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) scale[i] = p.row_scale[min(m0 + i * 16, p.M - 1)];
+  auto value = [&](int i, int j) {
+    return scaled4<GATE>(p.act, acc[i][j], acc[i][GATE ? NG + j : j], row_factor(scale[i]), col[j], other[j]);
+  };
+  auto emit = [&](auto kind) {
+    constexpr int OUT = decltype(kind)::value;
+    using T = typename ElemOf<OUT>::T;
+    const long step = 16 * p.ldo[0];
+    long at = m0 * p.ldo[0] + n0;
+    if constexpr (OUT != kF32 && NG % 2 == 0) {
+      if (inside && p.wide[0]) {
+        at += pair_at(g);
+#pragma unroll
+        for (int i = 0; i < MI; ++i, at += step)
+#pragma unroll
+          for (int j = 0; j < NG; j += 2)
+            put_pair<OUT>(static_cast<T*>(p.out[0]) + at + j * 16, value(i, j), value(i, j + 1));
+        return;
+      }
+    }
+    const bool whole = inside && p.vec[0];
+#pragma unroll
+    for (int i = 0; i < MI; ++i, at += step)
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const f4 v = value(i, j);
+        if (whole)
+          put_row4<OUT, true>(p.out[0], at + j * 16, v, 4);
+        else if (m0 + i * 16 < p.M && n0 + j * 16 < p.N)
+          put_row4<OUT, false>(p.out[0], at + j * 16, v, p.N - n0 - j * 16);
+      }
+  };
+  if (p.out_elem == kF32)
+    emit(std::integral_constant<int, kF32>{});
+  else if (p.out_elem == kF16)
+    emit(std::integral_constant<int, kF16>{});
+  else
+    emit(std::integral_constant<int, kBf16>{});
+}
+
 // ---- the product ------------------------------------------------------------------------
 
 // Operand layouts: rows with k contiguous (kRowK), or k rows with the operand's rows
@@ -314,9 +416,9 @@ struct TileOf {
   static __device__ __forceinline__ void place(int q, int wave, int lane, int& part, int& row, int& chunk) {
     const int b = (q * WAVES + wave) * 1024 + lane * 16;
     if constexpr (LAYOUT == kRowK) {
-      row = b / 128;
+      part = SUB == 1 ? 0 : b / 128 / kPart;
+      row = SUB == 1 ? b / 128 : b / 128 % kPart;
       chunk = ((b / 16) % 8) ^ swz_row(row);
-      part = 0;
     } else {
       part = b / (kPart * 128);
       const int w = b % (kPart * 128);
@@ -328,12 +430,13 @@ struct TileOf {
   // offset(kind(q)) + moved(q) rows of ld, the former in a register for each of kOffsets
   // kinds. (Rows, or k rows a period apart, differ by the uniform part alone.)
   static constexpr int kRows = LAYOUT == kRowK ? WAVES * 8 : WAVES * 1024 / kKRow;  // of one load of all waves
-  static_assert(LAYOUT == kColK || (SUB == 1 && kRows % 8 == 0), "whole permutations a load");
+  static_assert(LAYOUT == kColK || (kRows % 8 == 0 && kPart % 8 == 0), "whole permutations a load");
+  static_assert(LAYOUT == kColK || kPart % kRows == 0 || kRows == ROWS, "a load's rows lie alike in their parts");
   static constexpr int kOffsets =
       LAYOUT == kRowK || kRows >= kPeriod ? 1 : (kPeriod / kRows < kLoads ? kPeriod / kRows : kLoads);
   static constexpr __device__ int kind(int q) { return q % kOffsets; }
   static constexpr __device__ long moved(int q) {
-    return LAYOUT == kRowK ? q * kRows : (q * kRows) % BK / kPeriod * kPeriod;
+    return LAYOUT == kRowK ? (q * kRows) % kPart : (q * kRows) % BK / kPeriod * kPeriod;
   }
   static __device__ __forceinline__ unsigned offset(int q, int wave, int lane, long ld, int rows_left) {
     int part, row, chunk;
@@ -356,7 +459,7 @@ struct TileOf {
     int part, row, chunk;
     if constexpr (LAYOUT == kRowK) {
       place(0, wave, lane, part, row, chunk);
-      return chunk * VE >= k_left || row >= rows_left - q * kRows;
+      return chunk * VE >= k_left || row >= rows_left - moved(q);
     } else {
       place(q, wave, lane, part, row, chunk);
       return row >= k_left;
@@ -368,7 +471,7 @@ struct TileOf {
   static __device__ __forceinline__ s8v frag(const char* tile, int part, int r0, int kk, int lane) {
     const int g = lane >> 4, c = lane & 15;
     if constexpr (LAYOUT == kRowK) {
-      return *reinterpret_cast<const s8v*>(tile + (r0 + c) * 128 + (((kk * 4 + g) ^ swz_row(c)) * 16));
+      return *reinterpret_cast<const s8v*>(tile + (part * kPart + r0 + c) * 128 + (((kk * 4 + g) ^ swz_row(c)) * 16));
     } else if constexpr (EB == 2) {
       const int k = kk * 32 + 8 * g + (c >> 2);
       const int s = (((c >> 2) | (g << 2)) & (kUnits - 1)) ^ (r0 / 16);
@@ -398,6 +501,13 @@ __device__ __forceinline__ void multiply_row(f4 (&acc)[NJ], const s8v (&b)[NJ], 
     for (int q = 0; q < 4; ++q)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[j] = mfma_f32(__builtin_bit_cast(f4, b[j])[q], y[q], acc[j]);
+  } else if constexpr (KIND == kI8) {
+    // (the sums are integers in the accumulators' bits)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      acc[j] = __builtin_bit_cast(
+          f4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, b[j]), __builtin_bit_cast(i4, a),
+                                                    __builtin_bit_cast(i4, acc[j]), 0, 0, 0));
   } else {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -417,7 +527,8 @@ struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
 };
 
-// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad.
+// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad; of 8-bit integers
+// kEpiScale, kEpiScaleGate (two).
 //
 // A block takes tiles (and slices of K) one after another; the first two steps of the next one are
 // loaded before the epilogue of the last, so that they arrive under it. Two stages of LDS.
@@ -436,7 +547,7 @@ struct Shape {
 // instead of two changed nothing).
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
-  constexpr int SUB = EPI == kEpiGate ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
+  constexpr int SUB = EPI == kEpiGate || EPI == kEpiScaleGate ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
   using T = typename ElemOf<KIND>::T;
   constexpr int WAVES = S::WM * S::WN, TM = S::BM / S::WM, TN = S::BN / S::WN;
   constexpr int MI = TM / 16, NJ = TN / 16;
@@ -665,6 +776,8 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
             if (m0 + i * 16 < p.M && n0 + j * 16 < p.N)
               put_row4<KIND, false>(out, at + j * 16, acc[i][j], p.N - n0 - j * 16);
       }
+    } else if constexpr (KIND == kI8) {
+      scaled_out<MI, NJ / SUB, SUB == 2>(p, acc, m0, n0, g, inside);
     } else if constexpr (EPI == kEpiGate) {
       long h = m0 * p.epi.ldh + n0;
       float* kept = p.epi.saved ? p.epi.saved + ((long)m0 * p.N + n0) : nullptr;

@@ -453,6 +453,102 @@ int dp_gated_backward(dp_ops* ops, const dp_gated_shape* shape, const void* d_x,
                       const void* d_saved, const void* d_dy, void* d_dx, void* d_dw_gate,
                       void* d_dw_up, void* d_dw_down, void* stream);
 
+/*
+ * Checkpoints of activations in 8 bits: what the forward of a layer keeps of its input x [rows][cols] for the
+ * backward, 33 bits for every four values. A row's columns are in groups of 32 (the last one may be shorter). Each
+ * group has a unit, a power of two, 2^(floor(log2 max |x|) - 6) (at least 2^-133), and x is held as the multiple
+ * of it that is nearest (ties to the even one), at most 127 in magnitude: off by at most half a unit, or a
+ * whole one in the last 127th below the next power of two. What is restored is a number of all three types
+ * (in f16 where x was one); a group with an infinity or a NaN is restored as NaN.
+ * `kept`: dp_keep8_bytes bytes (0 for sizes that the calls refuse), 16-byte aligned: the integers [rows][cols up
+ * to a multiple of 32], then a byte for each group, the biased exponent of its largest value. With rows == 0 nothing
+ * is done.
+ */
+size_t dp_keep8_bytes(int64_t rows, int cols);
+int dp_keep8(dp_ops* ops, int type, int64_t rows, int cols, const void* d_x, int64_t ld_x,
+             void* d_kept, void* stream);
+int dp_restore8(dp_ops* ops, int type, int64_t rows, int cols, const void* d_kept, void* d_x,
+                int64_t ld_x, void* stream);
+
+/*
+ * dp_gated_backward from the checkpoint of x [rows][d_in] alone, with nothing kept by the forward (d_saved
+ * NULL): x w_gate and x w_up are formed again from the restored x, and the gradients are those of the block
+ * there. It keeps d_in * 33 / 32 bytes a row in place of x and 8 d_hidden. The workspace takes, for the
+ * time of the call, what the forward would have kept, which the calls of all layers on a stream share.
+ */
+int dp_gated_backward8(dp_ops* ops, const dp_gated_shape* shape, const void* d_kept,
+                       const void* d_w_gate, const void* d_w_up, const void* d_w_down,
+                       const void* d_dy, void* d_dx, void* d_dw_gate, void* d_dw_up,
+                       void* d_dw_down, void* stream);
+
+/*
+ * Products in 8-bit integers, to serve what was trained: weights with a scale for each output channel, laid out once,
+ * and rows of x (tokens, atoms) quantised in the call with a scale each. A row or channel is held as
+ *   scale = max |x| / 127,  q = x * (127 / max |x|) to the nearest integer (ties to the even one),
+ * both quotients rounded to fp32, the product with x exact. One whose largest magnitude is below 2^-119
+ * counts as zeros; one with an infinity or a NaN has a scale of NaN, and all that comes of it is NaN.
+ *
+ * dp_weights8: w [d_in][d_out] of a type -> d_w8 [d_out][ld_w8] integers (16-byte aligned; ld_w8 a multiple of 16, 0:
+ * d_in up to one; zeros past d_in) and d_scale [d_out].
+ */
+int dp_weights8(dp_ops* ops, int type, int d_in, int d_out, const void* d_w, int64_t ld_w,
+                void* d_w8, int64_t ld_w8, float* d_scale, void* stream);
+
+/*
+ * y = act(g), or act(g) * u with d_up (the gate half of the block; its down half is a call on y), where
+ * g = (sum over k of q_x q_w) scale_x scale_w, and u the same of the second weights: the sums are exact (d_in is at
+ * most 2^17), g and u are fp32, and y is rounded once. The integers may be any, from dp_weights8 or
+ * not; what lies past d_in in their rows is not looked at, but has to be readable up to a multiple of 16.
+ * The activations are those of the block, and DP_ACT_NONE.
+ */
+enum { DP_ACT_NONE = 3 };
+typedef struct {
+  int64_t rows;
+  int d_in, d_out;
+  int type, act;
+  int64_t ld_x, ld_y;
+  int64_t ld_w; /* of the 8-bit weights, both of them, in bytes: a multiple of 16 (0: d_in up to one) */
+} dp_linear8_shape;
+int dp_linear8(dp_ops* ops, const dp_linear8_shape* shape, const void* d_x, const void* d_w,
+               const float* d_w_scale, const void* d_up, const float* d_up_scale, void* d_y,
+               void* stream);
+
+/*
+ * Group norm with an activation, channels last: rows (atoms, positions) of `channels` in `groups` of neighbouring
+ * ones, rows of a frame (a cell, a sample) normalised together,
+ *   y = act(gamma (x - m) r + beta),  m the mean and r = 1 / sqrt(variance + eps) of the frame's rows over the
+ * group's channels (the variance around m, over their number). gamma and beta [channels] of the call's type, or
+ * NULL: ones, zeros. Frames are `frames` equal parts of the rows (rows of them: each row by itself), or with d_starts
+ * [frames + 1] (32-bit integers) the rows starts[f] .. starts[f + 1] - 1, not descending; a frame may be empty,
+ * and rows before the first and behind the last one are left as they were. What starts holds beyond the rows is cut
+ * off. d_stats: NULL, or [frames][groups] pairs of m and r in fp32 (8-byte aligned; zeros for an empty frame), for
+ * the backward. m, r and all sums are formed in fp32 or fp64 (never as a difference of large sums), y is rounded
+ * once. A NaN or an infinity makes its frame's group NaN. With rows == 0 nothing is done.
+ */
+typedef struct {
+  int64_t rows;
+  int channels, groups;
+  int frames;
+  int type, act; /* DP_ACT_NONE too */
+  float eps;
+  int64_t ld_x; /* x and dx */
+  int64_t ld_y; /* y and dy */
+} dp_norm_shape;
+int dp_group_norm(dp_ops* ops, const dp_norm_shape* shape, const void* d_x, const int* d_starts,
+                  const void* d_gamma, const void* d_beta, void* d_y, float* d_stats, void* stream);
+
+/*
+ * With v = (x - m) r, dz = dy act'(gamma v + beta) and w = gamma dz: dx = r (w - mean w - v mean(w v)), the means
+ * over the frame's rows and the group's channels, dgamma = sum of dz v and dbeta = sum of dz over all frames' rows.
+ * x, or in its place (d_x NULL) its checkpoint from dp_keep8, at whose values the gradients are then taken, with the
+ * forward's m and r. An output that is NULL is not formed; dx of rows that are in no frame is left as it was. With rows
+ * == 0 dgamma and dbeta are zeros.
+ */
+int dp_group_norm_grad(dp_ops* ops, const dp_norm_shape* shape, const void* d_x, const void* d_kept,
+                       const int* d_starts, const void* d_gamma, const void* d_beta,
+                       const float* d_stats, const void* d_dy, void* d_dx, void* d_dgamma,
+                       void* d_dbeta, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
