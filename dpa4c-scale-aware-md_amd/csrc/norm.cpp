@@ -39,12 +39,14 @@ NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
   const long length = std::max(1L, p.rows / p.frames);
   const bool affine = grad && (p.dgamma || p.dbeta);
   NormNeeds need{};
+  p.inv_chunks = 1.0f / (float)p.chunks_per, p.inv_per = 1.0f / (float)p.per;
   p.slices = 1;
   if (!p.starts && p.frames == p.rows && p.chunks <= 1024) {
     p.form = kNormRows;
-    const int T = p.chunks <= 16 ? 16 : p.chunks <= 256 ? 64 : 256;
-    p.lanes = lanes_of(p.groups, p.chunks_per, T);
-    p.blocks = (int)std::min((p.rows + 256 / T - 1) / (256 / T), 2L * ncu);
+    const int T = p.chunks <= 16 ? 16 : p.chunks <= 64 ? 64 : 256;
+    p.by_lanes = p.chunks_per <= 64 && (p.chunks_per & (p.chunks_per - 1)) == 0;
+    p.lanes = lanes_of(p.by_lanes ? 1 : p.groups, p.chunks_per, T);
+    p.blocks = (int)std::min((p.rows + 256 / T - 1) / (256 / T), (grad ? 4L : 8L) * ncu);
     if (affine) need.partial = 8 * (size_t)p.blocks * p.channels;
   } else {
     // whole groups a block, at least 16 chunks (256 bytes of a row) where that leaves no compute unit idle
@@ -54,6 +56,8 @@ NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
            (blocks(gp) < ncu || (blocks(gp) < 4 * ncu && (gp + 1) / 2 * p.chunks_per >= 16)) &&
            256 / ((gp + 1) / 2 * p.chunks_per) <= 2 * length)
       gp = (gp + 1) / 2;
+    // fewer columns where that lets a block hold its rows in registers (8 a thread), from 128 bytes of a row on
+    while (gp > 1 && (gp + 1) / 2 * p.chunks_per >= 8 && length > 6 * (256 / (gp * p.chunks_per))) gp = (gp + 1) / 2;
     const double bytes = 4.0 * p.rows * p.channels;
     const double each = 4.0 * length * gp * p.per * ((blocks(gp) + ncu - 1) / ncu);
     // us: a block's own pace, and three launches with all compute units at work

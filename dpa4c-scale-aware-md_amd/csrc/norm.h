@@ -21,6 +21,8 @@ struct NormArgs {
   int vec;     // channels a thread takes at once; `chunks` of them a row, `chunks_per` a group
   int chunks, chunks_per;
   int form;    // NormForm
+  bool by_lanes;              // kNormRows: a group's chunks are neighbouring lanes
+  float inv_chunks, inv_per;  // 1 / chunks_per, 1 / per
   int lanes;   // log2 of the lanes that sum one group's chunks
   int part;    // chunks of a block's columns (whole groups with kNormFrames), `parts` of them
   int parts, slices;

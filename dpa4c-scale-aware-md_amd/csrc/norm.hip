@@ -44,14 +44,82 @@ __device__ __forceinline__ Frame frame_of(const NormArgs& p, int f) {
   return Frame{a, (int)(b - a)};
 }
 
+// VE elements as they lie in memory: what is loaded ahead, or kept for long, takes no more registers than that
+// (held in words: single elements of 16 or 8 bits would take a register each).
+template <int KIND, int VE>
+struct Raw {
+  using E = typename ElemOf<KIND>::T;
+  static constexpr int kBytes = VE * sizeof(E), kWords = (kBytes + 3) / 4;
+  unsigned w[kWords];
+  __device__ __forceinline__ void load(const E* p) {
+    if constexpr (kBytes == 2)
+      w[0] = *p;
+    else
+      __builtin_memcpy(w, p, kBytes);  // (the hardware takes addresses of any alignment)
+  }
+  __device__ __forceinline__ void zeros() {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = 0;
+  }
+  __device__ __forceinline__ void ones() {
+    const unsigned one = KIND == kF32 ? 0x3f800000u : KIND == kBf16 ? 0x3f803f80u : 0x3c003c00u;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = one;
+  }
+  __device__ __forceinline__ void get(float (&out)[VE]) const {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      if constexpr (KIND == kF32)
+        out[e] = __builtin_bit_cast(float, w[e]);
+      else
+        out[e] = to_f32<KIND>((unsigned short)(w[e / 2] >> (16 * (e % 2))));
+    }
+  }
+};
+// the same of x or its checkpoint
+// v = x r - m r: one instruction a value. (m r is rounded, by no more than m itself is.)
+template <int KIND, int VE, bool KEPT>
+struct RawX : Raw<KIND, VE> {
+  __device__ __forceinline__ void load_at(const NormArgs& p, long row, int chunk) {
+    this->load(static_cast<const typename ElemOf<KIND>::T*>(p.x) + row * p.ld_x + (long)chunk * VE);
+  }
+  __device__ __forceinline__ void normalized(const Pair& s, float (&out)[VE]) const {
+    this->get(out);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) out[e] = __builtin_fmaf(out[e], s.b, -s.a * s.b);
+  }
+};
+template <int KIND, int VE>
+struct RawX<KIND, VE, true> {
+  static constexpr int kWords = (VE + 3) / 4;
+  unsigned w[kWords];
+  unsigned char field;
+  __device__ __forceinline__ void load_at(const NormArgs& p, long row, int chunk) {
+    const unsigned char* at = p.kept + row * p.wide + chunk * VE;
+    if constexpr (VE == 1) {
+      w[0] = *at;
+    } else if constexpr (VE == 2) {
+      unsigned short v;
+      __builtin_memcpy(&v, at, 2);
+      w[0] = v;
+    } else {
+      __builtin_memcpy(w, at, VE);
+    }
+    field = p.kept[p.rows * p.wide + row * (p.wide / 32) + chunk * VE / 32];
+  }
+  __device__ __forceinline__ void normalized(const Pair& s, float (&out)[VE]) const {
+    const float unit = unit_of(field) * s.b;
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      out[e] = __builtin_fmaf((float)(signed char)(w[e / 4] >> (8 * (e % 4))), unit, -s.a * s.b);
+  }
+};
+
 template <int KIND, int VE>
 __device__ __forceinline__ void load_vec(float (&v)[VE], const typename ElemOf<KIND>::T* p) {
-  struct Some {
-    typename ElemOf<KIND>::T v[VE];
-  } s;
-  __builtin_memcpy(&s, p, sizeof(s));  // (the hardware takes addresses of any alignment)
-#pragma unroll
-  for (int e = 0; e < VE; ++e) v[e] = to_f32<KIND>(s.v[e]);
+  Raw<KIND, VE> r;
+  r.load(p);
+  r.get(v);
 }
 template <int KIND, int VE>
 __device__ __forceinline__ void store_vec(typename ElemOf<KIND>::T* p, const float (&v)[VE]) {
@@ -61,21 +129,6 @@ __device__ __forceinline__ void store_vec(typename ElemOf<KIND>::T* p, const flo
 #pragma unroll
   for (int e = 0; e < VE; ++e) s.v[e] = from_f32<KIND>(v[e]);
   __builtin_memcpy(p, &s, sizeof(s));
-}
-// x at (row, chunk): the matrix's, or what the checkpoint restores
-template <int KIND, int VE, bool KEPT>
-__device__ __forceinline__ void load_x(const NormArgs& p, float (&v)[VE], long row, int chunk) {
-  if constexpr (KEPT) {
-    struct Some {
-      signed char v[VE];
-    } s;
-    __builtin_memcpy(&s, p.kept + row * p.wide + chunk * VE, sizeof(s));
-    const int field = p.kept[p.rows * p.wide + row * (p.wide / 32) + chunk * VE / 32];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) v[e] = restore_one(s.v[e], field);
-  } else {
-    load_vec<KIND, VE>(v, static_cast<const typename ElemOf<KIND>::T*>(p.x) + row * p.ld_x + (long)chunk * VE);
-  }
 }
 template <int KIND, int VE>
 __device__ __forceinline__ void load_affine(const NormArgs& p, int chunk, float (&gamma)[VE], float (&beta)[VE]) {
@@ -87,11 +140,11 @@ __device__ __forceinline__ void load_affine(const NormArgs& p, int chunk, float 
 }
 
 // act and its derivative over a thread's values (one uniform branch for all of them)
-template <int VE>
+template <int KIND, int VE>
 __device__ __forceinline__ void activate_vec(int act, const float (&z)[VE], float (&a)[VE], float (&da)[VE]) {
   auto all = [&](auto k) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) activate<decltype(k)::value>(z[e], a[e], da[e]);
+    for (int e = 0; e < VE; ++e) activate_as<KIND, decltype(k)::value>(z[e], a[e], da[e]);
   };
   if (act == kActNone) {
 #pragma unroll
@@ -104,27 +157,32 @@ __device__ __forceinline__ void activate_vec(int act, const float (&z)[VE], floa
     all(std::integral_constant<int, kActGelu>{});
   }
 }
-template <int VE>
-__device__ __forceinline__ void forward_vec(int act, float m, float r, const float (&gamma)[VE],
-                                            const float (&beta)[VE], float (&v)[VE]) {
+// x -> act(x scale + shift)
+template <int KIND, int VE>
+__device__ __forceinline__ void forward_vec(int act, const float (&scale)[VE], const float (&shift)[VE],
+                                            float (&x)[VE]) {
   float z[VE], da[VE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) z[e] = gamma[e] * ((v[e] - m) * r) + beta[e];
-  activate_vec<VE>(act, z, v, da);
+  for (int e = 0; e < VE; ++e) z[e] = __builtin_fmaf(x[e], scale[e], shift[e]);
+  activate_vec<KIND, VE>(act, z, x, da);
 }
-// x -> v and dy -> dz
-template <int VE>
-__device__ __forceinline__ void grad_vec(int act, float m, float r, const float (&gamma)[VE], const float (&beta)[VE],
-                                         float (&x)[VE], float (&dy)[VE]) {
+// dy -> dz
+template <int KIND, int VE>
+__device__ __forceinline__ void grad_vec(int act, const float (&gamma)[VE], const float (&beta)[VE],
+                                         const float (&v)[VE], float (&dy)[VE]) {
   float z[VE], a[VE], da[VE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    x[e] = (x[e] - m) * r;
-    z[e] = gamma[e] * x[e] + beta[e];
-  }
-  activate_vec<VE>(act, z, a, da);
+  for (int e = 0; e < VE; ++e) z[e] = __builtin_fmaf(gamma[e], v[e], beta[e]);
+  activate_vec<KIND, VE>(act, z, a, da);
 #pragma unroll
   for (int e = 0; e < VE; ++e) dy[e] *= da[e];
+}
+// w = gamma dz -> dx = r (w - mean w - v mean(w v))
+template <int VE>
+__device__ __forceinline__ void dx_vec(float r, const Pair& means, const float (&v)[VE], float (&w)[VE]) {
+  const float a = -r * means.a, b = -r * means.b;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) w[e] = __builtin_fmaf(v[e], b, __builtin_fmaf(w[e], r, a));
 }
 
 // mean and squared deviations of VE values
@@ -145,12 +203,24 @@ __device__ __forceinline__ void join_moments(Pair& p, float n, const Pair& q, fl
   p.b += q.b + d * d * n * w;
 }
 
+// v + that of another lane, in one instruction (DPP): within quads, halves of rows and rows of 16 lanes
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// The sum over 2^log_lanes neighbouring lanes, in each of them (every lane of the wave takes part).
 __device__ __forceinline__ float sum_lanes(float v, int log_lanes) {
-  for (int m = 0; m < log_lanes; ++m) v += __shfl_xor(v, 1 << m, kWave);
+  if (log_lanes > 0) v = add_dpp<0xB1>(v);   // lane ^ 1
+  if (log_lanes > 1) v = add_dpp<0x4E>(v);   // lane ^ 2
+  if (log_lanes > 2) v = add_dpp<0x141>(v);  // 7 - lane: the other quad, whose lanes are alike by now
+  if (log_lanes > 3) v = add_dpp<0x140>(v);  // 15 - lane
+  if (log_lanes > 4) v = add_xor16(v);
+  if (log_lanes > 5) v = add_xor32(v);
   return v;
 }
-__device__ __forceinline__ float deviation(float M, float n, float eps) {
-  return 1.0f / sqrtf(M / n + eps);
+// 1 / sqrt(M / n + eps), inv = 1 / n
+__device__ __forceinline__ float deviation(float M, float inv, float eps) {
+  return __builtin_amdgcn_rsqf(__builtin_fmaf(M, inv, eps));
 }
 
 // A barrier among the threads that share a row: a wave's, or the block's.
@@ -173,9 +243,13 @@ __device__ __forceinline__ void each_group(int t, int groups, int lanes, F&& f) 
 }
 
 // ---- every row a frame -----------------------------------------------------------------
-// T threads a row, C chunks of VE channels a thread (at neighbouring places for neighbouring threads). Parts
-// of a row in LDS: a pair for each chunk, then one for each group.
-template <int KIND, int VE, int T, int C>
+// T threads a row, C chunks of VE channels a thread (at neighbouring places for neighbouring threads). With
+// LANES a group is a power of two of chunks, at most 64, so that it is that many neighbouring lanes, which
+// add up without LDS or a barrier; else the parts of a row meet in LDS, a pair for each chunk and then one
+// for each group. (16,384 x 2048 in bf16, groups of 64, gelu: XXX.)
+// A block takes rows one after another: gamma and beta stay in registers, and the next row is loaded
+// while this one is computed.
+template <int KIND, int VE, int T, int C, bool LANES>
 __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
   extern __shared__ __align__(16) char lds[];
@@ -183,47 +257,80 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
   const int t = threadIdx.x % T, mine = threadIdx.x / T;
   Pair* parts = reinterpret_cast<Pair*>(lds) + (size_t)mine * (p.chunks + p.groups);
   Pair* whole = parts + p.chunks;
-  for (long row0 = (long)blockIdx.x * R; row0 < p.rows; row0 += (long)gridDim.x * R) {
-    const bool there = row0 + mine < p.rows;
-    const long row = there ? row0 + mine : p.rows - 1;
+  float gamma[C][VE], beta[C][VE];
+#pragma unroll
+  for (int k = 0; k < C; ++k) load_affine<KIND, VE>(p, min(k * T + t, p.chunks - 1), gamma[k], beta[k]);
+  Raw<KIND, VE> raw[C];
+  auto fetch = [&](long row) {
+    const E* x = static_cast<const E*>(p.x) + min(row, p.rows - 1) * p.ld_x;
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+      if (k * T + t < p.chunks) raw[k].load(x + (long)(k * T + t) * VE);
+  };
+  const long step = (long)gridDim.x * R;
+  fetch((long)blockIdx.x * R + mine);
+  for (long row0 = (long)blockIdx.x * R; row0 < p.rows; row0 += step) {
+    const long row = row0 + mine;
+    const bool there = row < p.rows;
     float v[C][VE];
+    Pair stat[C];
+    auto keep = [&](int q, const Pair& s) {
+      if (p.stats && there) *reinterpret_cast<Pair*>(p.stats + 2 * (row * p.groups + q)) = s;
+    };
+    if constexpr (LANES) {
 #pragma unroll
-    for (int k = 0; k < C; ++k)
-      if (k * T + t < p.chunks) load_x<KIND, VE, false>(p, v[k], row, k * T + t);
-#pragma unroll
-    for (int k = 0; k < C; ++k)
-      if (k * T + t < p.chunks) parts[k * T + t] = moments<VE>(v[k]);
-    row_sync<T>();
-    each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
-      const Pair* s = parts + q * p.chunks_per;
-      float m = 0.0f, M = 0.0f;
-      for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) m += s[k].a;
-      m = sum_lanes(m, p.lanes) / (float)p.chunks_per;
-      for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) M += s[k].b + VE * (s[k].a - m) * (s[k].a - m);
-      const float r = deviation(sum_lanes(M, p.lanes), (float)p.per, p.eps);
-      if (in && lane == 0) {
-        whole[q] = Pair{m, r};
-        if (p.stats && there) *reinterpret_cast<Pair*>(p.stats + 2 * (row * p.groups + q)) = Pair{m, r};
+      for (int k = 0; k < C; ++k) {
+        raw[k].get(v[k]);
+        const Pair s = moments<VE>(v[k]);
+        const float m = sum_lanes(s.a, p.lanes) * p.inv_chunks;
+        const float M = sum_lanes(s.b + VE * (s.a - m) * (s.a - m), p.lanes);
+        stat[k] = Pair{m, deviation(M, p.inv_per, p.eps)};
+        const int chunk = k * T + t;
+        if (chunk < p.chunks && (t & (p.chunks_per - 1)) == 0) keep(chunk / p.chunks_per, stat[k]);
       }
-    });
-    row_sync<T>();
+      if (row0 + step < p.rows) fetch(row + step);
+    } else {
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (k * T + t < p.chunks) {
+          raw[k].get(v[k]);
+          parts[k * T + t] = moments<VE>(v[k]);
+        }
+      if (row0 + step < p.rows) fetch(row + step);
+      row_sync<T>();
+      each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
+        const Pair* s = parts + q * p.chunks_per;
+        float m = 0.0f, M = 0.0f;
+        for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) m += s[k].a;
+        m = sum_lanes(m, p.lanes) * p.inv_chunks;
+        for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) M += s[k].b + VE * (s[k].a - m) * (s[k].a - m);
+        const Pair r = {m, deviation(sum_lanes(M, p.lanes), p.inv_per, p.eps)};
+        if (in && lane == 0) {
+          whole[q] = r;
+          keep(q, r);
+        }
+      });
+      row_sync<T>();
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (k * T + t < p.chunks) stat[k] = whole[(k * T + t) / p.chunks_per];
+      row_sync<T>();  // (the next row's parts go where these are read)
+    }
 #pragma unroll
     for (int k = 0; k < C; ++k) {
       const int chunk = k * T + t;
       if (chunk >= p.chunks) continue;
-      const Pair s = whole[chunk / p.chunks_per];
-      float gamma[VE], beta[VE];
-      load_affine<KIND, VE>(p, chunk, gamma, beta);
-      forward_vec<VE>(p.act, s.a, s.b, gamma, beta, v[k]);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[k][e] = __builtin_fmaf(v[k][e], stat[k].b, -stat[k].a * stat[k].b);
+      forward_vec<KIND, VE>(p.act, gamma[k], beta[k], v[k]);
       if (there) store_vec<KIND, VE>(static_cast<E*>(p.y) + row * p.ld_y + (long)chunk * VE, v[k]);
     }
-    row_sync<T>();  // (the next row's parts go where these are read)
   }
 }
 
 // Its gradients: dgamma and dbeta of a thread's channels are summed over all rows that its block takes, and
 // then over the block's row lanes; partial [blocks][2][channels].
-template <int KIND, int VE, int T, int C, bool KEPT>
+template <int KIND, int VE, int T, int C, bool LANES, bool KEPT>
 __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
   extern __shared__ __align__(16) char lds[];
@@ -231,61 +338,82 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
   const int t = threadIdx.x % T, mine = threadIdx.x / T;
   Pair* parts = reinterpret_cast<Pair*>(lds) + (size_t)mine * (p.chunks + p.groups);
   Pair* whole = parts + p.chunks;
-  float ga[C][VE] = {}, be[C][VE] = {};
-  for (long row0 = (long)blockIdx.x * R; row0 < p.rows; row0 += (long)gridDim.x * R) {
-    const bool there = row0 + mine < p.rows;
-    const long row = there ? row0 + mine : p.rows - 1;
-    float v[C][VE], dz[C][VE], r[C];
+  float gamma[C][VE], beta[C][VE];
 #pragma unroll
-    for (int k = 0; k < C; ++k)
-      if (k * T + t < p.chunks) {
-        load_x<KIND, VE, KEPT>(p, v[k], row, k * T + t);
-        load_vec<KIND, VE>(dz[k], static_cast<const E*>(p.dy) + row * p.ld_y + (long)(k * T + t) * VE);
-      }
+  for (int k = 0; k < C; ++k) load_affine<KIND, VE>(p, min(k * T + t, p.chunks - 1), gamma[k], beta[k]);
+  float ga[C][VE] = {}, be[C][VE] = {};
+  RawX<KIND, VE, KEPT> raw_x[C];
+  Raw<KIND, VE> raw_dy[C];
+  Pair stat[C];
+  auto fetch = [&](long row) {  // (dy of rows past the last: zeros)
+    const bool there = row < p.rows;
+    row = min(row, p.rows - 1);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
       const int chunk = k * T + t;
       if (chunk >= p.chunks) continue;
-      const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * (row * p.groups + chunk / p.chunks_per));
-      r[k] = s.b;
-      float gamma[VE], beta[VE];
-      load_affine<KIND, VE>(p, chunk, gamma, beta);
-      grad_vec<VE>(p.act, s.a, s.b, gamma, beta, v[k], dz[k]);
-      Pair sum = {0.0f, 0.0f};
+      raw_x[k].load_at(p, row, chunk);
+      if (there)
+        raw_dy[k].load(static_cast<const E*>(p.dy) + row * p.ld_y + (long)chunk * VE);
+      else
+        raw_dy[k].zeros();
+      stat[k] = *reinterpret_cast<const Pair*>(p.stats + 2 * (row * p.groups + chunk / p.chunks_per));
+    }
+  };
+  const long step = (long)gridDim.x * R;
+  fetch((long)blockIdx.x * R + mine);
+  for (long row0 = (long)blockIdx.x * R; row0 < p.rows; row0 += step) {
+    const long row = row0 + mine;
+    const bool there = row < p.rows;
+    float v[C][VE], w[C][VE], r[C];
+    Pair means[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int chunk = k * T + t;
+      means[k] = Pair{0.0f, 0.0f};
+      if (chunk >= p.chunks) continue;
+      raw_x[k].normalized(stat[k], v[k]);
+      raw_dy[k].get(w[k]);
+      r[k] = stat[k].b;
+      grad_vec<KIND, VE>(p.act, gamma[k], beta[k], v[k], w[k]);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float w = gamma[e] * dz[k][e];
-        sum.a += w;
-        sum.b += w * v[k][e];
-        if (there) {
-          be[k][e] += dz[k][e];
-          ga[k][e] += dz[k][e] * v[k][e];
-        }
+        be[k][e] += w[k][e];
+        ga[k][e] += w[k][e] * v[k][e];
+        w[k][e] *= gamma[k][e];
+        means[k].a += w[k][e];
+        means[k].b += w[k][e] * v[k][e];
       }
-      parts[chunk] = sum;
+      if constexpr (!LANES) parts[chunk] = means[k];
     }
-    row_sync<T>();
-    each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
-      const Pair* s = parts + q * p.chunks_per;
-      float a = 0.0f, b = 0.0f;
-      for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) a += s[k].a, b += s[k].b;
-      a = sum_lanes(a, p.lanes) / (float)p.per;
-      b = sum_lanes(b, p.lanes) / (float)p.per;
-      if (in && lane == 0) whole[q] = Pair{a, b};
-    });
-    row_sync<T>();
+    if (row0 + step < p.rows) fetch(row + step);
+    if constexpr (LANES) {
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        means[k] = Pair{sum_lanes(means[k].a, p.lanes) * p.inv_per, sum_lanes(means[k].b, p.lanes) * p.inv_per};
+    } else {
+      row_sync<T>();
+      each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
+        const Pair* s = parts + q * p.chunks_per;
+        float a = 0.0f, b = 0.0f;
+        for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) a += s[k].a, b += s[k].b;
+        a = sum_lanes(a, p.lanes) * p.inv_per;
+        b = sum_lanes(b, p.lanes) * p.inv_per;
+        if (in && lane == 0) whole[q] = Pair{a, b};
+      });
+      row_sync<T>();
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (k * T + t < p.chunks) means[k] = whole[(k * T + t) / p.chunks_per];
+      row_sync<T>();
+    }
 #pragma unroll
     for (int k = 0; k < C; ++k) {
       const int chunk = k * T + t;
-      if (chunk >= p.chunks) continue;
-      const Pair s = whole[chunk / p.chunks_per];
-      float gamma[VE], beta[VE];
-      load_affine<KIND, VE>(p, chunk, gamma, beta);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) dz[k][e] = r[k] * (gamma[e] * dz[k][e] - s.a - v[k][e] * s.b);
-      if (there && p.dx) store_vec<KIND, VE>(static_cast<E*>(p.dx) + row * p.ld_x + (long)chunk * VE, dz[k]);
+      if (chunk >= p.chunks || !there || !p.dx) continue;
+      dx_vec<VE>(r[k], means[k], v[k], w[k]);
+      store_vec<KIND, VE>(static_cast<E*>(p.dx) + row * p.ld_x + (long)chunk * VE, w[k]);
     }
-    row_sync<T>();
   }
   if (!p.partial) return;
   float* out = p.partial + (long)blockIdx.x * 2 * p.channels;
@@ -319,17 +447,17 @@ __device__ __forceinline__ Lay lay_of(int part, int cols) {
 
 constexpr int kBatch = 4;  // rows under way
 
-// Moments of a thread's chunk over rows first + tr, + TR, ... below first + count; n: their number
+// The moments s of a thread's chunk, joined with those of its rows from the `from`-th on: first + tr + i TR below
+// first + count
 template <int KIND, int VE>
-__device__ __forceinline__ Pair thread_moments(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                               int& n) {
-  Pair s = {0.0f, 0.0f};
-  n = 0;
-  int r = l.tr;
+__device__ __forceinline__ void thread_moments(const NormArgs& p, long first, int count, int chunk, const Lay& l,
+                                               int from, Pair& s) {
+  const typename ElemOf<KIND>::T* x = static_cast<const typename ElemOf<KIND>::T*>(p.x) + (long)chunk * VE;
+  int n = from, r = l.tr + from * l.TR;
   for (; r + (kBatch - 1) * l.TR < count; r += kBatch * l.TR) {
     float v[kBatch][VE];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) load_x<KIND, VE, false>(p, v[b], first + r + (long)b * l.TR, chunk);
+    for (int b = 0; b < kBatch; ++b) load_vec<KIND, VE>(v[b], x + (first + r + (long)b * l.TR) * p.ld_x);
     float m = 0.0f, M = 0.0f;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
@@ -345,115 +473,145 @@ __device__ __forceinline__ Pair thread_moments(const NormArgs& p, long first, in
   }
   for (; r < count; r += l.TR) {
     float v[VE];
-    load_x<KIND, VE, false>(p, v, first + r, chunk);
+    load_vec<KIND, VE>(v, x + (first + r) * p.ld_x);
     join_moments(s, (float)(n * VE), moments<VE>(v), (float)VE);
     ++n;
   }
-  return s;
 }
 // rows of a thread in row lane tr
 __device__ __forceinline__ int rows_of(int count, int tr, int TR) { return count > tr ? (count - tr + TR - 1) / TR : 0; }
 
-// y of a thread's chunk over its rows
+// y = act(x scale + shift) of a thread's chunk over its rows
 template <int KIND, int VE>
 __device__ __forceinline__ void thread_apply(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                             const Pair& s) {
+                                             int from, const float (&scale)[VE], const float (&shift)[VE]) {
   using E = typename ElemOf<KIND>::T;
-  float gamma[VE], beta[VE];
-  load_affine<KIND, VE>(p, chunk, gamma, beta);
+  const E* x = static_cast<const E*>(p.x) + (long)chunk * VE;
   E* y = static_cast<E*>(p.y) + (long)chunk * VE;
-  int r = l.tr;
+  int r = l.tr + from * l.TR;
   for (; r + (kBatch - 1) * l.TR < count; r += kBatch * l.TR) {
-    float v[kBatch][VE];
+    Raw<KIND, VE> raw[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) load_x<KIND, VE, false>(p, v[b], first + r + (long)b * l.TR, chunk);
+    for (int b = 0; b < kBatch; ++b) raw[b].load(x + (first + r + (long)b * l.TR) * p.ld_x);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      forward_vec<VE>(p.act, s.a, s.b, gamma, beta, v[b]);
-      store_vec<KIND, VE>(y + (first + r + (long)b * l.TR) * p.ld_y, v[b]);
+      float v[VE];
+      raw[b].get(v);
+      forward_vec<KIND, VE>(p.act, scale, shift, v);
+      store_vec<KIND, VE>(y + (first + r + (long)b * l.TR) * p.ld_y, v);
     }
   }
   for (; r < count; r += l.TR) {
     float v[VE];
-    load_x<KIND, VE, false>(p, v, first + r, chunk);
-    forward_vec<VE>(p.act, s.a, s.b, gamma, beta, v);
+    load_vec<KIND, VE>(v, x + (first + r) * p.ld_x);
+    forward_vec<KIND, VE>(p.act, scale, shift, v);
     store_vec<KIND, VE>(y + (first + r) * p.ld_y, v);
   }
 }
+// gamma v + beta = x scale + shift
+template <int VE>
+__device__ __forceinline__ void scale_shift(const Pair& s, const float (&gamma)[VE], const float (&beta)[VE],
+                                            float (&scale)[VE], float (&shift)[VE]) {
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    scale[e] = gamma[e] * s.b;
+    shift[e] = __builtin_fmaf(-s.a, scale[e], beta[e]);
+  }
+}
 
+// x and dy of a thread's chunk, both kRows rows of them, under way together.
+template <int KIND, int VE, bool KEPT, class F>
+__device__ __forceinline__ void thread_rows(const NormArgs& p, long first, int count, int chunk, const Lay& l,
+                                            int from, const Pair& s, F&& f) {
+  constexpr int kRows = 2;
+  using E = typename ElemOf<KIND>::T;
+  const E* dy = static_cast<const E*>(p.dy) + (long)chunk * VE;
+  for (int r = l.tr + from * l.TR; r < count; r += kRows * l.TR) {
+    RawX<KIND, VE, KEPT> raw_x[kRows];
+    Raw<KIND, VE> raw_dy[kRows];
+#pragma unroll
+    for (int b = 0; b < kRows; ++b)
+      if (r + b * l.TR < count) {
+        raw_x[b].load_at(p, first + r + (long)b * l.TR, chunk);
+        raw_dy[b].load(dy + (first + r + (long)b * l.TR) * p.ld_y);
+      }
+#pragma unroll
+    for (int b = 0; b < kRows; ++b)
+      if (r + b * l.TR < count) {
+        float v[VE], d[VE];
+        raw_x[b].normalized(s, v);
+        raw_dy[b].get(d);
+        f(v, d, first + r + (long)b * l.TR);
+      }
+  }
+}
 // dz and dz v of a thread's chunk summed over its rows
 template <int KIND, int VE, bool KEPT>
 __device__ __forceinline__ void thread_sums(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                            const Pair& s, const float (&gamma)[VE], const float (&beta)[VE],
-                                            float (&be)[VE], float (&ga)[VE]) {
-  using E = typename ElemOf<KIND>::T;
-  const E* dy = static_cast<const E*>(p.dy) + (long)chunk * VE;
-  auto add = [&](float (&v)[VE], float (&d)[VE]) {
-    grad_vec<VE>(p.act, s.a, s.b, gamma, beta, v, d);
+                                            int from, const Pair& s, const float (&gamma)[VE],
+                                            const float (&beta)[VE], float (&be)[VE], float (&ga)[VE]) {
+  thread_rows<KIND, VE, KEPT>(p, first, count, chunk, l, from, s, [&](float (&v)[VE], float (&d)[VE], long) {
+    grad_vec<KIND, VE>(p.act, gamma, beta, v, d);
 #pragma unroll
     for (int e = 0; e < VE; ++e) be[e] += d[e], ga[e] += d[e] * v[e];
-  };
-  int r = l.tr;
-  for (; r + l.TR < count; r += 2 * l.TR) {
-    float v[2][VE], d[2][VE];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      load_x<KIND, VE, KEPT>(p, v[b], first + r + (long)b * l.TR, chunk);
-      load_vec<KIND, VE>(d[b], dy + (first + r + (long)b * l.TR) * p.ld_y);
-    }
-    add(v[0], d[0]);
-    add(v[1], d[1]);
-  }
-  if (r < count) {
-    float v[VE], d[VE];
-    load_x<KIND, VE, KEPT>(p, v, first + r, chunk);
-    load_vec<KIND, VE>(d, dy + (first + r) * p.ld_y);
-    add(v, d);
-  }
+  });
 }
 template <int KIND, int VE, bool KEPT>
 __device__ __forceinline__ void thread_dx(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                          const Pair& s, const Pair& sums, const float (&gamma)[VE],
+                                          int from, const Pair& s, const Pair& means, const float (&gamma)[VE],
                                           const float (&beta)[VE]) {
   using E = typename ElemOf<KIND>::T;
-  const E* dy = static_cast<const E*>(p.dy) + (long)chunk * VE;
   E* dx = static_cast<E*>(p.dx) + (long)chunk * VE;
-  auto put = [&](float (&v)[VE], float (&d)[VE], long row) {
-    grad_vec<VE>(p.act, s.a, s.b, gamma, beta, v, d);
+  thread_rows<KIND, VE, KEPT>(p, first, count, chunk, l, from, s, [&](float (&v)[VE], float (&d)[VE], long row) {
+    grad_vec<KIND, VE>(p.act, gamma, beta, v, d);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) d[e] = s.b * (gamma[e] * d[e] - sums.a - v[e] * sums.b);
+    for (int e = 0; e < VE; ++e) d[e] *= gamma[e];
+    dx_vec<VE>(s.b, means, v, d);
     store_vec<KIND, VE>(dx + row * p.ld_x, d);
-  };
-  int r = l.tr;
-  for (; r + l.TR < count; r += 2 * l.TR) {
-    float v[2][VE], d[2][VE];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      load_x<KIND, VE, KEPT>(p, v[b], first + r + (long)b * l.TR, chunk);
-      load_vec<KIND, VE>(d[b], dy + (first + r + (long)b * l.TR) * p.ld_y);
-    }
-    put(v[0], d[0], first + r);
-    put(v[1], d[1], first + r + l.TR);
-  }
-  if (r < count) {
-    float v[VE], d[VE];
-    load_x<KIND, VE, KEPT>(p, v, first + r, chunk);
-    load_vec<KIND, VE>(d, dy + (first + r) * p.ld_y);
-    put(v, d, first + r);
-  }
+  });
 }
 
-// Whole frames: grid (parts, frames, or fewer in y: strided).
+// Whole frames: grid (parts, frames, or fewer in y: strided). A thread's first kHold rows stay in registers
+// between the sums and the output; what is beyond them is read again.
 template <int KIND, int VE>
 __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
+  using E = typename ElemOf<KIND>::T;
+  constexpr int kHold = 8;
   __shared__ Pair parts[kThreads], whole[kThreads];
   const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0), groups = cols / p.chunks_per;
   const Lay l = lay_of(p.part, cols);
   const int chunk = c0 + min(l.tc, cols - 1);
+  float gamma[VE], beta[VE];
+  load_affine<KIND, VE>(p, chunk, gamma, beta);
   for (int f = blockIdx.y; f < p.frames; f += gridDim.y) {
     const Frame w = frame_of(p, f);
-    int n = 0;
-    const Pair mine = l.in ? thread_moments<KIND, VE>(p, w.first, w.count, chunk, l, n) : Pair{0.0f, 0.0f};
+    const int have = l.in ? min(rows_of(w.count, l.tr, l.TR), kHold) : 0;
+    // (rows past the thread's last stay zeros)
+    Raw<KIND, VE> raw[kHold];
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+      raw[i].zeros();
+      if (i < have)
+        raw[i].load(static_cast<const E*>(p.x) + (w.first + l.tr + (long)i * l.TR) * p.ld_x + (long)chunk * VE);
+    }
+    Pair mine = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+      float v[VE];
+      raw[i].get(v);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) mine.a += v[e];
+    }
+    mine.a = have ? mine.a / (float)(have * VE) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+      if (i < have) {
+        float v[VE];
+        raw[i].get(v);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) mine.b += (v[e] - mine.a) * (v[e] - mine.a);
+      }
+    if (l.in) thread_moments<KIND, VE>(p, w.first, w.count, chunk, l, kHold, mine);
     parts[threadIdx.x] = mine;
     __syncthreads();
     const float total = (float)w.count * (float)p.per;
@@ -471,7 +629,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
         M += s.b + (float)(rows_of(w.count, tr, l.TR) * VE) * (s.a - m) * (s.a - m);
       }
       M = sum_lanes(M, p.lanes);
-      const Pair s = w.count ? Pair{m, deviation(M, total, p.eps)} : Pair{0.0f, 0.0f};
+      const Pair s = w.count ? Pair{m, deviation(M, 1.0f / total, p.eps)} : Pair{0.0f, 0.0f};
       if (in && lane == 0) {
         whole[q] = s;
         if (p.stats)
@@ -479,7 +637,19 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
       }
     });
     __syncthreads();
-    if (l.in) thread_apply<KIND, VE>(p, w.first, w.count, chunk, l, whole[l.tc / p.chunks_per]);
+    if (l.in) {
+      float scale[VE], shift[VE];
+      scale_shift<VE>(whole[l.tc / p.chunks_per], gamma, beta, scale, shift);
+#pragma unroll
+      for (int i = 0; i < kHold; ++i)
+        if (i < have) {
+          float v[VE];
+          raw[i].get(v);
+          forward_vec<KIND, VE>(p.act, scale, shift, v);
+          store_vec<KIND, VE>(static_cast<E*>(p.y) + (w.first + l.tr + (long)i * l.TR) * p.ld_y + (long)chunk * VE, v);
+        }
+      thread_apply<KIND, VE>(p, w.first, w.count, chunk, l, kHold, scale, shift);
+    }
     __syncthreads();
   }
 }
@@ -487,6 +657,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
 // partial [gridDim.y][2][channels]
 template <int KIND, int VE, bool KEPT>
 __global__ __launch_bounds__(kThreads) void k_norm_frames_grad(const NormArgs p) {
+  using E = typename ElemOf<KIND>::T;
+  constexpr int kHold = VE == 8 ? 4 : 8;  // rows whose v and dz stay in registers: 64 of these
   __shared__ Pair parts[kThreads], whole[kThreads];
   __shared__ float sums[kThreads * VE];
   const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0), groups = cols / p.chunks_per;
@@ -497,8 +669,30 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames_grad(const NormArgs p)
   for (int f = blockIdx.y; f < p.frames; f += gridDim.y) {
     const Frame w = frame_of(p, f);
     const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * ((long)f * p.groups + chunk / p.chunks_per));
-    float b[VE] = {}, g[VE] = {};
-    if (l.in) thread_sums<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, s, gamma, beta, b, g);
+    const int have = l.in ? min(rows_of(w.count, l.tr, l.TR), kHold) : 0;
+    RawX<KIND, VE, KEPT> raw_x[kHold];
+    Raw<KIND, VE> raw_dy[kHold];
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+      if (i < have) {
+        const long row = w.first + l.tr + (long)i * l.TR;
+        raw_x[i].load_at(p, row, chunk);
+        raw_dy[i].load(static_cast<const E*>(p.dy) + row * p.ld_y + (long)chunk * VE);
+      }
+    float b[VE] = {}, g[VE] = {}, v[kHold][VE], d[kHold][VE];
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+      if (i < have) {
+        raw_x[i].normalized(s, v[i]);
+        raw_dy[i].get(d[i]);
+        grad_vec<KIND, VE>(p.act, gamma, beta, v[i], d[i]);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          b[e] += d[i][e], g[e] += d[i][e] * v[i][e];
+          d[i][e] *= gamma[e];
+        }
+      }
+    if (l.in) thread_sums<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, kHold, s, gamma, beta, b, g);
     Pair sum = {0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
@@ -524,8 +718,16 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames_grad(const NormArgs p)
       if (in && lane == 0) whole[q] = Pair{x / total, y / total};
     });
     __syncthreads();
-    if (l.in)
-      thread_dx<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, s, whole[l.tc / p.chunks_per], gamma, beta);
+    if (l.in) {
+      const Pair q = whole[l.tc / p.chunks_per];
+#pragma unroll
+      for (int i = 0; i < kHold; ++i)
+        if (i < have) {
+          dx_vec<VE>(s.b, q, v[i], d[i]);
+          store_vec<KIND, VE>(static_cast<E*>(p.dx) + (w.first + l.tr + (long)i * l.TR) * p.ld_x + (long)chunk * VE, d[i]);
+        }
+      thread_dx<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, kHold, s, q, gamma, beta);
+    }
     __syncthreads();
   }
   if (!p.partial) return;
@@ -546,8 +748,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames_grad(const NormArgs p)
 // ---- frames cut into slices --------------------------------------------------------------------
 // Slice z of a frame's rows
 __device__ __forceinline__ Frame slice_of(const Frame& w, int z, int slices) {
-  const long a = (long)w.count * z / slices, b = (long)w.count * (z + 1) / slices;
-  return Frame{w.first + a, (int)(b - a)};
+  // (the first `more` slices have a row more)
+  const int each = w.count / slices, more = w.count - each * slices;
+  return Frame{w.first + (long)each * z + min(z, more), each + (z < more)};
 }
 
 // Moments of each chunk over a slice: pairs [frames][slices][chunks]. Grid (parts, slices, frames).
@@ -558,9 +761,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(const NormArgs p) {
   const Lay l = lay_of(p.part, cols);
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
     const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
-    int n = 0;
-    parts[threadIdx.x] =
-        l.in ? thread_moments<KIND, VE>(p, w.first, w.count, c0 + l.tc, l, n) : Pair{0.0f, 0.0f};
+    Pair mine = {0.0f, 0.0f};
+    if (l.in) thread_moments<KIND, VE>(p, w.first, w.count, c0 + l.tc, l, 0, mine);
+    parts[threadIdx.x] = mine;
     __syncthreads();
     if ((int)threadIdx.x < cols) {
       Pair s = parts[threadIdx.x];
@@ -593,25 +796,30 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_join(const NormArgs p) 
     const int f = (int)(at / p.groups), q = (int)(at % p.groups);
     const Frame w = frame_of(p, f);
     const float* s = p.pairs + 2 * ((long)f * p.slices * p.chunks + (long)q * p.chunks_per);
-    const long n = (long)p.slices * p.chunks_per;
-    auto entry = [&](long k, int& rows) {
-      const int z = (int)(k / p.chunks_per);
-      rows = slice_of(w, z, p.slices).count;
-      return *reinterpret_cast<const Pair*>(s + 2 * ((long)z * p.chunks + k % p.chunks_per));
+    const unsigned per = p.chunks_per, n = (unsigned)p.slices * per;
+    // an entry's moments, and how many values it stands for
+    auto entry = [&](unsigned k, Pair& e) {
+      const unsigned z = k / per;
+      e = *reinterpret_cast<const Pair*>(s + 2 * ((long)z * p.chunks + (k - z * per)));
+      return (double)(slice_of(w, z, p.slices).count * VE);
+    };
+    constexpr int kUnder = 4;
+    auto all = [&](auto f) {
+      for (unsigned k = threadIdx.x; k < n; k += kUnder * kThreads) {
+        Pair e[kUnder];
+        double count[kUnder];
+#pragma unroll
+        for (int u = 0; u < kUnder; ++u) count[u] = k + u * kThreads < n ? entry(k + u * kThreads, e[u]) : 0.0;
+#pragma unroll
+        for (int u = 0; u < kUnder; ++u)
+          if (k + u * kThreads < n) f(e[u], count[u]);
+      }
     };
     double m = 0.0, M = 0.0;
-    for (long k = threadIdx.x; k < n; k += kThreads) {
-      int rows;
-      const Pair e = entry(k, rows);
-      m += (double)rows * VE * e.a;
-    }
+    all([&](const Pair& e, double count) { m += count * e.a; });
     const double total = (double)w.count * p.per;
     m = block_sum(m, lds) / (total > 0.0 ? total : 1.0);
-    for (long k = threadIdx.x; k < n; k += kThreads) {
-      int rows;
-      const Pair e = entry(k, rows);
-      M += e.b + (double)rows * VE * (e.a - m) * (e.a - m);
-    }
+    all([&](const Pair& e, double count) { M += e.b + count * (e.a - m) * (e.a - m); });
     M = block_sum(M, lds);
     if (threadIdx.x == 0)
       *reinterpret_cast<Pair*>(p.stats + 2 * at) =
@@ -625,10 +833,14 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(const NormArgs p) {
   const Lay l = lay_of(p.part, cols);
   if (!l.in) return;
   const int chunk = c0 + l.tc;
+  float gamma[VE], beta[VE];
+  load_affine<KIND, VE>(p, chunk, gamma, beta);
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
     const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
     const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * ((long)f * p.groups + chunk / p.chunks_per));
-    thread_apply<KIND, VE>(p, w.first, w.count, chunk, l, s);
+    float scale[VE], shift[VE];
+    scale_shift<VE>(s, gamma, beta, scale, shift);
+    thread_apply<KIND, VE>(p, w.first, w.count, chunk, l, 0, scale, shift);
   }
 }
 
@@ -647,7 +859,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_sums(const NormArgs p) {
     const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
     const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * ((long)f * p.groups + chunk / p.chunks_per));
     float b[VE] = {}, g[VE] = {};
-    if (l.in) thread_sums<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, s, gamma, beta, b, g);
+    if (l.in) thread_sums<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, 0, s, gamma, beta, b, g);
     Pair sum = {0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
@@ -696,9 +908,11 @@ __global__ __launch_bounds__(kThreads) void k_norm_sums_join(const NormArgs p, i
       const int f = (int)(at / p.groups), q = (int)(at % p.groups);
       const float* s = p.pairs + 2 * ((long)f * p.slices * p.chunks + (long)q * p.chunks_per);
       double a = 0.0, b = 0.0;
-      const long n = (long)p.slices * p.chunks_per;
-      for (long k = threadIdx.x; k < n; k += kThreads) {
-        const Pair e = *reinterpret_cast<const Pair*>(s + 2 * (k / p.chunks_per * p.chunks + k % p.chunks_per));
+      const unsigned per = p.chunks_per, n = (unsigned)p.slices * per;
+#pragma unroll 4
+      for (unsigned k = threadIdx.x; k < n; k += kThreads) {
+        const unsigned z = k / per;
+        const Pair e = *reinterpret_cast<const Pair*>(s + 2 * ((long)z * p.chunks + (k - z * per)));
         a += e.a;
         b += e.b;
       }
@@ -712,11 +926,25 @@ __global__ __launch_bounds__(kThreads) void k_norm_sums_join(const NormArgs p, i
   const int slot = threadIdx.x % 16, share = threadIdx.x / 16;
   const long c = (long)(blockIdx.x - group_blocks) * 16 + slot;
   double a = 0.0, b = 0.0;
-  if (c < p.channels)
-    for (long k = parts * share / 16; k < parts * (share + 1) / 16; ++k) {
-      b += p.partial[k * 2 * p.channels + c];
-      a += p.partial[(k * 2 + 1) * p.channels + c];
+  if (c < p.channels) {
+    const long end = parts * (share + 1) / 16;
+    const float* s = p.partial + c;
+    long k = parts * share / 16;
+    for (; k + 8 <= end; k += 8) {
+      float x[8], y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        x[u] = s[(k + u) * 2 * p.channels];
+        y[u] = s[((k + u) * 2 + 1) * p.channels];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) b += x[u], a += y[u];
     }
+    for (; k < end; ++k) {
+      b += s[k * 2 * p.channels];
+      a += s[(k * 2 + 1) * p.channels];
+    }
+  }
   lds[0][threadIdx.x] = a;
   lds[1][threadIdx.x] = b;
   __syncthreads();
@@ -738,7 +966,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_dx(const NormArgs p) {
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
     const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
     const long at = 2 * ((long)f * p.groups + chunk / p.chunks_per);
-    thread_dx<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, *reinterpret_cast<const Pair*>(p.stats + at),
+    thread_dx<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, 0, *reinterpret_cast<const Pair*>(p.stats + at),
                               *reinterpret_cast<const Pair*>(p.sums + at), gamma, beta);
   }
 }
@@ -753,18 +981,24 @@ void by_vec(int vec, F&& f) {
   if (vec == 2) return f(std::integral_constant<int, 2>{});
   f(std::integral_constant<int, 1>{});
 }
-// threads of a row and chunks of a thread
+// threads of a row, chunks of a thread, and whether groups are lanes
 template <class F>
-void by_row(int chunks, F&& f) {
+void by_row(const NormArgs& p, F&& f) {
   using std::integral_constant;
-  if (chunks <= 16)
-    f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-  else if (chunks <= 64)
-    f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  else if (chunks <= 256)
-    f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  auto lanes = [&](auto t, auto c) {
+    if (p.by_lanes)
+      f(t, c, std::true_type{});
+    else
+      f(t, c, std::false_type{});
+  };
+  if (p.chunks <= 16)
+    lanes(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (p.chunks <= 64)
+    lanes(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (p.chunks <= 256)
+    lanes(integral_constant<int, 256>{}, integral_constant<int, 1>{});
   else
-    f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    lanes(integral_constant<int, 256>{}, integral_constant<int, 4>{});
 }
 size_t row_lds(const NormArgs& p, int T, int VE, bool grad) {
   const size_t parts = (size_t)(kThreads / T) * (p.chunks + p.groups) * sizeof(Pair);
@@ -782,11 +1016,11 @@ void norm_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
   by_vec(p.vec, [&](auto ve) {
     constexpr int VE = decltype(ve)::value;
     if (p.form == kNormRows) {
-      by_row(p.chunks, [&](auto t, auto c) {
+      by_row(p, [&](auto t, auto c, auto lanes) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
-        const long want = (p.rows + kThreads / T - 1) / (kThreads / T);
-        hipLaunchKernelGGL((k_norm_rows<KIND, VE, T, C>), dim3((unsigned)std::min(want, 1L << 20)), dim3(kThreads),
-                           row_lds(p, T, VE, false), st, p);
+        constexpr bool LANES = decltype(lanes)::value;
+        hipLaunchKernelGGL((k_norm_rows<KIND, VE, T, C, LANES>), dim3(p.blocks), dim3(kThreads),
+                           LANES ? 0 : row_lds(p, T, VE, false), st, p);
       });
     } else if (p.form == kNormFrames) {
       hipLaunchKernelGGL((k_norm_frames<KIND, VE>), frame_grid(p), dim3(kThreads), 0, st, p);
@@ -812,9 +1046,10 @@ void norm_grad_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
     int group_blocks = 0;
     long parts = 0;
     if (p.form == kNormRows) {
-      by_row(p.chunks, [&](auto t, auto c) {
+      by_row(p, [&](auto t, auto c, auto lanes) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
-        hipLaunchKernelGGL((k_norm_rows_grad<KIND, VE, T, C, KEPT>), dim3(p.blocks), dim3(kThreads),
+        constexpr bool LANES = decltype(lanes)::value;
+        hipLaunchKernelGGL((k_norm_rows_grad<KIND, VE, T, C, LANES, KEPT>), dim3(p.blocks), dim3(kThreads),
                            row_lds(p, T, VE, true), st, p);
       });
       parts = p.blocks;

@@ -141,6 +141,25 @@ struct Weights8Args {
 void weights8(hipStream_t st, int elem, const Weights8Args& args);
 // x [M][K] and weights [N][K] of integers, k contiguous; two weight matrices with `gate`
 void run_product8(hipStream_t st, bool gate, const ProductPlan& plan, ProductArgs& args);
+// for a few rows (linear8_rows.hip)
+constexpr int kLinear8Rows = 48;
+enum Linear8Form { kLinear8Tiles, kLinear8FewRows, kLinear8Fused };
+struct Linear8RowsArgs {
+  int rows, K, N, act, waves;
+  bool pairs;
+  const signed char* w[2];  // the second one null: no gate
+  long ld_w;
+  const float* col_scale[2];
+  const signed char* q;  // the rows in 8 bits, or null: x
+  long ld_q;
+  const float* row_scale;
+  const void* x;
+  long ld_x;
+  void* y;
+  long ld_y;
+};
+Linear8Form linear8_form(long rows, int K, int N);
+void run_linear8_rows(hipStream_t st, int elem, int ncu, Linear8RowsArgs& args);
 
 // Matrices [rows][cols] to be copied into rows of ld (a multiple of 8), with zeros past cols.
 struct PackItem {

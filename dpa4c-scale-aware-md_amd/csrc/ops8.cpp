@@ -47,8 +47,18 @@ void check_weights8(const void* w) {
 void linear8(dp_ops* O, const dp_linear8_shape& s, const void* x, const signed char* w, const float* w_scale,
              const signed char* up, const float* up_scale, void* y, hipStream_t st) {
   const int64_t ldq = ((int64_t)s.d_in + 15) / 16 * 16;
-  const ProductPlan plan =
-      plan_product(up ? kProdGate : kProdDown, kElemI8, s.rows, s.d_out, s.d_in, 1, 1, O->ncu);
+  const Linear8Form form = linear8_form((long)s.rows, s.d_in, s.d_out);
+  Linear8RowsArgs f{};
+  if (form != kLinear8Tiles) {
+    f.rows = (int)s.rows, f.K = s.d_in, f.N = s.d_out, f.act = s.act;
+    f.w[0] = w, f.w[1] = up, f.ld_w = (long)s.ld_w;
+    f.col_scale[0] = w_scale, f.col_scale[1] = up_scale;
+    f.x = x, f.ld_x = (long)s.ld_x, f.y = y, f.ld_y = (long)s.ld_y;
+    if (form == kLinear8Fused) return run_linear8_rows(st, elem_of(s.type), O->ncu, f);
+  }
+  ProductPlan plan{};
+  if (form == kLinear8Tiles)
+    plan = plan_product(up ? kProdGate : kProdDown, kElemI8, s.rows, s.d_out, s.d_in, 1, 1, O->ncu);
   Regions r;
   const size_t at_q = r.take((size_t)s.rows * ldq), at_s = r.take(sizeof(float) * (size_t)s.rows),
                at_part = r.take(plan.bytes);
@@ -59,6 +69,10 @@ void linear8(dp_ops* O, const dp_linear8_shape& s, const void* x, const signed c
   q.q = reinterpret_cast<signed char*>(ws + at_q);
   q.scale = reinterpret_cast<float*>(ws + at_s);
   rows8(st, elem_of(s.type), q);
+  if (form == kLinear8FewRows) {
+    f.q = q.q, f.ld_q = (long)ldq, f.row_scale = q.scale;
+    return run_linear8_rows(st, elem_of(s.type), O->ncu, f);
+  }
   ProductArgs p = product(Operand{q.q, (long)ldq}, Operand{w, (long)s.ld_w}, s.rows, s.d_out, s.d_in);
   p.b[1].p = up;
   p.act = s.act;

@@ -141,6 +141,28 @@ __device__ __forceinline__ void activate4(int act, const f4& g, f4& a, f4& da) {
     all(std::integral_constant<int, kActGelu>{});
 }
 
+// The same for results of 16 bits that are formed element by element (the norm, the 8-bit products), whose
+// vector instructions bound them: gelu's Phi(g) = 1 / (1 + exp(-g P(g^2))), P fitted to an even absolute error
+// of gelu up to |g| = 5.5 (1e-7; beyond it grows with g). gelu is off by 2e-7 of max(1, |g|), as silu is, and its
+// derivative by 2e-7: 18 instructions for 30 (forward; a rate of 4 counted as 4). Below -4, where gelu is under
+// 1.3e-4, its digits are not kept as the above keeps them.
+template <int KIND, int ACT>
+__device__ __forceinline__ void activate_as(float g, float& a, float& da) {
+  if constexpr (KIND == kF32 || ACT != kActGelu) {
+    activate<ACT>(g, a, da);
+  } else {
+    const float s = g * g;
+    const float l =
+        2.30220719f +
+        s * (0.104838343f +
+             s * (-9.5335357e-05f +
+                  s * (-0.000159458558f + s * (1.14574294e-05f + s * (-3.84952708e-07f + s * 5.20142374e-09f)))));
+    const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * l));
+    a = g * p;
+    da = p + g * __builtin_amdgcn_exp2f(-0.72134752f * s) * 0.39894228040143268f;
+  }
+}
+
 // ---- epilogues on four consecutive columns of one row, shared by the products and
 // by the sums over slices of K --------------------------------------------------------
 
@@ -247,12 +269,26 @@ __device__ __forceinline__ void put_pair(typename ElemOf<KIND>::T* p, const f4& 
 
 // ---- products of 8-bit integers -----------------------------------------------------------
 
-// act(g), or g itself
+// act(g), or g itself, for results of a kind
+template <int KIND>
 __device__ __forceinline__ f4 activated4(int act, const f4& g) {
   if (act == kActNone) return g;
-  f4 a, da;
-  activate4(act, g, a, da);
-  return a;
+  f4 v;
+  auto all = [&](auto k) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float a, da;
+      activate_as<KIND, decltype(k)::value>(g[r], a, da);
+      v[r] = a;
+    }
+  };
+  if (act == kActTanh)
+    all(std::integral_constant<int, kActTanh>{});
+  else if (act == kActSilu)
+    all(std::integral_constant<int, kActSilu>{});
+  else
+    all(std::integral_constant<int, kActGelu>{});
+  return v;
 }
 // A row's scale as two factors: with that of rows beyond 2^90 a sum (below 2^31) could leave fp32's range
 // before the column's scale brings it back.
@@ -264,19 +300,29 @@ __device__ __forceinline__ RowFactor row_factor(float scale) {
 }
 // Four columns of a row from the integer sums: act(g), or act(g) u; each sum in fp32 times the row's scale
 // and then the column's.
-template <bool GATE>
+template <int KIND, bool GATE>
 __device__ __forceinline__ f4 scaled4(int act, const f4& sums, const f4& other, const RowFactor& row, const f4& col,
                                       const f4& col_other) {
   const i4 s = __builtin_bit_cast(i4, sums), o = __builtin_bit_cast(i4, other);
   f4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = (float)s[e] * row.first * col[e] * row.last;
-  v = activated4(act, v);
+  v = activated4<KIND>(act, v);
   if constexpr (GATE) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= (float)o[e] * row.first * col_other[e] * row.last;
   }
   return v;
+}
+// Four consecutive elements at any alignment (which the hardware takes).
+template <int KIND>
+__device__ __forceinline__ void put_any4(typename ElemOf<KIND>::T* p, const f4& v) {
+  struct Four {
+    typename ElemOf<KIND>::T v[4];
+  } s;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s.v[e] = from_f32<KIND>(v[e]);
+  __builtin_memcpy(p, &s, sizeof(s));
 }
 // Scales of four columns, `count` of them there.
 __device__ __forceinline__ f4 scales4(const float* s, int count) {
@@ -303,11 +349,11 @@ __device__ __forceinline__ void scaled_out(const ProductArgs& p, const f4 (&acc)
   float scale[MI];
 #pragma unroll
   for (int i = 0; i < MI; ++i) scale[i] = p.row_scale[min(m0 + i * 16, p.M - 1)];
-  auto value = [&](int i, int j) {
-    return scaled4<GATE>(p.act, acc[i][j], acc[i][GATE ? NG + j : j], row_factor(scale[i]), col[j], other[j]);
-  };
   auto emit = [&](auto kind) {
     constexpr int OUT = decltype(kind)::value;
+    auto value = [&](int i, int j) {
+      return scaled4<OUT, GATE>(p.act, acc[i][j], acc[i][GATE ? NG + j : j], row_factor(scale[i]), col[j], other[j]);
+    };
     using T = typename ElemOf<OUT>::T;
     const long step = 16 * p.ldo[0];
     long at = m0 * p.ldo[0] + n0;
@@ -322,14 +368,13 @@ __device__ __forceinline__ void scaled_out(const ProductArgs& p, const f4 (&acc)
         return;
       }
     }
-    const bool whole = inside && p.vec[0];
 #pragma unroll
     for (int i = 0; i < MI; ++i, at += step)
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const f4 v = value(i, j);
-        if (whole)
-          put_row4<OUT, true>(p.out[0], at + j * 16, v, 4);
+        if (inside || (m0 + i * 16 < p.M && n0 + j * 16 + 4 <= p.N))
+          put_any4<OUT>(static_cast<T*>(p.out[0]) + at + j * 16, v);
         else if (m0 + i * 16 < p.M && n0 + j * 16 < p.N)
           put_row4<OUT, false>(p.out[0], at + j * 16, v, p.N - n0 - j * 16);
       }

@@ -42,15 +42,19 @@ __global__ __launch_bounds__(256) void k_join8(const ProductArgs p) {
   if (!in) return;
   const int count = p.N - n;
   const f4 col = scales4(p.col_scale[0] + n, count), other = GATE ? scales4(p.col_scale[1] + n, count) : f4{};
-  const f4 o = scaled4<GATE>(p.act, __builtin_bit_cast(f4, v[0]), __builtin_bit_cast(f4, v[SUB - 1]),
-                             row_factor(p.row_scale[row]), col, other);
   const long to = row * p.ldo[0] + n;
+  auto emit = [&](auto kind) {
+    constexpr int OUT = decltype(kind)::value;
+    const f4 o = scaled4<OUT, GATE>(p.act, __builtin_bit_cast(f4, v[0]), __builtin_bit_cast(f4, v[SUB - 1]),
+                                    row_factor(p.row_scale[row]), col, other);
+    put_row4<OUT, false>(p.out[0], to, o, count);
+  };
   if (p.out_elem == kF32)
-    put_row4<kF32, false>(p.out[0], to, o, count);
+    emit(std::integral_constant<int, kF32>{});
   else if (p.out_elem == kF16)
-    put_row4<kF16, false>(p.out[0], to, o, count);
+    emit(std::integral_constant<int, kF16>{});
   else
-    put_row4<kBf16, false>(p.out[0], to, o, count);
+    emit(std::integral_constant<int, kBf16>{});
 }
 
 template <bool GATE, class S>

@@ -104,22 +104,6 @@ __global__ __launch_bounds__(256) void k_restore8(const KeepArgs p) {
 }
 
 // ---- operands of the 8-bit products -------------------------------------------------------
-// s = max |x| / 127 and q = x (127 / max |x|) to nearest: both quotients are rounded to fp32, and the fused
-// multiply-add rounds their product with x once, to a whole number (the sum's last digit is 1), so that q
-// is the same on every machine.
-struct RowScale {
-  float inv, scale;
-};
-__device__ __forceinline__ RowScale row_scale(unsigned top) {
-  const float m = __builtin_bit_cast(float, top);
-  if (top >= 0x7f800000u) return RowScale{0.0f, __builtin_bit_cast(float, 0x7fc00000u)};
-  if (m < 0x1p-119f) return RowScale{0.0f, 0.0f};  // (below, the quotients leave fp32's range)
-  return RowScale{127.0f / m, m / 127.0f};
-}
-__device__ __forceinline__ unsigned quant8(float x, float inv) {
-  return low_byte(__builtin_fmaf(x, inv, kRound));
-}
-
 // A row by T threads of a block (64: a wave, four rows a block; 256), C eights a thread held in registers
 // between the maximum and the integers; what is beyond C T eights is read again, from the caches. Zeros up
 // to ld_q (a multiple of 16).
@@ -159,10 +143,7 @@ __global__ __launch_bounds__(256) void k_rows8(const Rows8Args p) {
     if (t == 0) p.scale[row] = s.scale;
     auto put = [&](int k, const float (&w)[8]) {
       if (k >= eights) return;
-      unsigned q[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[e / 4] |= quant8(s.inv == 0.0f ? 0.0f : w[e], s.inv) << (8 * (e % 4));
-      *reinterpret_cast<unsigned long long*>(p.q + row * p.ld_q + k * 8) = q[0] | (unsigned long long)q[1] << 32;
+      *reinterpret_cast<unsigned long long*>(p.q + row * p.ld_q + k * 8) = s.inv == 0.0f ? 0 : quantize8(w, s.inv);
     };
 #pragma unroll
     for (int k = 0; k < C; ++k) put(k * T + t, v[k]);
