@@ -40,6 +40,7 @@ NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
   const bool affine = grad && (p.dgamma || p.dbeta);
   NormNeeds need{};
   p.inv_chunks = 1.0f / (float)p.chunks_per, p.inv_per = 1.0f / (float)p.per;
+  p.once = past_caches((double)p.rows * p.channels * (elem == 2 ? 4 : 2));
   p.slices = 1;
   if (!p.starts && p.frames == p.rows && p.chunks <= 1024) {
     p.form = kNormRows;
@@ -73,9 +74,10 @@ NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
       p.form = kNormSlices;
       p.part = std::min(256, p.chunks);
       p.parts = (p.chunks + p.part - 1) / p.part;
-      const long want = std::max(1L, 8L * ncu / ((long)p.parts * p.frames));
+      const long want = std::max(1L, 4L * ncu / ((long)p.parts * p.frames));
       const int rows_block = 256 / p.part * 4;
       p.slices = (int)std::min(want, std::max(1L, length / rows_block));
+      p.out_slices = (int)std::min(2 * want, std::max(1L, length / rows_block));
       p.blocks = (int)std::min((long)p.frames, std::max(1L, 8L * ncu / ((long)p.parts * p.slices)));
       if (!grad || p.dx) need.pairs = 8 * (size_t)p.frames * p.slices * p.chunks;
       if (grad && p.dx) need.sums = 8 * (size_t)p.frames * p.groups;

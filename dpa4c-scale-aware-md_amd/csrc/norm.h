@@ -25,8 +25,9 @@ struct NormArgs {
   float inv_chunks, inv_per;  // 1 / chunks_per, 1 / per
   int lanes;   // log2 of the lanes that sum one group's chunks
   int part;    // chunks of a block's columns (whole groups with kNormFrames), `parts` of them
-  int parts, slices;
+  int parts, slices, out_slices;  // (the output's pass has slices of its own)
   int blocks;  // of the persistent kernels
+  bool once;   // y and dx are stored past the caches
   float* partial;  // dgamma and dbeta of blocks or slices, or null: none
   float* pairs;    // two sums of each chunk of a slice
   float* sums;     // [frames][groups][2]: means of gamma dz and gamma dz v

@@ -139,6 +139,22 @@ __device__ __forceinline__ void load_affine(const NormArgs& p, int chunk, float 
   if (p.beta) load_vec<KIND, VE>(beta, static_cast<const T*>(p.beta) + (long)chunk * VE);
 }
 
+// The same past the caches, where `once` (uniform).
+template <int KIND, int VE>
+__device__ __forceinline__ void store_out(typename ElemOf<KIND>::T* p, const float (&v)[VE], bool once) {
+  if constexpr (VE * sizeof(*p) == 16) {
+    if (once) {
+      struct Some {
+        typename ElemOf<KIND>::T v[VE];
+      } s;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s.v[e] = from_f32<KIND>(v[e]);
+      return store16<true>(p, __builtin_bit_cast(u4any, s));
+    }
+  }
+  store_vec<KIND, VE>(p, v);
+}
+
 // act and its derivative over a thread's values (one uniform branch for all of them)
 template <int KIND, int VE>
 __device__ __forceinline__ void activate_vec(int act, const float (&z)[VE], float (&a)[VE], float (&da)[VE]) {
@@ -323,7 +339,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) v[k][e] = __builtin_fmaf(v[k][e], stat[k].b, -stat[k].a * stat[k].b);
       forward_vec<KIND, VE>(p.act, gamma[k], beta[k], v[k]);
-      if (there) store_vec<KIND, VE>(static_cast<E*>(p.y) + row * p.ld_y + (long)chunk * VE, v[k]);
+      if (there) store_out<KIND, VE>(static_cast<E*>(p.y) + row * p.ld_y + (long)chunk * VE, v[k], p.once);
     }
   }
 }
@@ -342,27 +358,29 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
 #pragma unroll
   for (int k = 0; k < C; ++k) load_affine<KIND, VE>(p, min(k * T + t, p.chunks - 1), gamma[k], beta[k]);
   float ga[C][VE] = {}, be[C][VE] = {};
-  RawX<KIND, VE, KEPT> raw_x[C];
-  Raw<KIND, VE> raw_dy[C];
-  Pair stat[C];
-  auto fetch = [&](long row) {  // (dy of rows past the last: zeros)
+  // two rows are under way (with one, 16 waves of a compute unit wait for too few bytes)
+  struct Ahead {
+    RawX<KIND, VE, KEPT> x[C];
+    Raw<KIND, VE> dy[C];
+    Pair stat[C];
+  } ahead[2];
+  auto fetch = [&](long row, Ahead& to) {  // (dy of rows past the last: zeros)
     const bool there = row < p.rows;
     row = min(row, p.rows - 1);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
       const int chunk = k * T + t;
       if (chunk >= p.chunks) continue;
-      raw_x[k].load_at(p, row, chunk);
+      to.x[k].load_at(p, row, chunk);
       if (there)
-        raw_dy[k].load(static_cast<const E*>(p.dy) + row * p.ld_y + (long)chunk * VE);
+        to.dy[k].load(static_cast<const E*>(p.dy) + row * p.ld_y + (long)chunk * VE);
       else
-        raw_dy[k].zeros();
-      stat[k] = *reinterpret_cast<const Pair*>(p.stats + 2 * (row * p.groups + chunk / p.chunks_per));
+        to.dy[k].zeros();
+      to.stat[k] = *reinterpret_cast<const Pair*>(p.stats + 2 * (row * p.groups + chunk / p.chunks_per));
     }
   };
   const long step = (long)gridDim.x * R;
-  fetch((long)blockIdx.x * R + mine);
-  for (long row0 = (long)blockIdx.x * R; row0 < p.rows; row0 += step) {
+  auto compute = [&](long row0, Ahead& from) {
     const long row = row0 + mine;
     const bool there = row < p.rows;
     float v[C][VE], w[C][VE], r[C];
@@ -372,9 +390,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
       const int chunk = k * T + t;
       means[k] = Pair{0.0f, 0.0f};
       if (chunk >= p.chunks) continue;
-      raw_x[k].normalized(stat[k], v[k]);
-      raw_dy[k].get(w[k]);
-      r[k] = stat[k].b;
+      from.x[k].normalized(from.stat[k], v[k]);
+      from.dy[k].get(w[k]);
+      r[k] = from.stat[k].b;
       grad_vec<KIND, VE>(p.act, gamma[k], beta[k], v[k], w[k]);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
@@ -386,7 +404,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
       }
       if constexpr (!LANES) parts[chunk] = means[k];
     }
-    if (row0 + step < p.rows) fetch(row + step);
+    if (row0 + 2 * step < p.rows) fetch(row + 2 * step, from);
     if constexpr (LANES) {
 #pragma unroll
       for (int k = 0; k < C; ++k)
@@ -412,8 +430,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
       const int chunk = k * T + t;
       if (chunk >= p.chunks || !there || !p.dx) continue;
       dx_vec<VE>(r[k], means[k], v[k], w[k]);
-      store_vec<KIND, VE>(static_cast<E*>(p.dx) + row * p.ld_x + (long)chunk * VE, w[k]);
+      store_out<KIND, VE>(static_cast<E*>(p.dx) + row * p.ld_x + (long)chunk * VE, w[k], p.once);
     }
+  };
+  const long first = (long)blockIdx.x * R;
+  fetch(first + mine, ahead[0]);
+  if (first + step < p.rows) fetch(first + step + mine, ahead[1]);
+  for (long row0 = first; row0 < p.rows; row0 += 2 * step) {
+    compute(row0, ahead[0]);
+    if (row0 + step < p.rows) compute(row0 + step, ahead[1]);
   }
   if (!p.partial) return;
   float* out = p.partial + (long)blockIdx.x * 2 * p.channels;
@@ -498,14 +523,14 @@ __device__ __forceinline__ void thread_apply(const NormArgs& p, long first, int 
       float v[VE];
       raw[b].get(v);
       forward_vec<KIND, VE>(p.act, scale, shift, v);
-      store_vec<KIND, VE>(y + (first + r + (long)b * l.TR) * p.ld_y, v);
+      store_out<KIND, VE>(y + (first + r + (long)b * l.TR) * p.ld_y, v, p.once);
     }
   }
   for (; r < count; r += l.TR) {
     float v[VE];
     load_vec<KIND, VE>(v, x + (first + r) * p.ld_x);
     forward_vec<KIND, VE>(p.act, scale, shift, v);
-    store_vec<KIND, VE>(y + (first + r) * p.ld_y, v);
+    store_out<KIND, VE>(y + (first + r) * p.ld_y, v, p.once);
   }
 }
 // gamma v + beta = x scale + shift
@@ -567,7 +592,7 @@ __device__ __forceinline__ void thread_dx(const NormArgs& p, long first, int cou
 #pragma unroll
     for (int e = 0; e < VE; ++e) d[e] *= gamma[e];
     dx_vec<VE>(s.b, means, v, d);
-    store_vec<KIND, VE>(dx + row * p.ld_x, d);
+    store_out<KIND, VE>(dx + row * p.ld_x, d, p.once);
   });
 }
 
@@ -803,27 +828,34 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_join(const NormArgs p) 
       e = *reinterpret_cast<const Pair*>(s + 2 * ((long)z * p.chunks + (k - z * per)));
       return (double)(slice_of(w, z, p.slices).count * VE);
     };
-    constexpr int kUnder = 4;
-    auto all = [&](auto f) {
-      for (unsigned k = threadIdx.x; k < n; k += kUnder * kThreads) {
-        Pair e[kUnder];
-        double count[kUnder];
+    // one pass, around the first part's mean (in fp64, and the parts' means lie together)
+    Pair first;
+    entry(0, first);
+    constexpr int kUnder = 8;
+    double d = 0.0, M = 0.0;
+    for (unsigned k = threadIdx.x; k < n; k += kUnder * kThreads) {
+      Pair e[kUnder];
+      double count[kUnder];
 #pragma unroll
-        for (int u = 0; u < kUnder; ++u) count[u] = k + u * kThreads < n ? entry(k + u * kThreads, e[u]) : 0.0;
-#pragma unroll
-        for (int u = 0; u < kUnder; ++u)
-          if (k + u * kThreads < n) f(e[u], count[u]);
+      for (int u = 0; u < kUnder; ++u) {
+        count[u] = entry(min(k + u * kThreads, n - 1), e[u]);
+        if (k + u * kThreads >= n) count[u] = 0.0, e[u].b = 0.0f;
       }
-    };
-    double m = 0.0, M = 0.0;
-    all([&](const Pair& e, double count) { m += count * e.a; });
-    const double total = (double)w.count * p.per;
-    m = block_sum(m, lds) / (total > 0.0 ? total : 1.0);
-    all([&](const Pair& e, double count) { M += e.b + count * (e.a - m) * (e.a - m); });
-    M = block_sum(M, lds);
+#pragma unroll
+      for (int u = 0; u < kUnder; ++u) {
+        const double off = (double)e[u].a - first.a;
+        if (count[u] > 0.0) d += count[u] * off, M += e[u].b + count[u] * off * off;
+      }
+    }
+    const double total = (double)w.count * p.per, inv = total > 0.0 ? 1.0 / total : 0.0;
+    d = block_sum(d, lds) * inv;
+    M = block_sum(M, lds) - total * d * d;
+    const double m = first.a + d;
+    double var = M * inv;
+    if (var < 0.0) var = 0.0;  // (and a NaN stays one)
     if (threadIdx.x == 0)
       *reinterpret_cast<Pair*>(p.stats + 2 * at) =
-          total > 0.0 ? Pair{(float)m, (float)(1.0 / sqrt(M / total + (double)p.eps))} : Pair{0.0f, 0.0f};
+          total > 0.0 ? Pair{(float)m, (float)(1.0 / sqrt(var + (double)p.eps))} : Pair{0.0f, 0.0f};
   }
 }
 
@@ -836,7 +868,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(const NormArgs p) {
   float gamma[VE], beta[VE];
   load_affine<KIND, VE>(p, chunk, gamma, beta);
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
-    const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
+    const Frame w = slice_of(frame_of(p, f), gridDim.y - 1 - blockIdx.y, gridDim.y);
     const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * ((long)f * p.groups + chunk / p.chunks_per));
     float scale[VE], shift[VE];
     scale_shift<VE>(s, gamma, beta, scale, shift);
@@ -964,7 +996,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_dx(const NormArgs p) {
   float gamma[VE], beta[VE];
   load_affine<KIND, VE>(p, chunk, gamma, beta);
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
-    const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
+    const Frame w = slice_of(frame_of(p, f), gridDim.y - 1 - blockIdx.y, gridDim.y);
     const long at = 2 * ((long)f * p.groups + chunk / p.chunks_per);
     thread_dx<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, 0, *reinterpret_cast<const Pair*>(p.stats + at),
                               *reinterpret_cast<const Pair*>(p.sums + at), gamma, beta);
@@ -997,6 +1029,8 @@ void by_row(const NormArgs& p, F&& f) {
     lanes(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (p.chunks <= 256)
     lanes(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (p.chunks <= 512)
+    lanes(integral_constant<int, 256>{}, integral_constant<int, 2>{});
   else
     lanes(integral_constant<int, 256>{}, integral_constant<int, 4>{});
 }
@@ -1005,6 +1039,7 @@ size_t row_lds(const NormArgs& p, int T, int VE, bool grad) {
   return grad ? std::max(parts, (size_t)kThreads * VE * sizeof(float)) : parts;
 }
 dim3 frame_grid(const NormArgs& p) { return dim3(p.parts, std::min(p.frames, p.blocks)); }
+dim3 out_grid(const NormArgs& p) { return dim3(p.parts, p.out_slices, std::min(p.frames, 65535)); }
 dim3 slice_grid(const NormArgs& p, int most) { return dim3(p.parts, p.slices, std::min(p.frames, most)); }
 constexpr int kGrid = 65535;
 
@@ -1030,7 +1065,7 @@ void norm_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
       const long all = (long)p.frames * p.groups;
       hipLaunchKernelGGL((k_norm_stats_join<VE>), dim3((unsigned)std::min(all, 1L << 20)), dim3(kThreads), 0, st, p);
       DPAMD_LAUNCH_CHECK();
-      hipLaunchKernelGGL((k_norm_apply<KIND, VE>), slice_grid(p, kGrid), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_apply<KIND, VE>), out_grid(p), dim3(kThreads), 0, st, p);
     }
   });
   DPAMD_LAUNCH_CHECK();
@@ -1068,7 +1103,7 @@ void norm_grad_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
       DPAMD_LAUNCH_CHECK();
     }
     if (p.form == kNormSlices && p.dx) {
-      hipLaunchKernelGGL((k_norm_dx<KIND, VE, KEPT>), slice_grid(p, kGrid), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_dx<KIND, VE, KEPT>), out_grid(p), dim3(kThreads), 0, st, p);
       DPAMD_LAUNCH_CHECK();
     }
   };

@@ -52,6 +52,13 @@ ProductPlan plan_down(const dp_gated_shape& s, int ncu) {
 ProductPlan plan_gate_grad(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdGateGrad, elem_of(s.type), s.rows, s.d_hidden, s.d_out, 1, 1, ncu);
 }
+// (of the backward that forms g and u again: dh first, in fp32, and then the gate with its gradient)
+ProductPlan plan_dh(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdInput, elem_of(s.type), s.rows, s.d_hidden, s.d_out, 1, 1, ncu);
+}
+ProductPlan plan_gate_back(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdGateBack, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
+}
 ProductPlan plan_input(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdInput, elem_of(s.type), s.rows, s.d_in, s.d_hidden, 2, 1, ncu);
 }
@@ -123,7 +130,8 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
 }
 
 // The backward from x and the kept g and u (saved), or from the 8-bit checkpoint of x alone (kept): its values
-// are restored into an operand and x w_gate, x w_up are formed again, into the workspace.
+// are restored into an operand, dh is formed first, and the gate with its gradient in one product (with few outputs
+// g and u are formed into the workspace, for the kernels of these).
 void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const unsigned char* kept, const void* wg,
                     const void* wu, const void* wd, const void* saved, const void* dy, void* dx, void* dwg, void* dwu,
                     void* dwd, hipStream_t st) {
@@ -143,12 +151,13 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
     su = source_of(s.type, wu, s.ld_hidden, s.d_in, f, r, both);
   }
   const size_t hb = bytes_of(s.type) * (size_t)n * f8;
-  const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = kept || (dwd && !few) ? r.take(hb) : 0;
+  const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd && !few ? r.take(hb) : 0;
   const long ldx = (s.d_in + 7) / 8 * 8;
   const size_t at_x = kept ? r.take(bytes_of(s.type) * (size_t)n * ldx) : 0;
-  const size_t at_saved = kept ? r.take(8 * (size_t)n * f) : 0;
-  const ProductPlan p0 = kept ? plan_gate(s, O->ncu) : ProductPlan{};
-  const ProductPlan p1 = few ? ProductPlan{} : plan_gate_grad(s, O->ncu);
+  const ProductPlan p0 = !kept ? ProductPlan{} : few ? plan_gate(s, O->ncu) : plan_gate_back(s, O->ncu);
+  const ProductPlan p1 = few ? ProductPlan{} : kept ? plan_dh(s, O->ncu) : plan_gate_grad(s, O->ncu);
+  const long f4 = (f + 3) / 4 * 4;
+  const size_t at_saved = kept ? r.take(few ? 8 * (size_t)n * f : sizeof(float) * p1.split * (size_t)n * f4) : 0;
   const ProductPlan p2 = plan_input(s, O->ncu);
   const ProductPlan p3 = plan_weights(s, O->ncu);
   const ProductPlan p4 = few ? ProductPlan{} : plan_down_weight(s, O->ncu);
@@ -183,12 +192,25 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
     a.b[1] = ou;
     a.cols = (int)f8;
     a.act = s.act;
-    a.epi.h = ws + at_h;
     a.epi.ldh = f8;
-    a.epi.saved = reinterpret_cast<float*>(ws + at_saved);
     a.partial = part;
-    run_product(st, kProdGate, elem, p0, a);
-    saved = ws + at_saved;
+    if (few) {
+      a.epi.saved = reinterpret_cast<float*>(ws + at_saved);
+      run_product(st, kProdGate, elem, p0, a);
+      saved = ws + at_saved;
+    } else {
+      ProductArgs d = product(ody, od, n, f, s.d_out);
+      d.raw = true;
+      d.partial = reinterpret_cast<float*>(ws + at_saved);
+      run_product(st, kProdInput, elem, p1, d);
+      a.epi.h = dwd ? ws + at_h : nullptr;
+      a.epi.dg = ws + at_dg;
+      a.epi.du = ws + at_du;
+      a.epi.dh = d.partial;
+      a.epi.dh_slices = p1.split;
+      a.epi.dh_ld = f4, a.epi.dh_plane = n * f4;
+      run_product(st, kProdGateBack, elem, p0, a);
+    }
   }
   if (few) {
     q.dy = dy;
@@ -198,11 +220,11 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
     q.dwd = dwd;
     q.partial = dwd ? part : nullptr;
     run_outs_grad(st, elem, q);
-  } else {
+  } else if (!kept) {
     ProductArgs a = product(ody, od, n, f, s.d_out);
     a.cols = (int)f8;
     a.act = s.act;
-    a.epi.h = dwd && !kept ? ws + at_h : nullptr;
+    a.epi.h = dwd ? ws + at_h : nullptr;
     a.epi.dg = ws + at_dg;
     a.epi.du = ws + at_du;
     a.epi.ldh = f8;

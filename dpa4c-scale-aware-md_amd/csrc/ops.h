@@ -13,7 +13,7 @@ namespace dpamd {
 enum { kActTanh = 0, kActSilu = 1, kActGelu = 2, kActNone = 3 };
 
 // ---- tile products (product.h) ----
-enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2, kEpiScale = 3, kEpiScaleGate = 4 };
+enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2, kEpiScale = 3, kEpiScaleGate = 4, kEpiGateBack = 5 };
 
 // An operand of the products, of the call's type: 16-byte aligned, rows of whole 16-byte
 // chunks (ld elements), and the contiguous side ends with a chunk or is followed by zeros up to one.
@@ -37,6 +37,10 @@ struct EpiArgs {
   float* h32;  // h, not rounded, in place of `h` where no product follows (of a gate), or null
   long ldh;
   float* saved;
+  // of a gate whose gradient follows at once: dh, as `dh_slices` sums of rows of dh_ld, dh_plane apart
+  const float* dh;
+  int dh_slices;
+  long dh_ld, dh_plane;
 };
 
 struct ProductArgs {
@@ -59,6 +63,7 @@ struct ProductArgs {
   // products of 8-bit integers: scales of the rows and of each B matrix's columns, element kind of out[0]
   const float *row_scale, *col_scale[2];
   int out_elem;
+  bool raw;  // the slices' sums stay in `partial`
 };
 
 // What a product is: which layouts and epilogue.
@@ -66,7 +71,8 @@ enum ProductKind {
   kProdGate,      // x Wg, x Wu -> h                    rows k-contiguous by columns
   kProdDown,      // h Wd -> y
   kProdGateGrad,  // dy Wd^T -> dg, du, h               both k-contiguous
-  kProdInput,     // dg Wg^T + du Wu^T -> dx
+  kProdInput,     // dg Wg^T + du Wu^T -> dx            both k-contiguous
+  kProdGateBack,  // x Wg, x Wu and dh -> dg, du, h     rows k-contiguous by columns
   kProdWeight     // x^T dg, x^T du;  h^T dy            both k-strided
 };
 
@@ -160,6 +166,10 @@ struct Linear8RowsArgs {
 };
 Linear8Form linear8_form(long rows, int K, int N);
 void run_linear8_rows(hipStream_t st, int elem, int ncu, Linear8RowsArgs& args);
+
+// Outputs of so many bytes are stored past the caches: they would not be found there (256 MB, the last one) by
+// who reads them next, and what they push out has to be written back beside the next kernel's reads.
+inline bool past_caches(double bytes) { return bytes > 192e6; }
 
 // Matrices [rows][cols] to be copied into rows of ld (a multiple of 8), with zeros past cols.
 struct PackItem {

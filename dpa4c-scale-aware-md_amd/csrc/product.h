@@ -572,8 +572,8 @@ struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
 };
 
-// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad; of 8-bit integers
-// kEpiScale, kEpiScaleGate (two).
+// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad, kEpiGateBack (two); of 8-bit
+// integers kEpiScale, kEpiScaleGate (two).
 //
 // A block takes tiles (and slices of K) one after another; the first two steps of the next one are
 // loaded before the epilogue of the last, so that they arrive under it. Two stages of LDS.
@@ -592,7 +592,7 @@ struct Shape {
 // instead of two changed nothing).
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
-  constexpr int SUB = EPI == kEpiGate || EPI == kEpiScaleGate ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
+  constexpr int SUB = EPI == kEpiGate || EPI == kEpiScaleGate || EPI == kEpiGateBack ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
   using T = typename ElemOf<KIND>::T;
   constexpr int WAVES = S::WM * S::WN, TM = S::BM / S::WM, TN = S::BN / S::WN;
   constexpr int MI = TM / 16, NJ = TN / 16;
@@ -778,7 +778,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
     const int m0 = done.m0 + wm * TM + c, n0 = done.n0 + wn * (TN / SUB) + 4 * g;
     constexpr bool WIDE = KIND != kF32;  // pairs of fragments are stored together
     const bool inside = done.m0 + (wm + 1) * TM <= p.M && done.n0 + (wn + 1) * (TN / SUB) <= p.N;
-    if (p.split > 1) {
+    if (p.split > 1 || p.raw) {
       // a slice's sums, columns in rows of ldp (a multiple of 4)
       const int sub = SUB == 2 ? 2 : p.mats;
       float* o = p.partial + (((long)done.slice * sub + done.mat) * p.M + m0) * p.ldp + n0;
@@ -842,6 +842,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
           if (h32) {
 #pragma unroll
             for (int j = 0; j < NG; ++j) *reinterpret_cast<f4*>(h32 + h + j * 16) = v[j];
+          } else if (!to) {  // (g and u are all that is wanted)
           } else if constexpr (WIDE && NG % 2 == 0) {
 #pragma unroll
             for (int j = 0; j < NG; j += 2) put_pair<KIND>(to + h + pair_at(g) + j * 16, v[j], v[j + 1]);
@@ -860,11 +861,62 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
               const f4 v = gate_value<false>(p.act, count, acc[i][j], acc[i][j + NG]);
               if (h32)
                 *reinterpret_cast<f4*>(h32 + h + j * 16) = v;
-              else
+              else if (to)
                 put4<KIND>(to + h + j * 16, v);
               if (p.epi.saved) put_kept<false>(kept + j * 16, plane, count, acc[i][j], acc[i][j + NG]);
             }
       }
+    } else if constexpr (EPI == kEpiGateBack) {
+      // g and u are here, dh in memory: one number to read for each three to write, where the gate's
+      // gradient after a gate that kept g and u for it moves 22 bytes for these 14 (bf16). The next sixteen
+      // rows' dh are under way as the kept values are below.
+      constexpr int NG = NJ / SUB;
+      auto rows = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const float* dh_at = p.epi.dh + ((long)m0 * p.epi.dh_ld + n0);
+        long at = m0 * p.epi.ldh + n0;
+        auto fetch = [&](int i, f4* d) {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            d[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (FULL || (m0 + i * 16 < p.M && n0 + j * 16 < p.N)) {
+              const float* s = dh_at + i * 16l * p.epi.dh_ld + j * 16;
+              d[j] = *reinterpret_cast<const f4*>(s);
+              for (int z = 1; z < p.epi.dh_slices; ++z) d[j] += *reinterpret_cast<const f4*>(s + z * p.epi.dh_plane);
+            }
+          }
+        };
+        f4 dh[2][NG];
+        fetch(0, dh[0]);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          if (i + 1 < MI) fetch(i + 1, dh[(i + 1) & 1]);
+          GateGrad o[NG];
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+            o[j] = gate_grad<FULL>(p.act, p.N - n0 - j * 16, dh[i & 1][j], Kept{acc[i][j], acc[i][j + NG]});
+          vmem_wait_all();
+          const long row = at + i * 16 * p.epi.ldh;
+          if constexpr (FULL && WIDE && NG % 2 == 0) {
+            auto store = [&](void* out, auto member) {
+#pragma unroll
+              for (int j = 0; j < NG; j += 2)
+                put_pair<KIND>(static_cast<T*>(out) + row + pair_at(g) + j * 16, o[j].*member, o[j + 1].*member);
+            };
+            if (p.epi.h) store(p.epi.h, &GateGrad::h);
+            store(p.epi.dg, &GateGrad::dg);
+            store(p.epi.du, &GateGrad::du);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+              if (FULL || (m0 + i * 16 < p.M && n0 + j * 16 < p.cols)) put_gate_grad<KIND>(p.epi, row + j * 16, o[j]);
+          }
+        }
+      };
+      if (inside)
+        rows(std::true_type{});
+      else
+        rows(std::false_type{});
     } else {
       // The kept g, u of the next sixteen rows are under way while these rows' values are
       // computed, and are waited for before the stores that follow them are issued (a wait
@@ -923,11 +975,12 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 // 62 us, a chain of loads.
 template <int KIND, int EPI>
 __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
-  constexpr int SUB = EPI == kEpiGate ? 2 : 1;
+  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack;
+  constexpr int SUB = PAIR ? 2 : 1;
   __shared__ f4 part[SUB][256];
   const int G = p.join, per = 256 / G;
-  const int quads = p.ldp / 4, sub = EPI == kEpiGate ? 2 : p.mats;
-  const long rows = EPI == kEpiGate ? p.M : (long)p.M * p.mats;
+  const int quads = p.ldp / 4, sub = PAIR ? 2 : p.mats;
+  const long rows = PAIR ? p.M : (long)p.M * p.mats;
   const int slot = threadIdx.x % per, share = threadIdx.x / per;
   const long at = (long)blockIdx.x * per + slot;
   const bool in = at < rows * quads;
@@ -966,16 +1019,22 @@ __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
     }
   }
   if (!in) return;
-  const int mat = EPI == kEpiGate ? 0 : (int)(row / p.M);
-  const long m = EPI == kEpiGate ? row : row % p.M;
+  const int mat = PAIR ? 0 : (int)(row / p.M);
+  const long m = PAIR ? row : row % p.M;
   const long plane = (long)p.M * p.N;
   if constexpr (EPI == kEpiGate) {
     const f4 h = gate_value<false>(p.act, p.N - n, v, w);
     if (p.epi.h32)
       *reinterpret_cast<f4*>(p.epi.h32 + m * p.epi.ldh + n) = h;
-    else
+    else if (p.epi.h)
       put4<KIND>(static_cast<typename ElemOf<KIND>::T*>(p.epi.h) + m * p.epi.ldh + n, h);
     if (p.epi.saved) put_kept<false>(p.epi.saved + (m * p.N + n), plane, p.N - n, v, w);
+  } else if constexpr (EPI == kEpiGateBack) {
+    f4 dh = {0, 0, 0, 0};
+    if (n < p.N)
+      for (int z = 0; z < p.epi.dh_slices; ++z)
+        dh += *reinterpret_cast<const f4*>(p.epi.dh + z * p.epi.dh_plane + m * p.epi.dh_ld + n);
+    put_gate_grad<KIND>(p.epi, m * p.epi.ldh + n, gate_grad<false>(p.act, p.N - n, dh, Kept{v, w}));
   } else if constexpr (EPI == kEpiGateGrad) {
     const Kept k = load_kept<false>(p.epi.saved + (m * p.N + n), plane, p.N - n);
     put_gate_grad<KIND>(p.epi, m * p.epi.ldh + n, gate_grad<false>(p.act, p.N - n, v, k));

@@ -19,7 +19,8 @@ using Tiny = Shape<64, 32, 4, 1>;
 
 template <int KIND, int LA, int LB, int EPI, class S>
 void launch(hipStream_t st, ProductArgs& p) {
-  constexpr int SUB = EPI == kEpiGate ? 2 : 1;
+  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack;
+  constexpr int SUB = PAIR ? 2 : 1;
   p.tiles_m = (p.M + S::BM - 1) / S::BM;
   p.tiles_n1 = (p.N + S::BN / SUB - 1) / (S::BN / SUB);
   p.tiles_n = p.tiles_n1 * p.mats;
@@ -28,8 +29,8 @@ void launch(hipStream_t st, ProductArgs& p) {
   hipLaunchKernelGGL((k_product<KIND, LA, LB, EPI, S>), dim3((unsigned)std::min(items, (long)p.blocks)),
                      dim3(S::WM * S::WN * 64), 0, st, p);
   DPAMD_LAUNCH_CHECK();
-  if (p.split > 1) {
-    const long rows = (long)p.M * (EPI == kEpiGate ? 1 : p.mats), quads = p.ldp / 4;
+  if (p.split > 1 && !p.raw) {
+    const long rows = (long)p.M * (PAIR ? 1 : p.mats), quads = p.ldp / 4;
     // threads that share a quad's slices: up to 8 slices each, more where the quads fill the card
     p.join = 1;
     while (p.join < 64 && p.split > 8 * p.join && rows * quads * p.join < 1L << 18) p.join *= 2;
@@ -45,6 +46,7 @@ void launch_kind(hipStream_t st, ProductKind what, ProductArgs& p) {
     case kProdGate: return launch<KIND, kRowK, kColK, kEpiGate, S>(st, p);
     case kProdDown: return launch<KIND, kRowK, kColK, kEpiStore, S>(st, p);
     case kProdGateGrad: return launch<KIND, kRowK, kRowK, kEpiGateGrad, S>(st, p);
+    case kProdGateBack: return launch<KIND, kRowK, kColK, kEpiGateBack, S>(st, p);
     case kProdInput: return launch<KIND, kRowK, kRowK, kEpiStore, S>(st, p);
     case kProdWeight: return launch<KIND, kColK, kColK, kEpiStore, S>(st, p);
   }

@@ -47,7 +47,16 @@ __device__ __forceinline__ void load8(float (&v)[8], const typename ElemOf<KIND>
     for (int e = 0; e < 8; ++e) v[e] = e < count ? to_f32<KIND>(p[e]) : 0.0f;
   }
 }
-template <int KIND>
+// 16 bytes at the alignment of an element; with ONCE past the caches, for what is not read again soon
+typedef unsigned u4any __attribute__((ext_vector_type(4), aligned(2)));
+template <bool ONCE>
+__device__ __forceinline__ void store16(void* p, const u4any& v) {
+  if constexpr (ONCE)
+    __builtin_nontemporal_store(v, static_cast<u4any*>(p));
+  else
+    *static_cast<u4any*>(p) = v;
+}
+template <int KIND, bool ONCE = false>
 __device__ __forceinline__ void store8(typename ElemOf<KIND>::T* p, const float (&v)[8], int count) {
   struct Eight {
     typename ElemOf<KIND>::T v[8];
@@ -55,7 +64,12 @@ __device__ __forceinline__ void store8(typename ElemOf<KIND>::T* p, const float 
   if (count >= 8) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) s.v[e] = from_f32<KIND>(v[e]);
-    __builtin_memcpy(p, &s, sizeof(s));
+    struct Words {
+      u4any w[sizeof(Eight) / 16];
+    };
+    const Words w = __builtin_bit_cast(Words, s);
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(Eight) / 16); ++k) store16<ONCE>(reinterpret_cast<char*>(p) + 16 * k, w.w[k]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void k_keep8(const KeepArgs p) {
 }
 
 // Rows of `cols` columns and zeros up to `cols_out` (a multiple of eight where x is an operand).
-template <int KIND>
+template <int KIND, bool ONCE>
 __global__ __launch_bounds__(256) void k_restore8(const KeepArgs p) {
   using T = typename ElemOf<KIND>::T;
   const int per = (p.cols_out + 7) / 8;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void k_restore8(const KeepArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (at[k].c0 + e >= p.cols) f[e] = 0.0f;
-      store8<KIND>(x + at[k].row * p.ld + at[k].c0, f, p.cols_out - at[k].c0);
+      store8<KIND, ONCE>(x + at[k].row * p.ld + at[k].c0, f, p.cols_out - at[k].c0);
     }
   }
 }
@@ -220,7 +220,13 @@ void keep8(hipStream_t st, int elem, const KeepArgs& p) {
 void restore8(hipStream_t st, int elem, const KeepArgs& p) {
   if (p.rows <= 0) return;
   const dim3 grid(grid_of((p.rows * ((p.cols_out + 7) / 8) + kItems * 256 - 1) / (kItems * 256)));
-  by_kind(elem, [&](auto k) { hipLaunchKernelGGL((k_restore8<decltype(k)::value>), grid, dim3(256), 0, st, p); });
+  const bool once = past_caches(p.rows * p.cols_out * (elem == kF32 ? 4 : 2));
+  by_kind(elem, [&](auto k) {
+    if (once)
+      hipLaunchKernelGGL((k_restore8<decltype(k)::value, true>), grid, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((k_restore8<decltype(k)::value, false>), grid, dim3(256), 0, st, p);
+  });
   DPAMD_LAUNCH_CHECK();
 }
 
