@@ -91,7 +91,7 @@ void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride
 }
 
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu) {
-  const int sub = what == kProdGate || what == kProdGateBack ? 2 : 1, bk = elem == kF32 ? 32 : elem == kI8 ? 128 : 64;
+  const int sub = what == kProdGate || what == kProdGateBack || what == kProdGateOuts ? 2 : 1, bk = elem == kF32 ? 32 : elem == kI8 ? 128 : 64;
   ProductPlan best{};
   double best_us = 0;
   const long steps = (K + bk - 1) / bk * segs;
@@ -106,7 +106,7 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
     for (long split = 1; split <= most; split = split < 4 ? split + 1 : split + split / 4) {
       const long items = tiles * split, a_cu = (items + ncu - 1) / ncu, rounds = (items + slots - 1) / slots;
       const double bytes = split > 1 ? 4.0 * split * sub * mats * M * ((N + 7) / 8 * 8) : 0;
-      const double end = s.end_us[split > 1 ? 0 : what == kProdGate ? 1 : what == kProdGateGrad || what == kProdGateBack ? 2 : 0];
+      const double end = s.end_us[split > 1 ? 0 : what == kProdGate || what == kProdGateOuts ? 1 : what == kProdGateGrad || what == kProdGateBack ? 2 : 0];
       const double us = (double)((steps + split - 1) / split) * std::max(a_cu * share, rounds * s.alone_us) +
                         a_cu * end + 2.0 + (split > 1 ? 4 + 2 * bytes / 4e6 : 0);
       if (best_us == 0 || us < best_us) {
@@ -116,6 +116,13 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
     }
   }
   return best;
+}
+
+// waves' rows of the tiles: those of a tile by the waves that share them
+int gate_outs_slices(const ProductPlan& plan, int elem, long M) {
+  constexpr int kWaves[5] = {2, 2, 1, 4, 4};
+  const int bm = kShapes[elem == kF32][plan.shape].bm;
+  return (int)((M + bm - 1) / bm) * kWaves[plan.shape];
 }
 
 void tile_of(int shape, int elem, int& rows, int& cols) {

@@ -225,11 +225,16 @@ void run_outs_grad(hipStream_t st, int elem, const OutsArgs& p) {
       hipLaunchKernelGGL((k_outs_grad<K, decltype(o)::value>), dim3(p.slices, p.groups), dim3(256), 0, st, p);
     });
     DPAMD_LAUNCH_CHECK();
-    if (!p.partial) return;
-    const int each = 256 / kShares;
-    hipLaunchKernelGGL((k_outs_join<K>), dim3((p.f * p.o + each - 1) / each), dim3(256), 0, st, p);
-    DPAMD_LAUNCH_CHECK();
   });
+  if (p.partial) run_outs_join(st, elem, p);
+}
+
+void run_outs_join(hipStream_t st, int elem, const OutsArgs& p) {
+  const int each = 256 / kShares;
+  with_kind(elem, [&](auto kind) {
+    hipLaunchKernelGGL((k_outs_join<decltype(kind)::value>), dim3((p.f * p.o + each - 1) / each), dim3(256), 0, st, p);
+  });
+  DPAMD_LAUNCH_CHECK();
 }
 
 }  // namespace dpamd

@@ -89,10 +89,10 @@ __device__ __forceinline__ void quantize_rows(const Linear8RowsArgs& p, char* q,
 
 // F fragments of 16 rows, C of 16 channels (of each matrix); WAVES of a block share k. FUSED: x is quantised
 // here (F is 1).
-template <int KIND, int F, int C, bool GATE, int WAVES, bool FUSED>
+template <int KIND, int F, int C, bool GATE, int WAVES, bool FUSED, int AHEAD>
 __global__ __launch_bounds__(64 * WAVES) void k_linear8_rows(const Linear8RowsArgs p) {
   constexpr int MATS = GATE ? 2 : 1, W = MATS * C, T = 64 * WAVES;
-  constexpr int kAhead = 8 / C;  // steps whose weights are under way
+  constexpr int kAhead = AHEAD / C;  // steps whose weights are under way
   extern __shared__ __align__(16) char lds[];
   __shared__ float row_scales[kFusedRows];
   __shared__ unsigned tops[kFusedRows * WAVES];
@@ -199,15 +199,17 @@ template <int KIND, int F, int C, bool GATE, int WAVES, bool FUSED>
 void launch(hipStream_t st, const Linear8RowsArgs& p) {
   constexpr int kJoin = WAVES * F * C * (GATE ? 2 : 1) * 1024;
   static_assert(kJoin < 64 << 10, "the waves' parts are less than a block's LDS");
-  const int rows = FUSED ? p.rows * ((p.K + kStep - 1) / kStep * kStep + 16) : 0;
-  hipLaunchKernelGGL((k_linear8_rows<KIND, F, C, GATE, WAVES, FUSED>), dim3((p.N + 16 * C - 1) / (16 * C)),
-                     dim3(64 * WAVES), std::max(kJoin, rows), st, p);
+  const int steps = (p.K + kStep - 1) / kStep, rows = FUSED ? p.rows * (steps * kStep + 16) : 0;
+  const dim3 grid((p.N + 16 * C - 1) / (16 * C)), block(64 * WAVES);
+  if (steps >= 8 * WAVES)
+    hipLaunchKernelGGL((k_linear8_rows<KIND, F, C, GATE, WAVES, FUSED, 8>), grid, block, std::max(kJoin, rows), st, p);
+  else
+    hipLaunchKernelGGL((k_linear8_rows<KIND, F, C, GATE, WAVES, FUSED, 4>), grid, block, std::max(kJoin, rows), st, p);
   DPAMD_LAUNCH_CHECK();
 }
 
 template <int KIND, bool GATE, int WAVES>
 void by_rows(hipStream_t st, const Linear8RowsArgs& p) {
-  constexpr int FEW = GATE ? 4 : WAVES;  // (two matrices' parts of eight waves would be all of 64 KB)
   if (!p.q)
     launch<KIND, 1, 1, GATE, WAVES, true>(st, p);
   else if (p.rows <= 16)
@@ -223,7 +225,7 @@ void by_rows(hipStream_t st, const Linear8RowsArgs& p) {
   } else if (p.rows <= 32)
     launch<KIND, 2, 1, GATE, WAVES, false>(st, p);
   else
-    launch<KIND, 3, 1, GATE, FEW, false>(st, p);
+    launch<KIND, 3, 1, GATE, WAVES, false>(st, p);
 }
 
 template <int KIND>

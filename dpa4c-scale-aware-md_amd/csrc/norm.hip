@@ -219,11 +219,6 @@ __device__ __forceinline__ void join_moments(Pair& p, float n, const Pair& q, fl
   p.b += q.b + d * d * n * w;
 }
 
-// v + that of another lane, in one instruction (DPP): within quads, halves of rows and rows of 16 lanes
-template <int CTRL>
-__device__ __forceinline__ float add_dpp(float v) {
-  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
-}
 // The sum over 2^log_lanes neighbouring lanes, in each of them (every lane of the wave takes part).
 __device__ __forceinline__ float sum_lanes(float v, int log_lanes) {
   if (log_lanes > 0) v = add_dpp<0xB1>(v);   // lane ^ 1

@@ -59,6 +59,9 @@ ProductPlan plan_dh(const dp_gated_shape& s, int ncu) {
 ProductPlan plan_gate_back(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdGateBack, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
 }
+ProductPlan plan_gate_outs(const dp_gated_shape& s, int ncu) {
+  return plan_product(kProdGateOuts, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
+}
 ProductPlan plan_input(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdInput, elem_of(s.type), s.rows, s.d_in, s.d_hidden, 2, 1, ncu);
 }
@@ -131,7 +134,7 @@ void gated_forward(dp_ops* O, const dp_gated_shape& s, const void* x, const void
 
 // The backward from x and the kept g and u (saved), or from the 8-bit checkpoint of x alone (kept): its values
 // are restored into an operand, dh is formed first, and the gate with its gradient in one product (with few outputs
-// g and u are formed into the workspace, for the kernels of these).
+// dh too, or g and u into the workspace, for the kernels of these).
 void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const unsigned char* kept, const void* wg,
                     const void* wu, const void* wd, const void* saved, const void* dy, void* dx, void* dwg, void* dwu,
                     void* dwd, hipStream_t st) {
@@ -154,15 +157,23 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
   const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd && !few ? r.take(hb) : 0;
   const long ldx = (s.d_in + 7) / 8 * 8;
   const size_t at_x = kept ? r.take(bytes_of(s.type) * (size_t)n * ldx) : 0;
-  const ProductPlan p0 = !kept ? ProductPlan{} : few ? plan_gate(s, O->ncu) : plan_gate_back(s, O->ncu);
+  ProductPlan p0{};
+  if (kept) p0 = few ? plan_gate_outs(s, O->ncu) : plan_gate_back(s, O->ncu);
+  const bool outs = kept && few && p0.split == 1;  // (a sliced gate has its sums elsewhere)
+  if (kept && few && !outs) p0 = plan_gate(s, O->ncu);
   const ProductPlan p1 = few ? ProductPlan{} : kept ? plan_dh(s, O->ncu) : plan_gate_grad(s, O->ncu);
   const long f4 = (f + 3) / 4 * 4;
-  const size_t at_saved = kept ? r.take(few ? 8 * (size_t)n * f : sizeof(float) * p1.split * (size_t)n * f4) : 0;
+  const size_t at_saved =
+      kept && !outs ? r.take(few ? 8 * (size_t)n * f : sizeof(float) * p1.split * (size_t)n * f4) : 0;
   const ProductPlan p2 = plan_input(s, O->ncu);
   const ProductPlan p3 = plan_weights(s, O->ncu);
   const ProductPlan p4 = few ? ProductPlan{} : plan_down_weight(s, O->ncu);
   OutsArgs q = outs_of(s, wd);
-  const size_t down_bytes = few ? plan_outs_grad(O->ncu, q) : p4.bytes;
+  size_t down_bytes = few ? plan_outs_grad(O->ncu, q) : p4.bytes;
+  if (outs) {
+    q.slices = gate_outs_slices(p0, elem, n);
+    down_bytes = sizeof(float) * q.slices * (size_t)f * s.d_out;
+  }
   const size_t at_part = r.take(std::max({p0.bytes, p1.bytes, dx ? p2.bytes : 0, dwg ? p3.bytes : 0,
                                           dwd ? down_bytes : 0}));
   char* ws = workspace(O, st, r.used);
@@ -194,7 +205,18 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
     a.act = s.act;
     a.epi.ldh = f8;
     a.partial = part;
-    if (few) {
+    if (outs) {
+      a.epi.dg = ws + at_dg;
+      a.epi.du = ws + at_du;
+      a.epi.dy = dy, a.epi.ld_dy = s.ld_y;
+      a.epi.wd = wd, a.epi.ld_down = s.ld_down;
+      a.epi.outs = s.d_out;
+      a.epi.outs_partial = dwd ? part : nullptr;
+      run_product(st, kProdGateOuts, elem, p0, a);
+      q.dwd = dwd;
+      q.partial = part;
+      if (dwd) run_outs_join(st, elem, q);
+    } else if (few) {
       a.epi.saved = reinterpret_cast<float*>(ws + at_saved);
       run_product(st, kProdGate, elem, p0, a);
       saved = ws + at_saved;
@@ -212,7 +234,9 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
       run_product(st, kProdGateBack, elem, p0, a);
     }
   }
-  if (few) {
+  if (outs) {
+    // (formed with the gate)
+  } else if (few) {
     q.dy = dy;
     q.saved = static_cast<const float*>(saved);
     q.dg = ws + at_dg;

@@ -13,7 +13,7 @@ namespace dpamd {
 enum { kActTanh = 0, kActSilu = 1, kActGelu = 2, kActNone = 3 };
 
 // ---- tile products (product.h) ----
-enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2, kEpiScale = 3, kEpiScaleGate = 4, kEpiGateBack = 5 };
+enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2, kEpiScale = 3, kEpiScaleGate = 4, kEpiGateBack = 5, kEpiGateOuts = 6 };
 
 // An operand of the products, of the call's type: 16-byte aligned, rows of whole 16-byte
 // chunks (ld elements), and the contiguous side ends with a chunk or is followed by zeros up to one.
@@ -41,6 +41,12 @@ struct EpiArgs {
   const float* dh;
   int dh_slices;
   long dh_ld, dh_plane;
+  // of the same with few outputs: dh from dy [M][outs] and w_down [N][outs], and sums of h dy over each
+  // wave's rows, [slices][N][outs] (or null)
+  const void *dy, *wd;
+  int outs;
+  long ld_dy, ld_down;
+  float* outs_partial;
 };
 
 struct ProductArgs {
@@ -73,6 +79,7 @@ enum ProductKind {
   kProdGateGrad,  // dy Wd^T -> dg, du, h               both k-contiguous
   kProdInput,     // dg Wg^T + du Wu^T -> dx            both k-contiguous
   kProdGateBack,  // x Wg, x Wu and dh -> dg, du, h     rows k-contiguous by columns
+  kProdGateOuts,  // the same with up to four outputs
   kProdWeight     // x^T dg, x^T du;  h^T dy            both k-strided
 };
 
@@ -82,6 +89,7 @@ struct ProductPlan {
   size_t bytes;
 };
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu);
+int gate_outs_slices(const ProductPlan& plan, int elem, long M);
 void tile_of(int shape, int elem, int& rows, int& cols);  // of a plan's shape
 void run_product(hipStream_t st, ProductKind what, int elem, const ProductPlan& plan, ProductArgs& args);
 
@@ -116,6 +124,7 @@ bool few_outputs(int d_hidden, int d_out);
 void run_outs_down(hipStream_t st, int elem, int ncu, const OutsArgs& args);
 size_t plan_outs_grad(int ncu, OutsArgs& args);  // bytes of the partial sums
 void run_outs_grad(hipStream_t st, int elem, const OutsArgs& args);
+void run_outs_join(hipStream_t st, int elem, const OutsArgs& args);  // of `slices` sums, to dwd
 
 // ---- 8-bit forms (quant8.hip) and products (product8.hip) ----
 // Checkpoint of [rows][cols]: q [rows][wide] (wide: cols up to a multiple of 32), then a byte for each 32.

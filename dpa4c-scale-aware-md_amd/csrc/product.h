@@ -55,6 +55,16 @@ __device__ __forceinline__ typename ElemOf<KIND>::T from_f32(float v) {
     return to16<KIND>(v);
 }
 
+// v + that of another lane, in one instruction (DPP): within quads, halves of rows and rows of 16 lanes
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// The sum over a row of 16 lanes, in each of them.
+__device__ __forceinline__ float sum_rows16(float v) {
+  return add_dpp<0x140>(add_dpp<0x141>(add_dpp<0x4E>(add_dpp<0xB1>(v))));
+}
+
 // Four consecutive elements, aligned to them.
 template <int KIND>
 __device__ __forceinline__ void put4(typename ElemOf<KIND>::T* p, const f4& v) {
@@ -572,7 +582,7 @@ struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
 };
 
-// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad, kEpiGateBack (two); of 8-bit
+// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad, kEpiGateBack, kEpiGateOuts (two); of 8-bit
 // integers kEpiScale, kEpiScaleGate (two).
 //
 // A block takes tiles (and slices of K) one after another; the first two steps of the next one are
@@ -592,7 +602,7 @@ struct Shape {
 // instead of two changed nothing).
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
-  constexpr int SUB = EPI == kEpiGate || EPI == kEpiScaleGate || EPI == kEpiGateBack ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
+  constexpr int SUB = EPI == kEpiGate || EPI == kEpiScaleGate || EPI == kEpiGateBack || EPI == kEpiGateOuts ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
   using T = typename ElemOf<KIND>::T;
   constexpr int WAVES = S::WM * S::WN, TM = S::BM / S::WM, TN = S::BN / S::WN;
   constexpr int MI = TM / 16, NJ = TN / 16;
@@ -917,6 +927,65 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
         rows(std::true_type{});
       else
         rows(std::false_type{});
+    } else if constexpr (EPI == kEpiGateOuts) {
+      // dh from a few outputs' dy, here, and h dy summed over the wave's rows: neither g and u nor h meet
+      // memory. (31,920 rows of 70-96-1 in fp32: XXX)
+      constexpr int NG = NJ / SUB;
+      const int outs = p.epi.outs;
+      float w[NG][4][kFewOutputs], sum[NG][4][kFewOutputs] = {};
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int k = 0; k < kFewOutputs; ++k) {
+            const int n = n0 + j * 16 + e;
+            w[j][e][k] = k < outs && n < p.N
+                             ? to_f32<KIND>(static_cast<const T*>(p.epi.wd)[n * p.epi.ld_down + k])
+                             : 0.0f;
+          }
+      long at = m0 * p.epi.ldh + n0;
+#pragma unroll
+      for (int i = 0; i < MI; ++i, at += 16 * p.epi.ldh) {
+        const int m = m0 + i * 16;
+        const bool there = m < p.M;
+        float dy[kFewOutputs];
+#pragma unroll
+        for (int k = 0; k < kFewOutputs; ++k)
+          dy[k] = there && k < outs ? to_f32<KIND>(static_cast<const T*>(p.epi.dy)[m * p.epi.ld_dy + k]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          f4 dh = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < kFewOutputs; ++k)
+            if (k < outs)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dh[e] += dy[k] * w[j][e][k];
+          const GateGrad o =
+              gate_grad<false>(p.act, p.N - n0 - j * 16, dh, Kept{acc[i][j], acc[i][j + NG]});
+          if (!there) continue;  // (rows past the last hold anything)
+#pragma unroll
+          for (int k = 0; k < kFewOutputs; ++k)
+            if (k < outs)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[j][e][k] += o.h[e] * dy[k];
+          if (n0 + j * 16 < p.cols) put_gate_grad<KIND>(p.epi, at + j * 16, o);
+        }
+      }
+      if (p.epi.outs_partial) {
+        float* out = p.epi.outs_partial + (long)(done.m0 / S::BM * S::WM + wm) * p.N * outs;
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < kFewOutputs; ++k)
+              if (k < outs) {
+                const float v = sum_rows16(sum[j][e][k]);
+                const int n = n0 + j * 16 + e;
+                if (c == 0 && n < p.N) out[(long)n * outs + k] = v;
+              }
+      }
     } else {
       // The kept g, u of the next sixteen rows are under way while these rows' values are
       // computed, and are waited for before the stores that follow them are issued (a wait
@@ -975,7 +1044,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 // 62 us, a chain of loads.
 template <int KIND, int EPI>
 __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
-  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack;
+  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack || EPI == kEpiGateOuts;
   constexpr int SUB = PAIR ? 2 : 1;
   __shared__ f4 part[SUB][256];
   const int G = p.join, per = 256 / G;

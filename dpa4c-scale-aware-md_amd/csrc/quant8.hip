@@ -20,9 +20,8 @@ unsigned grid_of(long blocks) { return (unsigned)std::min(blocks, 1L << 20); }
 //
 // Eight columns a thread, four threads a group: 16-byte loads of 16-bit types, 8-byte stores of q. Bound by
 // the bytes.
-constexpr int kItems = 4;  // eights of a thread, 256 apart
-
-// Items of a block: kItems * 256 consecutive eights of the rows of `per` eights. Row and eight of each by one
+// Items of a block: ITEMS * 256 consecutive eights of the rows of `per` eights, 256 apart for a thread: four, or
+// one where four would leave compute units idle. Row and eight of each by one
 // 32-bit division from the block's first.
 struct Place {
   long row;
@@ -33,7 +32,7 @@ __device__ __forceinline__ Place place_of(long base_row, int base_off, int per, 
   return Place{base_row + r, (int)(o - r * (unsigned)per) * 8};
 }
 
-template <int KIND>
+template <int KIND, int kItems>
 __global__ __launch_bounds__(256) void k_keep8(const KeepArgs p) {
   using T = typename ElemOf<KIND>::T;
   const int wide = p.wide, per = wide / 8;
@@ -73,7 +72,7 @@ __global__ __launch_bounds__(256) void k_keep8(const KeepArgs p) {
 }
 
 // Rows of `cols` columns and zeros up to `cols_out` (a multiple of eight where x is an operand).
-template <int KIND, bool ONCE>
+template <int KIND, bool ONCE, int kItems>
 __global__ __launch_bounds__(256) void k_restore8(const KeepArgs p) {
   using T = typename ElemOf<KIND>::T;
   const int per = (p.cols_out + 7) / 8;
@@ -190,9 +189,15 @@ __global__ __launch_bounds__(256) void k_weights8(const Weights8Args p) {
   }
 }
 
+constexpr long kFewEights = 1L << 20;  // four for each thread of a full card
+dim3 blocks_of(long eights, int items) { return dim3(grid_of((eights + items * 256 - 1) / (items * 256))); }
+
+// A row to a wave, or to a block: few rows, or long ones.
 template <int KIND>
 void rows_kind(hipStream_t st, const Rows8Args& p) {
-  if (p.ld_q <= 64 * 8 * 4)
+  if (p.rows <= 1024 && p.ld_q <= 256 * 8)
+    hipLaunchKernelGGL((k_rows8<KIND, 256, 1>), dim3(grid_of(p.rows)), dim3(256), 0, st, p);
+  else if (p.ld_q <= 64 * 8 * 4)
     hipLaunchKernelGGL((k_rows8<KIND, 64, 4>), dim3(grid_of((p.rows + 3) / 4)), dim3(256), 0, st, p);
   else
     hipLaunchKernelGGL((k_rows8<KIND, 256, 4>), dim3(grid_of(p.rows)), dim3(256), 0, st, p);
@@ -212,20 +217,28 @@ void by_kind(int elem, F&& f) {
 
 void keep8(hipStream_t st, int elem, const KeepArgs& p) {
   if (p.rows <= 0) return;
-  const dim3 grid(grid_of((p.rows * (p.wide / 8) + kItems * 256 - 1) / (kItems * 256)));
-  by_kind(elem, [&](auto k) { hipLaunchKernelGGL((k_keep8<decltype(k)::value>), grid, dim3(256), 0, st, p); });
+  const long eights = p.rows * (p.wide / 8);
+  by_kind(elem, [&](auto k) {
+    if (eights < kFewEights)
+      hipLaunchKernelGGL((k_keep8<decltype(k)::value, 1>), blocks_of(eights, 1), dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((k_keep8<decltype(k)::value, 4>), blocks_of(eights, 4), dim3(256), 0, st, p);
+  });
   DPAMD_LAUNCH_CHECK();
 }
 
 void restore8(hipStream_t st, int elem, const KeepArgs& p) {
   if (p.rows <= 0) return;
-  const dim3 grid(grid_of((p.rows * ((p.cols_out + 7) / 8) + kItems * 256 - 1) / (kItems * 256)));
+  const long eights = p.rows * ((p.cols_out + 7) / 8);
   const bool once = past_caches(p.rows * p.cols_out * (elem == kF32 ? 4 : 2));
   by_kind(elem, [&](auto k) {
+    constexpr int KIND = decltype(k)::value;
     if (once)
-      hipLaunchKernelGGL((k_restore8<decltype(k)::value, true>), grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL((k_restore8<KIND, true, 4>), blocks_of(eights, 4), dim3(256), 0, st, p);
+    else if (eights < kFewEights)
+      hipLaunchKernelGGL((k_restore8<KIND, false, 1>), blocks_of(eights, 1), dim3(256), 0, st, p);
     else
-      hipLaunchKernelGGL((k_restore8<decltype(k)::value, false>), grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL((k_restore8<KIND, false, 4>), blocks_of(eights, 4), dim3(256), 0, st, p);
   });
   DPAMD_LAUNCH_CHECK();
 }
