@@ -1,6 +1,8 @@
 // C ABI of the group norm: argument checks, the choice of a form, workspaces.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "norm.h"
 #include "ops_host.h"
 
@@ -33,53 +35,71 @@ int lanes_of(int groups, int entries, int threads) {
 NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
   const int most = elem == 2 ? 4 : 8;  // 16 bytes
   p.per = p.channels / p.groups;
-  p.vec = p.per % most == 0 ? most : p.per % 2 == 0 ? 2 : 1;
-  p.chunks = p.channels / p.vec;
-  p.chunks_per = p.per / p.vec;
+  p.vec = p.channels < most ? 1 : most;
+  p.general = p.per % p.vec != 0;
+  p.vecs = (p.channels + p.vec - 1) / p.vec;
+  p.entries = p.general ? p.channels : p.vecs;
+  p.group_entries = p.general ? p.per : p.per / p.vec;
   const long length = std::max(1L, p.rows / p.frames);
   const bool affine = grad && (p.dgamma || p.dbeta);
   NormNeeds need{};
-  p.inv_chunks = 1.0f / (float)p.chunks_per, p.inv_per = 1.0f / (float)p.per;
+  p.inv_entries = 1.0f / (float)p.group_entries, p.inv_per = 1.0f / (float)p.per;
   p.once = past_caches((double)p.rows * p.channels * (elem == 2 ? 4 : 2));
-  p.slices = 1;
-  if (!p.starts && p.frames == p.rows && p.chunks <= 1024) {
+  p.slices = p.out_slices = 1;
+  if (!p.starts && p.frames == p.rows && p.vecs <= (p.general && elem != 2 ? 512 : 1024)) {
     p.form = kNormRows;
-    const int T = p.chunks <= 16 ? 16 : p.chunks <= 64 ? 64 : 256;
-    p.by_lanes = p.chunks_per <= 64 && (p.chunks_per & (p.chunks_per - 1)) == 0;
-    p.lanes = lanes_of(p.by_lanes ? 1 : p.groups, p.chunks_per, T);
+    const int T = p.vecs <= 16 ? 16 : p.vecs <= 64 ? 64 : 256;
+    p.by_lanes = !p.general && p.group_entries <= 64 && (p.group_entries & (p.group_entries - 1)) == 0;
+    p.lanes = lanes_of(p.by_lanes ? 1 : p.groups, p.group_entries, T);
     p.blocks = (int)std::min((p.rows + 256 / T - 1) / (256 / T), (grad ? 4L : 8L) * ncu);
     if (affine) need.partial = 8 * (size_t)p.blocks * p.channels;
   } else {
-    // whole groups a block, at least 16 chunks (256 bytes of a row) where that leaves no compute unit idle
-    int gp = std::max(1, std::min(p.groups, 256 / p.chunks_per));
+    // whole groups a block, at least 16 vectors (256 bytes of a row) where that leaves no compute unit idle
+    auto part = [&](int g) { return (int)(((long)g * p.per + p.vec - 1) / p.vec); };
     auto blocks = [&](int g) { return (long)p.frames * ((p.groups + g - 1) / g); };
-    while (gp > 1 && (gp + 1) / 2 * p.chunks_per >= 4 &&
-           (blocks(gp) < ncu || (blocks(gp) < 4 * ncu && (gp + 1) / 2 * p.chunks_per >= 16)) &&
-           256 / ((gp + 1) / 2 * p.chunks_per) <= 2 * length)
+    int gp = (int)std::max(1L, std::min((long)p.groups, 256L * p.vec / p.per));
+    while (gp > 1 && part((gp + 1) / 2) >= 4 &&
+           (blocks(gp) < ncu || (blocks(gp) < 4 * ncu && part((gp + 1) / 2) >= 16)) &&
+           256 / part((gp + 1) / 2) <= 2 * length)
       gp = (gp + 1) / 2;
     // fewer columns where that lets a block hold its rows in registers (8 a thread), from 128 bytes of a row on
-    while (gp > 1 && (gp + 1) / 2 * p.chunks_per >= 8 && length > 6 * (256 / (gp * p.chunks_per))) gp = (gp + 1) / 2;
-    const double bytes = 4.0 * p.rows * p.channels;
-    const double each = 4.0 * length * gp * p.per * ((blocks(gp) + ncu - 1) / ncu);
-    // us: a block's own pace, and three launches with all compute units at work
-    const bool slices = p.chunks_per > 256 || each / 15e3 > 10.0 + bytes / 2e6;
+    while (gp > 1 && part((gp + 1) / 2) >= 8 && length > 6 * (256 / part(gp))) gp = (gp + 1) / 2;
+    // us, fitted to a card's times: a block's chain of rows beyond those it holds, or the bytes, of which pieces of
+    // rows shorter than a few lines waste a part; against slices, which read all twice and take two launches more.
+    // (Ragged frames: up to twice the mean length.)
+    const int eb = elem == 2 ? 4 : 2, hold = grad && p.vec == 8 ? 4 : 8, batch = grad ? 2 : 4;
+    const double size = (double)eb * p.rows * p.channels, n_blocks = (double)blocks(gp);
+    const int lanes = 256 / std::min(256, part(gp));
+    const double more = std::max(0.0, (double)length * (p.starts ? 2 : 1) / lanes - hold);
+    const double again = std::max(0.0, 1.0 - (double)hold * lanes / length);  // rows that are read twice
+    const double waves = std::max(1.0, n_blocks / (3 * ncu)), piece = (double)gp * p.per * eb;
+    const double chain = 3 + waves * (1.2 + 2.4 * std::ceil(more / batch));
+    const double moved = size * (grad ? 3 + 2 * again : 2 + again) / 4.7e6 * (1 + (p.general ? 128 : 16) / piece);
+    const double whole = std::max(chain, moved * std::max(1.0, ncu / n_blocks));
+    const double cut = 10 + size * (grad ? 5 : 3) / 4.7e6;
+    const bool slices = part(gp) > 256 || whole > cut;
     if (!slices) {
       p.form = kNormFrames;
-      p.part = gp * p.chunks_per;
-      p.parts = (p.chunks + p.part - 1) / p.part;
-      p.lanes = lanes_of(gp, 256 / p.part * p.chunks_per, 256);
+      p.part = part(gp);
+      p.part_channels = gp * p.per;
+      p.parts = (p.groups + gp - 1) / gp;
+      p.lanes = lanes_of(gp, 256 / p.part * p.group_entries, 256);
       p.blocks = grad ? std::max(1, 8 * ncu / p.parts) : 65535;
       if (affine) need.partial = 8 * (size_t)std::min(p.frames, p.blocks) * p.channels;
     } else {
       p.form = kNormSlices;
-      p.part = std::min(256, p.chunks);
-      p.parts = (p.chunks + p.part - 1) / p.part;
+      p.part = std::min(256, p.vecs);
+      p.part_channels = p.part * p.vec;
+      p.parts = (p.vecs + p.part - 1) / p.part;
       const long want = std::max(1L, 4L * ncu / ((long)p.parts * p.frames));
-      const int rows_block = 256 / p.part * 4;
-      p.slices = (int)std::min(want, std::max(1L, length / rows_block));
-      p.out_slices = (int)std::min(2 * want, std::max(1L, length / rows_block));
+      // (of two rows a thread at least, and of one)
+      const int at_once = 256 / p.part;
+      p.slices = (int)std::min(want, std::max(1L, length / (2 * at_once)));
+      p.out_slices = (int)std::min(2 * want, std::max(1L, length / at_once));
+      p.part_groups = (int)std::min((long)p.groups, (long)p.part_channels / p.per + 2);
+      p.lanes = lanes_of(std::min(p.part_groups, 256), (std::min(p.per, p.part_channels) + p.vec - 1) / p.vec, 256);
       p.blocks = (int)std::min((long)p.frames, std::max(1L, 8L * ncu / ((long)p.parts * p.slices)));
-      if (!grad || p.dx) need.pairs = 8 * (size_t)p.frames * p.slices * p.chunks;
+      if (!grad || p.dx) need.pairs = 8 * (size_t)p.frames * p.slices * p.parts * p.part_groups;
       if (grad && p.dx) need.sums = 8 * (size_t)p.frames * p.groups;
       if (affine) need.partial = 8 * (size_t)p.blocks * p.slices * p.channels;
       if (!grad && !p.stats) need.stats = 8 * (size_t)p.frames * p.groups;

@@ -18,18 +18,21 @@ struct NormArgs {
   float* stats;  // [frames][groups][2]: mean, 1 / deviation
 
   // how it is cut
-  int vec;     // channels a thread takes at once; `chunks` of them a row, `chunks_per` a group
-  int chunks, chunks_per;
-  int form;    // NormForm
-  bool by_lanes;              // kNormRows: a group's chunks are neighbouring lanes
-  float inv_chunks, inv_per;  // 1 / chunks_per, 1 / per
-  int lanes;   // log2 of the lanes that sum one group's chunks
-  int part;    // chunks of a block's columns (whole groups with kNormFrames), `parts` of them
-  int parts, slices, out_slices;  // (the output's pass has slices of its own)
-  int blocks;  // of the persistent kernels
-  bool once;   // y and dx are stored past the caches
+  int vec, vecs;  // channels that a thread takes at once, and how many times that is a row
+  bool general;   // groups are not multiples of `vec`: the sums' entries are channels; else vectors
+  int entries, group_entries;    // of a row, of a group
+  float inv_entries, inv_per;    // 1 / group_entries, 1 / per
+  int form;       // NormForm
+  bool by_lanes;  // kNormRows: a group's vectors are neighbouring lanes
+  int lanes;      // log2 of the lanes that sum one group's entries
+  int part;       // vectors of a block's columns, `part_channels` channels (whole groups with kNormFrames)
+  int part_channels, parts;
+  int part_groups;  // kNormSlices: groups that a part may meet
+  int slices, out_slices;  // (the output's pass has slices of its own)
+  int blocks;              // of the persistent kernels
+  bool once;               // y and dx are stored past the caches
   float* partial;  // dgamma and dbeta of blocks or slices, or null: none
-  float* pairs;    // two sums of each chunk of a slice
+  float* pairs;    // two sums of each group of a slice and part
   float* sums;     // [frames][groups][2]: means of gamma dz and gamma dz v
 };
 

@@ -44,6 +44,44 @@ __device__ __forceinline__ Frame frame_of(const NormArgs& p, int f) {
   return Frame{a, (int)(b - a)};
 }
 
+// ---- a thread's channels -----------------------------------------------------------------
+// A thread takes VE neighbouring channels, 16 bytes, from c on; `count` of them are there (VE but at the
+// end of a row). Where groups are multiples of VE (not GEN) all of them are of one group, and are one entry of
+// the sums; else (GEN: groups of 5, of 47) each channel is an entry of its own, and knows its group. (With vectors as
+// narrow as a common divisor of groups and 16 bytes instead, odd groups went element by element:
+// 113,120 x 235 in groups of 5, bf16, with its gradients 491 us, so XXX.)
+struct Cols {
+  int c, count;
+};
+template <int VE, bool GEN>
+constexpr int entries_of() {
+  return GEN ? VE : 1;
+}
+// what each entry has: a mean and a deviation, two sums, ...
+template <int VE, bool GEN>
+struct Entries {
+  static constexpr int N = entries_of<VE, GEN>();
+  Pair e[N];
+  __device__ __forceinline__ const Pair& of(int channel) const { return e[GEN ? channel : 0]; }
+};
+// Pairs of the entries' groups, from an array of one for each group.
+template <int VE, bool GEN>
+__device__ __forceinline__ Entries<VE, GEN> of_groups(const Pair* groups, const Cols& x, int per) {
+  Entries<VE, GEN> s;
+  if constexpr (GEN) {
+    // (one division: the group's channels are counted from it)
+    int q = x.c / per, left = (q + 1) * per - x.c;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      s.e[e] = e < x.count ? groups[q] : Pair{0.0f, 0.0f};
+      if (--left == 0) ++q, left = per;
+    }
+  } else {
+    s.e[0] = groups[x.c / per];
+  }
+  return s;
+}
+
 // VE elements as they lie in memory: what is loaded ahead, or kept for long, takes no more registers than that
 // (held in words: single elements of 16 or 8 bits would take a register each).
 template <int KIND, int VE>
@@ -51,20 +89,28 @@ struct Raw {
   using E = typename ElemOf<KIND>::T;
   static constexpr int kBytes = VE * sizeof(E), kWords = (kBytes + 3) / 4;
   unsigned w[kWords];
-  __device__ __forceinline__ void load(const E* p) {
-    if constexpr (kBytes == 2)
-      w[0] = *p;
-    else
-      __builtin_memcpy(w, p, kBytes);  // (the hardware takes addresses of any alignment)
-  }
   __device__ __forceinline__ void zeros() {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) w[k] = 0;
   }
-  __device__ __forceinline__ void ones() {
-    const unsigned one = KIND == kF32 ? 0x3f800000u : KIND == kBf16 ? 0x3f803f80u : 0x3c003c00u;
+  // the elements from p on; those past x's count: zeros
+  template <bool GEN>
+  __device__ __forceinline__ void load(const E* p, const Cols& x) {
+    if constexpr (kBytes == 2) {
+      w[0] = *p;
+    } else if (!GEN || x.count == VE) {
+      __builtin_memcpy(w, p, kBytes);  // (the hardware takes addresses of any alignment)
+    } else {
+      zeros();
 #pragma unroll
-    for (int k = 0; k < kWords; ++k) w[k] = one;
+      for (int e = 0; e < VE; ++e)
+        if (e < x.count) {
+          if constexpr (KIND == kF32)
+            w[e] = __builtin_bit_cast(unsigned, p[e]);
+          else
+            w[e / 2] |= (unsigned)p[e] << (16 * (e % 2));
+        }
+    }
   }
   __device__ __forceinline__ void get(float (&out)[VE]) const {
 #pragma unroll
@@ -76,83 +122,83 @@ struct Raw {
     }
   }
 };
-// the same of x or its checkpoint
-// v = x r - m r: one instruction a value. (m r is rounded, by no more than m itself is.)
-template <int KIND, int VE, bool KEPT>
+// x or its checkpoint, and v = x r - m r from it: one instruction a value. (m r is rounded, by no more than m
+// itself is.)
+template <int KIND, int VE, bool GEN, bool KEPT>
 struct RawX : Raw<KIND, VE> {
-  __device__ __forceinline__ void load_at(const NormArgs& p, long row, int chunk) {
-    this->load(static_cast<const typename ElemOf<KIND>::T*>(p.x) + row * p.ld_x + (long)chunk * VE);
+  __device__ __forceinline__ void load_at(const NormArgs& p, long row, const Cols& x) {
+    this->template load<GEN>(static_cast<const typename ElemOf<KIND>::T*>(p.x) + row * p.ld_x + x.c, x);
   }
-  __device__ __forceinline__ void normalized(const Pair& s, float (&out)[VE]) const {
+  __device__ __forceinline__ void normalized(const Entries<VE, GEN>& s, float (&out)[VE]) const {
     this->get(out);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) out[e] = __builtin_fmaf(out[e], s.b, -s.a * s.b);
+    for (int e = 0; e < VE; ++e) out[e] = __builtin_fmaf(out[e], s.of(e).b, -s.of(e).a * s.of(e).b);
   }
 };
-template <int KIND, int VE>
-struct RawX<KIND, VE, true> {
+template <int KIND, int VE, bool GEN>
+struct RawX<KIND, VE, GEN, true> {
   static constexpr int kWords = (VE + 3) / 4;
   unsigned w[kWords];
-  unsigned char field;
-  __device__ __forceinline__ void load_at(const NormArgs& p, long row, int chunk) {
-    const unsigned char* at = p.kept + row * p.wide + chunk * VE;
-    if constexpr (VE == 1) {
+  unsigned char field, second;  // (GEN: the last elements may be of the next 32)
+  unsigned char split;          // elements of the first
+  __device__ __forceinline__ void load_at(const NormArgs& p, long row, const Cols& x) {
+    const unsigned char* at = p.kept + row * p.wide + x.c;
+    if constexpr (VE == 1)
       w[0] = *at;
-    } else if constexpr (VE == 2) {
-      unsigned short v;
-      __builtin_memcpy(&v, at, 2);
-      w[0] = v;
-    } else {
-      __builtin_memcpy(w, at, VE);
+    else
+      __builtin_memcpy(w, at, VE);  // (past a row's end are the next row's, or the fields: inside the buffer)
+    const unsigned char* fields = p.kept + p.rows * p.wide + row * (p.wide / 32);
+    field = fields[x.c / 32];
+    if constexpr (GEN) {
+      second = fields[min((x.c + VE - 1) / 32, p.wide / 32 - 1)];
+      split = (unsigned char)(32 - x.c % 32);
     }
-    field = p.kept[p.rows * p.wide + row * (p.wide / 32) + chunk * VE / 32];
   }
-  __device__ __forceinline__ void normalized(const Pair& s, float (&out)[VE]) const {
-    const float unit = unit_of(field) * s.b;
+  __device__ __forceinline__ void normalized(const Entries<VE, GEN>& s, float (&out)[VE]) const {
+    const float unit = unit_of(field), other = GEN ? unit_of(second) : unit;
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
-      out[e] = __builtin_fmaf((float)(signed char)(w[e / 4] >> (8 * (e % 4))), unit, -s.a * s.b);
+    for (int e = 0; e < VE; ++e) {
+      const float u = GEN && e >= split ? other : unit;
+      out[e] = __builtin_fmaf((float)(signed char)(w[e / 4] >> (8 * (e % 4))), u * s.of(e).b,
+                              -s.of(e).a * s.of(e).b);
+    }
   }
 };
 
-template <int KIND, int VE>
-__device__ __forceinline__ void load_vec(float (&v)[VE], const typename ElemOf<KIND>::T* p) {
-  Raw<KIND, VE> r;
-  r.load(p);
-  r.get(v);
-}
-template <int KIND, int VE>
-__device__ __forceinline__ void store_vec(typename ElemOf<KIND>::T* p, const float (&v)[VE]) {
+// With ONCE stored past the caches. (Not a test: the compiler makes one store of two, and that an ordinary one.)
+template <int KIND, int VE, bool GEN, bool ONCE>
+__device__ __forceinline__ void store_out(typename ElemOf<KIND>::T* p, const float (&v)[VE], const Cols& x) {
   struct Some {
     typename ElemOf<KIND>::T v[VE];
   } s;
 #pragma unroll
   for (int e = 0; e < VE; ++e) s.v[e] = from_f32<KIND>(v[e]);
-  __builtin_memcpy(p, &s, sizeof(s));
+  if constexpr (VE == 1) {
+    *p = s.v[0];
+  } else if (!GEN || x.count == VE) {
+    static_assert(sizeof(s) == 16, "a thread's channels are 16 bytes");
+    store16<ONCE>(p, __builtin_bit_cast(u4any, s));
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (e < x.count) p[e] = s.v[e];
+  }
 }
-template <int KIND, int VE>
-__device__ __forceinline__ void load_affine(const NormArgs& p, int chunk, float (&gamma)[VE], float (&beta)[VE]) {
+
+template <int KIND, int VE, bool GEN>
+__device__ __forceinline__ void load_affine(const NormArgs& p, const Cols& x, float (&gamma)[VE], float (&beta)[VE]) {
   using T = typename ElemOf<KIND>::T;
 #pragma unroll
   for (int e = 0; e < VE; ++e) gamma[e] = 1.0f, beta[e] = 0.0f;
-  if (p.gamma) load_vec<KIND, VE>(gamma, static_cast<const T*>(p.gamma) + (long)chunk * VE);
-  if (p.beta) load_vec<KIND, VE>(beta, static_cast<const T*>(p.beta) + (long)chunk * VE);
-}
-
-// The same past the caches, where `once` (uniform).
-template <int KIND, int VE>
-__device__ __forceinline__ void store_out(typename ElemOf<KIND>::T* p, const float (&v)[VE], bool once) {
-  if constexpr (VE * sizeof(*p) == 16) {
-    if (once) {
-      struct Some {
-        typename ElemOf<KIND>::T v[VE];
-      } s;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) s.v[e] = from_f32<KIND>(v[e]);
-      return store16<true>(p, __builtin_bit_cast(u4any, s));
-    }
+  Raw<KIND, VE> r;
+  if (p.gamma) {
+    r.template load<GEN>(static_cast<const T*>(p.gamma) + x.c, x);
+    r.get(gamma);
   }
-  store_vec<KIND, VE>(p, v);
+  if (p.beta) {
+    r.template load<GEN>(static_cast<const T*>(p.beta) + x.c, x);
+    r.get(beta);
+  }
 }
 
 // act and its derivative over a thread's values (one uniform branch for all of them)
@@ -182,6 +228,16 @@ __device__ __forceinline__ void forward_vec(int act, const float (&scale)[VE], c
   for (int e = 0; e < VE; ++e) z[e] = __builtin_fmaf(x[e], scale[e], shift[e]);
   activate_vec<KIND, VE>(act, z, x, da);
 }
+// gamma v + beta = x scale + shift
+template <int VE, bool GEN>
+__device__ __forceinline__ void scale_shift(const Entries<VE, GEN>& s, const float (&gamma)[VE],
+                                            const float (&beta)[VE], float (&scale)[VE], float (&shift)[VE]) {
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    scale[e] = gamma[e] * s.of(e).b;
+    shift[e] = __builtin_fmaf(-s.of(e).a, scale[e], beta[e]);
+  }
+}
 // dy -> dz
 template <int KIND, int VE>
 __device__ __forceinline__ void grad_vec(int act, const float (&gamma)[VE], const float (&beta)[VE],
@@ -193,30 +249,69 @@ __device__ __forceinline__ void grad_vec(int act, const float (&gamma)[VE], cons
 #pragma unroll
   for (int e = 0; e < VE; ++e) dy[e] *= da[e];
 }
-// w = gamma dz -> dx = r (w - mean w - v mean(w v))
-template <int VE>
-__device__ __forceinline__ void dx_vec(float r, const Pair& means, const float (&v)[VE], float (&w)[VE]) {
-  const float a = -r * means.a, b = -r * means.b;
+// w = gamma dz -> dx = r (w - mean w - v mean(w v)); s: m and r, means: of w and w v
+template <int VE, bool GEN>
+__device__ __forceinline__ void dx_vec(const Entries<VE, GEN>& s, const Entries<VE, GEN>& means, const float (&v)[VE],
+                                       float (&w)[VE]) {
 #pragma unroll
-  for (int e = 0; e < VE; ++e) w[e] = __builtin_fmaf(v[e], b, __builtin_fmaf(w[e], r, a));
+  for (int e = 0; e < VE; ++e) {
+    const float r = s.of(e).b;
+    w[e] = __builtin_fmaf(v[e], -r * means.of(e).b, __builtin_fmaf(w[e], r, -r * means.of(e).a));
+  }
 }
 
-// mean and squared deviations of VE values
-template <int VE>
-__device__ __forceinline__ Pair moments(const float (&v)[VE]) {
-  float s = 0.0f, q = 0.0f;
+// ---- sums --------------------------------------------------------------------------------
+// Mean and squared deviations of ROWS rows of each entry (of VE values, or one, a row)
+template <int VE, bool GEN, int ROWS>
+__device__ __forceinline__ Entries<VE, GEN> moments(const float (&v)[ROWS][VE]) {
+  constexpr int N = entries_of<VE, GEN>(), W = VE / N;
+  Entries<VE, GEN> s;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) s += v[e];
-  const float m = s * (1.0f / VE);
+  for (int i = 0; i < N; ++i) {
+    float m = 0.0f, M = 0.0f;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) q += (v[e] - m) * (v[e] - m);
-  return Pair{m, q};
+    for (int b = 0; b < ROWS; ++b)
+#pragma unroll
+      for (int w = 0; w < W; ++w) m += v[b][i * W + w];
+    m *= 1.0f / (ROWS * W);
+#pragma unroll
+    for (int b = 0; b < ROWS; ++b)
+#pragma unroll
+      for (int w = 0; w < W; ++w) M += (v[b][i * W + w] - m) * (v[b][i * W + w] - m);
+    s.e[i] = Pair{m, M};
+  }
+  return s;
 }
 // (m, M) of n values joined with that of k more
 __device__ __forceinline__ void join_moments(Pair& p, float n, const Pair& q, float k) {
   const float d = q.a - p.a, w = n == 0.0f ? 1.0f : k * __builtin_amdgcn_rcpf(n + k);
   p.a += d * w;
   p.b += q.b + d * d * n * w;
+}
+template <int VE, bool GEN>
+__device__ __forceinline__ void join_rows(Entries<VE, GEN>& s, int n, const Entries<VE, GEN>& q, int k) {
+  constexpr int N = entries_of<VE, GEN>(), W = VE / N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) join_moments(s.e[i], (float)(n * W), q.e[i], (float)(k * W));
+}
+// Sums of each entry's channels: of b (a) and of g (b)
+template <int VE, bool GEN>
+__device__ __forceinline__ Entries<VE, GEN> entry_sums(const float (&b)[VE], const float (&g)[VE]) {
+  constexpr int N = entries_of<VE, GEN>(), W = VE / N;
+  Entries<VE, GEN> s;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s.e[i] = Pair{0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) s.e[i].a += b[i * W + w], s.e[i].b += g[i * W + w];
+  }
+  return s;
+}
+template <int VE, bool GEN>
+__device__ __forceinline__ void put_entries(Pair* to, const Entries<VE, GEN>& s, const Cols& x) {
+#pragma unroll
+  for (int i = 0; i < entries_of<VE, GEN>(); ++i)
+    if (!GEN || i < x.count) to[i] = s.e[i];
 }
 
 // The sum over 2^log_lanes neighbouring lanes, in each of them (every lane of the wave takes part).
@@ -254,67 +349,72 @@ __device__ __forceinline__ void each_group(int t, int groups, int lanes, F&& f) 
 }
 
 // ---- every row a frame -----------------------------------------------------------------
-// T threads a row, C chunks of VE channels a thread (at neighbouring places for neighbouring threads). With
-// LANES a group is a power of two of chunks, at most 64, so that it is that many neighbouring lanes, which
-// add up without LDS or a barrier; else the parts of a row meet in LDS, a pair for each chunk and then one
-// for each group. (16,384 x 2048 in bf16, groups of 64, gelu: XXX.)
-// A block takes rows one after another: gamma and beta stay in registers, and the next row is loaded
-// while this one is computed.
-template <int KIND, int VE, int T, int C, bool LANES>
+// T threads a row, C vectors of VE channels a thread (at neighbouring places for neighbouring threads). With
+// LANES a group is a power of two of vectors, at most 64, so that it is that many neighbouring lanes, which
+// add up without LDS or a barrier; else the entries of a row meet in LDS, and then a pair for each group.
+// (16,384 x 2048 in bf16, groups of 64, gelu: 50 us through LDS, 38 by lanes, and 29 with gelu's short form; a copy's
+// rate would be 26.) A block takes rows one after another: gamma and beta stay in registers, and the next row is
+// loaded while this one is computed.
+template <int KIND, int VE, bool GEN, int T, int C, bool LANES, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
+  constexpr int W = VE / entries_of<VE, GEN>();
   extern __shared__ __align__(16) char lds[];
   constexpr int R = kThreads / T;
   const int t = threadIdx.x % T, mine = threadIdx.x / T;
-  Pair* parts = reinterpret_cast<Pair*>(lds) + (size_t)mine * (p.chunks + p.groups);
-  Pair* whole = parts + p.chunks;
+  Pair* parts = reinterpret_cast<Pair*>(lds) + (size_t)mine * (p.entries + p.groups);
+  Pair* whole = parts + p.entries;
+  Cols x[C];
   float gamma[C][VE], beta[C][VE];
 #pragma unroll
-  for (int k = 0; k < C; ++k) load_affine<KIND, VE>(p, min(k * T + t, p.chunks - 1), gamma[k], beta[k]);
+  for (int k = 0; k < C; ++k) {
+    const int c = min(k * T + t, p.vecs - 1) * VE;
+    x[k] = Cols{c, min(VE, p.channels - c)};
+    load_affine<KIND, VE, GEN>(p, x[k], gamma[k], beta[k]);
+  }
   Raw<KIND, VE> raw[C];
   auto fetch = [&](long row) {
-    const E* x = static_cast<const E*>(p.x) + min(row, p.rows - 1) * p.ld_x;
+    const E* at = static_cast<const E*>(p.x) + min(row, p.rows - 1) * p.ld_x;
 #pragma unroll
     for (int k = 0; k < C; ++k)
-      if (k * T + t < p.chunks) raw[k].load(x + (long)(k * T + t) * VE);
+      if (k * T + t < p.vecs) raw[k].template load<GEN>(at + x[k].c, x[k]);
   };
   const long step = (long)gridDim.x * R;
   fetch((long)blockIdx.x * R + mine);
   for (long row0 = (long)blockIdx.x * R; row0 < p.rows; row0 += step) {
     const long row = row0 + mine;
     const bool there = row < p.rows;
-    float v[C][VE];
-    Pair stat[C];
+    float v[C][1][VE];
+    Entries<VE, GEN> stat[C];
     auto keep = [&](int q, const Pair& s) {
       if (p.stats && there) *reinterpret_cast<Pair*>(p.stats + 2 * (row * p.groups + q)) = s;
     };
     if constexpr (LANES) {
 #pragma unroll
       for (int k = 0; k < C; ++k) {
-        raw[k].get(v[k]);
-        const Pair s = moments<VE>(v[k]);
-        const float m = sum_lanes(s.a, p.lanes) * p.inv_chunks;
+        raw[k].get(v[k][0]);
+        const Pair s = moments<VE, GEN, 1>(v[k]).e[0];
+        const float m = sum_lanes(s.a, p.lanes) * p.inv_entries;
         const float M = sum_lanes(s.b + VE * (s.a - m) * (s.a - m), p.lanes);
-        stat[k] = Pair{m, deviation(M, p.inv_per, p.eps)};
-        const int chunk = k * T + t;
-        if (chunk < p.chunks && (t & (p.chunks_per - 1)) == 0) keep(chunk / p.chunks_per, stat[k]);
+        stat[k].e[0] = Pair{m, deviation(M, p.inv_per, p.eps)};
+        if (k * T + t < p.vecs && (t & (p.group_entries - 1)) == 0) keep(x[k].c / p.per, stat[k].e[0]);
       }
       if (row0 + step < p.rows) fetch(row + step);
     } else {
 #pragma unroll
       for (int k = 0; k < C; ++k)
-        if (k * T + t < p.chunks) {
-          raw[k].get(v[k]);
-          parts[k * T + t] = moments<VE>(v[k]);
+        if (k * T + t < p.vecs) {
+          raw[k].get(v[k][0]);
+          put_entries<VE, GEN>(parts + x[k].c / W, moments<VE, GEN, 1>(v[k]), x[k]);
         }
       if (row0 + step < p.rows) fetch(row + step);
       row_sync<T>();
       each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
-        const Pair* s = parts + q * p.chunks_per;
+        const Pair* s = parts + q * p.group_entries;
         float m = 0.0f, M = 0.0f;
-        for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) m += s[k].a;
-        m = sum_lanes(m, p.lanes) * p.inv_chunks;
-        for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) M += s[k].b + VE * (s[k].a - m) * (s[k].a - m);
+        for (int k = lane; k < p.group_entries; k += 1 << p.lanes) m += s[k].a;
+        m = sum_lanes(m, p.lanes) * p.inv_entries;
+        for (int k = lane; k < p.group_entries; k += 1 << p.lanes) M += s[k].b + W * (s[k].a - m) * (s[k].a - m);
         const Pair r = {m, deviation(sum_lanes(M, p.lanes), p.inv_per, p.eps)};
         if (in && lane == 0) {
           whole[q] = r;
@@ -324,92 +424,105 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
       row_sync<T>();
 #pragma unroll
       for (int k = 0; k < C; ++k)
-        if (k * T + t < p.chunks) stat[k] = whole[(k * T + t) / p.chunks_per];
+        if (k * T + t < p.vecs) stat[k] = of_groups<VE, GEN>(whole, x[k], p.per);
       row_sync<T>();  // (the next row's parts go where these are read)
     }
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int chunk = k * T + t;
-      if (chunk >= p.chunks) continue;
+      if (k * T + t >= p.vecs) continue;
 #pragma unroll
-      for (int e = 0; e < VE; ++e) v[k][e] = __builtin_fmaf(v[k][e], stat[k].b, -stat[k].a * stat[k].b);
-      forward_vec<KIND, VE>(p.act, gamma[k], beta[k], v[k]);
-      if (there) store_out<KIND, VE>(static_cast<E*>(p.y) + row * p.ld_y + (long)chunk * VE, v[k], p.once);
+      for (int e = 0; e < VE; ++e)
+        v[k][0][e] = __builtin_fmaf(v[k][0][e], stat[k].of(e).b, -stat[k].of(e).a * stat[k].of(e).b);
+      forward_vec<KIND, VE>(p.act, gamma[k], beta[k], v[k][0]);
+      if (there) store_out<KIND, VE, GEN, ONCE>(static_cast<E*>(p.y) + row * p.ld_y + x[k].c, v[k][0], x[k]);
     }
   }
 }
 
 // Its gradients: dgamma and dbeta of a thread's channels are summed over all rows that its block takes, and
-// then over the block's row lanes; partial [blocks][2][channels].
-template <int KIND, int VE, int T, int C, bool LANES, bool KEPT>
+// then over the block's row lanes; partial [blocks][2][channels]. (16,384 x 2048 from the checkpoint in bf16: 74 us
+// with one row under way, 49 with two, 33 at a copy's rate.)
+template <int KIND, int VE, bool GEN, int T, int C, bool LANES, bool KEPT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
+  constexpr int W = VE / entries_of<VE, GEN>();
   extern __shared__ __align__(16) char lds[];
   constexpr int R = kThreads / T;
   const int t = threadIdx.x % T, mine = threadIdx.x / T;
-  Pair* parts = reinterpret_cast<Pair*>(lds) + (size_t)mine * (p.chunks + p.groups);
-  Pair* whole = parts + p.chunks;
-  float gamma[C][VE], beta[C][VE];
+  Pair* parts = reinterpret_cast<Pair*>(lds) + (size_t)mine * (p.entries + p.groups);
+  Pair* whole = parts + p.entries;
+  Cols x[C];
+  float gamma[C][VE], beta[C][VE], ga[C][VE] = {}, be[C][VE] = {};
 #pragma unroll
-  for (int k = 0; k < C; ++k) load_affine<KIND, VE>(p, min(k * T + t, p.chunks - 1), gamma[k], beta[k]);
-  float ga[C][VE] = {}, be[C][VE] = {};
+  for (int k = 0; k < C; ++k) {
+    const int c = min(k * T + t, p.vecs - 1) * VE;
+    x[k] = Cols{c, min(VE, p.channels - c)};
+    load_affine<KIND, VE, GEN>(p, x[k], gamma[k], beta[k]);
+  }
   // two rows are under way (with one, 16 waves of a compute unit wait for too few bytes)
+  // (GEN: m and r of each channel would take too many registers for that: they are loaded at the row's turn)
   struct Ahead {
-    RawX<KIND, VE, KEPT> x[C];
+    RawX<KIND, VE, GEN, KEPT> x[C];
     Raw<KIND, VE> dy[C];
-    Pair stat[C];
+    Entries<VE, false> stat[C];
   } ahead[2];
+  auto stats_of = [&](long row, const Cols& c) {
+    return of_groups<VE, GEN>(reinterpret_cast<const Pair*>(p.stats + 2 * row * p.groups), c, p.per);
+  };
   auto fetch = [&](long row, Ahead& to) {  // (dy of rows past the last: zeros)
     const bool there = row < p.rows;
     row = min(row, p.rows - 1);
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int chunk = k * T + t;
-      if (chunk >= p.chunks) continue;
-      to.x[k].load_at(p, row, chunk);
+      if (k * T + t >= p.vecs) continue;
+      to.x[k].load_at(p, row, x[k]);
       if (there)
-        to.dy[k].load(static_cast<const E*>(p.dy) + row * p.ld_y + (long)chunk * VE);
+        to.dy[k].template load<GEN>(static_cast<const E*>(p.dy) + row * p.ld_y + x[k].c, x[k]);
       else
         to.dy[k].zeros();
-      to.stat[k] = *reinterpret_cast<const Pair*>(p.stats + 2 * (row * p.groups + chunk / p.chunks_per));
+      if constexpr (!GEN) to.stat[k] = stats_of(row, x[k]);
     }
   };
   const long step = (long)gridDim.x * R;
   auto compute = [&](long row0, Ahead& from) {
     const long row = row0 + mine;
     const bool there = row < p.rows;
-    float v[C][VE], w[C][VE], r[C];
-    Pair means[C];
+    float v[C][VE], w[C][VE];
+    Entries<VE, GEN> means[C], stat[C];
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int chunk = k * T + t;
-      means[k] = Pair{0.0f, 0.0f};
-      if (chunk >= p.chunks) continue;
-      from.x[k].normalized(from.stat[k], v[k]);
+      means[k] = Entries<VE, GEN>{};
+      if (k * T + t >= p.vecs) continue;
+      if constexpr (GEN)
+        stat[k] = stats_of(min(row, p.rows - 1), x[k]);
+      else
+        stat[k] = from.stat[k];
+      from.x[k].normalized(stat[k], v[k]);
       from.dy[k].get(w[k]);
-      r[k] = from.stat[k].b;
       grad_vec<KIND, VE>(p.act, gamma[k], beta[k], v[k], w[k]);
+      float wv[VE];
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         be[k][e] += w[k][e];
         ga[k][e] += w[k][e] * v[k][e];
         w[k][e] *= gamma[k][e];
-        means[k].a += w[k][e];
-        means[k].b += w[k][e] * v[k][e];
+        wv[e] = w[k][e] * v[k][e];
       }
-      if constexpr (!LANES) parts[chunk] = means[k];
+      means[k] = entry_sums<VE, GEN>(w[k], wv);
+      if constexpr (!LANES) put_entries<VE, GEN>(parts + x[k].c / W, means[k], x[k]);
     }
     if (row0 + 2 * step < p.rows) fetch(row + 2 * step, from);
     if constexpr (LANES) {
 #pragma unroll
       for (int k = 0; k < C; ++k)
-        means[k] = Pair{sum_lanes(means[k].a, p.lanes) * p.inv_per, sum_lanes(means[k].b, p.lanes) * p.inv_per};
+        means[k].e[0] = Pair{sum_lanes(means[k].e[0].a, p.lanes) * p.inv_per,
+                             sum_lanes(means[k].e[0].b, p.lanes) * p.inv_per};
     } else {
       row_sync<T>();
       each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
-        const Pair* s = parts + q * p.chunks_per;
+        const Pair* s = parts + q * p.group_entries;
         float a = 0.0f, b = 0.0f;
-        for (int k = lane; k < p.chunks_per; k += 1 << p.lanes) a += s[k].a, b += s[k].b;
+        for (int k = lane; k < p.group_entries; k += 1 << p.lanes) a += s[k].a, b += s[k].b;
         a = sum_lanes(a, p.lanes) * p.inv_per;
         b = sum_lanes(b, p.lanes) * p.inv_per;
         if (in && lane == 0) whole[q] = Pair{a, b};
@@ -417,15 +530,14 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
       row_sync<T>();
 #pragma unroll
       for (int k = 0; k < C; ++k)
-        if (k * T + t < p.chunks) means[k] = whole[(k * T + t) / p.chunks_per];
+        if (k * T + t < p.vecs) means[k] = of_groups<VE, GEN>(whole, x[k], p.per);
       row_sync<T>();
     }
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int chunk = k * T + t;
-      if (chunk >= p.chunks || !there || !p.dx) continue;
-      dx_vec<VE>(r[k], means[k], v[k], w[k]);
-      store_out<KIND, VE>(static_cast<E*>(p.dx) + row * p.ld_x + (long)chunk * VE, w[k], p.once);
+      if (k * T + t >= p.vecs || !there || !p.dx) continue;
+      dx_vec<VE, GEN>(stat[k], means[k], v[k], w[k]);
+      store_out<KIND, VE, GEN, ONCE>(static_cast<E*>(p.dx) + row * p.ld_x + x[k].c, w[k], x[k]);
     }
   };
   const long first = (long)blockIdx.x * R;
@@ -454,106 +566,102 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
 }
 
 // ---- a block's part of a frame ---------------------------------------------------------------
-// Threads (column tc of `part` chunks, row tr): part is at most 256; the threads left over by 256 / part
-// idle. Rows tr, tr + TR, ...
+// Threads (vector tc of `part`, row lane tr): part is at most 256; the threads left over by 256 / part
+// idle. Rows tr, tr + TR, ... The part's channels: from c0 on, `channels` of them.
 struct Lay {
-  int tc, tr, TR;
+  int tc, tr, TR, c0, channels;
+  Cols x;
   bool in;
 };
-__device__ __forceinline__ Lay lay_of(int part, int cols) {
-  const int TR = kThreads / part, tr = threadIdx.x / part, tc = threadIdx.x - tr * part;
-  return Lay{tc, tr, TR, tr < TR && tc < cols};
+template <int VE>
+__device__ __forceinline__ Lay lay_of(const NormArgs& p) {
+  Lay l;
+  l.TR = kThreads / p.part;
+  l.tr = threadIdx.x / p.part;
+  l.tc = threadIdx.x - l.tr * p.part;
+  l.c0 = blockIdx.x * p.part_channels;
+  l.channels = min(p.part_channels, p.channels - l.c0);
+  l.in = l.tr < l.TR && l.tc * VE < l.channels;
+  const int at = l.in ? l.tc * VE : 0;
+  l.x = Cols{l.c0 + at, min(VE, l.channels - at)};
+  return l;
 }
+// rows of row lane tr
+__device__ __forceinline__ int rows_of(int count, int tr, int TR) { return count > tr ? (count - tr + TR - 1) / TR : 0; }
 
 constexpr int kBatch = 4;  // rows under way
 
-// The moments s of a thread's chunk, joined with those of its rows from the `from`-th on: first + tr + i TR below
+// The moments s of a thread's entries, joined with those of its rows from the `from`-th on: first + tr + i TR below
 // first + count
-template <int KIND, int VE>
-__device__ __forceinline__ void thread_moments(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                               int from, Pair& s) {
-  const typename ElemOf<KIND>::T* x = static_cast<const typename ElemOf<KIND>::T*>(p.x) + (long)chunk * VE;
+template <int KIND, int VE, bool GEN>
+__device__ __forceinline__ void thread_moments(const NormArgs& p, long first, int count, const Lay& l, int from,
+                                               Entries<VE, GEN>& s) {
+  const typename ElemOf<KIND>::T* x = static_cast<const typename ElemOf<KIND>::T*>(p.x) + l.x.c;
   int n = from, r = l.tr + from * l.TR;
   for (; r + (kBatch - 1) * l.TR < count; r += kBatch * l.TR) {
     float v[kBatch][VE];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) load_vec<KIND, VE>(v[b], x + (first + r + (long)b * l.TR) * p.ld_x);
-    float m = 0.0f, M = 0.0f;
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) m += v[b][e];
-    m *= 1.0f / (kBatch * VE);
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) M += (v[b][e] - m) * (v[b][e] - m);
-    join_moments(s, (float)(n * VE), Pair{m, M}, (float)(kBatch * VE));
+    for (int b = 0; b < kBatch; ++b) {
+      Raw<KIND, VE> raw;
+      raw.template load<GEN>(x + (first + r + (long)b * l.TR) * p.ld_x, l.x);
+      raw.get(v[b]);
+    }
+    join_rows<VE, GEN>(s, n, moments<VE, GEN, kBatch>(v), kBatch);
     n += kBatch;
   }
   for (; r < count; r += l.TR) {
-    float v[VE];
-    load_vec<KIND, VE>(v, x + (first + r) * p.ld_x);
-    join_moments(s, (float)(n * VE), moments<VE>(v), (float)VE);
+    float v[1][VE];
+    Raw<KIND, VE> raw;
+    raw.template load<GEN>(x + (first + r) * p.ld_x, l.x);
+    raw.get(v[0]);
+    join_rows<VE, GEN>(s, n, moments<VE, GEN, 1>(v), 1);
     ++n;
   }
 }
-// rows of a thread in row lane tr
-__device__ __forceinline__ int rows_of(int count, int tr, int TR) { return count > tr ? (count - tr + TR - 1) / TR : 0; }
 
-// y = act(x scale + shift) of a thread's chunk over its rows
-template <int KIND, int VE>
-__device__ __forceinline__ void thread_apply(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                             int from, const float (&scale)[VE], const float (&shift)[VE]) {
+// y = act(x scale + shift) of a thread's channels over its rows
+template <int KIND, int VE, bool GEN, bool ONCE>
+__device__ __forceinline__ void thread_apply(const NormArgs& p, long first, int count, const Lay& l, int from,
+                                             const float (&scale)[VE], const float (&shift)[VE]) {
   using E = typename ElemOf<KIND>::T;
-  const E* x = static_cast<const E*>(p.x) + (long)chunk * VE;
-  E* y = static_cast<E*>(p.y) + (long)chunk * VE;
+  const E* x = static_cast<const E*>(p.x) + l.x.c;
+  E* y = static_cast<E*>(p.y) + l.x.c;
   int r = l.tr + from * l.TR;
+  Raw<KIND, VE> raw[kBatch];
+  float v[VE];
   for (; r + (kBatch - 1) * l.TR < count; r += kBatch * l.TR) {
-    Raw<KIND, VE> raw[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) raw[b].load(x + (first + r + (long)b * l.TR) * p.ld_x);
+    for (int b = 0; b < kBatch; ++b) raw[b].template load<GEN>(x + (first + r + (long)b * l.TR) * p.ld_x, l.x);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      float v[VE];
       raw[b].get(v);
       forward_vec<KIND, VE>(p.act, scale, shift, v);
-      store_out<KIND, VE>(y + (first + r + (long)b * l.TR) * p.ld_y, v, p.once);
+      store_out<KIND, VE, GEN, ONCE>(y + (first + r + (long)b * l.TR) * p.ld_y, v, l.x);
     }
   }
   for (; r < count; r += l.TR) {
-    float v[VE];
-    load_vec<KIND, VE>(v, x + (first + r) * p.ld_x);
+    raw[0].template load<GEN>(x + (first + r) * p.ld_x, l.x);
+    raw[0].get(v);
     forward_vec<KIND, VE>(p.act, scale, shift, v);
-    store_out<KIND, VE>(y + (first + r) * p.ld_y, v, p.once);
-  }
-}
-// gamma v + beta = x scale + shift
-template <int VE>
-__device__ __forceinline__ void scale_shift(const Pair& s, const float (&gamma)[VE], const float (&beta)[VE],
-                                            float (&scale)[VE], float (&shift)[VE]) {
-#pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    scale[e] = gamma[e] * s.b;
-    shift[e] = __builtin_fmaf(-s.a, scale[e], beta[e]);
+    store_out<KIND, VE, GEN, ONCE>(y + (first + r) * p.ld_y, v, l.x);
   }
 }
 
-// x and dy of a thread's chunk, both kRows rows of them, under way together.
-template <int KIND, int VE, bool KEPT, class F>
-__device__ __forceinline__ void thread_rows(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                            int from, const Pair& s, F&& f) {
+// f(v, dy, row) over a thread's rows, two of them under way together.
+template <int KIND, int VE, bool GEN, bool KEPT, class F>
+__device__ __forceinline__ void thread_rows(const NormArgs& p, long first, int count, const Lay& l, int from,
+                                            const Entries<VE, GEN>& s, F&& f) {
   constexpr int kRows = 2;
   using E = typename ElemOf<KIND>::T;
-  const E* dy = static_cast<const E*>(p.dy) + (long)chunk * VE;
+  const E* dy = static_cast<const E*>(p.dy) + l.x.c;
   for (int r = l.tr + from * l.TR; r < count; r += kRows * l.TR) {
-    RawX<KIND, VE, KEPT> raw_x[kRows];
+    RawX<KIND, VE, GEN, KEPT> raw_x[kRows];
     Raw<KIND, VE> raw_dy[kRows];
 #pragma unroll
     for (int b = 0; b < kRows; ++b)
       if (r + b * l.TR < count) {
-        raw_x[b].load_at(p, first + r + (long)b * l.TR, chunk);
-        raw_dy[b].load(dy + (first + r + (long)b * l.TR) * p.ld_y);
+        raw_x[b].load_at(p, first + r + (long)b * l.TR, l.x);
+        raw_dy[b].template load<GEN>(dy + (first + r + (long)b * l.TR) * p.ld_y, l.x);
       }
 #pragma unroll
     for (int b = 0; b < kRows; ++b)
@@ -565,44 +673,60 @@ __device__ __forceinline__ void thread_rows(const NormArgs& p, long first, int c
       }
   }
 }
-// dz and dz v of a thread's chunk summed over its rows
-template <int KIND, int VE, bool KEPT>
-__device__ __forceinline__ void thread_sums(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                            int from, const Pair& s, const float (&gamma)[VE],
+// dz and dz v of a thread's channels summed over its rows
+template <int KIND, int VE, bool GEN, bool KEPT>
+__device__ __forceinline__ void thread_sums(const NormArgs& p, long first, int count, const Lay& l, int from,
+                                            const Entries<VE, GEN>& s, const float (&gamma)[VE],
                                             const float (&beta)[VE], float (&be)[VE], float (&ga)[VE]) {
-  thread_rows<KIND, VE, KEPT>(p, first, count, chunk, l, from, s, [&](float (&v)[VE], float (&d)[VE], long) {
+  thread_rows<KIND, VE, GEN, KEPT>(p, first, count, l, from, s, [&](float (&v)[VE], float (&d)[VE], long) {
     grad_vec<KIND, VE>(p.act, gamma, beta, v, d);
 #pragma unroll
     for (int e = 0; e < VE; ++e) be[e] += d[e], ga[e] += d[e] * v[e];
   });
 }
-template <int KIND, int VE, bool KEPT>
-__device__ __forceinline__ void thread_dx(const NormArgs& p, long first, int count, int chunk, const Lay& l,
-                                          int from, const Pair& s, const Pair& means, const float (&gamma)[VE],
-                                          const float (&beta)[VE]) {
+template <int KIND, int VE, bool GEN, bool KEPT, bool ONCE>
+__device__ __forceinline__ void thread_dx(const NormArgs& p, long first, int count, const Lay& l, int from,
+                                          const Entries<VE, GEN>& s, const Entries<VE, GEN>& means,
+                                          const float (&gamma)[VE], const float (&beta)[VE]) {
   using E = typename ElemOf<KIND>::T;
-  E* dx = static_cast<E*>(p.dx) + (long)chunk * VE;
-  thread_rows<KIND, VE, KEPT>(p, first, count, chunk, l, from, s, [&](float (&v)[VE], float (&d)[VE], long row) {
+  E* dx = static_cast<E*>(p.dx) + l.x.c;
+  thread_rows<KIND, VE, GEN, KEPT>(p, first, count, l, from, s, [&](float (&v)[VE], float (&d)[VE], long row) {
     grad_vec<KIND, VE>(p.act, gamma, beta, v, d);
 #pragma unroll
     for (int e = 0; e < VE; ++e) d[e] *= gamma[e];
-    dx_vec<VE>(s.b, means, v, d);
-    store_out<KIND, VE>(dx + row * p.ld_x, d, p.once);
+    dx_vec<VE, GEN>(s, means, v, d);
+    store_out<KIND, VE, GEN, ONCE>(dx + row * p.ld_x, d, l.x);
   });
+}
+// be and ga of the block's threads summed over its row lanes, to out [2][channels] at the part's channels
+template <int VE>
+__device__ __forceinline__ void put_channel_sums(const NormArgs& p, const Lay& l, const float (&ga)[VE],
+                                                 const float (&be)[VE], float* sums, float* out) {
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VE; ++e) sums[threadIdx.x * VE + e] = which ? be[e] : ga[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < l.channels; c += kThreads) {
+      float v = 0.0f;
+      for (int m = 0; m < l.TR; ++m) v += sums[m * p.part * VE + c];
+      out[which * p.channels + l.c0 + c] = v;
+    }
+  }
 }
 
 // Whole frames: grid (parts, frames, or fewer in y: strided). A thread's first kHold rows stay in registers
-// between the sums and the output; what is beyond them is read again.
-template <int KIND, int VE>
+// between the sums and the output; what is beyond them is read again. (64 ragged frames of 12,288 x 1600 in fp32: 50 us
+// reading all rows twice, 41 so; 30 at a copy's rate.)
+template <int KIND, int VE, bool GEN, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
-  constexpr int kHold = 8;
-  __shared__ Pair parts[kThreads], whole[kThreads];
-  const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0), groups = cols / p.chunks_per;
-  const Lay l = lay_of(p.part, cols);
-  const int chunk = c0 + min(l.tc, cols - 1);
+  constexpr int kHold = 8, N = entries_of<VE, GEN>(), W = VE / N;
+  __shared__ Pair parts[kThreads * N], whole[kThreads * N];
+  const Lay l = lay_of<VE>(p);
+  const int wide = p.part * N, groups = l.channels / p.per;  // entries of a row lane
   float gamma[VE], beta[VE];
-  load_affine<KIND, VE>(p, chunk, gamma, beta);
+  load_affine<KIND, VE, GEN>(p, l.x, gamma, beta);
   for (int f = blockIdx.y; f < p.frames; f += gridDim.y) {
     const Frame w = frame_of(p, f);
     const int have = l.in ? min(rows_of(w.count, l.tr, l.TR), kHold) : 0;
@@ -612,92 +736,99 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
     for (int i = 0; i < kHold; ++i) {
       raw[i].zeros();
       if (i < have)
-        raw[i].load(static_cast<const E*>(p.x) + (w.first + l.tr + (long)i * l.TR) * p.ld_x + (long)chunk * VE);
+        raw[i].template load<GEN>(static_cast<const E*>(p.x) + (w.first + l.tr + (long)i * l.TR) * p.ld_x + l.x.c, l.x);
     }
-    Pair mine = {0.0f, 0.0f};
+    Entries<VE, GEN> mine{};
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
       float v[VE];
       raw[i].get(v);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) mine.a += v[e];
+      for (int e = 0; e < VE; ++e) mine.e[GEN ? e : 0].a += v[e];
     }
-    mine.a = have ? mine.a / (float)(have * VE) : 0.0f;
+    const float inv = have ? 1.0f / (float)(have * W) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine.e[i].a *= inv;
 #pragma unroll
     for (int i = 0; i < kHold; ++i)
       if (i < have) {
         float v[VE];
         raw[i].get(v);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) mine.b += (v[e] - mine.a) * (v[e] - mine.a);
+        for (int e = 0; e < VE; ++e) {
+          const float d = v[e] - mine.of(e).a;
+          mine.e[GEN ? e : 0].b += d * d;
+        }
       }
-    if (l.in) thread_moments<KIND, VE>(p, w.first, w.count, chunk, l, kHold, mine);
-    parts[threadIdx.x] = mine;
+    if (l.in) {
+      thread_moments<KIND, VE, GEN>(p, w.first, w.count, l, kHold, mine);
+      put_entries<VE, GEN>(parts + l.tr * wide + l.tc * N, mine, l.x);
+    }
     __syncthreads();
     const float total = (float)w.count * (float)p.per;
     each_group<kThreads>(threadIdx.x, groups, p.lanes, [&](int q, int lane, bool in) {
       float m = 0.0f, M = 0.0f;
-      const int all = l.TR * p.chunks_per;
+      const int all = l.TR * p.group_entries;
       for (int k = lane; k < all; k += 1 << p.lanes) {
-        const int tr = k / p.chunks_per;
-        m += (float)rows_of(w.count, tr, l.TR) * parts[tr * p.part + q * p.chunks_per + k - tr * p.chunks_per].a;
+        const int tr = k / p.group_entries;
+        m += (float)rows_of(w.count, tr, l.TR) * parts[tr * wide + q * p.group_entries + k - tr * p.group_entries].a;
       }
-      m = sum_lanes(m, p.lanes) * VE / total;
+      m = sum_lanes(m, p.lanes) * W / total;
       for (int k = lane; k < all; k += 1 << p.lanes) {
-        const int tr = k / p.chunks_per;
-        const Pair s = parts[tr * p.part + q * p.chunks_per + k - tr * p.chunks_per];
-        M += s.b + (float)(rows_of(w.count, tr, l.TR) * VE) * (s.a - m) * (s.a - m);
+        const int tr = k / p.group_entries, rows = rows_of(w.count, tr, l.TR);
+        const Pair s = parts[tr * wide + q * p.group_entries + k - tr * p.group_entries];
+        M += s.b + (float)(rows * W) * (s.a - m) * (s.a - m);
       }
       M = sum_lanes(M, p.lanes);
       const Pair s = w.count ? Pair{m, deviation(M, 1.0f / total, p.eps)} : Pair{0.0f, 0.0f};
       if (in && lane == 0) {
         whole[q] = s;
-        if (p.stats)
-          *reinterpret_cast<Pair*>(p.stats + 2 * ((long)f * p.groups + c0 / p.chunks_per + q)) = s;
+        if (p.stats) *reinterpret_cast<Pair*>(p.stats + 2 * ((long)f * p.groups + l.c0 / p.per + q)) = s;
       }
     });
     __syncthreads();
     if (l.in) {
       float scale[VE], shift[VE];
-      scale_shift<VE>(whole[l.tc / p.chunks_per], gamma, beta, scale, shift);
+      scale_shift<VE, GEN>(of_groups<VE, GEN>(whole, Cols{l.x.c - l.c0, l.x.count}, p.per), gamma, beta, scale, shift);
 #pragma unroll
       for (int i = 0; i < kHold; ++i)
         if (i < have) {
           float v[VE];
           raw[i].get(v);
           forward_vec<KIND, VE>(p.act, scale, shift, v);
-          store_vec<KIND, VE>(static_cast<E*>(p.y) + (w.first + l.tr + (long)i * l.TR) * p.ld_y + (long)chunk * VE, v);
+          store_out<KIND, VE, GEN, ONCE>(static_cast<E*>(p.y) + (w.first + l.tr + (long)i * l.TR) * p.ld_y + l.x.c, v, l.x);
         }
-      thread_apply<KIND, VE>(p, w.first, w.count, chunk, l, kHold, scale, shift);
+      thread_apply<KIND, VE, GEN, ONCE>(p, w.first, w.count, l, kHold, scale, shift);
     }
     __syncthreads();
   }
 }
 
 // partial [gridDim.y][2][channels]
-template <int KIND, int VE, bool KEPT>
+template <int KIND, int VE, bool GEN, bool KEPT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_frames_grad(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
   constexpr int kHold = VE == 8 ? 4 : 8;  // rows whose v and dz stay in registers: 64 of these
-  __shared__ Pair parts[kThreads], whole[kThreads];
+  constexpr int N = entries_of<VE, GEN>();
+  __shared__ Pair parts[kThreads * N], whole[kThreads * N];
   __shared__ float sums[kThreads * VE];
-  const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0), groups = cols / p.chunks_per;
-  const Lay l = lay_of(p.part, cols);
-  const int chunk = c0 + min(l.tc, cols - 1);
+  const Lay l = lay_of<VE>(p);
+  const int wide = p.part * N, groups = l.channels / p.per;
   float gamma[VE], beta[VE], ga[VE] = {}, be[VE] = {};
-  load_affine<KIND, VE>(p, chunk, gamma, beta);
+  load_affine<KIND, VE, GEN>(p, l.x, gamma, beta);
   for (int f = blockIdx.y; f < p.frames; f += gridDim.y) {
     const Frame w = frame_of(p, f);
-    const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * ((long)f * p.groups + chunk / p.chunks_per));
+    const Entries<VE, GEN> s =
+        of_groups<VE, GEN>(reinterpret_cast<const Pair*>(p.stats + 2 * (long)f * p.groups), l.x, p.per);
     const int have = l.in ? min(rows_of(w.count, l.tr, l.TR), kHold) : 0;
-    RawX<KIND, VE, KEPT> raw_x[kHold];
+    RawX<KIND, VE, GEN, KEPT> raw_x[kHold];
     Raw<KIND, VE> raw_dy[kHold];
 #pragma unroll
     for (int i = 0; i < kHold; ++i)
       if (i < have) {
         const long row = w.first + l.tr + (long)i * l.TR;
-        raw_x[i].load_at(p, row, chunk);
-        raw_dy[i].load(static_cast<const E*>(p.dy) + row * p.ld_y + (long)chunk * VE);
+        raw_x[i].load_at(p, row, l.x);
+        raw_dy[i].template load<GEN>(static_cast<const E*>(p.dy) + row * p.ld_y + l.x.c, l.x);
       }
     float b[VE] = {}, g[VE] = {}, v[kHold][VE], d[kHold][VE];
 #pragma unroll
@@ -712,57 +843,45 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames_grad(const NormArgs p)
           d[i][e] *= gamma[e];
         }
       }
-    if (l.in) thread_sums<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, kHold, s, gamma, beta, b, g);
-    Pair sum = {0.0f, 0.0f};
+    if (l.in) thread_sums<KIND, VE, GEN, KEPT>(p, w.first, w.count, l, kHold, s, gamma, beta, b, g);
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      sum.a += gamma[e] * b[e];
-      sum.b += gamma[e] * g[e];
       be[e] += b[e];
       ga[e] += g[e];
+      b[e] *= gamma[e];
+      g[e] *= gamma[e];
     }
     if (!p.dx) continue;
-    parts[threadIdx.x] = sum;
+    if (l.in) put_entries<VE, GEN>(parts + l.tr * wide + l.tc * N, entry_sums<VE, GEN>(b, g), l.x);
     __syncthreads();
     const float total = fmaxf((float)w.count * (float)p.per, 1.0f);
     each_group<kThreads>(threadIdx.x, groups, p.lanes, [&](int q, int lane, bool in) {
-      float x = 0.0f, y = 0.0f;
-      for (int k = lane; k < l.TR * p.chunks_per; k += 1 << p.lanes) {
-        const int tr = k / p.chunks_per;
-        const Pair v = parts[tr * p.part + q * p.chunks_per + k - tr * p.chunks_per];
-        x += v.a;
-        y += v.b;
+      float a = 0.0f, c = 0.0f;
+      for (int k = lane; k < l.TR * p.group_entries; k += 1 << p.lanes) {
+        const int tr = k / p.group_entries;
+        const Pair u = parts[tr * wide + q * p.group_entries + k - tr * p.group_entries];
+        a += u.a;
+        c += u.b;
       }
-      x = sum_lanes(x, p.lanes);
-      y = sum_lanes(y, p.lanes);
-      if (in && lane == 0) whole[q] = Pair{x / total, y / total};
+      a = sum_lanes(a, p.lanes);
+      c = sum_lanes(c, p.lanes);
+      if (in && lane == 0) whole[q] = Pair{a / total, c / total};
     });
     __syncthreads();
     if (l.in) {
-      const Pair q = whole[l.tc / p.chunks_per];
+      const Entries<VE, GEN> means = of_groups<VE, GEN>(whole, Cols{l.x.c - l.c0, l.x.count}, p.per);
 #pragma unroll
       for (int i = 0; i < kHold; ++i)
         if (i < have) {
-          dx_vec<VE>(s.b, q, v[i], d[i]);
-          store_vec<KIND, VE>(static_cast<E*>(p.dx) + (w.first + l.tr + (long)i * l.TR) * p.ld_x + (long)chunk * VE, d[i]);
+          dx_vec<VE, GEN>(s, means, v[i], d[i]);
+          store_out<KIND, VE, GEN, ONCE>(static_cast<E*>(p.dx) + (w.first + l.tr + (long)i * l.TR) * p.ld_x + l.x.c, d[i],
+                                   l.x);
         }
-      thread_dx<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, kHold, s, q, gamma, beta);
+      thread_dx<KIND, VE, GEN, KEPT, ONCE>(p, w.first, w.count, l, kHold, s, means, gamma, beta);
     }
     __syncthreads();
   }
-  if (!p.partial) return;
-  float* out = p.partial + (long)blockIdx.y * 2 * p.channels + (long)c0 * VE;
-  for (int which = 0; which < 2; ++which) {
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < VE; ++e) sums[threadIdx.x * VE + e] = which ? be[e] : ga[e];
-    __syncthreads();
-    for (int c = threadIdx.x; c < cols * VE; c += kThreads) {
-      float v = 0.0f;
-      for (int m = 0; m < l.TR; ++m) v += sums[m * p.part * VE + c];
-      out[which * p.channels + c] = v;
-    }
-  }
+  if (p.partial) put_channel_sums<VE>(p, l, ga, be, sums, p.partial + (long)blockIdx.y * 2 * p.channels);
 }
 
 // ---- frames cut into slices --------------------------------------------------------------------
@@ -773,28 +892,64 @@ __device__ __forceinline__ Frame slice_of(const Frame& w, int z, int slices) {
   return Frame{w.first + (long)each * z + min(z, more), each + (z < more)};
 }
 
-// Moments of each chunk over a slice: pairs [frames][slices][chunks]. Grid (parts, slices, frames).
-template <int KIND, int VE>
+// The groups that a part of the columns meets (the first and the last one may go on beyond it), and
+// where their sums of a slice are: pairs [frames][slices][parts][part_groups].
+struct PartGroups {
+  int first, count;
+};
+__device__ __forceinline__ PartGroups groups_of(const NormArgs& p, const Lay& l) {
+  const int q = l.c0 / p.per;
+  return PartGroups{q, (l.c0 + l.channels - 1) / p.per - q + 1};
+}
+__device__ __forceinline__ Pair* slice_pairs(const NormArgs& p, int f, int z, int part) {
+  return reinterpret_cast<Pair*>(p.pairs) + (((long)f * p.slices + z) * p.parts + part) * p.part_groups;
+}
+// f(group's place in the part, its first entry there, the one past its last, lane, whether there is such a group)
+template <class F>
+__device__ __forceinline__ void each_part_group(const NormArgs& p, const Lay& l, int W, F&& f) {
+  const PartGroups g = groups_of(p, l);
+  each_group<kThreads>(threadIdx.x, g.count, p.lanes, [&](int k, int lane, bool in) {
+    const int a = max((g.first + k) * p.per - l.c0, 0), b = min((g.first + k + 1) * p.per - l.c0, l.channels);
+    f(k, a / W, b / W, lane, in);
+  });
+}
+
+// Moments of each group over a slice, or of its channels in this part. Grid (parts, slices, frames).
+template <int KIND, int VE, bool GEN>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(const NormArgs p) {
-  __shared__ Pair parts[kThreads];
-  const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0);
-  const Lay l = lay_of(p.part, cols);
+  constexpr int N = entries_of<VE, GEN>(), W = VE / N;
+  __shared__ Pair parts[kThreads * N];
+  const Lay l = lay_of<VE>(p);
+  const int wide = p.part * N, entries = (l.channels + W - 1) / W;
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
     const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
-    Pair mine = {0.0f, 0.0f};
-    if (l.in) thread_moments<KIND, VE>(p, w.first, w.count, c0 + l.tc, l, 0, mine);
-    parts[threadIdx.x] = mine;
+    Entries<VE, GEN> mine{};
+    if (l.in) {
+      thread_moments<KIND, VE, GEN>(p, w.first, w.count, l, 0, mine);
+      put_entries<VE, GEN>(parts + l.tr * wide + l.tc * N, mine, l.x);
+    }
     __syncthreads();
-    if ((int)threadIdx.x < cols) {
-      Pair s = parts[threadIdx.x];
+    for (int k = threadIdx.x; k < entries; k += kThreads) {
+      Pair s = parts[k];
       int have = rows_of(w.count, 0, l.TR);
       for (int tr = 1; tr < l.TR; ++tr) {
-        const int k = rows_of(w.count, tr, l.TR);
-        if (k) join_moments(s, (float)(have * VE), parts[tr * p.part + threadIdx.x], (float)(k * VE));
-        have += k;
+        const int n = rows_of(w.count, tr, l.TR);
+        if (n) join_moments(s, (float)(have * W), parts[tr * wide + k], (float)(n * W));
+        have += n;
       }
-      *reinterpret_cast<Pair*>(p.pairs + 2 * (((long)f * p.slices + blockIdx.y) * p.chunks + c0 + threadIdx.x)) = s;
+      parts[k] = s;
     }
+    __syncthreads();
+    Pair* out = slice_pairs(p, f, blockIdx.y, blockIdx.x);
+    each_part_group(p, l, W, [&](int q, int e0, int e1, int lane, bool in) {
+      float m = 0.0f, M = 0.0f;
+      for (int k = e0 + lane; k < e1; k += 1 << p.lanes) m += parts[k].a;
+      m = sum_lanes(m, p.lanes) / (float)(e1 - e0);
+      const float each = (float)(w.count * W);
+      for (int k = e0 + lane; k < e1; k += 1 << p.lanes) M += parts[k].b + each * (parts[k].a - m) * (parts[k].a - m);
+      M = sum_lanes(M, p.lanes);
+      if (in && lane == 0) out[q] = Pair{m, M};
+    });
     __syncthreads();
   }
 }
@@ -807,34 +962,50 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
+// The parts and slices that a group's sums come from: part p0 + k % parts, slice k / parts.
+struct GroupSums {
+  int p0, parts;
+  unsigned n;
+  __device__ __forceinline__ GroupSums(const NormArgs& p, int q) {
+    p0 = q * p.per / p.part_channels;
+    parts = ((q + 1) * p.per - 1) / p.part_channels - p0 + 1;
+    n = (unsigned)p.slices * parts;
+  }
+  // (and how many of the group's channels are in the part)
+  __device__ __forceinline__ Pair get(const NormArgs& p, int f, int q, unsigned k, int& z, int& channels) const {
+    z = (int)(k / (unsigned)parts);
+    const int part = p0 + (int)(k - (unsigned)z * parts), c0 = part * p.part_channels;
+    channels = min((q + 1) * p.per, c0 + p.part_channels) - max(q * p.per, c0);
+    return slice_pairs(p, f, z, part)[q - c0 / p.per];
+  }
+};
+
 // The slices' moments of each (frame, group) joined, in fp64: a block each.
-template <int VE>
 __global__ __launch_bounds__(kThreads) void k_norm_stats_join(const NormArgs p) {
   __shared__ double lds[4];
   const long all = (long)p.frames * p.groups;
   for (long at = blockIdx.x; at < all; at += gridDim.x) {
     const int f = (int)(at / p.groups), q = (int)(at % p.groups);
     const Frame w = frame_of(p, f);
-    const float* s = p.pairs + 2 * ((long)f * p.slices * p.chunks + (long)q * p.chunks_per);
-    const unsigned per = p.chunks_per, n = (unsigned)p.slices * per;
-    // an entry's moments, and how many values it stands for
+    const GroupSums sums(p, q);
+    // a part's moments, and how many values it stands for
     auto entry = [&](unsigned k, Pair& e) {
-      const unsigned z = k / per;
-      e = *reinterpret_cast<const Pair*>(s + 2 * ((long)z * p.chunks + (k - z * per)));
-      return (double)(slice_of(w, z, p.slices).count * VE);
+      int z, channels;
+      e = sums.get(p, f, q, k, z, channels);
+      return (double)slice_of(w, z, p.slices).count * channels;
     };
     // one pass, around the first part's mean (in fp64, and the parts' means lie together)
     Pair first;
     entry(0, first);
-    constexpr int kUnder = 8;
+    constexpr int kUnder = 4;
     double d = 0.0, M = 0.0;
-    for (unsigned k = threadIdx.x; k < n; k += kUnder * kThreads) {
+    for (unsigned k = threadIdx.x; k < sums.n; k += kUnder * kThreads) {
       Pair e[kUnder];
       double count[kUnder];
 #pragma unroll
       for (int u = 0; u < kUnder; ++u) {
-        count[u] = entry(min(k + u * kThreads, n - 1), e[u]);
-        if (k + u * kThreads >= n) count[u] = 0.0, e[u].b = 0.0f;
+        count[u] = entry(min(k + u * kThreads, sums.n - 1), e[u]);
+        if (k + u * kThreads >= sums.n) count[u] = 0.0;
       }
 #pragma unroll
       for (int u = 0; u < kUnder; ++u) {
@@ -854,73 +1025,71 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_join(const NormArgs p) 
   }
 }
 
-template <int KIND, int VE>
+// (The output's slices from the last one on: what the sums' pass has read last is in the last cache yet.)
+template <int KIND, int VE, bool GEN, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(const NormArgs p) {
-  const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0);
-  const Lay l = lay_of(p.part, cols);
+  const Lay l = lay_of<VE>(p);
   if (!l.in) return;
-  const int chunk = c0 + l.tc;
   float gamma[VE], beta[VE];
-  load_affine<KIND, VE>(p, chunk, gamma, beta);
+  load_affine<KIND, VE, GEN>(p, l.x, gamma, beta);
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
     const Frame w = slice_of(frame_of(p, f), gridDim.y - 1 - blockIdx.y, gridDim.y);
-    const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * ((long)f * p.groups + chunk / p.chunks_per));
     float scale[VE], shift[VE];
-    scale_shift<VE>(s, gamma, beta, scale, shift);
-    thread_apply<KIND, VE>(p, w.first, w.count, chunk, l, 0, scale, shift);
+    scale_shift<VE, GEN>(of_groups<VE, GEN>(reinterpret_cast<const Pair*>(p.stats + 2 * (long)f * p.groups), l.x, p.per),
+                         gamma, beta, scale, shift);
+    thread_apply<KIND, VE, GEN, ONCE>(p, w.first, w.count, l, 0, scale, shift);
   }
 }
 
-// Sums of w and w v over a slice for each chunk: pairs [frames][slices][chunks]. dgamma and dbeta over all frames
+// Sums of w and w v over a slice for each group, or its channels in this part. dgamma and dbeta over all frames
 // that a block takes: partial [gridDim.z][slices][2][channels].
-template <int KIND, int VE, bool KEPT>
+template <int KIND, int VE, bool GEN, bool KEPT>
 __global__ __launch_bounds__(kThreads) void k_norm_sums(const NormArgs p) {
-  __shared__ Pair parts[kThreads];
+  constexpr int N = entries_of<VE, GEN>(), W = VE / N;
+  __shared__ Pair parts[kThreads * N];
   __shared__ float sums[kThreads * VE];
-  const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0);
-  const Lay l = lay_of(p.part, cols);
-  const int chunk = c0 + min(l.tc, cols - 1);
+  const Lay l = lay_of<VE>(p);
+  const int wide = p.part * N, entries = (l.channels + W - 1) / W;
   float gamma[VE], beta[VE], ga[VE] = {}, be[VE] = {};
-  load_affine<KIND, VE>(p, chunk, gamma, beta);
+  load_affine<KIND, VE, GEN>(p, l.x, gamma, beta);
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
     const Frame w = slice_of(frame_of(p, f), blockIdx.y, p.slices);
-    const Pair s = *reinterpret_cast<const Pair*>(p.stats + 2 * ((long)f * p.groups + chunk / p.chunks_per));
+    const Entries<VE, GEN> s =
+        of_groups<VE, GEN>(reinterpret_cast<const Pair*>(p.stats + 2 * (long)f * p.groups), l.x, p.per);
     float b[VE] = {}, g[VE] = {};
-    if (l.in) thread_sums<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, 0, s, gamma, beta, b, g);
-    Pair sum = {0.0f, 0.0f};
+    if (l.in) thread_sums<KIND, VE, GEN, KEPT>(p, w.first, w.count, l, 0, s, gamma, beta, b, g);
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      sum.a += gamma[e] * b[e];
-      sum.b += gamma[e] * g[e];
       be[e] += b[e];
       ga[e] += g[e];
+      b[e] *= gamma[e];
+      g[e] *= gamma[e];
     }
     if (!p.dx) continue;
     __syncthreads();
-    parts[threadIdx.x] = sum;
+    if (l.in) put_entries<VE, GEN>(parts + l.tr * wide + l.tc * N, entry_sums<VE, GEN>(b, g), l.x);
     __syncthreads();
-    if ((int)threadIdx.x < cols) {
+    for (int k = threadIdx.x; k < entries; k += kThreads) {
+      Pair sum = parts[k];
       for (int tr = 1; tr < l.TR; ++tr) {
-        const Pair q = parts[tr * p.part + threadIdx.x];
+        const Pair q = parts[tr * wide + k];
         sum.a += q.a;
         sum.b += q.b;
       }
-      *reinterpret_cast<Pair*>(p.pairs + 2 * (((long)f * p.slices + blockIdx.y) * p.chunks + chunk)) = sum;
+      parts[k] = sum;
     }
-  }
-  if (!p.partial) return;
-  float* out = p.partial + ((long)blockIdx.z * p.slices + blockIdx.y) * 2 * p.channels + (long)c0 * VE;
-  for (int which = 0; which < 2; ++which) {
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < VE; ++e) sums[threadIdx.x * VE + e] = which ? be[e] : ga[e];
-    __syncthreads();
-    for (int c = threadIdx.x; c < cols * VE; c += kThreads) {
-      float v = 0.0f;
-      for (int m = 0; m < l.TR; ++m) v += sums[m * p.part * VE + c];
-      out[which * p.channels + c] = v;
-    }
+    Pair* out = slice_pairs(p, f, blockIdx.y, blockIdx.x);
+    each_part_group(p, l, W, [&](int q, int e0, int e1, int lane, bool in) {
+      float a = 0.0f, c = 0.0f;
+      for (int k = e0 + lane; k < e1; k += 1 << p.lanes) a += parts[k].a, c += parts[k].b;
+      a = sum_lanes(a, p.lanes);
+      c = sum_lanes(c, p.lanes);
+      if (in && lane == 0) out[q] = Pair{a, c};
+    });
   }
+  if (p.partial)
+    put_channel_sums<VE>(p, l, ga, be, sums, p.partial + ((long)blockIdx.z * p.slices + blockIdx.y) * 2 * p.channels);
 }
 
 // The slices' (or blocks') sums joined in fp64. The first `group_blocks` blocks: means of w and w v for each
@@ -933,13 +1102,12 @@ __global__ __launch_bounds__(kThreads) void k_norm_sums_join(const NormArgs p, i
     const long all = (long)p.frames * p.groups;
     for (long at = blockIdx.x; at < all; at += group_blocks) {
       const int f = (int)(at / p.groups), q = (int)(at % p.groups);
-      const float* s = p.pairs + 2 * ((long)f * p.slices * p.chunks + (long)q * p.chunks_per);
+      const GroupSums sums(p, q);
       double a = 0.0, b = 0.0;
-      const unsigned per = p.chunks_per, n = (unsigned)p.slices * per;
 #pragma unroll 4
-      for (unsigned k = threadIdx.x; k < n; k += kThreads) {
-        const unsigned z = k / per;
-        const Pair e = *reinterpret_cast<const Pair*>(s + 2 * ((long)z * p.chunks + (k - z * per)));
+      for (unsigned k = threadIdx.x; k < sums.n; k += kThreads) {
+        int z, channels;
+        const Pair e = sums.get(p, f, q, k, z, channels);
         a += e.a;
         b += e.b;
       }
@@ -982,55 +1150,63 @@ __global__ __launch_bounds__(kThreads) void k_norm_sums_join(const NormArgs p, i
   if (p.dbeta) static_cast<E*>(p.dbeta)[c] = from_f32<KIND>((float)a);
 }
 
-template <int KIND, int VE, bool KEPT>
+template <int KIND, int VE, bool GEN, bool KEPT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_dx(const NormArgs p) {
-  const int c0 = blockIdx.x * p.part, cols = min(p.part, p.chunks - c0);
-  const Lay l = lay_of(p.part, cols);
+  const Lay l = lay_of<VE>(p);
   if (!l.in) return;
-  const int chunk = c0 + l.tc;
   float gamma[VE], beta[VE];
-  load_affine<KIND, VE>(p, chunk, gamma, beta);
+  load_affine<KIND, VE, GEN>(p, l.x, gamma, beta);
   for (int f = blockIdx.z; f < p.frames; f += gridDim.z) {
     const Frame w = slice_of(frame_of(p, f), gridDim.y - 1 - blockIdx.y, gridDim.y);
-    const long at = 2 * ((long)f * p.groups + chunk / p.chunks_per);
-    thread_dx<KIND, VE, KEPT>(p, w.first, w.count, chunk, l, 0, *reinterpret_cast<const Pair*>(p.stats + at),
-                              *reinterpret_cast<const Pair*>(p.sums + at), gamma, beta);
+    const long at = 2 * (long)f * p.groups;
+    thread_dx<KIND, VE, GEN, KEPT, ONCE>(
+        p, w.first, w.count, l, 0, of_groups<VE, GEN>(reinterpret_cast<const Pair*>(p.stats + at), l.x, p.per),
+        of_groups<VE, GEN>(reinterpret_cast<const Pair*>(p.sums + at), l.x, p.per), gamma, beta);
   }
 }
 
 // ---- launches ---------------------------------------------------------------------------------
+// channels of a thread, and whether groups are anything but multiples of them
 template <class F>
-void by_vec(int vec, F&& f) {
-  if constexpr (ELEM_KIND != kF32)
-    if (vec == 8) return f(std::integral_constant<int, 8>{});
-  if constexpr (ELEM_KIND == kF32)
-    if (vec == 4) return f(std::integral_constant<int, 4>{});
-  if (vec == 2) return f(std::integral_constant<int, 2>{});
-  f(std::integral_constant<int, 1>{});
+void by_vec(const NormArgs& p, F&& f) {
+  using std::integral_constant;
+  constexpr int kMost = ELEM_KIND == kF32 ? 4 : 8;
+  if (p.vec == 1)
+    f(integral_constant<int, 1>{}, std::false_type{});
+  else if (p.general)
+    f(integral_constant<int, kMost>{}, std::true_type{});
+  else
+    f(integral_constant<int, kMost>{}, std::false_type{});
 }
-// threads of a row, chunks of a thread, and whether groups are lanes
 template <class F>
+void with(bool b, F&& f) {
+  if (b)
+    f(std::true_type{});
+  else
+    f(std::false_type{});
+}
+// threads of a row, vectors of a thread, and whether groups are lanes
+template <bool GEN, class F>
 void by_row(const NormArgs& p, F&& f) {
   using std::integral_constant;
   auto lanes = [&](auto t, auto c) {
-    if (p.by_lanes)
-      f(t, c, std::true_type{});
-    else
-      f(t, c, std::false_type{});
+    if constexpr (!GEN)
+      if (p.by_lanes) return f(t, c, std::true_type{});
+    f(t, c, std::false_type{});
   };
-  if (p.chunks <= 16)
+  if (p.vecs <= 16)
     lanes(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-  else if (p.chunks <= 64)
+  else if (p.vecs <= 64)
     lanes(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  else if (p.chunks <= 256)
+  else if (p.vecs <= 256)
     lanes(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  else if (p.chunks <= 512)
+  else if (p.vecs <= 512)
     lanes(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  else
+  else if constexpr (!GEN || ELEM_KIND == kF32)
     lanes(integral_constant<int, 256>{}, integral_constant<int, 4>{});
 }
-size_t row_lds(const NormArgs& p, int T, int VE, bool grad) {
-  const size_t parts = (size_t)(kThreads / T) * (p.chunks + p.groups) * sizeof(Pair);
+size_t row_lds(const NormArgs& p, int T, int VE, bool grad, bool lanes) {
+  const size_t parts = lanes ? 0 : (size_t)(kThreads / T) * (p.entries + p.groups) * sizeof(Pair);
   return grad ? std::max(parts, (size_t)kThreads * VE * sizeof(float)) : parts;
 }
 dim3 frame_grid(const NormArgs& p) { return dim3(p.parts, std::min(p.frames, p.blocks)); }
@@ -1043,26 +1219,28 @@ constexpr int kGrid = 65535;
 template <>
 void norm_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
   constexpr int KIND = ELEM_KIND;
-  by_vec(p.vec, [&](auto ve) {
+  auto launch = [&](auto ve, auto gen, auto past) {
     constexpr int VE = decltype(ve)::value;
+    constexpr bool GEN = decltype(gen)::value, ONCE = decltype(past)::value;
     if (p.form == kNormRows) {
-      by_row(p, [&](auto t, auto c, auto lanes) {
+      by_row<GEN>(p, [&](auto t, auto c, auto lanes) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         constexpr bool LANES = decltype(lanes)::value;
-        hipLaunchKernelGGL((k_norm_rows<KIND, VE, T, C, LANES>), dim3(p.blocks), dim3(kThreads),
-                           LANES ? 0 : row_lds(p, T, VE, false), st, p);
+        hipLaunchKernelGGL((k_norm_rows<KIND, VE, GEN, T, C, LANES, ONCE>), dim3(p.blocks), dim3(kThreads),
+                           row_lds(p, T, VE, false, LANES), st, p);
       });
     } else if (p.form == kNormFrames) {
-      hipLaunchKernelGGL((k_norm_frames<KIND, VE>), frame_grid(p), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_frames<KIND, VE, GEN, ONCE>), frame_grid(p), dim3(kThreads), 0, st, p);
     } else {
-      hipLaunchKernelGGL((k_norm_stats<KIND, VE>), slice_grid(p, kGrid), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_stats<KIND, VE, GEN>), slice_grid(p, kGrid), dim3(kThreads), 0, st, p);
       DPAMD_LAUNCH_CHECK();
       const long all = (long)p.frames * p.groups;
-      hipLaunchKernelGGL((k_norm_stats_join<VE>), dim3((unsigned)std::min(all, 1L << 20)), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL(k_norm_stats_join, dim3((unsigned)std::min(all, 1L << 20)), dim3(kThreads), 0, st, p);
       DPAMD_LAUNCH_CHECK();
-      hipLaunchKernelGGL((k_norm_apply<KIND, VE>), out_grid(p), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_apply<KIND, VE, GEN, ONCE>), out_grid(p), dim3(kThreads), 0, st, p);
     }
-  });
+  };
+  by_vec(p, [&](auto ve, auto gen) { with(p.once, [&](auto past) { launch(ve, gen, past); }); });
   DPAMD_LAUNCH_CHECK();
 }
 
@@ -1070,24 +1248,24 @@ template <>
 void norm_grad_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
   constexpr int KIND = ELEM_KIND;
   const int channel_blocks = p.dgamma || p.dbeta ? (p.channels + 15) / 16 : 0;
-  auto launch = [&](auto ve, auto kept) {
+  auto launch = [&](auto ve, auto gen, auto kept, auto past) {
     constexpr int VE = decltype(ve)::value;
-    constexpr bool KEPT = decltype(kept)::value;
+    constexpr bool GEN = decltype(gen)::value, KEPT = decltype(kept)::value, ONCE = decltype(past)::value;
     int group_blocks = 0;
     long parts = 0;
     if (p.form == kNormRows) {
-      by_row(p, [&](auto t, auto c, auto lanes) {
+      by_row<GEN>(p, [&](auto t, auto c, auto lanes) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         constexpr bool LANES = decltype(lanes)::value;
-        hipLaunchKernelGGL((k_norm_rows_grad<KIND, VE, T, C, LANES, KEPT>), dim3(p.blocks), dim3(kThreads),
-                           row_lds(p, T, VE, true), st, p);
+        hipLaunchKernelGGL((k_norm_rows_grad<KIND, VE, GEN, T, C, LANES, KEPT, ONCE>), dim3(p.blocks), dim3(kThreads),
+                           row_lds(p, T, VE, true, LANES), st, p);
       });
       parts = p.blocks;
     } else if (p.form == kNormFrames) {
-      hipLaunchKernelGGL((k_norm_frames_grad<KIND, VE, KEPT>), frame_grid(p), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_frames_grad<KIND, VE, GEN, KEPT, ONCE>), frame_grid(p), dim3(kThreads), 0, st, p);
       parts = frame_grid(p).y;
     } else {
-      hipLaunchKernelGGL((k_norm_sums<KIND, VE, KEPT>), slice_grid(p, p.blocks), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_sums<KIND, VE, GEN, KEPT>), slice_grid(p, p.blocks), dim3(kThreads), 0, st, p);
       parts = (long)slice_grid(p, p.blocks).z * p.slices;
       if (p.dx) group_blocks = (int)std::min((long)p.frames * p.groups, 1L << 20);
     }
@@ -1098,15 +1276,12 @@ void norm_grad_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
       DPAMD_LAUNCH_CHECK();
     }
     if (p.form == kNormSlices && p.dx) {
-      hipLaunchKernelGGL((k_norm_dx<KIND, VE, KEPT>), out_grid(p), dim3(kThreads), 0, st, p);
+      hipLaunchKernelGGL((k_norm_dx<KIND, VE, GEN, KEPT, ONCE>), out_grid(p), dim3(kThreads), 0, st, p);
       DPAMD_LAUNCH_CHECK();
     }
   };
-  by_vec(p.vec, [&](auto ve) {
-    if (p.kept)
-      launch(ve, std::true_type{});
-    else
-      launch(ve, std::false_type{});
+  by_vec(p, [&](auto ve, auto gen) {
+    with(p.kept != nullptr, [&](auto kept) { with(p.once, [&](auto past) { launch(ve, gen, kept, past); }); });
   });
 }
 
