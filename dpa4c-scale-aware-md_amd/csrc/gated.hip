@@ -48,25 +48,35 @@ __global__ __launch_bounds__(256) void k_zero(unsigned char* dst, long rows, lon
 
 // One step (128 bytes of k) of one block, measured: its share of a compute unit's time
 // among others, and its time alone; what a tile's epilogue adds (a plain store, the gate, the gate's
-// gradient); and the blocks that a compute unit holds. Measured with each shape forced, every
+// gradient, the gate with its gradient, the same with few outputs); and the blocks that a compute unit holds. Measured with each shape forced, every
 // product of training steps of ten sizes, 33 to 131,072 rows: the one picked here took within 6 % of
 // the best one's time but for eleven of 108, of which the worst took 24 % more. (fp32: the
 // matrix cores are slow enough that 256 x 256 tiles gain nothing over 128 x 128. 16 bits: 128 x 32
 // was nowhere ahead of both neighbours.)
 struct TileShape {
   int bm, bn, per_cu;
-  double share_us, alone_us, end_us[3];
+  double share_us, alone_us, end_us[5];
 };
-const TileShape kShapes[2][5] = {{{256, 256, 1, 1.8, 1.8, {14, 24, 66}},
-                                {128, 128, 2, 0.62, 1.0, {5, 8, 23}},
-                                {64, 128, 3, 0.40, 0.9, {2.2, 3.2, 7}},
+int end_of(ProductKind what) {
+  switch (what) {
+    case kProdGate: return 1;
+    case kProdGateGrad: return 2;
+    case kProdGateBack: return 3;
+    case kProdGateOuts:
+    case kProdGateOne: return 4;
+    default: return 0;
+  }
+}
+const TileShape kShapes[2][5] = {{{256, 256, 1, 1.8, 1.8, {14, 24, 66, 23, 24}},
+                                {128, 128, 2, 0.62, 1.0, {5, 8, 23, 6, 8}},
+                                {64, 128, 3, 0.40, 0.9, {2.2, 3.2, 7, 3.6, 3.2}},
                                 {},
-                                {64, 32, 6, 0.22, 0.55, {0.7, 1, 1.5}}},
+                                {64, 32, 6, 0.22, 0.55, {0.7, 1, 1.5, 1, 1}}},
                                {{},
-                                {128, 128, 2, 2.05, 2.26, {5, 8, 23}},
-                                {64, 128, 3, 1.05, 1.27, {2.2, 3.2, 7}},
-                                {128, 32, 4, 0.575, 0.75, {1.5, 1.5, 3.5}},
-                                {64, 32, 6, 0.33, 0.5, {0.7, 1, 1.5}}}};
+                                {128, 128, 2, 2.05, 2.26, {5, 8, 23, 8, 8}},
+                                {64, 128, 3, 1.05, 1.27, {2.2, 3.2, 7, 3.9, 3.2}},
+                                {128, 32, 4, 0.575, 0.75, {1.5, 1.5, 3.5, 2.3, 1.5}},
+                                {64, 32, 6, 0.33, 0.5, {0.7, 1, 1.5, 1.4, 1}}}};
 
 // (a grid holds fewer than 2^32 threads: the kernels stride over what is beyond)
 unsigned blocks_for(long threads) { return (unsigned)std::min((threads + 255) / 256, 1L << 20); }
@@ -91,13 +101,14 @@ void fill_zero(hipStream_t st, void* dst, long rows, long row_bytes, long stride
 }
 
 ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int segs, int mats, int ncu) {
-  const int sub = what == kProdGate || what == kProdGateBack || what == kProdGateOuts ? 2 : 1, bk = elem == kF32 ? 32 : elem == kI8 ? 128 : 64;
+  const int sub = what == kProdDown || what == kProdGateGrad || what == kProdInput || what == kProdWeight ? 1 : 2, bk = elem == kF32 ? 32 : elem == kI8 ? 128 : 64;
   ProductPlan best{};
   double best_us = 0;
   const long steps = (K + bk - 1) / bk * segs;
   for (int k = 0; k < 5; ++k) {
     const TileShape& s = kShapes[elem == kF32][k];
-    if (!s.bm) continue;
+    // (two to four outputs' sums take the 128 x 128 tile's second block of a compute unit: 385 us so 322)
+    if (!s.bm || (what == kProdGateOuts && s.bm == 128 && s.bn == 128)) continue;
     // (k-strided tiles of 32 columns have too few banks apart)
     const double share = s.share_us * (what == kProdWeight && s.bn == 32 ? 1.3 : 1.0);
     const long tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn / sub - 1) / (s.bn / sub)) * mats;
@@ -106,7 +117,7 @@ ProductPlan plan_product(ProductKind what, int elem, long M, long N, long K, int
     for (long split = 1; split <= most; split = split < 4 ? split + 1 : split + split / 4) {
       const long items = tiles * split, a_cu = (items + ncu - 1) / ncu, rounds = (items + slots - 1) / slots;
       const double bytes = split > 1 ? 4.0 * split * sub * mats * M * ((N + 7) / 8 * 8) : 0;
-      const double end = s.end_us[split > 1 ? 0 : what == kProdGate || what == kProdGateOuts ? 1 : what == kProdGateGrad || what == kProdGateBack ? 2 : 0];
+      const double end = s.end_us[split > 1 ? 0 : end_of(what)];
       const double us = (double)((steps + split - 1) / split) * std::max(a_cu * share, rounds * s.alone_us) +
                         a_cu * end + 2.0 + (split > 1 ? 4 + 2 * bytes / 4e6 : 0);
       if (best_us == 0 || us < best_us) {

@@ -60,7 +60,7 @@ ProductPlan plan_gate_back(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdGateBack, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
 }
 ProductPlan plan_gate_outs(const dp_gated_shape& s, int ncu) {
-  return plan_product(kProdGateOuts, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
+  return plan_product(s.d_out == 1 ? kProdGateOne : kProdGateOuts, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
 }
 ProductPlan plan_input(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdInput, elem_of(s.type), s.rows, s.d_in, s.d_hidden, 2, 1, ncu);
@@ -212,7 +212,7 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
       a.epi.wd = wd, a.epi.ld_down = s.ld_down;
       a.epi.outs = s.d_out;
       a.epi.outs_partial = dwd ? part : nullptr;
-      run_product(st, kProdGateOuts, elem, p0, a);
+      run_product(st, s.d_out == 1 ? kProdGateOne : kProdGateOuts, elem, p0, a);
       q.dwd = dwd;
       q.partial = part;
       if (dwd) run_outs_join(st, elem, q);

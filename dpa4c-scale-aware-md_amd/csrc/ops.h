@@ -12,8 +12,10 @@ namespace dpamd {
 // activations, with the codes of the model files
 enum { kActTanh = 0, kActSilu = 1, kActGelu = 2, kActNone = 3 };
 
+constexpr int kFewOutputs = 4;
+
 // ---- tile products (product.h) ----
-enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2, kEpiScale = 3, kEpiScaleGate = 4, kEpiGateBack = 5, kEpiGateOuts = 6 };
+enum { kEpiStore = 0, kEpiGate = 1, kEpiGateGrad = 2, kEpiScale = 3, kEpiScaleGate = 4, kEpiGateBack = 5, kEpiGateOuts = 6, kEpiGateOne = 7 };
 
 // An operand of the products, of the call's type: 16-byte aligned, rows of whole 16-byte
 // chunks (ld elements), and the contiguous side ends with a chunk or is followed by zeros up to one.
@@ -79,7 +81,8 @@ enum ProductKind {
   kProdGateGrad,  // dy Wd^T -> dg, du, h               both k-contiguous
   kProdInput,     // dg Wg^T + du Wu^T -> dx            both k-contiguous
   kProdGateBack,  // x Wg, x Wu and dh -> dg, du, h     rows k-contiguous by columns
-  kProdGateOuts,  // the same with up to four outputs
+  kProdGateOuts,  // the same with two to four outputs
+  kProdGateOne,   // and with one
   kProdWeight     // x^T dg, x^T du;  h^T dy            both k-strided
 };
 
@@ -108,7 +111,6 @@ size_t plan_rows(int elem, int ncu, RowsArgs& args);  // bytes of the partial su
 void run_rows(hipStream_t st, int elem, RowsArgs& args);
 
 // ---- the block's down side for few outputs (gated_outs.hip) ----
-constexpr int kFewOutputs = 4;
 struct OutsArgs {
   long rows;
   int f, o, act;

@@ -582,7 +582,7 @@ struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
 };
 
-// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad, kEpiGateBack, kEpiGateOuts (two); of 8-bit
+// EPI: kEpiStore, kEpiGate (two B matrices, BN / 2 columns of each), kEpiGateGrad, kEpiGateBack, kEpiGateOuts, kEpiGateOne (two); of 8-bit
 // integers kEpiScale, kEpiScaleGate (two).
 //
 // A block takes tiles (and slices of K) one after another; the first two steps of the next one are
@@ -602,7 +602,11 @@ struct Shape {
 // instead of two changed nothing).
 template <int KIND, int LA, int LB, int EPI, class S>
 __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs p) {
-  constexpr int SUB = EPI == kEpiGate || EPI == kEpiScaleGate || EPI == kEpiGateBack || EPI == kEpiGateOuts ? 2 : 1, EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
+  constexpr int SUB = EPI == kEpiGate || EPI == kEpiScaleGate || EPI == kEpiGateBack ||
+                              EPI == kEpiGateOuts || EPI == kEpiGateOne
+                          ? 2
+                          : 1,
+                EB = sizeof(typename ElemOf<KIND>::T), BK = 128 / EB;
   using T = typename ElemOf<KIND>::T;
   constexpr int WAVES = S::WM * S::WN, TM = S::BM / S::WM, TN = S::BN / S::WN;
   constexpr int MI = TM / 16, NJ = TN / 16;
@@ -927,18 +931,18 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
         rows(std::true_type{});
       else
         rows(std::false_type{});
-    } else if constexpr (EPI == kEpiGateOuts) {
+    } else if constexpr (EPI == kEpiGateOuts || EPI == kEpiGateOne) {
       // dh from a few outputs' dy, here, and h dy summed over the wave's rows: neither g and u nor h meet
       // memory. (31,920 rows of 70-96-1 in fp32: XXX)
-      constexpr int NG = NJ / SUB;
-      const int outs = p.epi.outs;
-      float w[NG][4][kFewOutputs], sum[NG][4][kFewOutputs] = {};
+      constexpr int NG = NJ / SUB, O = EPI == kEpiGateOne ? 1 : kFewOutputs;
+      const int outs = O == 1 ? 1 : p.epi.outs;
+      float w[NG][4][O], sum[NG][4][O] = {};
 #pragma unroll
       for (int j = 0; j < NG; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int k = 0; k < kFewOutputs; ++k) {
+          for (int k = 0; k < O; ++k) {
             const int n = n0 + j * 16 + e;
             w[j][e][k] = k < outs && n < p.N
                              ? to_f32<KIND>(static_cast<const T*>(p.epi.wd)[n * p.epi.ld_down + k])
@@ -949,15 +953,15 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
       for (int i = 0; i < MI; ++i, at += 16 * p.epi.ldh) {
         const int m = m0 + i * 16;
         const bool there = m < p.M;
-        float dy[kFewOutputs];
+        float dy[O];
 #pragma unroll
-        for (int k = 0; k < kFewOutputs; ++k)
+        for (int k = 0; k < O; ++k)
           dy[k] = there && k < outs ? to_f32<KIND>(static_cast<const T*>(p.epi.dy)[m * p.epi.ld_dy + k]) : 0.0f;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
           f4 dh = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int k = 0; k < kFewOutputs; ++k)
+          for (int k = 0; k < O; ++k)
             if (k < outs)
 #pragma unroll
               for (int e = 0; e < 4; ++e) dh[e] += dy[k] * w[j][e][k];
@@ -965,7 +969,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
               gate_grad<false>(p.act, p.N - n0 - j * 16, dh, Kept{acc[i][j], acc[i][j + NG]});
           if (!there) continue;  // (rows past the last hold anything)
 #pragma unroll
-          for (int k = 0; k < kFewOutputs; ++k)
+          for (int k = 0; k < O; ++k)
             if (k < outs)
 #pragma unroll
               for (int e = 0; e < 4; ++e) sum[j][e][k] += o.h[e] * dy[k];
@@ -979,7 +983,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int k = 0; k < kFewOutputs; ++k)
+            for (int k = 0; k < O; ++k)
               if (k < outs) {
                 const float v = sum_rows16(sum[j][e][k]);
                 const int n = n0 + j * 16 + e;
@@ -1044,7 +1048,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 // 62 us, a chain of loads.
 template <int KIND, int EPI>
 __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
-  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack || EPI == kEpiGateOuts;
+  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack || EPI == kEpiGateOuts || EPI == kEpiGateOne;
   constexpr int SUB = PAIR ? 2 : 1;
   __shared__ f4 part[SUB][256];
   const int G = p.join, per = 256 / G;

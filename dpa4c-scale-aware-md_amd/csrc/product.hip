@@ -19,7 +19,7 @@ using Tiny = Shape<64, 32, 4, 1>;
 
 template <int KIND, int LA, int LB, int EPI, class S>
 void launch(hipStream_t st, ProductArgs& p) {
-  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack || EPI == kEpiGateOuts;
+  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack || EPI == kEpiGateOuts || EPI == kEpiGateOne;
   constexpr int SUB = PAIR ? 2 : 1;
   p.tiles_m = (p.M + S::BM - 1) / S::BM;
   p.tiles_n1 = (p.N + S::BN / SUB - 1) / (S::BN / SUB);
@@ -29,7 +29,7 @@ void launch(hipStream_t st, ProductArgs& p) {
   hipLaunchKernelGGL((k_product<KIND, LA, LB, EPI, S>), dim3((unsigned)std::min(items, (long)p.blocks)),
                      dim3(S::WM * S::WN * 64), 0, st, p);
   DPAMD_LAUNCH_CHECK();
-  if (EPI == kEpiGateOuts && p.split > 1) throw HipError{hipErrorInvalidValue, "gated block: a sliced gate"};
+  if ((EPI == kEpiGateOuts || EPI == kEpiGateOne) && p.split > 1) throw HipError{hipErrorInvalidValue, "gated block: a sliced gate"};
   if (p.split > 1 && !p.raw) {
     const long rows = (long)p.M * (PAIR ? 1 : p.mats), quads = p.ldp / 4;
     // threads that share a quad's slices: up to 8 slices each, more where the quads fill the card
@@ -48,7 +48,10 @@ void launch_kind(hipStream_t st, ProductKind what, ProductArgs& p) {
     case kProdDown: return launch<KIND, kRowK, kColK, kEpiStore, S>(st, p);
     case kProdGateGrad: return launch<KIND, kRowK, kRowK, kEpiGateGrad, S>(st, p);
     case kProdGateBack: return launch<KIND, kRowK, kColK, kEpiGateBack, S>(st, p);
-    case kProdGateOuts: return launch<KIND, kRowK, kColK, kEpiGateOuts, S>(st, p);
+    case kProdGateOuts:
+      if constexpr (S::BM != 128 || S::BN != 128) launch<KIND, kRowK, kColK, kEpiGateOuts, S>(st, p);
+      return;  // (the other shape is not planned for it)
+    case kProdGateOne: return launch<KIND, kRowK, kColK, kEpiGateOne, S>(st, p);
     case kProdInput: return launch<KIND, kRowK, kRowK, kEpiStore, S>(st, p);
     case kProdWeight: return launch<KIND, kColK, kColK, kEpiStore, S>(st, p);
   }

@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void k_restore8(const KeepArgs p) {
 }
 
 // ---- operands of the 8-bit products -------------------------------------------------------
-// A row by T threads of a block (64: a wave, four rows a block; 256), C eights a thread held in registers
+// A row by T threads of a block (16; 64, a wave; 256), C eights a thread held in registers
 // between the maximum and the integers; what is beyond C T eights is read again, from the caches. Zeros up
 // to ld_q (a multiple of 16).
 template <int KIND, int T, int C>
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256) void k_rows8(const Rows8Args p) {
       for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(unsigned, w[e]) & 0x7fffffffu);
     }
 #pragma unroll
-    for (int m = 1; m < 64; m *= 2) top = max(top, (unsigned)__shfl_xor((int)top, m, kWave));
+    for (int m = 1; m < (T < 64 ? T : 64); m *= 2) top = max(top, (unsigned)__shfl_xor((int)top, m, kWave));
     if constexpr (T == 256) {
       __syncthreads();
       if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
@@ -192,13 +192,19 @@ __global__ __launch_bounds__(256) void k_weights8(const Weights8Args p) {
 constexpr long kFewEights = 1L << 20;  // four for each thread of a full card
 dim3 blocks_of(long eights, int items) { return dim3(grid_of((eights + items * 256 - 1) / (items * 256))); }
 
-// A row to a wave, or to a block: few rows, or long ones.
+// A row to 16 lanes, to a wave, or to a block: by its length, and few rows to blocks.
 template <int KIND>
 void rows_kind(hipStream_t st, const Rows8Args& p) {
-  if (p.rows <= 1024 && p.ld_q <= 256 * 8)
+  if (p.ld_q <= 16 * 8)
+    hipLaunchKernelGGL((k_rows8<KIND, 16, 1>), dim3(grid_of((p.rows + 15) / 16)), dim3(256), 0, st, p);
+  else if (p.ld_q <= 16 * 8 * 4 && p.rows > 1024)
+    hipLaunchKernelGGL((k_rows8<KIND, 16, 4>), dim3(grid_of((p.rows + 15) / 16)), dim3(256), 0, st, p);
+  else if (p.rows <= 1024 && p.ld_q <= 256 * 8)
     hipLaunchKernelGGL((k_rows8<KIND, 256, 1>), dim3(grid_of(p.rows)), dim3(256), 0, st, p);
   else if (p.ld_q <= 64 * 8 * 4)
     hipLaunchKernelGGL((k_rows8<KIND, 64, 4>), dim3(grid_of((p.rows + 3) / 4)), dim3(256), 0, st, p);
+  else if (p.ld_q <= 64 * 8 * 8 && p.rows > 2048)
+    hipLaunchKernelGGL((k_rows8<KIND, 64, 8>), dim3(grid_of((p.rows + 3) / 4)), dim3(256), 0, st, p);
   else
     hipLaunchKernelGGL((k_rows8<KIND, 256, 4>), dim3(grid_of(p.rows)), dim3(256), 0, st, p);
 }
