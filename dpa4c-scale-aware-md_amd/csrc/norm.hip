@@ -49,7 +49,7 @@ __device__ __forceinline__ Frame frame_of(const NormArgs& p, int f) {
 // end of a row). Where groups are multiples of VE (not GEN) all of them are of one group, and are one entry of
 // the sums; else (GEN: groups of 5, of 47) each channel is an entry of its own, and knows its group. (With vectors as
 // narrow as a common divisor of groups and 16 bytes instead, odd groups went element by element:
-// 113,120 x 235 in groups of 5, bf16, with its gradients 491 us, so XXX.)
+// 113,120 x 235 in groups of 5, bf16, with its gradients 491 us, so 147.)
 struct Cols {
   int c, count;
 };
@@ -142,11 +142,19 @@ struct RawX<KIND, VE, GEN, true> {
   unsigned char field, second;  // (GEN: the last elements may be of the next 32)
   unsigned char split;          // elements of the first
   __device__ __forceinline__ void load_at(const NormArgs& p, long row, const Cols& x) {
-    const unsigned char* at = p.kept + row * p.wide + x.c;
-    if constexpr (VE == 1)
-      w[0] = *at;
-    else
-      __builtin_memcpy(w, at, VE);  // (past a row's end are the next row's, or the fields: inside the buffer)
+    const unsigned char* at = p.kept + row * p.wide;
+    if constexpr (VE == 1) {
+      w[0] = at[x.c];
+    } else if constexpr (GEN) {
+      // (from any channel on, but not past the row's end: there the last ones, shifted)
+      const int c = min(x.c, p.wide - VE);
+      std::conditional_t<VE == 8, unsigned long long, unsigned> v;
+      __builtin_memcpy(&v, at + c, VE);
+      v >>= 8 * (x.c - c);
+      __builtin_memcpy(w, &v, VE);
+    } else {
+      __builtin_memcpy(w, at + x.c, VE);
+    }
     const unsigned char* fields = p.kept + p.rows * p.wide + row * (p.wide / 32);
     field = fields[x.c / 32];
     if constexpr (GEN) {

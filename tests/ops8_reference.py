@@ -91,25 +91,30 @@ def norm(dtype, act, x, gamma, beta, frames, groups, eps, dy=None, at=None):
     per = ch // groups
     u, tiny = ref.HALF_ULP[dtype], ref.TINY[dtype]
     gm, bt = gamma.reshape(groups, per), beta.reshape(groups, per)
+    first, each = frames[0]
+    if each and all(f == (first + k * each, each) for k, f in enumerate(frames)):
+        batches = [(0, len(frames), first, each)]  # (all at once)
+    else:
+        batches = [(f, 1, first, count) for f, (first, count) in enumerate(frames)]
     out = {"y": [torch.full_like(x, math.nan) for _ in range(2)],
-           "stats": [torch.zeros(len(frames), groups, 2, dtype=torch.float64) for _ in range(2)]}
+           "stats": [x.new_zeros(len(frames), groups, 2) for _ in range(2)]}
     if dy is not None:
         out["dx"] = [torch.full_like(x, math.nan) for _ in range(2)]
         for k in ("dgamma", "dbeta"):
-            out[k] = [torch.zeros(groups, per, dtype=torch.float64) for _ in range(2)]
+            out[k] = [x.new_zeros(groups, per) for _ in range(2)]
     sums = (n + 32) * 2.0 ** -23
-    for f, (first, count) in enumerate(frames):
+    for f, many, first, count in batches:
         if not count:
             continue
-        rows = slice(first, first + count)
-        a = x[rows].reshape(count, groups, per)
+        rows, shape = slice(first, first + many * count), (many, count, groups, per)
+        a = x[rows].reshape(shape)
         number = count * per
         # a value passes at most 32 additions in its thread's batch, a join for every fourth row,
         # and 256 parts of a block
         g = (min(number, 300 + count // 4) + 32) * 2.0 ** -23
 
         def mean(v):
-            return v.mean((0, 2), keepdim=True)
+            return v.mean((1, 3), keepdim=True)
 
         m = mean(a)
         bm = g * mean(a.abs())
@@ -117,8 +122,8 @@ def norm(dtype, act, x, gamma, beta, frames, groups, eps, dy=None, at=None):
         bvar = g * var + 2 * bm * var.sqrt() + bm ** 2
         r = (var + eps) ** -0.5
         br = ((var - bvar).clamp(min=0) + eps) ** -0.5 - r + 4 * E32 * r
-        out["stats"][0][f] = torch.stack([m, r], -1).reshape(groups, 2)
-        out["stats"][1][f] = torch.stack([bm + E32 * m.abs(), br], -1).reshape(groups, 2)
+        out["stats"][0][f:f + many] = torch.stack([m, r], -1).reshape(many, groups, 2)
+        out["stats"][1][f:f + many] = torch.stack([bm + E32 * m.abs(), br], -1).reshape(many, groups, 2)
 
         def value(t):
             d = t - m
@@ -130,13 +135,13 @@ def norm(dtype, act, x, gamma, beta, frames, groups, eps, dy=None, at=None):
         v, bv, z, bz = value(a)
         y = act64(act, z)[0]
         by = act_bound(act, y, bz, ref.SLOPE)
-        out["y"][0][rows] = y.reshape(count, ch)
-        out["y"][1][rows] = (by + u * (y.abs() + by) + tiny).reshape(count, ch)
+        out["y"][0][rows] = y.reshape(many * count, ch)
+        out["y"][1][rows] = (by + u * (y.abs() + by) + tiny).reshape(many * count, ch)
         if dy is None:
             continue
         if at is not None:
-            v, bv, z, bz = value(at[rows].reshape(count, groups, per))
-        d = dy[rows].reshape(count, groups, per)
+            v, bv, z, bz = value(at[rows].reshape(shape))
+        d = dy[rows].reshape(shape)
         da = act64(act, z)[1]
         dz = d * da
         bdz = d.abs() * act_bound(act, z, bz, ref.BEND) + 2 * E32 * dz.abs()
@@ -148,12 +153,12 @@ def norm(dtype, act, x, gamma, beta, frames, groups, eps, dy=None, at=None):
         bi = bw + b1 + v.abs() * b2 + bv * (s2.abs() + b2) + 4 * E32 * (w.abs() + s1.abs() + (v * s2).abs())
         dx = r * inner
         bx = (r + br) * bi + br * inner.abs() + 2 * E32 * dx.abs()
-        out["dx"][0][rows] = dx.reshape(count, ch)
-        out["dx"][1][rows] = (bx + u * (dx.abs() + bx) + tiny).reshape(count, ch)
+        out["dx"][0][rows] = dx.reshape(many * count, ch)
+        out["dx"][1][rows] = (bx + u * (dx.abs() + bx) + tiny).reshape(many * count, ch)
         dv, bdv = dz * v, bdz * (v.abs() + bv) + dz.abs() * bv + 2 * E32 * (dz * v).abs()
         for k, t, b in (("dgamma", dv, bdv), ("dbeta", dz, bdz)):
-            out[k][0] += t.sum(0)
-            out[k][1] += (b + sums * (t.abs() + b)).sum(0)
+            out[k][0] += t.sum((0, 1))
+            out[k][1] += (b + sums * (t.abs() + b)).sum((0, 1))
     if dy is not None:
         for k in ("dgamma", "dbeta"):
             t, b = (z.reshape(ch) for z in out[k])

@@ -323,3 +323,64 @@ def test_every_tile_shape_is_run(dp):
         assert seen == {(256, 256), (128, 128), (64, 128), (64, 32)}, (gate, seen)
         assert any(tiles(dp, *s, gate)[2] > 1 for s in TILED + PRODUCTS if s[0] > 64)
         assert any(tiles(dp, *s, gate)[2] == 1 for s in TILED + PRODUCTS if s[0] > 64)
+
+
+def test_products_past_32_bits(ops, dp):
+    """More than 2^32 integers in the rows' 8-bit form, and 2^31 in y's bytes: the first rows and the last."""
+    n, d, o = 2 ** 21 + 9, 2064, 520
+    x = torch.empty(n, d, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator().manual_seed(1)
+    ends = torch.randn(32, d, generator=gen).bfloat16()
+    x.fill_(1.0)
+    x[:16], x[-16:] = ends[:16].cuda(), ends[16:].cuda()
+    w, ws = weights(gen, o, d)
+    gw, gs, y = w.cuda(), ws.cuda(), torch.empty(n, o, dtype=torch.bfloat16, device="cuda")
+    ops.linear8(dp.ops.Linear8Shape(n, d, o, dtype="bf16"), x.data_ptr(), gw.data_ptr(), gs.data_ptr(), y.data_ptr(),
+                stream=stream())
+    torch.cuda.synchronize()
+    v, b = ref8.linear8("bf16", "none", ends.double(), w[:, :d], ws)
+    check(torch.cat([y[:16], y[-16:]]), (v, b), "ends")
+    assert bool((y[16:-16] == y[16]).all())
+
+
+@pytest.mark.parametrize("o", [1, 8])
+def test_backward_from_a_checkpoint_past_32_bits(ops, dp, o):
+    """More than 2^32 hidden values: dx of the first rows and the last, and a w_down gradient over all."""
+    n, d, f = 2 ** 21 + 40, 8, 2072
+    gen = torch.Generator().manual_seed(4)
+    host = {"wg": rand(gen, "bf16", d, f, d ** -0.5), "wu": rand(gen, "bf16", d, f, d ** -0.5),
+            "wd": rand(gen, "bf16", f, o, f ** -0.5)}
+    xe, dye = rand(gen, "bf16", 32, d), rand(gen, "bf16", 32, o)
+    g = {k: v.cuda() for k, v in host.items()}
+    x, dy = (torch.zeros(n, c, dtype=torch.bfloat16, device="cuda") for c in (d, o))
+    for m, e in ((x, xe), (dy, dye)):
+        m[:16], m[-16:] = e[:16].cuda(), e[16:].cuda()
+    dx, dwd = torch.empty_like(x), torch.empty_like(g["wd"])
+    kept = kept_of(dp, n, d)
+    shape = dp.ops.GatedShape(n, d, f, o, dtype="bf16")
+    ops.keep8(x.data_ptr(), kept.data_ptr(), n, d, "bf16", stream=stream())
+    ops.gated_backward8(shape, kept.data_ptr(), *(g[k].data_ptr() for k in ("wg", "wu", "wd")), dy.data_ptr(),
+                        dx.data_ptr(), d_dw_down=dwd.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    # (the rows between are zeros, whose gradients are: sums over the 32 rows, and over many zeros)
+    want = ref.gated("bf16", "silu", ref8.restored(xe.double()), *(host[k].double() for k in ("wg", "wu", "wd")),
+                     dye.double())
+    check(torch.cat([dx[:16], dx[-16:]]), want["dx"], "dx")
+    check(dwd, want["dwd"], "dwd")
+    assert bool((dx[16:-16] == 0).all())
+
+
+def test_restored_past_the_caches(ops, dp):
+    """Outputs of over 192 MB are stored in another way."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for dtype, cols in (("bf16", 1043), ("f32", 1040)):
+        x = torch.randn(100000, cols, generator=gen, device="cuda").to(ref.TORCH[dtype])
+        kept, out, part = kept_of(dp, 100000, cols), torch.empty_like(x), torch.empty(1000, cols, dtype=x.dtype,
+                                                                                     device="cuda")
+        ops.keep8(x.data_ptr(), kept.data_ptr(), 100000, cols, dtype, stream=stream())
+        ops.restore8(kept.data_ptr(), out.data_ptr(), 100000, cols, dtype, stream=stream())
+        few = kept_of(dp, 1000, cols)
+        for at in (0, 50000, 99000):
+            ops.keep8(x[at:].data_ptr(), few.data_ptr(), 1000, cols, dtype, stream=stream())
+            ops.restore8(few.data_ptr(), part.data_ptr(), 1000, cols, dtype, stream=stream())
+            assert torch.equal(out[at:at + 1000], part)

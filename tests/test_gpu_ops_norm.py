@@ -65,8 +65,9 @@ def norm_case(ops, dp, dtype, act, rows, ch, groups, frames=1, lengths=None, fir
         assert torch.equal(alone, m["y"].view)
     one, zero = torch.ones(ch, dtype=torch.float64), torch.zeros(ch, dtype=torch.float64)
     args = [host["x"].double(), gamma[0].double() if affine else one, beta[0].double() if affine else zero]
-    back = ref8.restored(host["x"].double()) if kept else None
-    want = ref8.norm(dtype, act, *args, parts, groups, eps, host["dy"].double(), back)
+    back = ref8.restored(host["x"].double()).to(at) if kept else None
+    want = ref8.norm(dtype, act, *(v.to(at) for v in args), parts, groups, eps, host["dy"].double().to(at), back)
+    want = {k: (v.cpu(), b.cpu()) for k, (v, b) in want.items()}
     what = (dtype, act, rows, ch, groups, frames, kept)
     check(st[:-4].reshape(frames, groups, 2), want["stats"], ("stats",) + what)
     assert bool((st[-4:] == 7.0).all())
@@ -226,3 +227,69 @@ def test_against_differences(ops, dp, frames):
         slope = (loss(x.double() + step) - loss(x.double() - step)) / (2 * h)
         # second order: h^2 times third derivatives of up to about 10^3; fp32: 1e-5 of sums below 10
         assert abs(float(dx[r, c]) - float(slope)) < 1e-4 + 1e-4 * abs(float(slope))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3])
+@pytest.mark.parametrize("ch,groups", [(32, 16), (96, 16), (35, 5), (64, 1), (8, 8), (9, 3), (7, 7)])
+def test_checkpoints_of_a_few_rows(ops, dp, dtype, rows, ch, groups):
+    """Frames named by starts, whose parts begin at any channel: reads of the checkpoint end with it."""
+    norm_case(ops, dp, dtype, "silu", rows, ch, groups, lengths=[rows], kept=True, eps=1e-3)
+    norm_case(ops, dp, dtype, "silu", rows, ch, groups, frames=1, kept=True, eps=1e-3)
+
+
+@pytest.mark.parametrize("rows,ch,groups,frames", [(3000, 235, 47, 5), (2000, 1001, 7, 1), (900, 5005, 5, 2),
+                                                   (700, 4100, 4100, 1), (260, 2310, 11, 260), (300, 9001, 1, 3),
+                                                   (5000, 6, 2, 1), (1200, 12, 12, 40)])
+def test_groups_across_vectors_and_parts(ops, dp, rows, ch, groups, frames):
+    """Groups that no vector of 16 bytes divides, that go over several parts of the columns or are one
+    channel each."""
+    for k, dtype in enumerate(TYPES):
+        norm_case(ops, dp, dtype, ("silu", "none", "gelu")[k], rows, ch, groups, frames)
+        norm_case(ops, dp, dtype, ("gelu", "tanh", "none")[k], rows, ch, groups, frames, kept=True, eps=1e-3)
+
+
+@pytest.mark.parametrize("rows,ch,groups,frames", [(70000, 1024, 32, 1), (70000, 1030, 103, 4), (70000, 1024, 16, 70000),
+                                                   (70016, 1024, 64, 547)])
+def test_outputs_past_the_caches(ops, dp, rows, ch, groups, frames):
+    """Outputs of over 192 MB, which are stored in another way, in each form."""
+    norm_case(ops, dp, "f32", "silu", rows, ch, groups, frames, at="cuda")
+
+
+@pytest.mark.parametrize("frames", [1, "rows"])
+def test_past_32_bits(ops, dp, frames):
+    """More than 2^32 values: y, dx and the sums of the last rows, whose places pass 32 bits."""
+    rows, ch, groups = 2 ** 21 + 32, 2080, 65
+    x = torch.empty(rows, ch, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for a in range(0, rows, 2 ** 18):
+        x[a:a + 2 ** 18] = torch.randn(min(2 ** 18, rows - a), ch, generator=gen, device="cuda", dtype=torch.float32)
+    n = rows if frames == "rows" else 1
+    y, stats = torch.empty_like(x), torch.empty(n, groups, 2, device="cuda")
+    shape = dp.ops.NormShape(rows, ch, groups, frames=n, dtype="bf16")
+    ops.group_norm(shape, x.data_ptr(), 0, 0, y.data_ptr(), stats=stats.data_ptr(), stream=stream())
+    dx, dgamma, dbeta = torch.empty_like(x), *(torch.empty(ch, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ops.group_norm_grad(shape, x.data_ptr(), 0, 0, stats.data_ptr(), y.data_ptr(), dx.data_ptr(), dgamma.data_ptr(),
+                        dbeta.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    for part in (slice(0, 8), slice(rows - 8, rows)):
+        a = x[part].double().reshape(8, groups, -1)
+        if n == 1:
+            # mean 0 and deviation 1 of 6.7e7 values each: off by 5 / sqrt of that, and its square root of two
+            assert float(stats[0, :, 0].abs().max()) < 7e-4 and float((stats[0, :, 1] - 1).abs().max()) < 7e-4
+            m, r = (stats[0, :, k].double()[:, None] for k in (0, 1))
+        else:
+            m = a.mean(2, keepdim=True)
+            r = ((a - m).square().mean(2, keepdim=True) + 1e-5) ** -0.5
+        want = ((a - m) * r).reshape(8, ch)
+        got = y[part].double()
+        assert bool(((got - want).abs() <= (2.0 ** -8 + 1e-5) * want.abs() + 1e-5).all())
+        # dy = y = v (rounded): w = v, so dx = r (v - mean v - v mean v^2), small, as mean v^2 is nearly 1
+        v, w = want.reshape(8, groups, -1), got.reshape(8, groups, -1)
+        s1, s2 = (0.0, 1.0) if n == 1 else (w.mean(2, keepdim=True), (w * v).mean(2, keepdim=True))
+        dxw = (r * (w - s1 - v * s2)).reshape(8, ch)
+        # (n = 1: the means of w and w v to 1e-3, as above; both: rounded to bf16, terms of up to 5 in fp32)
+        assert bool(((dx[part].double() - dxw).abs() <= 2.0 ** -8 * dxw.abs() + (1e-2 if n == 1 else 2e-5)).all())
+    # dgamma = sum of y v, about the number of rows; dbeta = sum of y, a sum of 2^21 roundings and signs
+    assert bool(((dgamma.double() / rows - 1).abs() < 2.0 ** -7).all())
+    assert bool((dbeta.double().abs() < 6 * math.sqrt(rows)).all())
