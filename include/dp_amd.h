@@ -344,7 +344,7 @@ size_t dp_device_bytes(const dp_model* model);
 
 /*
  * Operators of trainable heads: what a per-atom (or per-token) net on top of
- * descriptors or embeddings needs, forward and backward. No counterpart in the
+ * descriptors or embeddings needs, forward and backward, and served in 8 bits. No counterpart in the
  * reference, whose nets are evaluated inside its model. Every array is device memory
  * on the handle's GPU; work is ordered on `stream` (a hipStream_t, NULL = default
  * stream) and the calls return without waiting for it. Matrices are row-major;
@@ -474,7 +474,7 @@ int dp_restore8(dp_ops* ops, int type, int64_t rows, int cols, const void* d_kep
  * dp_gated_backward from the checkpoint of x [rows][d_in] alone, with nothing kept by the forward (d_saved
  * NULL): x w_gate and x w_up are formed again from the restored x, and the gradients are those of the block
  * there. It keeps d_in * 33 / 32 bytes a row in place of x and 8 d_hidden. The workspace takes, for the
- * time of the call, what the forward would have kept, which the calls of all layers on a stream share.
+ * time of the call, x and at most what the forward would have kept, which the calls of all layers on a stream share.
  */
 int dp_gated_backward8(dp_ops* ops, const dp_gated_shape* shape, const void* d_kept,
                        const void* d_w_gate, const void* d_w_up, const void* d_w_down,
