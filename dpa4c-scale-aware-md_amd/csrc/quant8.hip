@@ -172,7 +172,8 @@ __global__ __launch_bounds__(256) void k_weights8(const Weights8Args p) {
   __syncthreads();
   const RowScale s = row_scale(max(max(tops[0][c], tops[1][c]), max(tops[2][c], tops[3][c])));
   if (in && part == 0) p.scale[col] = s.scale;
-  for (int k0 = 0; k0 < p.ld_q; k0 += 64) {
+  const int whole = (p.d_in + 15) / 16 * 16;  // (what lies between the rows beyond it is the caller's)
+  for (int k0 = 0; k0 < whole; k0 += 64) {
     __syncthreads();
     for (int k = part; k < 64; k += 4) {
       const float v = in && k0 + k < p.d_in && s.inv != 0.0f ? to_f32<KIND>(w[(k0 + k) * p.ld_w]) : 0.0f;
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256) void k_weights8(const Weights8Args p) {
     // 16 threads a channel, four integers each
     for (int r = threadIdx.x / 16; r < 64; r += 16) {
       const int k = (threadIdx.x % 16) * 4;
-      if (blockIdx.x * 64 + r < p.d_out && k0 + k < p.ld_q)
+      if (blockIdx.x * 64 + r < p.d_out && k0 + k < whole)
         *reinterpret_cast<unsigned*>(p.q + (long)(blockIdx.x * 64 + r) * p.ld_q + k0 + k) =
             *reinterpret_cast<const unsigned*>(&tile[r][k]);
     }

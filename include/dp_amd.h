@@ -489,7 +489,8 @@ int dp_gated_backward8(dp_ops* ops, const dp_gated_shape* shape, const void* d_k
  * counts as zeros; one with an infinity or a NaN has a scale of NaN, and all that comes of it is NaN.
  *
  * dp_weights8: w [d_in][d_out] of a type -> d_w8 [d_out][ld_w8] integers (16-byte aligned; ld_w8 a multiple of 16, 0:
- * d_in up to one; zeros past d_in) and d_scale [d_out].
+ * d_in up to one) and d_scale [d_out]. Past d_in there are zeros up to a multiple of 16, and what lies between the
+ * rows beyond it is left as it was.
  */
 int dp_weights8(dp_ops* ops, int type, int d_in, int d_out, const void* d_w, int64_t ld_w,
                 void* d_w8, int64_t ld_w8, float* d_scale, void* stream);

@@ -201,9 +201,38 @@ def test_weights(ops, dp, dtype, d, o, pad, skip, more):
     want, s = ref8.rows8(host.T.double())
     got = q[:o * ld].cpu().reshape(o, ld)
     assert torch.equal(got[:, :d].double(), want)
-    assert bool((got[:, d:] == 0).all()) and bool((q[o * ld:] == 0x55).all())
+    assert bool((got[:, d:ld - more] == 0).all()) and bool((got[:, ld - more:] == 0x55).all())
+    assert bool((q[o * ld:] == 0x55).all())
     assert torch.equal(torch.nan_to_num(scale[:o].cpu(), nan=-1.0), torch.nan_to_num(s[:, 0].float(), nan=-1.0))
     assert bool((scale[o:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,o", [(70, 33), (640, 100)])
+def test_weights_side_by_side(ops, dp, dtype, d, o):
+    """Two matrices whose rows alternate in one array, written one after the other, and multiplied from there."""
+    gen = torch.Generator().manual_seed(d)
+    whole = (d + 15) // 16 * 16
+    host = [rand(gen, dtype, d, o) for _ in range(2)]
+    q = torch.full((2 * whole * o + 64,), 0x55, dtype=torch.int8, device="cuda")
+    scale = torch.empty(2, o, device="cuda")
+    dev = [h.cuda() for h in host]
+    for k in (1, 0):
+        ops.weights8(dev[k].data_ptr(), q[k * whole:].data_ptr(), scale[k].data_ptr(), d, o, dtype, ld_w8=2 * whole,
+                     stream=stream())
+    x = rand(gen, dtype, 5, d)
+    xd, y = x.cuda(), torch.empty(5, o, dtype=x.dtype, device="cuda")
+    shape = dp.ops.Linear8Shape(5, d, o, dtype=dtype, act="silu", ld_w=2 * whole)
+    ops.linear8(shape, xd.data_ptr(), q.data_ptr(), scale[0].data_ptr(), y.data_ptr(), d_up=q[whole:].data_ptr(),
+                d_up_scale=scale[1].data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    want = [ref8.rows8(h.T.double()) for h in host]
+    got = q[:2 * whole * o].cpu().reshape(o, 2, whole)
+    for k in range(2):
+        assert torch.equal(got[:, k, :d].double(), want[k][0]) and bool((got[:, k, d:] == 0).all())
+    assert bool((q[2 * whole * o:] == 0x55).all())
+    check(y.cpu(), ref8.linear8(dtype, "silu", x.double(), got[:, 0, :d], want[0][1][:, 0], got[:, 1, :d],
+                                want[1][1][:, 0]), (dtype, d, o))
 
 
 def weights(gen, o, d, more=0):
