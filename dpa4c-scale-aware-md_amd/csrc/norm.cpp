@@ -76,7 +76,9 @@ NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
     const double chain = 3 + waves * (1.2 + 2.4 * std::ceil(more / batch));
     const double moved = size * (grad ? 3 + 2 * again : 2 + again) / 4.7e6 * (1 + (p.general ? 128 : 16) / piece);
     const double whole = std::max(chain, moved * std::max(1.0, ncu / n_blocks));
-    const double cut = 10 + size * (grad ? 5 : 3) / 4.7e6;
+    // (and a block of the slices' join for each frame and group: 50,000 frames of two rows of 256 in 32 groups, bf16,
+    // 2,741 us in slices and 231 as frames)
+    const double cut = 10 + size * (grad ? 5 : 3) / 4.7e6 + 1.7e-3 * p.frames * p.groups;
     const bool slices = part(gp) > 256 || whole > cut;
     if (!slices) {
       p.form = kNormFrames;

@@ -293,3 +293,11 @@ def test_past_32_bits(ops, dp, frames):
     # dgamma = sum of y v, about the number of rows; dbeta = sum of y, a sum of 2^21 roundings and signs
     assert bool(((dgamma.double() / rows - 1).abs() < 2.0 ** -7).all())
     assert bool((dbeta.double().abs() < 6 * math.sqrt(rows)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ch,groups", [(128, 32), (90, 18)])
+def test_many_short_frames(ops, dp, dtype, ch, groups):
+    """Thousands of frames of none to three rows (small molecules of a batch)."""
+    lengths = [(7 * k) % 4 for k in range(3000)]
+    norm_case(ops, dp, dtype, "silu", sum(lengths) + 5, ch, groups, lengths=lengths, first=2)
