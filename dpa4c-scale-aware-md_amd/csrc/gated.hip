@@ -48,7 +48,8 @@ __global__ __launch_bounds__(256) void k_zero(unsigned char* dst, long rows, lon
 
 // One step (128 bytes of k) of one block, measured: its share of a compute unit's time
 // among others, and its time alone; what a tile's epilogue adds (a plain store, the gate, the gate's
-// gradient, the gate with its gradient, the same with few outputs); and the blocks that a compute unit holds. Measured with each shape forced, every
+// gradient, the gate with its gradient, the same with few outputs); and the blocks that a compute unit holds (8-bit
+// integers: as 16 bits). Measured with each shape forced, every
 // product of training steps of ten sizes, 33 to 131,072 rows: the one picked here took within 6 % of
 // the best one's time but for eleven of 108, of which the worst took 24 % more. (fp32: the
 // matrix cores are slow enough that 256 x 256 tiles gain nothing over 128 x 128. 16 bits: 128 x 32

@@ -2,7 +2,9 @@
 // memory straight into the operands of v_mfma_i32_16x16x64_i8, 16 output channels by 64 of k in one 16-byte load
 // a lane; the rows of x, in fragments of 16, are its other operand. A block takes 16 channels, its waves share
 // k and join their integers through LDS, so that no sum leaves the block and all of the weights' loads
-// are under way at once. The bytes of the weights bound it.
+// are under way at once. The bytes of the weights bound it: 5.9 us for one row of 2048 -> 8192 (2.8 TB/s, start and end of
+// the launch in it; 3.2 at a copy's rate). With more rows each block reads all of them again from L2: 33 rows of
+// a gate of 2048 -> 2 x 5000 11.9 us.
 #include <algorithm>
 
 #include "quant8.h"
@@ -12,7 +14,7 @@ namespace dpamd {
 namespace {
 
 constexpr int kStep = 64;   // k of one product
-constexpr int kFusedRows = 2;
+constexpr int kFusedRows = 2;  // (2048 -> 8192: two rows 6.4 us, and four 10.5, where five with a launch of their own take 8.9)
 constexpr int kFusedBytes = 48 << 10;
 
 // The 8-bit rows of x in LDS, rows `ld` bytes apart, and their scales: for up to kFusedRows rows each
@@ -245,7 +247,9 @@ void rows_kind(hipStream_t st, const Linear8RowsArgs& p) {
 
 }  // namespace
 
-// Whether so many rows are for these kernels, and whether they quantise x themselves.
+// Whether so many rows are for these kernels, and whether they quantise x themselves. Against tiles, in us: 2048 -> 8192
+// 33 rows 12.2 and 15, 48 rows 12.9 and 14.5; but 8192 -> 2048, whose k only waves share here and blocks share there,
+// 33 to 48 rows 19 to 21 and 16.3; a gate of 2048 -> 8192 with 64 rows 21.7 and 19.2.
 Linear8Form linear8_form(long rows, int K, int N) {
   if (rows > kLinear8Rows || (rows > 32 && K > 2 * N)) return kLinear8Tiles;
   const long ld = (K + kStep - 1) / kStep * kStep + 16;
@@ -254,7 +258,11 @@ Linear8Form linear8_form(long rows, int K, int N) {
 
 void run_linear8_rows(hipStream_t st, int elem, int ncu, Linear8RowsArgs& p) {
   const int steps = (p.K + kStep - 1) / kStep, blocks = (p.N + 15) / 16;
-  p.waves = blocks < 2 * ncu && steps >= 64 ? 8 : 4;
+  // eight waves where compute units are left over and each wave has eight steps yet: 8192 -> 2048, one row 8.1 us and 10.5
+  // with four, 16 rows 13.7 and 14.2; but 4096 -> 4096 16 rows 11.7 and 10.9
+  p.waves = blocks < ncu && steps >= 64 ? 8 : 4;
+  // 32 channels a block where that leaves a block for each: 2048 -> 8192 33 rows 11.2 us and 11.9, 4096 -> 8192 17.2 and
+  // 20.8
   p.pairs = blocks >= 2 * ncu;
   if (elem == kBf16)
     rows_kind<kBf16>(st, p);

@@ -1,5 +1,5 @@
 // C ABI of the operators of trainable heads (dp_ops): argument checks, workspaces, and
-// the order of the kernels of product.hip, gated.hip and lookup.hip.
+// the order of the kernels of product.hip, gated.hip and lookup.hip. (ops8.cpp, norm.cpp: the other operators.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

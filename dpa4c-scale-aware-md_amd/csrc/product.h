@@ -1,6 +1,7 @@
 // Tile products on the matrix cores: C[m][n] = sum_k A(m, k) B(n, k), with an
-// epilogue on the fp32 sums. The products of the gated block (gated.hip), for bf16, f16 and
-// fp32 operands (v_mfma_f32_16x16x32_bf16 / _f16, v_mfma_f32_16x16x4_f32).
+// epilogue on the sums. The products of the gated block (gated.hip), for bf16, f16 and
+// fp32 operands (v_mfma_f32_16x16x32_bf16 / _f16, v_mfma_f32_16x16x4_f32), and those of 8-bit integers
+// (product8.hip, v_mfma_i32_16x16x64_i8).
 #pragma once
 
 #include <type_traits>

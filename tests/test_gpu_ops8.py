@@ -413,3 +413,12 @@ def test_restored_past_the_caches(ops, dp):
             ops.keep8(x[at:].data_ptr(), few.data_ptr(), 1000, cols, dtype, stream=stream())
             ops.restore8(few.data_ptr(), part.data_ptr(), 1000, cols, dtype, stream=stream())
             assert torch.equal(out[at:at + 1000], part)
+
+
+@pytest.mark.parametrize("pad,skip", [(0, 0), (3, 1)])
+@pytest.mark.parametrize("n,d", [(70, 100), (1100, 100), (1030, 500), (300, 520), (8200, 513), (8203, 1024), (1200, 1031),
+                                 (70, 2050), (1100, 4099), (70, 8192), (66, 8200), (1100, 9000)])
+def test_rows_of_every_length(ops, dp, n, d, pad, skip):
+    """Rows quantised by 16 lanes, a wave or a block, ending inside and beyond what these hold."""
+    for k, dtype in enumerate(TYPES):
+        linear8_case(ops, dp, dtype, ("tanh", "none", "silu")[k], n, d, 9, pad=pad, skip=skip)
