@@ -301,3 +301,11 @@ def test_many_short_frames(ops, dp, dtype, ch, groups):
     """Thousands of frames of none to three rows (small molecules of a batch)."""
     lengths = [(7 * k) % 4 for k in range(3000)]
     norm_case(ops, dp, dtype, "silu", sum(lengths) + 5, ch, groups, lengths=lengths, first=2)
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("dtype,ch,groups", [("f32", 564, 4), ("bf16", 1064, 8), ("f16", 1100, 4), ("bf16", 2080, 16),
+                                             ("f16", 2600, 4), ("f32", 2100, 3)])
+def test_slices_of_uneven_widths(ops, dp, dtype, ch, groups, kept):
+    """Rows that are cut into parts of columns, groups that go on beyond them."""
+    norm_case(ops, dp, dtype, "silu", 4100, ch, groups, kept=kept)
