@@ -48,9 +48,15 @@ NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
   p.slices = p.out_slices = 1;
   if (!p.starts && p.frames == p.rows && p.vecs <= (p.general && elem != 2 ? 512 : 1024)) {
     p.form = kNormRows;
-    const int T = p.vecs <= 16 ? 16 : p.vecs <= 64 ? 64 : 256;
+    // (threads of a row, as few of them idle as may be: bf16, forward, 30,000 x 960 24 us with 128 and 40 with 256, 60,000 x
+    // 256 12 with 32 and 18 with 64, 400,000 x 12 in 2 groups 19 with 4 and 56 with 16)
+    const int T = p.vecs <= 4 ? 4 : p.vecs <= 16 ? 16 : p.vecs <= 32 ? 32 : p.vecs <= 64 ? 64 : p.vecs <= 128 ? 128 : 256;
     p.by_lanes = !p.general && p.group_entries <= 64 && (p.group_entries & (p.group_entries - 1)) == 0;
-    p.lanes = lanes_of(p.by_lanes ? 1 : p.groups, p.group_entries, T);
+    // (bf16, gradients, channels as entries and pieces: 30,000 x 2500 in 4 groups 667 and 349 us, 2,712 x 4042 in 2 98 and
+    // 57; but fp32, whose vectors are half as long, 30,000 x 1010 in 10 110 and 120, and 20,000 x 2500 in 2 435 and 420)
+    p.pieces = p.general && p.per >= p.vec && (p.vec == 8 || p.vecs > 256);
+    if (p.pieces) p.entries = 2 * p.vecs;
+    p.lanes = lanes_of(p.by_lanes ? 1 : p.groups, p.pieces ? p.per / p.vec + 1 : p.group_entries, T);
     p.blocks = (int)std::min((p.rows + 256 / T - 1) / (256 / T), (grad ? 4L : 8L) * ncu);
     if (affine) need.partial = 8 * (size_t)p.blocks * p.channels;
   } else {

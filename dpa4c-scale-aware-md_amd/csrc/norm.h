@@ -22,6 +22,7 @@ struct NormArgs {
   bool general;   // groups are not multiples of `vec`: the sums' entries are channels; else vectors
   int entries, group_entries;    // of a row, of a group
   float inv_entries, inv_per;    // 1 / group_entries, 1 / per
+  bool pieces;    // kNormRows: groups of `vec` channels or more, of which a vector meets two at most: two entries a vector
   int form;       // NormForm
   bool by_lanes;  // kNormRows: a group's vectors are neighbouring lanes
   int lanes;      // log2 of the lanes that sum one group's entries

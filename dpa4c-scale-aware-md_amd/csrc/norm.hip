@@ -49,26 +49,44 @@ __device__ __forceinline__ Frame frame_of(const NormArgs& p, int f) {
 // end of a row). Where groups are multiples of VE (not GEN) all of them are of one group, and are one entry of
 // the sums; else (GEN: groups of 5, of 47) each channel is an entry of its own, and knows its group. (With vectors as
 // narrow as a common divisor of groups and 16 bytes instead, odd groups went element by element:
-// 113,120 x 235 in groups of 5, bf16, with its gradients 491 us, so 147.)
+// 113,120 x 235 in groups of 5, bf16, with its gradients 491 us, so 147.) With groups of VE channels or more (GEN ==
+// kPieces, every row a frame) a thread's channels are of two groups at most, and are two entries.
+constexpr int kPieces = 2;
 struct Cols {
   int c, count;
 };
-template <int VE, bool GEN>
+template <int VE, int GEN>
 constexpr int entries_of() {
-  return GEN ? VE : 1;
+  return GEN == kPieces ? 2 : GEN ? VE : 1;
 }
+// channels from c on to the end of its group
+__device__ __forceinline__ int left_of(const Cols& x, int per) { return per - x.c % per; }
 // what each entry has: a mean and a deviation, two sums, ...
-template <int VE, bool GEN>
+template <int VE, int GEN>
 struct Entries {
   static constexpr int N = entries_of<VE, GEN>();
   Pair e[N];
   __device__ __forceinline__ const Pair& of(int channel) const { return e[GEN ? channel : 0]; }
 };
+template <int VE>
+struct Entries<VE, kPieces> {
+  static constexpr int N = 2;
+  Pair e[N];
+  int left;  // channels of the first
+  __device__ __forceinline__ Pair of(int channel) const {
+    return Pair{channel < left ? e[0].a : e[1].a, channel < left ? e[0].b : e[1].b};
+  }
+};
 // Pairs of the entries' groups, from an array of one for each group.
-template <int VE, bool GEN>
+template <int VE, int GEN>
 __device__ __forceinline__ Entries<VE, GEN> of_groups(const Pair* groups, const Cols& x, int per) {
   Entries<VE, GEN> s;
-  if constexpr (GEN) {
+  if constexpr (GEN == kPieces) {
+    const int q = x.c / per;
+    s.left = (q + 1) * per - x.c;
+    s.e[0] = groups[q];
+    s.e[1] = s.left < x.count ? groups[q + 1] : s.e[0];
+  } else if constexpr (GEN) {
     // (one division: the group's channels are counted from it)
     int q = x.c / per, left = (q + 1) * per - x.c;
 #pragma unroll
@@ -94,7 +112,7 @@ struct Raw {
     for (int k = 0; k < kWords; ++k) w[k] = 0;
   }
   // the elements from p on; those past x's count: zeros
-  template <bool GEN>
+  template <int GEN>
   __device__ __forceinline__ void load(const E* p, const Cols& x) {
     if constexpr (kBytes == 2) {
       w[0] = *p;
@@ -124,7 +142,7 @@ struct Raw {
 };
 // x or its checkpoint, and v = x r - m r from it: one instruction a value. (m r is rounded, by no more than m
 // itself is.)
-template <int KIND, int VE, bool GEN, bool KEPT>
+template <int KIND, int VE, int GEN, bool KEPT>
 struct RawX : Raw<KIND, VE> {
   __device__ __forceinline__ void load_at(const NormArgs& p, long row, const Cols& x) {
     this->template load<GEN>(static_cast<const typename ElemOf<KIND>::T*>(p.x) + row * p.ld_x + x.c, x);
@@ -135,7 +153,7 @@ struct RawX : Raw<KIND, VE> {
     for (int e = 0; e < VE; ++e) out[e] = __builtin_fmaf(out[e], s.of(e).b, -s.of(e).a * s.of(e).b);
   }
 };
-template <int KIND, int VE, bool GEN>
+template <int KIND, int VE, int GEN>
 struct RawX<KIND, VE, GEN, true> {
   static constexpr int kWords = (VE + 3) / 4;
   unsigned w[kWords];
@@ -174,7 +192,7 @@ struct RawX<KIND, VE, GEN, true> {
 };
 
 // With ONCE stored past the caches. (Not a test: the compiler makes one store of two, and that an ordinary one.)
-template <int KIND, int VE, bool GEN, bool ONCE>
+template <int KIND, int VE, int GEN, bool ONCE>
 __device__ __forceinline__ void store_out(typename ElemOf<KIND>::T* p, const float (&v)[VE], const Cols& x) {
   struct Some {
     typename ElemOf<KIND>::T v[VE];
@@ -193,7 +211,7 @@ __device__ __forceinline__ void store_out(typename ElemOf<KIND>::T* p, const flo
   }
 }
 
-template <int KIND, int VE, bool GEN>
+template <int KIND, int VE, int GEN>
 __device__ __forceinline__ void load_affine(const NormArgs& p, const Cols& x, float (&gamma)[VE], float (&beta)[VE]) {
   using T = typename ElemOf<KIND>::T;
 #pragma unroll
@@ -237,7 +255,7 @@ __device__ __forceinline__ void forward_vec(int act, const float (&scale)[VE], c
   activate_vec<KIND, VE>(act, z, x, da);
 }
 // gamma v + beta = x scale + shift
-template <int VE, bool GEN>
+template <int VE, int GEN>
 __device__ __forceinline__ void scale_shift(const Entries<VE, GEN>& s, const float (&gamma)[VE],
                                             const float (&beta)[VE], float (&scale)[VE], float (&shift)[VE]) {
 #pragma unroll
@@ -258,7 +276,7 @@ __device__ __forceinline__ void grad_vec(int act, const float (&gamma)[VE], cons
   for (int e = 0; e < VE; ++e) dy[e] *= da[e];
 }
 // w = gamma dz -> dx = r (w - mean w - v mean(w v)); s: m and r, means: of w and w v
-template <int VE, bool GEN>
+template <int VE, int GEN>
 __device__ __forceinline__ void dx_vec(const Entries<VE, GEN>& s, const Entries<VE, GEN>& means, const float (&v)[VE],
                                        float (&w)[VE]) {
 #pragma unroll
@@ -270,7 +288,7 @@ __device__ __forceinline__ void dx_vec(const Entries<VE, GEN>& s, const Entries<
 
 // ---- sums --------------------------------------------------------------------------------
 // Mean and squared deviations of ROWS rows of each entry (of VE values, or one, a row)
-template <int VE, bool GEN, int ROWS>
+template <int VE, int GEN, int ROWS>
 __device__ __forceinline__ Entries<VE, GEN> moments(const float (&v)[ROWS][VE]) {
   constexpr int N = entries_of<VE, GEN>(), W = VE / N;
   Entries<VE, GEN> s;
@@ -296,14 +314,14 @@ __device__ __forceinline__ void join_moments(Pair& p, float n, const Pair& q, fl
   p.a += d * w;
   p.b += q.b + d * d * n * w;
 }
-template <int VE, bool GEN>
+template <int VE, int GEN>
 __device__ __forceinline__ void join_rows(Entries<VE, GEN>& s, int n, const Entries<VE, GEN>& q, int k) {
   constexpr int N = entries_of<VE, GEN>(), W = VE / N;
 #pragma unroll
   for (int i = 0; i < N; ++i) join_moments(s.e[i], (float)(n * W), q.e[i], (float)(k * W));
 }
 // Sums of each entry's channels: of b (a) and of g (b)
-template <int VE, bool GEN>
+template <int VE, int GEN>
 __device__ __forceinline__ Entries<VE, GEN> entry_sums(const float (&b)[VE], const float (&g)[VE]) {
   constexpr int N = entries_of<VE, GEN>(), W = VE / N;
   Entries<VE, GEN> s;
@@ -315,7 +333,40 @@ __device__ __forceinline__ Entries<VE, GEN> entry_sums(const float (&b)[VE], con
   }
   return s;
 }
-template <int VE, bool GEN>
+// Both for two pieces: moments of one row, and sums.
+template <int VE>
+__device__ __forceinline__ Entries<VE, kPieces> piece_moments(const float (&v)[VE], const Cols& x, int left) {
+  Entries<VE, kPieces> s;
+  s.left = left;
+  const int n = min(left, x.count);
+  float m[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < VE; ++e) m[0] += e < n ? v[e] : 0.0f, m[1] += e >= n && e < x.count ? v[e] : 0.0f;
+  m[0] *= 1.0f / (float)n;
+  m[1] *= 1.0f / (float)max(x.count - n, 1);
+  float M[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    const float d = v[e] - (e < n ? m[0] : m[1]), dd = d * d;
+    M[0] += e < n ? dd : 0.0f, M[1] += e >= n && e < x.count ? dd : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) s.e[i] = Pair{m[i], M[i]};
+  return s;
+}
+template <int VE>
+__device__ __forceinline__ Entries<VE, kPieces> piece_sums(const float (&b)[VE], const float (&g)[VE], int left) {
+  Entries<VE, kPieces> s;
+  s.left = left;
+  s.e[0] = s.e[1] = Pair{0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    s.e[0].a += e < left ? b[e] : 0.0f, s.e[0].b += e < left ? g[e] : 0.0f;
+    s.e[1].a += e < left ? 0.0f : b[e], s.e[1].b += e < left ? 0.0f : g[e];
+  }
+  return s;
+}
+template <int VE, int GEN>
 __device__ __forceinline__ void put_entries(Pair* to, const Entries<VE, GEN>& s, const Cols& x) {
 #pragma unroll
   for (int i = 0; i < entries_of<VE, GEN>(); ++i)
@@ -356,6 +407,19 @@ __device__ __forceinline__ void each_group(int t, int groups, int lanes, F&& f) 
   }
 }
 
+// f(entry, its channels) for the entries of group q of a row, every 2^lanes-th of them.
+template <int VE, int GEN, class F>
+__device__ __forceinline__ void each_entry(const NormArgs& p, const Pair* parts, int q, int lane, F&& f) {
+  if constexpr (GEN == kPieces) {
+    const int first = q * p.per, end = first + p.per, last = (end - 1) / VE;
+    for (int v = first / VE + lane; v <= last; v += 1 << p.lanes)
+      f(parts[2 * v + (v * VE < first)], (float)(min(end, (v + 1) * VE) - max(first, v * VE)));
+  } else {
+    const Pair* s = parts + q * p.group_entries;
+    for (int k = lane; k < p.group_entries; k += 1 << p.lanes) f(s[k], (float)(VE / entries_of<VE, GEN>()));
+  }
+}
+
 // ---- every row a frame -----------------------------------------------------------------
 // T threads a row, C vectors of VE channels a thread (at neighbouring places for neighbouring threads). With
 // LANES a group is a power of two of vectors, at most 64, so that it is that many neighbouring lanes, which
@@ -363,10 +427,10 @@ __device__ __forceinline__ void each_group(int t, int groups, int lanes, F&& f) 
 // (16,384 x 2048 in bf16, groups of 64, gelu: 50 us through LDS, 38 by lanes, and 29 with gelu's short form; a copy's
 // rate would be 26.) A block takes rows one after another: gamma and beta stay in registers, and the next row is
 // loaded while this one is computed.
-template <int KIND, int VE, bool GEN, int T, int C, bool LANES, bool ONCE>
+template <int KIND, int VE, int GEN, int T, int C, bool LANES, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
-  constexpr int W = VE / entries_of<VE, GEN>();
+  constexpr int W = VE / entries_of<VE, GEN>();  // (kPieces: a vector is two entries too)
   extern __shared__ __align__(16) char lds[];
   constexpr int R = kThreads / T;
   const int t = threadIdx.x % T, mine = threadIdx.x / T;
@@ -413,16 +477,18 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
       for (int k = 0; k < C; ++k)
         if (k * T + t < p.vecs) {
           raw[k].get(v[k][0]);
-          put_entries<VE, GEN>(parts + x[k].c / W, moments<VE, GEN, 1>(v[k]), x[k]);
+          if constexpr (GEN == kPieces)
+            put_entries<VE, GEN>(parts + x[k].c / W, piece_moments<VE>(v[k][0], x[k], left_of(x[k], p.per)), x[k]);
+          else
+            put_entries<VE, GEN>(parts + x[k].c / W, moments<VE, GEN, 1>(v[k]), x[k]);
         }
       if (row0 + step < p.rows) fetch(row + step);
       row_sync<T>();
       each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
-        const Pair* s = parts + q * p.group_entries;
         float m = 0.0f, M = 0.0f;
-        for (int k = lane; k < p.group_entries; k += 1 << p.lanes) m += s[k].a;
-        m = sum_lanes(m, p.lanes) * p.inv_entries;
-        for (int k = lane; k < p.group_entries; k += 1 << p.lanes) M += s[k].b + W * (s[k].a - m) * (s[k].a - m);
+        each_entry<VE, GEN>(p, parts, q, lane, [&](const Pair& s, float n) { m += n * s.a; });
+        m = sum_lanes(m, p.lanes) * p.inv_per;
+        each_entry<VE, GEN>(p, parts, q, lane, [&](const Pair& s, float n) { M += s.b + n * (s.a - m) * (s.a - m); });
         const Pair r = {m, deviation(sum_lanes(M, p.lanes), p.inv_per, p.eps)};
         if (in && lane == 0) {
           whole[q] = r;
@@ -450,10 +516,10 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows(const NormArgs p) {
 // Its gradients: dgamma and dbeta of a thread's channels are summed over all rows that its block takes, and
 // then over the block's row lanes; partial [blocks][2][channels]. (16,384 x 2048 from the checkpoint in bf16: 74 us
 // with one row under way, 49 with two, 33 at a copy's rate.)
-template <int KIND, int VE, bool GEN, int T, int C, bool LANES, bool KEPT, bool ONCE>
+template <int KIND, int VE, int GEN, int T, int C, bool LANES, bool KEPT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
-  constexpr int W = VE / entries_of<VE, GEN>();
+  constexpr int W = VE / entries_of<VE, GEN>();  // (kPieces: a vector is two entries too)
   extern __shared__ __align__(16) char lds[];
   constexpr int R = kThreads / T;
   const int t = threadIdx.x % T, mine = threadIdx.x / T;
@@ -468,11 +534,11 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
     load_affine<KIND, VE, GEN>(p, x[k], gamma[k], beta[k]);
   }
   // two rows are under way (with one, 16 waves of a compute unit wait for too few bytes)
-  // (GEN: m and r of each channel would take too many registers for that: they are loaded at the row's turn)
+  // (m and r of each channel would take too many registers for that: they are loaded at the row's turn)
   struct Ahead {
     RawX<KIND, VE, GEN, KEPT> x[C];
     Raw<KIND, VE> dy[C];
-    Entries<VE, false> stat[C];
+    Entries<VE, GEN == 1 ? 0 : GEN> stat[C];
   } ahead[2];
   auto stats_of = [&](long row, const Cols& c) {
     return of_groups<VE, GEN>(reinterpret_cast<const Pair*>(p.stats + 2 * row * p.groups), c, p.per);
@@ -488,7 +554,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
         to.dy[k].template load<GEN>(static_cast<const E*>(p.dy) + row * p.ld_y + x[k].c, x[k]);
       else
         to.dy[k].zeros();
-      if constexpr (!GEN) to.stat[k] = stats_of(row, x[k]);
+      if constexpr (GEN != 1) to.stat[k] = stats_of(row, x[k]);
     }
   };
   const long step = (long)gridDim.x * R;
@@ -501,7 +567,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
     for (int k = 0; k < C; ++k) {
       means[k] = Entries<VE, GEN>{};
       if (k * T + t >= p.vecs) continue;
-      if constexpr (GEN)
+      if constexpr (GEN == 1)
         stat[k] = stats_of(min(row, p.rows - 1), x[k]);
       else
         stat[k] = from.stat[k];
@@ -516,7 +582,10 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
         w[k][e] *= gamma[k][e];
         wv[e] = w[k][e] * v[k][e];
       }
-      means[k] = entry_sums<VE, GEN>(w[k], wv);
+      if constexpr (GEN == kPieces)
+        means[k] = piece_sums<VE>(w[k], wv, left_of(x[k], p.per));
+      else
+        means[k] = entry_sums<VE, GEN>(w[k], wv);
       if constexpr (!LANES) put_entries<VE, GEN>(parts + x[k].c / W, means[k], x[k]);
     }
     if (row0 + 2 * step < p.rows) fetch(row + 2 * step, from);
@@ -528,9 +597,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_rows_grad(const NormArgs p) {
     } else {
       row_sync<T>();
       each_group<T>(t, p.groups, p.lanes, [&](int q, int lane, bool in) {
-        const Pair* s = parts + q * p.group_entries;
         float a = 0.0f, b = 0.0f;
-        for (int k = lane; k < p.group_entries; k += 1 << p.lanes) a += s[k].a, b += s[k].b;
+        each_entry<VE, GEN>(p, parts, q, lane, [&](const Pair& s, float) { a += s.a, b += s.b; });
         a = sum_lanes(a, p.lanes) * p.inv_per;
         b = sum_lanes(b, p.lanes) * p.inv_per;
         if (in && lane == 0) whole[q] = Pair{a, b};
@@ -601,7 +669,7 @@ constexpr int kBatch = 4;  // rows under way
 
 // The moments s of a thread's entries, joined with those of its rows from the `from`-th on: first + tr + i TR below
 // first + count
-template <int KIND, int VE, bool GEN>
+template <int KIND, int VE, int GEN>
 __device__ __forceinline__ void thread_moments(const NormArgs& p, long first, int count, const Lay& l, int from,
                                                Entries<VE, GEN>& s) {
   const typename ElemOf<KIND>::T* x = static_cast<const typename ElemOf<KIND>::T*>(p.x) + l.x.c;
@@ -628,7 +696,7 @@ __device__ __forceinline__ void thread_moments(const NormArgs& p, long first, in
 }
 
 // y = act(x scale + shift) of a thread's channels over its rows
-template <int KIND, int VE, bool GEN, bool ONCE>
+template <int KIND, int VE, int GEN, bool ONCE>
 __device__ __forceinline__ void thread_apply(const NormArgs& p, long first, int count, const Lay& l, int from,
                                              const float (&scale)[VE], const float (&shift)[VE]) {
   using E = typename ElemOf<KIND>::T;
@@ -656,7 +724,7 @@ __device__ __forceinline__ void thread_apply(const NormArgs& p, long first, int 
 }
 
 // f(v, dy, row) over a thread's rows, two of them under way together.
-template <int KIND, int VE, bool GEN, bool KEPT, class F>
+template <int KIND, int VE, int GEN, bool KEPT, class F>
 __device__ __forceinline__ void thread_rows(const NormArgs& p, long first, int count, const Lay& l, int from,
                                             const Entries<VE, GEN>& s, F&& f) {
   constexpr int kRows = 2;
@@ -682,7 +750,7 @@ __device__ __forceinline__ void thread_rows(const NormArgs& p, long first, int c
   }
 }
 // dz and dz v of a thread's channels summed over its rows
-template <int KIND, int VE, bool GEN, bool KEPT>
+template <int KIND, int VE, int GEN, bool KEPT>
 __device__ __forceinline__ void thread_sums(const NormArgs& p, long first, int count, const Lay& l, int from,
                                             const Entries<VE, GEN>& s, const float (&gamma)[VE],
                                             const float (&beta)[VE], float (&be)[VE], float (&ga)[VE]) {
@@ -692,7 +760,7 @@ __device__ __forceinline__ void thread_sums(const NormArgs& p, long first, int c
     for (int e = 0; e < VE; ++e) be[e] += d[e], ga[e] += d[e] * v[e];
   });
 }
-template <int KIND, int VE, bool GEN, bool KEPT, bool ONCE>
+template <int KIND, int VE, int GEN, bool KEPT, bool ONCE>
 __device__ __forceinline__ void thread_dx(const NormArgs& p, long first, int count, const Lay& l, int from,
                                           const Entries<VE, GEN>& s, const Entries<VE, GEN>& means,
                                           const float (&gamma)[VE], const float (&beta)[VE]) {
@@ -726,7 +794,7 @@ __device__ __forceinline__ void put_channel_sums(const NormArgs& p, const Lay& l
 // Whole frames: grid (parts, frames, or fewer in y: strided). A thread's first kHold rows stay in registers
 // between the sums and the output; what is beyond them is read again. (64 ragged frames of 12,288 x 1600 in fp32: 50 us
 // reading all rows twice, 41 so; 30 at a copy's rate.)
-template <int KIND, int VE, bool GEN, bool ONCE>
+template <int KIND, int VE, int GEN, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
   constexpr int kHold = 8, N = entries_of<VE, GEN>(), W = VE / N;
@@ -813,7 +881,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
 }
 
 // partial [gridDim.y][2][channels]
-template <int KIND, int VE, bool GEN, bool KEPT, bool ONCE>
+template <int KIND, int VE, int GEN, bool KEPT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_frames_grad(const NormArgs p) {
   using E = typename ElemOf<KIND>::T;
   constexpr int kHold = VE == 8 ? 4 : 8;  // rows whose v and dz stay in registers: 64 of these
@@ -923,7 +991,7 @@ __device__ __forceinline__ void each_part_group(const NormArgs& p, const Lay& l,
 }
 
 // Moments of each group over a slice, or of its channels in this part. Grid (parts, slices, frames).
-template <int KIND, int VE, bool GEN>
+template <int KIND, int VE, int GEN>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(const NormArgs p) {
   constexpr int N = entries_of<VE, GEN>(), W = VE / N;
   __shared__ Pair parts[kThreads * N];
@@ -1034,7 +1102,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_join(const NormArgs p) 
 }
 
 // (The output's slices from the last one on: what the sums' pass has read last is in the last cache yet.)
-template <int KIND, int VE, bool GEN, bool ONCE>
+template <int KIND, int VE, int GEN, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(const NormArgs p) {
   const Lay l = lay_of<VE>(p);
   if (!l.in) return;
@@ -1051,7 +1119,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(const NormArgs p) {
 
 // Sums of w and w v over a slice for each group, or its channels in this part. dgamma and dbeta over all frames
 // that a block takes: partial [gridDim.z][slices][2][channels].
-template <int KIND, int VE, bool GEN, bool KEPT>
+template <int KIND, int VE, int GEN, bool KEPT>
 __global__ __launch_bounds__(kThreads) void k_norm_sums(const NormArgs p) {
   constexpr int N = entries_of<VE, GEN>(), W = VE / N;
   __shared__ Pair parts[kThreads * N];
@@ -1158,7 +1226,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_sums_join(const NormArgs p, i
   if (p.dbeta) static_cast<E*>(p.dbeta)[c] = from_f32<KIND>((float)a);
 }
 
-template <int KIND, int VE, bool GEN, bool KEPT, bool ONCE>
+template <int KIND, int VE, int GEN, bool KEPT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_norm_dx(const NormArgs p) {
   const Lay l = lay_of<VE>(p);
   if (!l.in) return;
@@ -1193,19 +1261,28 @@ void with(bool b, F&& f) {
   else
     f(std::false_type{});
 }
-// threads of a row, vectors of a thread, and whether groups are lanes
-template <bool GEN, class F>
+// threads of a row, vectors of a thread, whether groups are lanes, and what a thread's entries are
+template <int GEN, class F>
 void by_row(const NormArgs& p, F&& f) {
   using std::integral_constant;
   auto lanes = [&](auto t, auto c) {
-    if constexpr (!GEN)
-      if (p.by_lanes) return f(t, c, std::true_type{});
-    f(t, c, std::false_type{});
+    if constexpr (!GEN) {
+      if (p.by_lanes) return f(t, c, std::true_type{}, integral_constant<int, 0>{});
+    } else if constexpr (ELEM_KIND != kF32 || decltype(c)::value > 1) {
+      if (p.pieces) return f(t, c, std::false_type{}, integral_constant<int, kPieces>{});
+    }
+    f(t, c, std::false_type{}, integral_constant<int, GEN>{});
   };
-  if (p.vecs <= 16)
+  if (p.vecs <= 4)
+    lanes(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else if (p.vecs <= 16)
     lanes(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (p.vecs <= 32)
+    lanes(integral_constant<int, 32>{}, integral_constant<int, 1>{});
   else if (p.vecs <= 64)
     lanes(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (p.vecs <= 128)
+    lanes(integral_constant<int, 128>{}, integral_constant<int, 1>{});
   else if (p.vecs <= 256)
     lanes(integral_constant<int, 256>{}, integral_constant<int, 1>{});
   else if (p.vecs <= 512)
@@ -1229,12 +1306,12 @@ void norm_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
   constexpr int KIND = ELEM_KIND;
   auto launch = [&](auto ve, auto gen, auto past) {
     constexpr int VE = decltype(ve)::value;
-    constexpr bool GEN = decltype(gen)::value, ONCE = decltype(past)::value;
+    constexpr int GEN = decltype(gen)::value, ONCE = decltype(past)::value;
     if (p.form == kNormRows) {
-      by_row<GEN>(p, [&](auto t, auto c, auto lanes) {
+      by_row<GEN>(p, [&](auto t, auto c, auto lanes, auto entries) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         constexpr bool LANES = decltype(lanes)::value;
-        hipLaunchKernelGGL((k_norm_rows<KIND, VE, GEN, T, C, LANES, ONCE>), dim3(p.blocks), dim3(kThreads),
+        hipLaunchKernelGGL((k_norm_rows<KIND, VE, decltype(entries)::value, T, C, LANES, ONCE>), dim3(p.blocks), dim3(kThreads),
                            row_lds(p, T, VE, false, LANES), st, p);
       });
     } else if (p.form == kNormFrames) {
@@ -1258,14 +1335,14 @@ void norm_grad_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
   const int channel_blocks = p.dgamma || p.dbeta ? (p.channels + 15) / 16 : 0;
   auto launch = [&](auto ve, auto gen, auto kept, auto past) {
     constexpr int VE = decltype(ve)::value;
-    constexpr bool GEN = decltype(gen)::value, KEPT = decltype(kept)::value, ONCE = decltype(past)::value;
+    constexpr int GEN = decltype(gen)::value, KEPT = decltype(kept)::value, ONCE = decltype(past)::value;
     int group_blocks = 0;
     long parts = 0;
     if (p.form == kNormRows) {
-      by_row<GEN>(p, [&](auto t, auto c, auto lanes) {
+      by_row<GEN>(p, [&](auto t, auto c, auto lanes, auto entries) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         constexpr bool LANES = decltype(lanes)::value;
-        hipLaunchKernelGGL((k_norm_rows_grad<KIND, VE, GEN, T, C, LANES, KEPT, ONCE>), dim3(p.blocks), dim3(kThreads),
+        hipLaunchKernelGGL((k_norm_rows_grad<KIND, VE, decltype(entries)::value, T, C, LANES, KEPT, ONCE>), dim3(p.blocks), dim3(kThreads),
                            row_lds(p, T, VE, true, LANES), st, p);
       });
       parts = p.blocks;

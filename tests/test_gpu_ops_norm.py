@@ -309,3 +309,18 @@ def test_many_short_frames(ops, dp, dtype, ch, groups):
 def test_slices_of_uneven_widths(ops, dp, dtype, ch, groups, kept):
     """Rows that are cut into parts of columns, groups that go on beyond them."""
     norm_case(ops, dp, dtype, "silu", 4100, ch, groups, kept=kept)
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,ch,groups", [(37, 27, 3), (700, 90, 6), (300, 123, 3), (65, 235, 5), (130, 1010, 10),
+                                            (40, 2500, 4), (33, 1476, 41), (9, 3999, 31), (21, 45, 5), (50, 4090, 409), (1000, 12, 2), (259, 30, 2),
+                                            (300, 16, 4), (70, 3, 3)])
+def test_rows_of_odd_groups(ops, dp, dtype, rows, ch, groups, kept):
+    """Each row by itself, groups that end inside a thread's channels: of so many channels or more, and of fewer."""
+    norm_case(ops, dp, dtype, "gelu", rows, ch, groups, frames=rows, kept=kept)
+
+
+@pytest.mark.parametrize("shift", [30.0, 3000.0])
+def test_rows_of_odd_groups_far_from_zero(ops, dp, shift):
+    norm_case(ops, dp, "f32", "none", 64, 245, 7, frames=64, shift=shift)
