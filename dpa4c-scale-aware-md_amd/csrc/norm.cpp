@@ -49,8 +49,9 @@ NormNeeds plan_norm(int elem, int ncu, bool grad, NormArgs& p) {
   if (!p.starts && p.frames == p.rows && p.vecs <= (p.general && elem != 2 ? 512 : 1024)) {
     p.form = kNormRows;
     // (threads of a row, as few of them idle as may be: bf16, forward, 30,000 x 960 24 us with 128 and 40 with 256, 60,000 x
-    // 256 12 with 32 and 18 with 64, 400,000 x 12 in 2 groups 19 with 4 and 56 with 16)
-    const int T = p.vecs <= 4 ? 4 : p.vecs <= 16 ? 16 : p.vecs <= 32 ? 32 : p.vecs <= 64 ? 64 : p.vecs <= 128 ? 128 : 256;
+    // 256 12 with 32 and 18 with 64, 400,000 x 12 in 2 groups 19 with 4 and 56 with 16,
+    // 100,000 x 64 7.3 with 8 and 9.9 with 16)
+    const int T = p.vecs <= 4 ? 4 : p.vecs <= 8 ? 8 : p.vecs <= 16 ? 16 : p.vecs <= 32 ? 32 : p.vecs <= 64 ? 64 : p.vecs <= 128 ? 128 : 256;
     p.by_lanes = !p.general && p.group_entries <= 64 && (p.group_entries & (p.group_entries - 1)) == 0;
     // (bf16, gradients, channels as entries and pieces: 30,000 x 2500 in 4 groups 667 and 349 us, 2,712 x 4042 in 2 98 and
     // 57; but fp32, whose vectors are half as long, 30,000 x 1010 in 10 110 and 120, and 20,000 x 2500 in 2 435 and 420)

@@ -1275,6 +1275,8 @@ void by_row(const NormArgs& p, F&& f) {
   };
   if (p.vecs <= 4)
     lanes(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else if (p.vecs <= 8)
+    lanes(integral_constant<int, 8>{}, integral_constant<int, 1>{});
   else if (p.vecs <= 16)
     lanes(integral_constant<int, 16>{}, integral_constant<int, 1>{});
   else if (p.vecs <= 32)

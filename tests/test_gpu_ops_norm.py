@@ -324,3 +324,10 @@ def test_rows_of_odd_groups(ops, dp, dtype, rows, ch, groups, kept):
 @pytest.mark.parametrize("shift", [30.0, 3000.0])
 def test_rows_of_odd_groups_far_from_zero(ops, dp, shift):
     norm_case(ops, dp, "f32", "none", 64, 245, 7, frames=64, shift=shift)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ch,groups", [(4095, 1365), (4096, 4096), (2049, 2049), (62, 31), (64, 4), (61, 1), (33, 11)])
+def test_rows_of_many_and_of_few_groups(ops, dp, dtype, ch, groups):
+    """As many entries as a row may have in LDS, and rows of a few lanes."""
+    norm_case(ops, dp, dtype, "silu", 90, ch, groups, frames=90)
