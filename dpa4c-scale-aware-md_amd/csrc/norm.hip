@@ -1262,7 +1262,8 @@ void with(bool b, F&& f) {
     f(std::false_type{});
 }
 // threads of a row, vectors of a thread, whether groups are lanes, and what a thread's entries are
-template <int GEN, class F>
+// (VE is 1 for rows of less than 16 bytes: seven vectors at most)
+template <int VE, int GEN, class F>
 void by_row(const NormArgs& p, F&& f) {
   using std::integral_constant;
   auto lanes = [&](auto t, auto c) {
@@ -1274,9 +1275,11 @@ void by_row(const NormArgs& p, F&& f) {
     f(t, c, std::false_type{}, integral_constant<int, GEN>{});
   };
   if (p.vecs <= 4)
-    lanes(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  else if (p.vecs <= 8)
-    lanes(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    return lanes(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  if (p.vecs <= 8)
+    return lanes(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  if constexpr (VE == 1)
+    return;
   else if (p.vecs <= 16)
     lanes(integral_constant<int, 16>{}, integral_constant<int, 1>{});
   else if (p.vecs <= 32)
@@ -1310,7 +1313,7 @@ void norm_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
     constexpr int VE = decltype(ve)::value;
     constexpr int GEN = decltype(gen)::value, ONCE = decltype(past)::value;
     if (p.form == kNormRows) {
-      by_row<GEN>(p, [&](auto t, auto c, auto lanes, auto entries) {
+      by_row<VE, GEN>(p, [&](auto t, auto c, auto lanes, auto entries) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         constexpr bool LANES = decltype(lanes)::value;
         hipLaunchKernelGGL((k_norm_rows<KIND, VE, decltype(entries)::value, T, C, LANES, ONCE>), dim3(p.blocks), dim3(kThreads),
@@ -1341,7 +1344,7 @@ void norm_grad_launch<ELEM_KIND>(hipStream_t st, const NormArgs& p) {
     int group_blocks = 0;
     long parts = 0;
     if (p.form == kNormRows) {
-      by_row<GEN>(p, [&](auto t, auto c, auto lanes, auto entries) {
+      by_row<VE, GEN>(p, [&](auto t, auto c, auto lanes, auto entries) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         constexpr bool LANES = decltype(lanes)::value;
         hipLaunchKernelGGL((k_norm_rows_grad<KIND, VE, decltype(entries)::value, T, C, LANES, KEPT, ONCE>), dim3(p.blocks), dim3(kThreads),
