@@ -59,8 +59,17 @@ ProductPlan plan_dh(const dp_gated_shape& s, int ncu) {
 ProductPlan plan_gate_back(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdGateBack, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
 }
-ProductPlan plan_gate_outs(const dp_gated_shape& s, int ncu) {
-  return plan_product(s.d_out == 1 ? kProdGateOne : kProdGateOuts, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
+// The gate's product of that backward, and what it is: with up to four outputs dh is formed in its epilogue, and a
+// sliced one, whose sums are elsewhere, keeps g and u for the kernels of few outputs.
+struct Gate8 {
+  ProductKind what;
+  ProductPlan plan;
+};
+Gate8 plan_gate8(const dp_gated_shape& s, int ncu) {
+  if (!few_outputs(s.d_hidden, s.d_out)) return {kProdGateBack, plan_gate_back(s, ncu)};
+  const ProductKind outs = s.d_out == 1 ? kProdGateOne : kProdGateOuts;
+  const ProductPlan p = plan_product(outs, elem_of(s.type), s.rows, s.d_hidden, s.d_in, 1, 1, ncu);
+  return p.split == 1 ? Gate8{outs, p} : Gate8{kProdGate, plan_gate(s, ncu)};
 }
 ProductPlan plan_input(const dp_gated_shape& s, int ncu) {
   return plan_product(kProdInput, elem_of(s.type), s.rows, s.d_in, s.d_hidden, 2, 1, ncu);
@@ -157,10 +166,9 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
   const size_t at_dg = r.take(hb), at_du = r.take(hb), at_h = dwd && !few ? r.take(hb) : 0;
   const long ldx = (s.d_in + 7) / 8 * 8;
   const size_t at_x = kept ? r.take(bytes_of(s.type) * (size_t)n * ldx) : 0;
-  ProductPlan p0{};
-  if (kept) p0 = few ? plan_gate_outs(s, O->ncu) : plan_gate_back(s, O->ncu);
-  const bool outs = kept && few && p0.split == 1;  // (a sliced gate has its sums elsewhere)
-  if (kept && few && !outs) p0 = plan_gate(s, O->ncu);
+  const Gate8 gate = kept ? plan_gate8(s, O->ncu) : Gate8{};
+  const ProductPlan& p0 = gate.plan;
+  const bool outs = kept && few && gate.what != kProdGate;
   const ProductPlan p1 = few ? ProductPlan{} : kept ? plan_dh(s, O->ncu) : plan_gate_grad(s, O->ncu);
   const long f4 = (f + 3) / 4 * 4;
   const size_t at_saved =
@@ -212,7 +220,7 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
       a.epi.wd = wd, a.epi.ld_down = s.ld_down;
       a.epi.outs = s.d_out;
       a.epi.outs_partial = dwd ? part : nullptr;
-      run_product(st, s.d_out == 1 ? kProdGateOne : kProdGateOuts, elem, p0, a);
+      run_product(st, gate.what, elem, p0, a);
       q.dwd = dwd;
       q.partial = part;
       if (dwd) run_outs_join(st, elem, q);
@@ -396,6 +404,29 @@ int dp_debug_gated_plan(const dp_gated_shape* shape, int compute_units, int* pla
     put(3, plan_input(s, compute_units));
     put(4, plan_weights(s, compute_units));
     if (!few) put(5, plan_down_weight(s, compute_units));
+    return DP_OK;
+  } catch (...) {
+    return DP_ERR_ARG;
+  }
+}
+
+int dp_debug_gated_plan8(const dp_gated_shape* shape, int compute_units, int* plan) {
+  if (!plan || compute_units < 1) return DP_ERR_ARG;
+  try {
+    const dp_gated_shape s = checked(shape);
+    std::fill(plan, plan + 3 * DP_GATED_PRODUCTS8, 0);
+    if (s.rows == 0) return DP_OK;
+    auto put = [&](int k, const ProductPlan& p) {
+      tile_of(p.shape, elem_of(s.type), plan[3 * k], plan[3 * k + 1]);
+      plan[3 * k + 2] = p.split;
+    };
+    const bool few = few_outputs(s.d_hidden, s.d_out);
+    const Gate8 gate = plan_gate8(s, compute_units);
+    put(gate.what == kProdGate ? 0 : gate.what == kProdGateBack ? 1 : gate.what == kProdGateOuts ? 2 : 3, gate.plan);
+    if (!few) put(4, plan_dh(s, compute_units));
+    put(5, plan_input(s, compute_units));
+    put(6, plan_weights(s, compute_units));
+    if (!few) put(7, plan_down_weight(s, compute_units));
     return DP_OK;
   } catch (...) {
     return DP_ERR_ARG;

@@ -18,8 +18,9 @@ ACTS = {"tanh": ACT_TANH, "silu": ACT_SILU, "gelu": ACT_GELU, "none": ACT_NONE}
 EXPORTED = ("dp_ops_create", "dp_ops_destroy", "dp_ops_last_error", "dp_ops_device_bytes", "dp_embed",
             "dp_embed_grad", "dp_gated_saved_bytes", "dp_gated_forward", "dp_gated_backward", "dp_debug_gated_plan",
             "dp_keep8_bytes", "dp_keep8", "dp_restore8", "dp_gated_backward8", "dp_weights8", "dp_linear8",
-            "dp_group_norm", "dp_group_norm_grad")
+            "dp_group_norm", "dp_group_norm_grad", "dp_debug_gated_plan8")
 PRODUCTS = ("gate", "down", "gate_grad", "dx", "dw", "dw_down")
+PRODUCTS8 = ("gate", "gate_back", "gate_outs", "gate_one", "dh", "dx", "dw", "dw_down")
 
 
 class _Shape(C.Structure):
@@ -53,7 +54,8 @@ def bind(L):
     L.dp_embed_grad.argtypes = [P, I, N, I, I, P, P, N, C.c_float, P, N, P]
     L.dp_gated_saved_bytes.argtypes = [S]
     L.dp_gated_saved_bytes.restype = C.c_size_t
-    L.dp_debug_gated_plan.argtypes = [S, I, C.POINTER(C.c_int)]
+    for plan in (L.dp_debug_gated_plan, L.dp_debug_gated_plan8):
+        plan.argtypes = [S, I, C.POINTER(C.c_int)]
     L.dp_gated_forward.argtypes = [P, S, P, P, P, P, P, P, P]
     L.dp_gated_backward.argtypes = [P, S, P, P, P, P, P, P, P, P, P, P, P]
     L.dp_keep8_bytes.argtypes = [N, I]
@@ -93,11 +95,18 @@ class GatedShape:
 
     def plan(self, compute_units: int = 256) -> dict:
         """{product: (tile rows, tile columns, slices)} of those that run as tiles (dp_debug_gated_plan)."""
+        return self._plan("dp_debug_gated_plan", PRODUCTS, compute_units)
+
+    def plan8(self, compute_units: int = 256) -> dict:
+        """The same of gated_backward8 (dp_debug_gated_plan8)."""
+        return self._plan("dp_debug_gated_plan8", PRODUCTS8, compute_units)
+
+    def _plan(self, call, products, compute_units):
         from . import DeepmdException, lib
-        p = (C.c_int * (3 * len(PRODUCTS)))()
-        if lib().dp_debug_gated_plan(C.byref(self.c), compute_units, p) != 0:
-            raise DeepmdException("dp_debug_gated_plan: a shape that the calls refuse")
-        return {k: tuple(p[3 * i:3 * i + 3]) for i, k in enumerate(PRODUCTS) if p[3 * i]}
+        p = (C.c_int * (3 * len(products)))()
+        if getattr(lib(), call)(C.byref(self.c), compute_units, p) != 0:
+            raise DeepmdException(call + ": a shape that the calls refuse")
+        return {k: tuple(p[3 * i:3 * i + 3]) for i, k in enumerate(products) if p[3 * i]}
 
 
 class Linear8Shape:

@@ -481,6 +481,12 @@ int dp_gated_backward8(dp_ops* ops, const dp_gated_shape* shape, const void* d_k
                        const void* d_dy, void* d_dx, void* d_dw_gate, void* d_dw_up,
                        void* d_dw_down, void* stream);
 
+/* dp_debug_gated_plan for it: the gate that keeps x w_gate and x w_up (up to four outputs, where it is sliced), the
+ * gate with its gradient of five outputs and more, of two to four, of one (one of these four runs), dh, dx, dw_gate
+ * and dw_up, dw_down. */
+enum { DP_GATED_PRODUCTS8 = 8 };
+int dp_debug_gated_plan8(const dp_gated_shape* shape, int compute_units, int* plan);
+
 /*
  * Products in 8-bit integers, to serve what was trained: weights with a scale for each output channel, laid out once,
  * and rows of x (tokens, atoms) quantised in the call with a scale each. A row or channel is held as
