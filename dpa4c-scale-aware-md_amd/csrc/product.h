@@ -1050,7 +1050,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
 // 62 us, a chain of loads.
 template <int KIND, int EPI>
 __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
-  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack || EPI == kEpiGateOuts || EPI == kEpiGateOne;
+  constexpr bool PAIR = EPI == kEpiGate || EPI == kEpiGateBack;
   constexpr int SUB = PAIR ? 2 : 1;
   __shared__ f4 part[SUB][256];
   const int G = p.join, per = 256 / G;

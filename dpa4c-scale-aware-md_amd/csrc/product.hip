@@ -26,11 +26,14 @@ void launch(hipStream_t st, ProductArgs& p) {
   p.tiles_n = p.tiles_n1 * p.mats;
   const long items = (long)p.tiles_m * p.tiles_n * p.split;
   if (items >= 1L << 31) throw HipError{hipErrorInvalidValue, "gated block: too many tiles"};
+  // (a slice has no h of its own to sum with dy)
+  constexpr bool WHOLE = EPI == kEpiGateOuts || EPI == kEpiGateOne;
+  if (WHOLE && p.split > 1) throw HipError{hipErrorInvalidValue, "gated block: a sliced gate of few outputs"};
   hipLaunchKernelGGL((k_product<KIND, LA, LB, EPI, S>), dim3((unsigned)std::min(items, (long)p.blocks)),
                      dim3(S::WM * S::WN * 64), 0, st, p);
   DPAMD_LAUNCH_CHECK();
-  if ((EPI == kEpiGateOuts || EPI == kEpiGateOne) && p.split > 1) throw HipError{hipErrorInvalidValue, "gated block: a sliced gate"};
-  if (p.split > 1 && !p.raw) {
+  if constexpr (!WHOLE) {
+    if (p.split == 1 || p.raw) return;
     const long rows = (long)p.M * (PAIR ? 1 : p.mats), quads = p.ldp / 4;
     // threads that share a quad's slices: up to 8 slices each, more where the quads fill the card
     p.join = 1;
@@ -49,8 +52,9 @@ void launch_kind(hipStream_t st, ProductKind what, ProductArgs& p) {
     case kProdGateGrad: return launch<KIND, kRowK, kRowK, kEpiGateGrad, S>(st, p);
     case kProdGateBack: return launch<KIND, kRowK, kColK, kEpiGateBack, S>(st, p);
     case kProdGateOuts:
-      if constexpr (S::BM != 128 || S::BN != 128) launch<KIND, kRowK, kColK, kEpiGateOuts, S>(st, p);
-      return;  // (the other shape is not planned for it)
+      // (the plan leaves out 128 x 128)
+      if constexpr (S::BM != 128 || S::BN != 128) return launch<KIND, kRowK, kColK, kEpiGateOuts, S>(st, p);
+      throw HipError{hipErrorInvalidValue, "gated block: a tile that few outputs do not have"};
     case kProdGateOne: return launch<KIND, kRowK, kColK, kEpiGateOne, S>(st, p);
     case kProdInput: return launch<KIND, kRowK, kRowK, kEpiStore, S>(st, p);
     case kProdWeight: return launch<KIND, kColK, kColK, kEpiStore, S>(st, p);

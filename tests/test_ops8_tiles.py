@@ -1,7 +1,11 @@
 """The sizes of ops8_tiles.py reach every tile that the library takes for a product of the gated block's gradients from
 a checkpoint on 256 compute units, whole and sliced (what it takes is asked of it for shapes drawn over the range)."""
 import math
+import os
 import random
+import re
+import shutil
+import subprocess
 
 import pytest
 
@@ -33,6 +37,27 @@ def test_heads_are_sliced(dp):
     for s in HEADS:
         plan = dp.ops.GatedShape(*s, dtype="bf16").plan8()
         assert plan["gate" if s[3] <= 4 else "gate_back"][2] > 1, s
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gates_that_no_join_follows(dp, dtype):
+    """The gate that sums h dy in its tiles is never sliced, and has no tile of 128 x 128 with two to four outputs."""
+    rng = random.Random(1)
+    for _ in range(5000):
+        n, d, f = (round(math.exp(rng.uniform(0, math.log(m)))) for m in (100000, 4096, 8192))
+        plan = dp.ops.GatedShape(n, d, f, rng.randint(1, 4), dtype=dtype).plan8()
+        assert plan.get("gate_outs", (0, 0, 1))[2] == plan.get("gate_one", (0, 0, 1))[2] == 1
+        assert plan.get("gate_outs", (0, 0, 1))[:2] != (128, 128)
+
+
+def test_no_join_is_built_for_them(dp):
+    """A kernel that no call may reach is not in the library (kEpiGateOuts is 6, kEpiGateOne 7)."""
+    if not (shutil.which("nm") and os.path.exists(dp.LIB_PATH)):
+        pytest.skip("no nm, or the library is not built")
+    names = subprocess.run(["nm", "-C", dp.LIB_PATH], check=True, capture_output=True, text=True).stdout
+    built = {m for m in re.findall(r"k_join<(\d), (\d)>", names)}
+    assert {("0", "1"), ("0", "2"), ("0", "5")} <= built
+    assert not [b for b in built if b[1] in "67"]
 
 
 def test_plan(dp):
