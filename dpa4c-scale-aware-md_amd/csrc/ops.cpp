@@ -182,7 +182,8 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
     q.slices = gate_outs_slices(p0, elem, n);
     down_bytes = sizeof(float) * q.slices * (size_t)f * s.d_out;
   }
-  const size_t at_part = r.take(std::max({p0.bytes, p1.bytes, dx ? p2.bytes : 0, dwg ? p3.bytes : 0,
+  // (dh's slices from a checkpoint are in at_saved)
+  const size_t at_part = r.take(std::max({p0.bytes, kept ? 0 : p1.bytes, dx ? p2.bytes : 0, dwg ? p3.bytes : 0,
                                           dwd ? down_bytes : 0}));
   char* ws = workspace(O, st, r.used);
   float* part = reinterpret_cast<float*>(ws + at_part);

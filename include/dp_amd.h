@@ -473,8 +473,12 @@ int dp_restore8(dp_ops* ops, int type, int64_t rows, int cols, const void* d_kep
 /*
  * dp_gated_backward from the checkpoint of x [rows][d_in] alone, with nothing kept by the forward (d_saved
  * NULL): x w_gate and x w_up are formed again from the restored x, and the gradients are those of the block
- * there. It keeps d_in * 33 / 32 bytes a row in place of x and 8 d_hidden. The workspace takes, for the
- * time of the call, x and at most what the forward would have kept, which the calls of all layers on a stream share.
+ * there. It keeps d_in * 33 / 32 bytes a row in place of x and 8 d_hidden. The workspace, which the calls of all layers
+ * on a stream share, takes for the time of the call x, dg, du and (for d_w_down) h in the call's type, and in fp32 dh: once, or
+ * with few rows once for each slice of its sum (64 rows of 64-512-4096: 15). With up to four outputs there is neither h
+ * nor dh, but x w_gate and x w_up in fp32 where their sums are sliced. (2048-8192-2048 in bf16: 84 KB a row for the call
+ * of one layer, where each layer's forward would keep 64.) Beside them stand the operands that are not whole 16-byte
+ * chunks and the slices of the largest product, as in dp_gated_backward.
  */
 int dp_gated_backward8(dp_ops* ops, const dp_gated_shape* shape, const void* d_kept,
                        const void* d_w_gate, const void* d_w_up, const void* d_w_down,
