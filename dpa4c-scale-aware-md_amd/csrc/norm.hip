@@ -312,7 +312,7 @@ __device__ __forceinline__ Entries<VE, GEN> moments(const float (&v)[ROWS][VE]) 
 __device__ __forceinline__ void join_moments(Pair& p, float n, const Pair& q, float k) {
   const float d = q.a - p.a, w = n == 0.0f ? 1.0f : k * __builtin_amdgcn_rcpf(n + k);
   p.a += d * w;
-  p.b += q.b + d * d * n * w;
+  p.b += q.b + d * (d * (n * w));  // (with n == 0 d is q's mean, whose square may leave the range)
 }
 template <int VE, int GEN>
 __device__ __forceinline__ void join_rows(Entries<VE, GEN>& s, int n, const Entries<VE, GEN>& q, int k) {

@@ -1,0 +1,46 @@
+"""Group norm at the ends of fp32's range and at lengths whose products leave 32-bit integers, in each of its
+forms: rows by themselves, frames of a block, frames in slices."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_ops import stream
+
+pytestmark = pytest.mark.gpu
+
+# rows, channels, groups, frames: as above, the last two in slices
+FORMS = [(64, 64, 4, 64), (640, 64, 4, 10), (20000, 64, 4, 1), (20000, 65, 5, 1)]
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ops(dp):
+    return dp.ops.Operators()
+
+
+def norm(ops, dp, x, groups, frames, eps, starts=0):
+    """y and stats of x without gamma and beta."""
+    dtype = next(k for k, t in TYPES.items() if t == x.dtype)
+    y, stats = torch.zeros_like(x), torch.empty(frames, groups, 2, device="cuda")
+    shape = dp.ops.NormShape(*x.shape, groups, frames=frames, dtype=dtype, eps=eps)
+    ops.group_norm(shape, x.data_ptr(), 0, 0, y.data_ptr(), stats=stats.data_ptr(), starts=starts, stream=stream())
+    torch.cuda.synchronize()
+    return y, stats
+
+
+@pytest.mark.parametrize("dtype,step", [("f32", 54), ("bf16", 58)])
+@pytest.mark.parametrize("rows,ch,groups,frames", FORMS)
+def test_means_whose_squares_leave_the_range(ops, dp, dtype, step, rows, ch, groups, frames):
+    """2^65 and one step more: the mean's square passes 2^128, those of the deviations and their sums (in bf16 of a
+    slice's rows) do not. The mean is off by 32 roundings of a batch's sum and one of each of at most 320 joins,
+    2^-24 of it each: below 352 * 2^41 < 2^50, an eighth of the deviations (2^53 and more); y (one in magnitude) by that
+    and by its rounding."""
+    gen = torch.Generator().manual_seed(rows + ch)
+    x = (2.0 ** 65 + 2.0 ** step * torch.randint(0, 2, (rows, ch), generator=gen).double()).to(TYPES[dtype])
+    y, _ = norm(ops, dp, x.cuda(), groups, frames, 0.0)
+    a = x.double().reshape(frames, rows // frames, groups, -1)
+    m = a.mean((1, 3), keepdim=True)
+    want = ((a - m) / (a - m).square().mean((1, 3), keepdim=True).sqrt()).reshape(rows, ch)
+    assert bool(torch.isfinite(y).all())
+    assert float((y.double().cpu() - want).abs().max()) < 0.25 * float(want.abs().max())
