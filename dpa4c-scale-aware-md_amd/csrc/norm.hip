@@ -383,9 +383,12 @@ __device__ __forceinline__ float sum_lanes(float v, int log_lanes) {
   if (log_lanes > 5) v = add_xor32(v);
   return v;
 }
-// 1 / sqrt(M / n + eps), inv = 1 / n
+// 1 / sqrt(M / n + eps), inv = 1 / n. NaN where squares or their sum have left fp32's range (1 / sqrt would be zero,
+// and y act(beta) without a word), and infinite below the normal numbers, whose squares have lost their digits.
 __device__ __forceinline__ float deviation(float M, float inv, float eps) {
-  return __builtin_amdgcn_rsqf(__builtin_fmaf(M, inv, eps));
+  const float var = __builtin_fmaf(M, inv, eps);
+  const float r = var < __builtin_inff() ? __builtin_amdgcn_rsqf(var) : __builtin_nanf("");
+  return var < 0x1p-126f ? __builtin_inff() : r;
 }
 
 // A barrier among the threads that share a row: a wave's, or the block's.
@@ -1095,9 +1098,10 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats_join(const NormArgs p) 
     const double m = first.a + d;
     double var = M * inv;
     if (var < 0.0) var = 0.0;  // (and a NaN stays one)
-    if (threadIdx.x == 0)
-      *reinterpret_cast<Pair*>(p.stats + 2 * at) =
-          total > 0.0 ? Pair{(float)m, (float)(1.0 / sqrt(var + (double)p.eps))} : Pair{0.0f, 0.0f};
+    var += (double)p.eps;
+    // (as deviation() has it)
+    const float r = var < 0x1p-126 ? __builtin_inff() : var < __builtin_inf() ? (float)(1.0 / sqrt(var)) : __builtin_nanf("");
+    if (threadIdx.x == 0) *reinterpret_cast<Pair*>(p.stats + 2 * at) = total > 0.0 ? Pair{(float)m, r} : Pair{0.0f, 0.0f};
   }
 }
 

@@ -535,7 +535,9 @@ int dp_linear8(dp_ops* ops, const dp_linear8_shape* shape, const void* d_x, cons
  * off. d_stats: NULL, or [frames][groups] pairs of m and r in fp32 (8-byte aligned; zeros for an empty frame), for
  * the backward. m, r and all sums are formed in fp32 or fp64 (never as a difference of large sums), y is rounded
  * once. The activations are those of the block, gelu to 2e-7 of max(1, |z|) in 16 bits. A NaN or an infinity makes
- * its frame's group NaN. With rows == 0 nothing is done.
+ * its frame's group NaN, and so do values whose sum, or deviations whose squares' sum, leaves fp32's range (deviations of
+ * 1e19, or of 1e16 over a million values; means may be of any size). A variance + eps below 2^-126 (which takes an eps
+ * of 0, or almost) counts as zero: r is infinite. With rows == 0 nothing is done.
  */
 typedef struct {
   int64_t rows;

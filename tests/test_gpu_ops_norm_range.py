@@ -44,3 +44,32 @@ def test_means_whose_squares_leave_the_range(ops, dp, dtype, step, rows, ch, gro
     want = ((a - m) / (a - m).square().mean((1, 3), keepdim=True).sqrt()).reshape(rows, ch)
     assert bool(torch.isfinite(y).all())
     assert float((y.double().cpu() - want).abs().max()) < 0.25 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,ch,groups,frames", FORMS)
+def test_deviations_whose_squares_leave_the_range(ops, dp, dtype, rows, ch, groups, frames):
+    """Deviations of 10^20: their group is NaN, as with an infinity, and not act(beta); other groups are not."""
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, ch, generator=gen)
+    x[:, ch // groups:2 * ch // groups] *= 1e20
+    y, stats = norm(ops, dp, x.to(TYPES[dtype]).cuda(), groups, frames, 1e-5)
+    bad = torch.zeros(ch, dtype=torch.bool)
+    bad[ch // groups:2 * ch // groups] = True
+    assert bool(torch.isnan(y[:, bad]).all()) and bool(torch.isfinite(y[:, ~bad]).all())
+    assert bool(torch.isnan(stats[:, 1, 1]).all())
+
+
+@pytest.mark.parametrize("rows,ch,groups,frames", FORMS)
+def test_variances_below_the_normal_numbers(ops, dp, rows, ch, groups, frames):
+    """Deviations of 2^-70 with eps 0: a variance below 2^-126 counts as zero, whose r is infinite, in each form; one of
+    2^-122 does not."""
+    gen = torch.Generator().manual_seed(rows)
+    sign = torch.randint(0, 2, (rows, ch), generator=gen).float() * 2 - 1
+    y, stats = norm(ops, dp, (sign * 2.0 ** -70).cuda(), groups, frames, 0.0)
+    assert bool((stats[..., 1] == math.inf).all()) and not bool(torch.isfinite(y).any())
+    y, stats = norm(ops, dp, (sign * 2.0 ** -61).cuda(), groups, frames, 0.0)
+    assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(stats).all())
+    # (an eps of its own makes both ordinary)
+    y, stats = norm(ops, dp, (sign * 2.0 ** -70).cuda(), groups, frames, 2.0 ** -100)
+    assert bool((y.abs() < 2.0 ** -19).all()) and bool((stats[..., 1] == 2.0 ** 50).all())
