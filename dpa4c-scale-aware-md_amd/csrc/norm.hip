@@ -308,7 +308,8 @@ __device__ __forceinline__ Entries<VE, GEN> moments(const float (&v)[ROWS][VE]) 
   }
   return s;
 }
-// (m, M) of n values joined with that of k more
+// (m, M) of n values joined with that of k more. (Numbers of values are floats: a frame of 2^28 rows has more than
+// an integer counts.)
 __device__ __forceinline__ void join_moments(Pair& p, float n, const Pair& q, float k) {
   const float d = q.a - p.a, w = n == 0.0f ? 1.0f : k * __builtin_amdgcn_rcpf(n + k);
   p.a += d * w;
@@ -318,7 +319,7 @@ template <int VE, int GEN>
 __device__ __forceinline__ void join_rows(Entries<VE, GEN>& s, int n, const Entries<VE, GEN>& q, int k) {
   constexpr int N = entries_of<VE, GEN>(), W = VE / N;
 #pragma unroll
-  for (int i = 0; i < N; ++i) join_moments(s.e[i], (float)(n * W), q.e[i], (float)(k * W));
+  for (int i = 0; i < N; ++i) join_moments(s.e[i], (float)n * W, q.e[i], (float)k * W);
 }
 // Sums of each entry's channels: of b (a) and of g (b)
 template <int VE, int GEN>
@@ -825,7 +826,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) mine.e[GEN ? e : 0].a += v[e];
     }
-    const float inv = have ? 1.0f / (float)(have * W) : 0.0f;
+    const float inv = have ? 1.0f / ((float)have * W) : 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) mine.e[i].a *= inv;
 #pragma unroll
@@ -856,7 +857,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_frames(const NormArgs p) {
       for (int k = lane; k < all; k += 1 << p.lanes) {
         const int tr = k / p.group_entries, rows = rows_of(w.count, tr, l.TR);
         const Pair s = parts[tr * wide + q * p.group_entries + k - tr * p.group_entries];
-        M += s.b + (float)(rows * W) * (s.a - m) * (s.a - m);
+        M += s.b + (float)rows * W * (s.a - m) * (s.a - m);
       }
       M = sum_lanes(M, p.lanes);
       const Pair s = w.count ? Pair{m, deviation(M, 1.0f / total, p.eps)} : Pair{0.0f, 0.0f};
@@ -1013,7 +1014,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(const NormArgs p) {
       int have = rows_of(w.count, 0, l.TR);
       for (int tr = 1; tr < l.TR; ++tr) {
         const int n = rows_of(w.count, tr, l.TR);
-        if (n) join_moments(s, (float)(have * W), parts[tr * wide + k], (float)(n * W));
+        if (n) join_moments(s, (float)have * W, parts[tr * wide + k], (float)n * W);
         have += n;
       }
       parts[k] = s;
@@ -1024,7 +1025,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(const NormArgs p) {
       float m = 0.0f, M = 0.0f;
       for (int k = e0 + lane; k < e1; k += 1 << p.lanes) m += parts[k].a;
       m = sum_lanes(m, p.lanes) / (float)(e1 - e0);
-      const float each = (float)(w.count * W);
+      const float each = (float)w.count * W;
       for (int k = e0 + lane; k < e1; k += 1 << p.lanes) M += parts[k].b + each * (parts[k].a - m) * (parts[k].a - m);
       M = sum_lanes(M, p.lanes);
       if (in && lane == 0) out[q] = Pair{m, M};
