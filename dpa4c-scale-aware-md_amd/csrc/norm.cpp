@@ -147,8 +147,9 @@ NormArgs norm_args(const dp_norm_shape* shape, const void* starts) {
   require(s.rows >= 0 && s.rows <= kMaxRows, "rows out of range");
   require(s.channels >= 1 && s.channels <= kMaxDim, "channels must be 1 .. 2^20");
   require(s.groups >= 1 && s.groups <= s.channels && s.channels % s.groups == 0, "groups must divide channels");
-  require(s.frames >= 1 && s.frames <= kMaxRows, "frames must be 1 .. 2^30");
-  require(starts || s.rows % s.frames == 0, "rows are not the same number for each frame, and there are no starts");
+  // (as many frames as rows, where there are none)
+  require(s.frames >= (s.rows ? 1 : 0) && s.frames <= kMaxRows, "frames must be 1 .. 2^30");
+  require(starts || s.rows == 0 || s.rows % s.frames == 0, "rows are not the same number for each frame, and there are no starts");
   require(s.eps >= 0.0f && s.eps < 1e30f, "eps must be a number from 0 on");
   NormArgs p{};
   p.rows = (long)s.rows;

@@ -529,7 +529,7 @@ int dp_linear8(dp_ops* ops, const dp_linear8_shape* shape, const void* d_x, cons
  * ones, rows of a frame (a cell, a sample) normalised together,
  *   y = act(gamma (x - m) r + beta),  m the mean and r = 1 / sqrt(variance + eps) of the frame's rows over the
  * group's channels (the variance around m, over their number). gamma and beta [channels] of the call's type, or
- * NULL: ones, zeros. Frames are `frames` equal parts of the rows (rows of them: each row by itself), or with d_starts
+ * NULL: ones, zeros. Frames are `frames` equal parts of the rows (rows of them, 0 of 0: each row by itself), or with d_starts
  * [frames + 1] (32-bit integers) the rows starts[f] .. starts[f + 1] - 1, not descending; a frame may be empty,
  * and rows before the first and behind the last one are left as they were. What starts holds beyond the rows is cut
  * off. d_stats: NULL, or [frames][groups] pairs of m and r in fp32 (8-byte aligned; zeros for an empty frame), for
