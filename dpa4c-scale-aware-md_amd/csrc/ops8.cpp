@@ -8,8 +8,10 @@ using namespace dpamd;
 
 namespace {
 
-// A product of two integers is at most 127^2, and a sum of so many of them stays below 2^31.
+// A product of two integers is at most 127 * 128 (a row's are quantised here, weights may hold -128), and a sum of so
+// many of them stays below 2^31.
 constexpr int64_t kMaxIn8 = 1 << 17;
+static_assert(127 * 128 * kMaxIn8 < int64_t(1) << 31, "sums of 8-bit products are 32-bit integers");
 
 void check_type(int type) {
   require(type == DP_TYPE_F32 || type == DP_TYPE_BF16 || type == DP_TYPE_F16, "unknown type");
