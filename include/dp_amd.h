@@ -510,7 +510,8 @@ int dp_weights8(dp_ops* ops, int type, int d_in, int d_out, const void* d_w, int
  * g = (sum over k of q_x q_w) scale_x scale_w, and u the same of the second weights: the sums are exact (d_in is at
  * most 2^17), g and u are fp32, and y is rounded once. The integers may be any, from dp_weights8 or
  * not; what lies past d_in in their rows is not looked at, but has to be readable up to a multiple of 16.
- * The activations are those of the block, and DP_ACT_NONE; with results of 16 bits gelu is off by 2e-7 of max(1, |g|).
+ * The activations are those of the block, and DP_ACT_NONE; with results of 16 bits gelu's normal distribution is off by
+ * 2.2e-7, or by 2.2e-5 of itself in the tail, where that is less.
  */
 enum { DP_ACT_NONE = 3 };
 typedef struct {
@@ -534,7 +535,7 @@ int dp_linear8(dp_ops* ops, const dp_linear8_shape* shape, const void* d_x, cons
  * and rows before the first and behind the last one are left as they were. What starts holds beyond the rows is cut
  * off. d_stats: NULL, or [frames][groups] pairs of m and r in fp32 (8-byte aligned; zeros for an empty frame), for
  * the backward. m, r and all sums are formed in fp32 or fp64 (never as a difference of large sums), y is rounded
- * once. The activations are those of the block, gelu to 2e-7 of max(1, |z|) in 16 bits. A NaN or an infinity makes
+ * once. The activations are those of the block, in 16 bits gelu as in dp_linear8. A NaN or an infinity makes
  * its frame's group NaN, and so do values whose sum, or deviations whose squares' sum, leaves fp32's range (deviations of
  * 1e19, or of 1e16 over a million values; means may be of any size). A variance + eps below 2^-126 (which takes an eps
  * of 0, or almost) counts as zero: r is infinite. With rows == 0 nothing is done.
