@@ -37,8 +37,9 @@ struct NormArgs {
   float* sums;     // [frames][groups][2]: means of gamma dz and gamma dz v
 };
 
-// kNormRows: every row a frame of its own, a wave or a block a row, in registers.
-// kNormFrames: a block takes whole frames over a part of the groups, and reads them twice.
+// kNormRows: every row a frame of its own, 4 to 256 threads a row, in registers.
+// kNormFrames: a block takes whole frames over a part of the groups; each thread's first rows stay in registers, what
+// is beyond them is read twice.
 // kNormSlices: frames cut into slices of rows, whose sums meet in memory.
 enum NormForm { kNormRows = 0, kNormFrames = 1, kNormSlices = 2 };
 

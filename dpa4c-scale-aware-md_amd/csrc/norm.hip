@@ -13,7 +13,7 @@
 // holds, around their own mean, and parts are joined by
 //   m = sum n_i m_i / n,  M = sum M_i + sum n_i (m_i - m)^2,
 // so that no difference of large sums occurs whatever the mean is. All in fp32; slices are joined in
-// fp64. Sums have an order that sizes alone fix.
+// fp64. Sums have an order that sizes, row lengths and the card's compute units fix.
 #include <algorithm>
 
 #include "norm.h"
