@@ -226,6 +226,7 @@ void gated_backward(dp_ops* O, const dp_gated_shape& s, const void* x, const uns
       q.partial = part;
       if (dwd) run_outs_join(st, elem, q);
     } else if (few) {
+      a.epi.h = ws + at_dg;  // (written and not read: dg comes after it)
       a.epi.saved = reinterpret_cast<float*>(ws + at_saved);
       run_product(st, kProdGate, elem, p0, a);
       saved = ws + at_saved;

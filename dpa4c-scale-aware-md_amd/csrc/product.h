@@ -492,7 +492,7 @@ struct TileOf {
       LAYOUT == kRowK || kRows >= kPeriod ? 1 : (kPeriod / kRows < kLoads ? kPeriod / kRows : kLoads);
   static constexpr __device__ int kind(int q) { return q % kOffsets; }
   static constexpr __device__ long moved(int q) {
-    return LAYOUT == kRowK ? (q * kRows) % kPart : (q * kRows) % BK / kPeriod * kPeriod;
+    return LAYOUT == kRowK ? (SUB == 1 ? q * kRows : (q * kRows) % kPart) : (q * kRows) % BK / kPeriod * kPeriod;
   }
   static __device__ __forceinline__ unsigned offset(int q, int wave, int lane, long ld, int rows_left) {
     int part, row, chunk;
@@ -515,7 +515,7 @@ struct TileOf {
     int part, row, chunk;
     if constexpr (LAYOUT == kRowK) {
       place(0, wave, lane, part, row, chunk);
-      return chunk * VE >= k_left || row >= rows_left - moved(q);
+      return chunk * VE >= k_left || row >= rows_left - (int)moved(q);
     } else {
       place(q, wave, lane, part, row, chunk);
       return row >= k_left;
@@ -793,7 +793,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
     const int m0 = done.m0 + wm * TM + c, n0 = done.n0 + wn * (TN / SUB) + 4 * g;
     constexpr bool WIDE = KIND != kF32;  // pairs of fragments are stored together
     const bool inside = done.m0 + (wm + 1) * TM <= p.M && done.n0 + (wn + 1) * (TN / SUB) <= p.N;
-    if (p.split > 1 || p.raw) {
+    if (p.split > 1 || (EPI == kEpiStore && LB == kRowK && p.raw)) {
       // a slice's sums, columns in rows of ldp (a multiple of 4)
       const int sub = SUB == 2 ? 2 : p.mats;
       float* o = p.partial + (((long)done.slice * sub + done.mat) * p.M + m0) * p.ldp + n0;
@@ -857,7 +857,6 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
           if (h32) {
 #pragma unroll
             for (int j = 0; j < NG; ++j) *reinterpret_cast<f4*>(h32 + h + j * 16) = v[j];
-          } else if (!to) {  // (g and u are all that is wanted)
           } else if constexpr (WIDE && NG % 2 == 0) {
 #pragma unroll
             for (int j = 0; j < NG; j += 2) put_pair<KIND>(to + h + pair_at(g) + j * 16, v[j], v[j + 1]);
@@ -876,7 +875,7 @@ __global__ __launch_bounds__(S::WM* S::WN * 64) void k_product(const ProductArgs
               const f4 v = gate_value<false>(p.act, count, acc[i][j], acc[i][j + NG]);
               if (h32)
                 *reinterpret_cast<f4*>(h32 + h + j * 16) = v;
-              else if (to)
+              else
                 put4<KIND>(to + h + j * 16, v);
               if (p.epi.saved) put_kept<false>(kept + j * 16, plane, count, acc[i][j], acc[i][j + NG]);
             }
@@ -1101,7 +1100,7 @@ __global__ __launch_bounds__(256) void k_join(const ProductArgs p) {
     const f4 h = gate_value<false>(p.act, p.N - n, v, w);
     if (p.epi.h32)
       *reinterpret_cast<f4*>(p.epi.h32 + m * p.epi.ldh + n) = h;
-    else if (p.epi.h)
+    else
       put4<KIND>(static_cast<typename ElemOf<KIND>::T*>(p.epi.h) + m * p.epi.ldh + n, h);
     if (p.epi.saved) put_kept<false>(p.epi.saved + (m * p.N + n), plane, p.N - n, v, w);
   } else if constexpr (EPI == kEpiGateBack) {
