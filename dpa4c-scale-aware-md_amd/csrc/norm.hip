@@ -435,7 +435,7 @@ __device__ __forceinline__ void each_entry(const NormArgs& p, const Pair* parts,
 // T threads a row, C vectors of VE channels a thread (at neighbouring places for neighbouring threads). With
 // LANES a group is a power of two of vectors, at most 64, so that it is that many neighbouring lanes, which
 // add up without LDS or a barrier; else the entries of a row meet in LDS, and then a pair for each group.
-// (16,384 x 2048 in bf16, groups of 64, gelu: 50 us through LDS, 38 by lanes, and 29 with gelu's short form; a copy's
+// (16,384 x 2048 in bf16, groups of 64, gelu: 50 us through LDS, 38 by lanes, and 34 with gelu in six terms; a copy's
 // rate would be 26.) A block takes rows one after another: gamma and beta stay in registers, and the next row is
 // loaded while this one is computed.
 template <int KIND, int VE, int GEN, int T, int C, bool LANES, bool ONCE>
