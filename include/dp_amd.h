@@ -540,7 +540,7 @@ int dp_linear8(dp_ops* ops, const dp_linear8_shape* shape, const void* d_x, cons
  * the backward. m, r and all sums are formed in fp32 or fp64 (never as a difference of large sums), y is rounded
  * once. The activations are those of the block, in 16 bits gelu as in dp_linear8. A NaN or an infinity makes
  * its frame's group NaN, and so do values whose sum, or deviations whose squares' sum, leaves fp32's range (deviations of
- * 1e19, or of 1e16 over a million values; means may be of any size). A variance + eps below 2^-126 (which takes an eps
+ * 1e19, or of 1e16 over a million values; a mean of 1e32 over as many). A variance + eps below 2^-126 (which takes an eps
  * of 0, or almost) counts as zero: r is infinite. With rows == 0 nothing is done.
  */
 typedef struct {
